@@ -230,6 +230,42 @@ int st_kv_attn(const void* q, int64_t qs, int64_t B, int64_t Hq, const void* kv,
                const int32_t* starts, void* out, int64_t os, float* wo, float* wml, double scale, int64_t S,
                int64_t minpps, void* stream);
 
+/* ---- KV pages in 8 bits ------------------------------------------------------------------------------------------ */
+/* No counterpart in the reference.  kv uint8 [blocks, H, 2 (K/V), 16, D] e4m3 codes, exps int8 [blocks, H, 2]; a code stands for
+ * e4m3(code) * 2^exp, -64 <= exp <= 56, so every value is a BF16 number.  D is 64 or 128; at 128 the 16-byte piece c of row r lies at
+ * place c ^ (r & 6) ^ 4 (r & 1).  2 * 16 * H * D bytes a page. */
+int64_t st_kv8_page_bytes(int64_t H, int64_t D);
+/* Append N tokens: K, V BF16 [N, H, D] (heads contiguous, token strides ks / vs in elements, multiples of 8); slot int64 [N] = block *
+ * 16 + row (negative or beyond the cache: not stored; the same slot twice: the last one counts).  With cos_t / sin_t (float [max_pos,
+ * D / 2]) keys are rotated by the tokens' positions pos[i * pos_step] (clamped to the tables; pos_step 0: one position for all) on
+ * pairs (2i, 2i + 1) (interleaved) or (i, i + D/2); with wk (BF16 [D]) they are RMS-normalised before.  Q (may be NULL; BF16 [N, Hq,
+ * D], stride qs) goes the same way with wq into q_out (stride qos; may be Q).  fp32 arithmetic, one rounding at the end.
+ * A unit's exponent (page, head, K or V) is the smallest that holds its new rows, or its old one if that is larger; the other rows are
+ * then rounded again.  A page written at row 0 starts anew: rows not written in the call become zero.  Values that are not finite, or
+ * beyond 448 * 2^56, are cut off there (NaN: zero) and *bad (int32) is set to 1.
+ * marks: int32 [17 * nblocks], zero on entry and on exit; may be NULL for calls of up to 512 tokens. */
+int st_kv8_append(const void* K, const void* V, int64_t ks, int64_t vs, const int64_t* slot, int64_t N, int64_t H, int64_t D, void* kv,
+                  int8_t* exps, int64_t nblocks, const int64_t* pos, int64_t pos_step, const float* cos_t, const float* sin_t,
+                  int64_t max_pos, int interleaved, const void* wk, const void* Q, int64_t qs, const void* wq, int64_t Hq, void* q_out,
+                  int64_t qos, double eps, int32_t* marks, int32_t* bad, void* stream);
+/* Listed pages (blocks NULL: the first n) -> dense BF16 [n, 16, H, D], exact; ids outside [0, nblocks) give zeros. */
+int st_kv8_dequant_blocks(const void* kv, const int8_t* exps, int64_t nblocks, int64_t H, int64_t D, const int32_t* blocks, int64_t n,
+                          void* Kd, void* Vd, void* stream);
+/* Decode attention, one query token per sequence: q, out BF16 [B, Hq, D] (16-byte aligned, token strides qs / os multiples of 8); bt
+ * int32 [B, bts]; keys [max(starts, lens - window), lens) take part (starts int32 [B] or NULL, window 0: none); a sequence without
+ * any gives zeros.  S splits with >= minpps pages each; wo float [B, Hq, S, D], wml float [B, Hq, S, 2] when S > 1. */
+int st_kv8_attn(const void* q, int64_t qs, int64_t B, int64_t Hq, const void* kv, const int8_t* exps, int64_t nblocks, int64_t Hkv,
+                int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens, const int32_t* starts, int64_t window, void* out,
+                int64_t os, float* wo, float* wml, double scale, int64_t S, int64_t minpps, void* stream);
+/* Causal attention of several query tokens per sequence, whose keys are in the pages already: q, out BF16 [T, Hq, D]; cu int32 [B + 1]:
+ * sequence b's queries are rows cu[b] .. cu[b + 1] - 1, the last at position lens[b] - 1 (cu NULL: one each).  A query at position p
+ * sees keys [max(starts, p - window + 1), p].  Rows of q behind cu[B] are left alone in out.  wo float [T, Hq, S, D], wml float [T, Hq,
+ * S, 2] when S > 1. */
+int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
+                      const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens,
+                      const int32_t* starts, int64_t window, void* out, int64_t os, float* wo, float* wml, double scale, int64_t S,
+                      void* stream);
+
 /* st_gemv (1 <= B <= 8) of a fused gate/up projection with the SwiGLU gate in the epilogue: the M = 2 I rows of the tree
  * are the gate and up projections interleaved in 16-row tiles (tile 2j = gate rows 16j .. 16j + 15, tile 2j + 1 = the
  * same rows of up); act BF16 [B, I] = silu(gate) * up with the rounding points of st_silu_mul (both products to BF16,

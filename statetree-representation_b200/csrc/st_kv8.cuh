@@ -1,0 +1,49 @@
+// The 8-bit KV page shared by its kernels (st_kv8.cu, st_kv8_chunk.cu).
+//
+// Page: uint8 [blocks, H, 2 (K/V), 16, D] e4m3 codes and int8 exps [blocks, H, 2]; value = e4m3(code) * 2^exp, exp in [E8_MIN, E8_MAX].
+// A power of two, because the codes are floating point: a finer scale would not make them more precise, and a page whose largest value
+// grows as tokens arrive changes its exponent without rounding again (but for codes that become subnormal).  Every value has four
+// significant bits, so it is a BF16 number exactly and the tensor cores read it without a rounding of their own.
+//
+// At D = 128 the 16-byte pieces of a row are kept in another order (piece8): rows are 128 B apart, and both ways in which a warp of the
+// decode kernel reads a page (eight rows x four pieces for keys, four even or odd rows x two pieces for values) then touch every bank
+// of shared memory once per eight lanes.
+#pragma once
+#include "st_common.cuh"
+
+namespace st {
+constexpr int E8_MIN = -64, E8_MAX = 56;
+constexpr int MAX_D8 = 128;
+
+template <int D>
+__device__ __forceinline__ int piece8(int row, int c) {
+  return D == 128 ? c ^ (row & 6) ^ ((row & 1) << 2) : c;
+}
+template <int D>
+__device__ __forceinline__ size_t page8_off(long long blk, int H, int h, int kvi) {
+  return (((size_t)blk * H + h) * 2 + kvi) * (PAGE * D);
+}
+__device__ __forceinline__ int page8_exp(int e) { return min(max(e, E8_MIN), E8_MAX); }
+// 2^e, e in [-126, 127]
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+
+// Four codes -> their BF16 bit patterns times 2^-120: the four exponent and three mantissa bits are put at the low end of BF16's
+// exponent field and the top of its mantissa, code 0 .. 7 of an exponent (subnormal) becoming subnormals, so the value is exact
+// without a multiplication; 2^120 goes into a factor that is applied anyway.  High bytes hi = s0000eee, low bytes lo = emmm0000.
+// (The codes 0x7F and 0xFF, which no append writes, read as +-480.)
+__device__ __forceinline__ void codes_split(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  hi = ((w & 0x70707070u) >> 4) | (w & 0x80808080u);
+  lo = (w & 0x0F0F0F0Fu) << 4;
+}
+__device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t& p01, uint32_t& p23) {
+  uint32_t lo, hi;
+  codes_split(w, lo, hi);
+  p01 = __byte_perm(lo, hi, 0x5140);
+  p23 = __byte_perm(lo, hi, 0x7362);
+}
+// the value of a BF16 pattern from codes_to_bf16 (low or high half) without its 2^-120 and with 2^e
+__device__ __forceinline__ float2 codes_value(uint32_t p, float up) {      // up = 2^(20 + e)
+  constexpr float C = 1.2676506002282294e30f;                             // 2^100
+  return make_float2(__uint_as_float(p << 16) * C * up, __uint_as_float(p & 0xFFFF0000u) * C * up);
+}
+}  // namespace st

@@ -81,6 +81,104 @@ class PageStore:
         return int(self.pcnt[0].item()), self.pool.shape[0]
 
 
+def _rows(t, D):
+    """t as the 8-bit kernels read it: heads contiguous, 16-byte aligned, token stride a multiple of 8 (copied if it is not)"""
+    if t.numel() == 0 or (t.stride(2) == 1 and (t.stride(1) == D or t.size(1) == 1) and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class PageStore8:
+    """Pages of one attention layer in 8 bits (256 B per token and head of dimension 128; a PageStore's take 400 and are lossless):
+    pages uint8 [blocks, H, 2 (keys, values), 16, D] of e4m3 codes and exps int8 [blocks, H, 2], a value being e4m3(code) * 2^exp
+    with one exponent per page, head and keys / values; the head dimension D is 64 or 128.  Same calls as PageStore; besides, append()
+    takes a rotation and norms, and chunk_attention() several query tokens per sequence.  All calls go to the current stream, allocate
+    only outputs and workspaces of their own (calls on several streams, and captured ones, do not meet there) and can be captured."""
+
+    def __init__(self, num_blocks, num_kv_heads, device, head_dim=128):
+        pages = torch.zeros(num_blocks, num_kv_heads, 2, PAGE, head_dim, dtype=torch.uint8, device=device)
+        self._take(pages, torch.full((num_blocks, num_kv_heads, 2), -64, dtype=torch.int8, device=device))
+
+    @classmethod
+    def over(cls, pages, exps):
+        """a store over page tensors that exist already (another store's, or part of a larger buffer)"""
+        self = cls.__new__(cls)
+        self._take(pages, exps)
+        return self
+
+    def _take(self, pages, exps):
+        kv_ext()._pages8("PageStore8", pages, exps)
+        self.pages, self.exps, self.device = pages, exps, pages.device
+        self.H, self.D = pages.shape[1], pages.shape[4]
+        self.marks = torch.zeros(17 * pages.shape[0], dtype=torch.int32, device=pages.device)    # the append's; zero between calls
+        self.bad = torch.zeros(1, dtype=torch.int32, device=pages.device)
+
+    def append(self, K, V, slots, positions=None, cos=None, sin=None, interleaved=True, q=None, q_norm=None, k_norm=None, eps=1e-6,
+               q_out=None):
+        """K, V [N, H, D] bf16, slots int64 [N] = block * 16 + row, -1 = padding token; the same slot twice: the last token counts.
+        With cos / sin (float32 [P, D / 2]) keys are rotated at positions int64 [N] (or [1]: one for all), on pairs (2i, 2i + 1), or
+        (i, i + D/2) with interleaved=False; with k_norm (bf16 [D]) they are RMS-normalised before.  q [N, Hq, D] goes the same way
+        (q_norm) into q_out, which is returned.  A page is written from row 0 on: doing that again starts it anew (its other rows
+        become zero); tokens that follow raise its exponent where they need to."""
+        K, V = _rows(K, self.D), _rows(V, self.D)
+        if q is not None:
+            q = _rows(q, self.D)
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        kv_ext().kv8_append(K, V, slots, self.pages, self.exps, self.marks, self.bad, positions, cos, sin, interleaved, k_norm, q, q_norm,
+                            q_out, eps)
+        return q_out
+
+    def attention(self, q, block_table, lens, scale, splits=None, starts=None, min_pages=4, out=None, window=0):
+        """one query token per sequence: q [B, Hq, D] bf16 -> [B, Hq, D] bf16; tokens [max(starts, lens - window), lens) take part
+        (window 0: from starts on).  splits: how many CTAs share a sequence (None: by batch size and table width)"""
+        q = _rows(q, self.D)
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        if splits is None:
+            splits = decode_splits(q.shape[0], self.H, block_table.shape[1])
+        wo, wml = self._partials(q, splits)
+        kv_ext().kv8_attn(q, self.pages, self.exps, block_table, lens, out, scale, splits, wo, wml, starts, min_pages, window)
+        return out
+
+    def chunk_attention(self, q, cu, block_table, lens, scale, splits=None, starts=None, out=None, window=0):
+        """causal attention of several query tokens per sequence, after their keys and values have been appended: q [T, Hq, D] bf16,
+        sequence b's rows are cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1]), the last of them at position lens[b] - 1 -> [T, Hq, D];
+        rows behind cu[B] of a given `out` stay as they are"""
+        q = _rows(q, self.D)
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        if splits is None:
+            splits = 1
+        wo, wml = self._partials(q, splits)
+        kv_ext().kv8_chunk_attn(q, cu, self.pages, self.exps, block_table, lens, out, scale, splits, wo, wml, starts, window)
+        return out
+
+    def _partials(self, q, splits):
+        """(wo, wml) of a call whose sequences are split: its own, from the caching allocator"""
+        if splits <= 1:
+            return None, None
+        rows = q.shape[0] * q.shape[1] * splits
+        flat = torch.empty(rows * (self.D + 2), dtype=torch.float32, device=q.device)
+        return flat[:rows * self.D], flat[rows * self.D:]
+
+    def dense(self, blocks=None):
+        """pages (all, or the listed block ids) as exact BF16 Kd, Vd [n, 16, H, D]"""
+        n = self.pages.shape[0] if blocks is None else blocks.numel()
+        Kd = torch.empty(n, PAGE, self.H, self.D, dtype=torch.bfloat16, device=self.device)
+        Vd = torch.empty_like(Kd)
+        kv_ext().kv8_dequant_blocks(self.pages, self.exps, None if blocks is None else blocks.to(torch.int32).contiguous(), Kd, Vd)
+        return Kd, Vd
+
+    def check(self):
+        """raise if a value that is not finite (or beyond 448 * 2^56) was appended: it was cut off, a NaN stored as zero"""
+        if int(self.bad.item()):
+            raise RuntimeError("PageStore8: values that are not finite were appended")
+
+    def reset(self):
+        self.bad.zero_()
+
+
 class PagedKVCache:
     """Static paged cache for a decoder: per-layer pages, one block table [B, max_pages] (sequence b owns pages
     b * max_pages ...), a GPU-side token count so decode steps are CUDA-graph safe."""

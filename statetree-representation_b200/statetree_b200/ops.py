@@ -59,6 +59,14 @@ _SIGNATURES = {
     "st_kv_append": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _int, _vp]),
     "st_kv_dequant": (_int, [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
     "st_kv_dequant_blocks": (_int, [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "st_kv8_page_bytes": (_i64, [_i64, _i64]),
+    "st_kv8_append": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _vp, _vp,
+                             _i64, _vp, _i64, _vp, _i64, _dbl, _vp, _vp, _vp]),
+    "st_kv8_dequant_blocks": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "st_kv8_attn": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _dbl,
+                           _i64, _i64, _vp]),
+    "st_kv8_chunk_attn": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64,
+                                 _vp, _vp, _dbl, _i64, _vp]),
     "st_gemv_swiglu_supported": (_int, [_i64, _i64, _i64]),
     "st_gemv_swiglu": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "st_rope_kv_append": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _dbl, _vp, _vp, _i64,
@@ -562,6 +570,138 @@ class _KV:
             _check(lib().st_kv_attn(_ptr(q), q.stride(0), B, Hq, _ptr(kv), kv.size(0), Hkv, _ptr(pool), pool.size(0),
                                     _ptr(bt), bt.stride(0), _ptr(lens), _ptr(starts), _ptr(out), out.stride(0),
                                     _ptr(wo), _ptr(wml), float(scale), int(S), int(minpps), _stream(q)))
+
+    # ---- pages in 8 bits (no counterpart in the reference)
+    @staticmethod
+    def _pages8(who, kv, exps, *others):
+        """(H, D) of the pages kv uint8 [blocks, H, 2, 16, D] with exps int8 [blocks, H, 2]; `others` lie on their device"""
+        if not (kv.dtype == torch.uint8 and kv.dim() == 5 and kv.shape[2:4] == (2, 16) and kv.shape[4] in (64, 128) and kv.is_contiguous()):
+            raise RuntimeError(f"{who}: cache uint8 [blocks, H, 2, 16, 64 or 128]")
+        if not (exps.dtype == torch.int8 and exps.shape == kv.shape[:3] and exps.is_contiguous()):
+            raise RuntimeError(f"{who}: exponents int8 [blocks, H, 2]")
+        for t in (exps, *others):
+            if t is not None and t.device != kv.device:
+                raise RuntimeError(f"{who}: a tensor on {t.device}, the cache on {kv.device}")
+        return kv.shape[1], kv.shape[4]
+
+    @staticmethod
+    def _rows8(who, name, t, D):
+        """t is BF16 [N, heads, D] with heads contiguous, as the kernels read it (16-byte vectors)"""
+        if not (t.dtype == torch.bfloat16 and t.dim() == 3 and t.size(2) == D):
+            raise RuntimeError(f"{who}: {name} BF16 [N, heads, {D}]")
+        if t.numel() and not (t.stride(2) == 1 and (t.stride(1) == D or t.size(1) == 1) and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0):
+            raise RuntimeError(f"{who}: {name} with heads contiguous, 16-byte aligned, token stride a multiple of 8")
+
+    @staticmethod
+    def kv8_append(K, V, slot, kv, exps, marks, bad, positions=None, cos=None, sin=None, interleaved=True, wk=None, Q=None, wq=None,
+                   q_out=None, eps=1e-6):
+        """K, V [N, H, D] (K normalised with wk and rotated by positions, if given) into the pages at slot [N]; Q [N, Hq, D] likewise
+        into q_out"""
+        who = "kv8_append"
+        H, D = _KV._pages8(who, kv, exps, K, V, slot, marks, bad, positions, cos, sin, wk, Q, wq, q_out)
+        for name, t in (("K", K), ("V", V)):
+            _KV._rows8(who, name, t, D)
+        N = K.size(0)
+        if K.size(1) != H or V.shape != K.shape:
+            raise RuntimeError(f"{who}: K and V of the cache's {H} heads")
+        if not (slot.dtype == torch.int64 and slot.is_contiguous() and slot.numel() == N):
+            raise RuntimeError(f"{who}: slots int64 [N]")
+        if not (marks.dtype == torch.int32 and marks.is_contiguous() and marks.numel() >= 17 * kv.size(0) and bad.dtype == torch.int32
+                and bad.numel() >= 1):
+            raise RuntimeError(f"{who}: marks int32 [17 * blocks], bad int32 [1]")
+        step, span = 0, 0
+        if (cos is None) != (sin is None) or (cos is not None and positions is None):
+            raise RuntimeError(f"{who}: a rotation takes positions, cos and sin")
+        if cos is not None:
+            if not (positions.dtype == torch.int64 and positions.is_contiguous() and positions.numel() in (1, N)):
+                raise RuntimeError(f"{who}: positions int64 [N] or [1]")
+            if not (cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and cos.size(1) == D // 2
+                    and cos.size(0) > 0 and cos.is_contiguous() and sin.is_contiguous()):
+                raise RuntimeError(f"{who}: cos and sin float32 [positions, {D // 2}]")
+            step, span = int(positions.numel() > 1), cos.size(0)
+        for w in (wk, wq):
+            if w is not None and not (w.dtype == torch.bfloat16 and w.numel() == D and w.is_contiguous() and w.data_ptr() % 16 == 0):
+                raise RuntimeError(f"{who}: norm weights BF16 [{D}], 16-byte aligned")
+        Hq = qs = qos = 0
+        if Q is not None:
+            if q_out is None or Q.size(0) != N or q_out.shape != Q.shape:
+                raise RuntimeError(f"{who}: Q and q_out [N, Hq, {D}]")
+            _KV._rows8(who, "Q", Q, D)
+            _KV._rows8(who, "q_out", q_out, D)
+            Hq, qs, qos = Q.size(1), Q.stride(0), q_out.stride(0)
+        if N == 0:
+            return
+        with _ctx(kv):
+            _check(lib().st_kv8_append(K.data_ptr(), V.data_ptr(), K.stride(0), V.stride(0), slot.data_ptr(), N, H, D, kv.data_ptr(),
+                                       exps.data_ptr(), kv.size(0), None if cos is None else positions.data_ptr(), step, _ptr(cos),
+                                       _ptr(sin), span, 1 if interleaved else 0, _ptr(wk), _ptr(Q), qs, _ptr(wq), Hq, _ptr(q_out), qos,
+                                       float(eps), marks.data_ptr(), bad.data_ptr(), _stream(kv)))
+
+    @staticmethod
+    def kv8_dequant_blocks(kv, exps, blocks, Kd, Vd):
+        """listed pages (int32; None: all) as BF16 [n, 16, H, D]"""
+        who = "kv8_dequant_blocks"
+        H, D = _KV._pages8(who, kv, exps, blocks, Kd, Vd)
+        if blocks is not None and not (blocks.dtype == torch.int32 and blocks.is_contiguous() and blocks.dim() == 1):
+            raise RuntimeError(f"{who}: blocks int32 [n]")
+        n = kv.size(0) if blocks is None else blocks.numel()
+        for t in (Kd, Vd):
+            if not (t.dtype == torch.bfloat16 and t.is_contiguous() and t.numel() == n * 16 * H * D):
+                raise RuntimeError(f"{who}: outputs BF16 [n, 16, H, D]")
+        if n == 0:
+            return
+        with _ctx(kv):
+            _check(lib().st_kv8_dequant_blocks(kv.data_ptr(), exps.data_ptr(), kv.size(0), H, D, _ptr(blocks), n, Kd.data_ptr(),
+                                               Vd.data_ptr(), _stream(kv)))
+
+    @staticmethod
+    def _attn8(who, q, cu, kv, exps, bt, lens, out, starts, window, S, wo, wml):
+        H, D = _KV._pages8(who, kv, exps, q, cu, bt, lens, out, starts, wo, wml)
+        _KV._rows8(who, "q", q, D)
+        _KV._rows8(who, "out", out, D)
+        B, Hq = bt.size(0), q.size(1)
+        if Hq % H or out.shape != q.shape:
+            raise RuntimeError(f"{who}: q and out [tokens, a multiple of {H} heads, {D}]")
+        if not (bt.dtype == torch.int32 and bt.dim() == 2 and bt.stride(1) == 1 and lens.dtype == torch.int32 and lens.is_contiguous()
+                and lens.numel() == B):
+            raise RuntimeError(f"{who}: block table int32 [B, pages], lens int32 [B]")
+        if starts is not None and not (starts.dtype == torch.int32 and starts.is_contiguous() and starts.numel() == B):
+            raise RuntimeError(f"{who}: starts int32 [B]")
+        if window < 0 or S < 1:
+            raise RuntimeError(f"{who}: window / splits")
+        if S > 1 and not (wo is not None and wml is not None and wo.dtype == wml.dtype == torch.float32
+                          and wo.numel() >= q.size(0) * Hq * S * D and wml.numel() >= q.size(0) * Hq * S * 2):
+            raise RuntimeError(f"{who}: workspace")
+        return B, Hq, H, D
+
+    @staticmethod
+    def kv8_attn(q, kv, exps, bt, lens, out, scale, S=1, wo=None, wml=None, starts=None, minpps=1, window=0):
+        """one query token per sequence, q [B, Hq, D]"""
+        B, Hq, H, D = _KV._attn8("kv8_attn", q, None, kv, exps, bt, lens, out, starts, window, S, wo, wml)
+        if q.size(0) != B:
+            raise RuntimeError("kv8_attn: one query per sequence of the block table")
+        if B == 0:
+            return
+        with _ctx(kv):
+            _check(lib().st_kv8_attn(q.data_ptr(), q.stride(0), B, Hq, kv.data_ptr(), exps.data_ptr(), kv.size(0), H, D, bt.data_ptr(),
+                                     bt.stride(0), lens.data_ptr(), _ptr(starts), int(window), out.data_ptr(), out.stride(0), _ptr(wo),
+                                     _ptr(wml), float(scale), int(S), int(minpps), _stream(kv)))
+
+    @staticmethod
+    def kv8_chunk_attn(q, cu, kv, exps, bt, lens, out, scale, S=1, wo=None, wml=None, starts=None, window=0):
+        """causal attention of the query rows cu[b] .. cu[b + 1] - 1 of every sequence b, q [T, Hq, D]"""
+        who = "kv8_chunk_attn"
+        B, Hq, H, D = _KV._attn8(who, q, cu, kv, exps, bt, lens, out, starts, window, S, wo, wml)
+        if cu is None and q.size(0) != B:
+            raise RuntimeError(f"{who}: without cu every sequence has one query")
+        if cu is not None and not (cu.dtype == torch.int32 and cu.is_contiguous() and cu.numel() == B + 1):
+            raise RuntimeError(f"{who}: cu int32 [B + 1]")
+        if q.size(0) == 0 or B == 0:
+            return
+        with _ctx(kv):
+            _check(lib().st_kv8_chunk_attn(q.data_ptr(), q.stride(0), q.size(0), Hq, _ptr(cu), B, kv.data_ptr(), exps.data_ptr(),
+                                           kv.size(0), H, D, bt.data_ptr(), bt.stride(0), lens.data_ptr(), _ptr(starts), int(window),
+                                           out.data_ptr(), out.stride(0), _ptr(wo), _ptr(wml), float(scale), int(S), _stream(kv)))
 
 
 def ext():
