@@ -2,6 +2,8 @@
 // The page and why it is laid out so: st_kv8.cuh.
 #include <math.h>
 
+#include <atomic>
+
 #include "../../include/statetree_b200.h"
 #include "st_host.h"
 #include "st_kv8.cuh"
@@ -393,6 +395,348 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(const Attn8 a) {
   for (int d = 0; d < PL; d += 2)
     *reinterpret_cast<uint32_t*>(a.out + t * a.out_stride + (size_t)hq * D + PL * lane + d) = pack_bf16(o[d] * inv, o[d + 1] * inv);
 }
+// ------------------------------------------------------------------------------------------------ attention, one token per sequence
+// Orientation.  A decode step has few query heads per KV head, so the heads of a group go on the 8-wide N side of mma.m16n8k16 and
+// tokens / dims on the 16-wide M side (groups of more than eight take a CTA per eight heads):
+//     S^T [16 tokens x 8 heads] = K [16 tokens x D dims] . Q^T        O^T [D dims x 8 heads] += V^T [D dims x 16 tokens] . P^T
+// The order of the k index is free as long as both operands agree on it: lane (g, t) = (lane / 4, lane % 4) takes for keys the
+// 16-byte pieces t and t + 4 of rows g and g + 8 as they lie in the page, four dims per MMA, and q in the same order; for values the
+// piece g of tokens 2t, 2t + 1, 2t + 8, 2t + 9, two dims per MMA, the codes of two tokens being paired by a byte permute.  So a page
+// goes from its codes to fragments with 1.75 (keys) and 2 (values) integer operations a code and no transposition through memory.
+//
+// Scales.  Codes become BF16 numbers times 2^-120 (codes_split); q carries 2^60 and P 2^(60 + exponent of the page's values), so no
+// operand or sum leaves fp32's range for values within the format's, and the page's key exponent joins the softmax scale.
+// P is rounded to BF16 (2^-9 of each probability at most, unbiased), everything else is fp32: maxima, sums, partial results.
+//
+// Softmax: a head's reference maximum m is raised when a page holds a score more than 8 above it (base 2), one vote per page.
+//
+// Work split: grid = sequences x KV heads x head blocks x splits; a CTA's pages go round-robin to its warps, each of which streams its
+// own through a private ring of bulk copies (a page of one head is contiguous, 2 * 16 * D bytes), so there is no barrier in the loop.
+// Block-table entries and exponents come 32 pages at a time, one batch ahead.
+constexpr float RAISE8 = 8.f;
+
+struct Parts8 { float* o; float* ml; int splits, min_pages; };
+
+// q times 2^60, exactly (BF16 keeps its eight bits)
+__device__ __forceinline__ uint32_t q_up(uint32_t q) {
+  const __nv_bfloat162 c = __floats2bfloat162_rn(1152921504606846976.f, 1152921504606846976.f);
+  const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&q), c);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float over_rows_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
+  return fmaxf(v, __shfl_xor_sync(FULL, v, 16));
+}
+__device__ __forceinline__ float over_rows_sum(float v) {
+  v += __shfl_xor_sync(FULL, v, 4);
+  v += __shfl_xor_sync(FULL, v, 8);
+  return v + __shfl_xor_sync(FULL, v, 16);
+}
+
+template <int D, int NW, int STG>
+__global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 a, const Parts8 parts, int* status) {
+  constexpr int PB = 2 * PAGE * D, KT = D / 16, VT = D / 16;             // bytes of a page, MMAs of its keys and of its values
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + NW * STG * PB);
+  uint32_t* const s_exp = reinterpret_cast<uint32_t*>(bars + NW * STG);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int G = a.Hq / a.H, blocks_of_heads = (G + 7) / 8;
+  const int split = blockIdx.x % parts.splits;
+  int rest = blockIdx.x / parts.splits;
+  const int hb = rest % blocks_of_heads;
+  rest /= blocks_of_heads;
+  const int kvh = rest % a.H, seq = rest / a.H;
+  const int heads = min(8, G - 8 * hb), first_head = kvh * G + 8 * hb;
+  uint8_t* const ring = smem + warp * STG * PB;
+  uint64_t* const bar = bars + warp * STG;
+  uint32_t* const my_exp = s_exp + warp * STG;
+  if (lane == 0) {
+    for (int s = 0; s < STG; ++s) mbar_init(bar + s, 1);
+    fence_barrier_init();
+  }
+  const uint64_t stream_policy = policy_evict_first();
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int len = a.lens[seq];
+  int lo = a.starts ? max(a.starts[seq], 0) : 0;
+  if (a.window > 0) lo = max(lo, len - a.window);
+  uint32_t qf[KT][2];
+  {
+    const uint16_t* const qrow = a.q + (size_t)seq * a.q_stride + (size_t)(first_head + (g < heads ? g : 0)) * D;
+#pragma unroll
+    for (int p = 0; p < D / 64; ++p) {
+      const uint4* const at = reinterpret_cast<const uint4*>(qrow + 16 * (t + 4 * p));
+      const uint4 u = at[0], v = at[1];
+      qf[4 * p][0] = u.x; qf[4 * p][1] = u.y; qf[4 * p + 1][0] = u.z; qf[4 * p + 1][1] = u.w;
+      qf[4 * p + 2][0] = v.x; qf[4 * p + 2][1] = v.y; qf[4 * p + 3][0] = v.z; qf[4 * p + 3][1] = v.w;
+    }
+  }
+  const int first_page = lo / PAGE;
+  const int end_page = len > lo ? (int)min((long long)(len - 1) / PAGE + 1, a.table_stride) : 0;
+  const int per_split = max(parts.min_pages, (end_page - first_page + parts.splits - 1) / parts.splits);
+  const int lo_page = first_page + split * per_split, hi_page = min(end_page, lo_page + per_split);
+  const int my_first = lo_page + warp;
+  const int my_count = hi_page > my_first ? (hi_page - my_first + NW - 1) / NW : 0;
+
+  const int* const my_table = a.table + (size_t)seq * a.table_stride + my_first;
+  auto entry = [&](int i) { return i + lane < my_count ? __ldg(my_table + (long long)(i + lane) * NW) : 0; };
+  auto inside = [&](int e) -> long long { return e < 0 ? 0 : (e >= a.nblocks ? a.nblocks - 1 : e); };
+  auto exps_of = [&](int e) -> uint32_t {                         // (both exponents of the page in one load)
+    return __ldg(reinterpret_cast<const uint16_t*>(a.exps) + (size_t)inside(e) * a.H + kvh);
+  };
+  int now = entry(0), next = entry(32);
+  uint32_t now_x = exps_of(now), next_x = 0;
+  auto fetch = [&](int i) {                                       // this warp's i-th page -> stage i % STG (whole warp, i in order)
+    if ((i & 31) == 0 && i > 0) {
+      now = next;
+      now_x = next_x;
+      next = entry(i + 32);
+    }
+    if ((i & 31) == 16) next_x = exps_of(next);
+    const long long blk = inside(__shfl_sync(FULL, now, i & 31));
+    const uint32_t x = __shfl_sync(FULL, now_x, i & 31);
+    const int s = i % STG;
+    if (elect_one()) {
+      my_exp[s] = x;
+      mbar_expect_tx(bar + s, PB);
+      bulk_g2s(ring + s * PB, a.kv + page8_off<D>(blk, a.H, kvh, 0), PB, bar + s, stream_policy);
+    }
+  };
+  __syncwarp();
+  for (int i = 0; i < min(my_count, STG); ++i) fetch(i);
+#pragma unroll
+  for (int k = 0; k < KT; ++k) {                                  // columns beyond the heads are zero
+    qf[k][0] = g < heads ? q_up(qf[k][0]) : 0u;
+    qf[k][1] = g < heads ? q_up(qf[k][1]) : 0u;
+  }
+  const bool head0 = 2 * t < heads, head1 = 2 * t + 1 < heads;
+  float m0 = head0 ? -INFINITY : 0.f, m1 = head1 ? -INFINITY : 0.f, l0 = 0.f, l1 = 0.f;
+  float acc[VT][4];                                               // MMA j: [0], [1] dim D/8 g + 2j, [2], [3] the next; heads 2t, 2t + 1
+#pragma unroll
+  for (int j = 0; j < VT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  bool gave_up = false;
+  __syncwarp();
+
+  for (int i = 0; i < my_count; ++i) {
+    const int s = i % STG, page = my_first + i * NW;
+    if (!mbar_wait(bar + s, (uint32_t)(i / STG) & 1u)) {
+      if (lane == 0) atomicExch(status, ERR_WAIT_FULL);
+      for (int k = i + 1; k < min(my_count, i + STG); ++k)        // let the copies still in flight land
+        (void)mbar_wait(bar + k % STG, (uint32_t)(k / STG) & 1u);
+      gave_up = true;
+      break;
+    }
+    const uint8_t* const pg = ring + s * PB;
+    const uint32_t x = my_exp[s];
+    const int ek = page8_exp((int8_t)(x & 0xFF)), ev = page8_exp((int8_t)(x >> 8));
+    float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < D / 64; ++p) {
+      const uint8_t* const at = pg + g * D + 16 * piece8<D>(g, t + 4 * p);
+      const uint4 u = *reinterpret_cast<const uint4*>(at), v = *reinterpret_cast<const uint4*>(at + 8 * D);
+      const uint32_t wu[4] = {u.x, u.y, u.z, u.w}, wv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t a0, a1, a2, a3;
+        codes_to_bf16(wu[k], a0, a2);
+        codes_to_bf16(wv[k], a1, a3);
+        mma_bf16_r(k & 1 ? sd : sc, a0, a1, a2, a3, qf[4 * p + k][0], qf[4 * p + k][1]);
+      }
+    }
+    const float c = a.scale_log2 * pow2i(60 + ek);
+    const int tok = page * PAGE + g;
+    const bool v_lo = tok >= lo && tok < len, v_hi = tok + 8 >= lo && tok + 8 < len;
+    const float x00 = v_lo && head0 ? (sc[0] + sd[0]) * c : -INFINITY, x01 = v_lo && head1 ? (sc[1] + sd[1]) * c : -INFINITY;
+    const float x10 = v_hi && head0 ? (sc[2] + sd[2]) * c : -INFINITY, x11 = v_hi && head1 ? (sc[3] + sd[3]) * c : -INFINITY;
+    const float top0 = fmaxf(x00, x10), top1 = fmaxf(x01, x11);
+    if (__any_sync(FULL, top0 > m0 + RAISE8 || top1 > m1 + RAISE8)) {
+      const float n0 = fmaxf(m0, over_rows_max(top0)), n1 = fmaxf(m1, over_rows_max(top1));
+      const float f0 = n0 == m0 ? 1.f : exp2f(m0 - n0), f1 = n1 == m1 ? 1.f : exp2f(m1 - n1);
+      l0 *= f0;
+      l1 *= f1;
+#pragma unroll
+      for (int j = 0; j < VT; ++j) { acc[j][0] *= f0; acc[j][1] *= f1; acc[j][2] *= f0; acc[j][3] *= f1; }
+      m0 = n0;
+      m1 = n1;
+    }
+    const float p00 = exp2f(x00 - m0), p01 = exp2f(x01 - m1), p10 = exp2f(x10 - m0), p11 = exp2f(x11 - m1);
+    l0 += p00 + p10;
+    l1 += p01 + p11;
+    const float up = pow2i(60 + ev);
+    const uint32_t b0 = movmatrix_t(pack_bf16(p00 * up, p01 * up)), b1 = movmatrix_t(pack_bf16(p10 * up, p11 * up));
+    const uint8_t* const vp = pg + PAGE * D;
+    constexpr int WORDS = D / 32;                                 // of a lane's dims of one token: D / 8 codes
+    uint32_t w[4][WORDS];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = 2 * t + (k & 1) + 8 * (k >> 1);
+      if (D == 128) {
+        const uint4 u = *reinterpret_cast<const uint4*>(vp + r * D + 16 * piece8<D>(r, g));
+        w[k][0] = u.x; w[k][1] = u.y; w[k][WORDS > 2 ? 2 : 0] = u.z; w[k][WORDS > 2 ? 3 : 0] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(vp + r * D + 8 * g);
+        w[k][0] = u.x; w[k][1] = u.y;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k)
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {                               // dims 4k + 2d, 4k + 2d + 1 of the lane
+        uint32_t a0, a1, a2, a3;
+        codes_to_bf16(__byte_perm(w[0][k], w[1][k], d ? 0x7362 : 0x5140), a0, a1);
+        codes_to_bf16(__byte_perm(w[2][k], w[3][k], d ? 0x7362 : 0x5140), a2, a3);
+        mma_bf16_r(acc[2 * k + d], a0, a1, a2, a3, b0, b1);
+      }
+    __syncwarp();                                                 // every lane has read this stage
+    if (i + STG < my_count) {
+      fence_proxy_async();
+      fetch(i + STG);
+    }
+  }
+  if (gave_up) { m0 = head0 ? -INFINITY : 0.f; m1 = head1 ? -INFINITY : 0.f; l0 = l1 = 0.f; }
+  l0 = over_rows_sum(l0);
+  l1 = over_rows_sum(l1);
+
+  // ---- the CTA's warps together.  The rings are idle now; each warp parks (O^T, m, l) of its heads there.
+  __syncthreads();
+  constexpr int ROW = D + 2, PER_WARP = 8 * ROW;
+  static_assert(PER_WARP * 4 <= STG * PB, "parked partials must fit in the ring");
+  float* const park = reinterpret_cast<float*>(smem);
+  float* const mine = park + warp * PER_WARP;
+#pragma unroll
+  for (int j = 0; j < VT; ++j) {
+    const int d = D / 8 * g + 2 * j;
+    if (head0) *reinterpret_cast<float2*>(mine + 2 * t * ROW + d) = make_float2(acc[j][0], acc[j][2]);
+    if (head1) *reinterpret_cast<float2*>(mine + (2 * t + 1) * ROW + d) = make_float2(acc[j][1], acc[j][3]);
+  }
+  if (g == 0) {
+    if (head0) *reinterpret_cast<float2*>(mine + 2 * t * ROW + D) = make_float2(m0, l0);
+    if (head1) *reinterpret_cast<float2*>(mine + (2 * t + 1) * ROW + D) = make_float2(m1, l1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < heads * D; e += NW * 32) {
+    const int h = e / D, d = e % D;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, park[w * PER_WARP + h * ROW + D]);
+    float den = 0.f, num = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float* const pw = park + w * PER_WARP + h * ROW;
+      if (pw[D] == -INFINITY) continue;                           // a warp without pages
+      const float f = exp2f(pw[D] - top);
+      den += f * pw[D + 1];
+      num += f * pw[d];
+    }
+    num *= 1152921504606846976.f;                                 // 2^60
+    const int hq = first_head + h;
+    if (parts.splits == 1) {
+      const __nv_bfloat16 v = __float2bfloat16_rn(den > 0.f ? num / den : den);        // (a sum that is not a number stays one)
+      a.out[(size_t)seq * a.out_stride + (size_t)hq * D + d] = *reinterpret_cast<const uint16_t*>(&v);
+    } else {
+      const size_t ix = ((size_t)seq * a.Hq + hq) * parts.splits + split;
+      parts.o[ix * D + d] = num;
+      if (d == 0) { parts.ml[ix * 2] = top; parts.ml[ix * 2 + 1] = den; }
+    }
+  }
+}
+
+// Weighs the split partials of a (token, query head) by exp2(m_j - max m) and normalises.  Latency bounds it: WPR warps share a row
+// (four beyond four splits), lane j takes (m, l) of split j, a round's partials are all in flight.  The splits are added in an order
+// of their own, whichever finished first.
+constexpr int MERGE8 = 4;
+template <int D, int WPR>
+__global__ void __launch_bounds__(MERGE8 * 32) kv8_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                                                                const int* __restrict__ cu, int B, uint16_t* __restrict__ out,
+                                                                long long out_stride, int Hq, int splits, long long rows) {
+  constexpr int PL = D / 32;
+  __shared__ float s_num[MERGE8][D];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
+  const long long row = (long long)blockIdx.x * (MERGE8 / WPR) + warp / WPR;
+  if (row >= rows) return;                                        // (WPR = 4: one row per CTA, never beyond)
+  if (cu && (row / Hq < cu[0] || row / Hq >= cu[B])) return;      // rows of no sequence (the whole CTA with WPR = 4)
+  const float* const ml = part_ml + row * splits * 2;
+  const float* const po = part_o + row * splits * D + PL * lane;
+  float top = -INFINITY;
+  for (int j = lane; j < splits; j += 32) top = fmaxf(top, ml[2 * j]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
+  float den = 0.f, num[PL];
+#pragma unroll
+  for (int d = 0; d < PL; ++d) num[d] = 0.f;
+  for (int c = 0; c < splits; c += 32) {
+    float m = -INFINITY, l = 0.f;
+    if (c + lane < splits) { m = ml[2 * (c + lane)]; l = ml[2 * (c + lane) + 1]; }
+    const float f = m == -INFINITY ? 0.f : exp2f(m - top);        // (a split without tokens weighs nothing)
+    den += f * l;
+    constexpr int U = WPR == 1 ? 4 : 8;
+    for (int k0 = 0; k0 < 32 && c + k0 < splits; k0 += U * WPR) {
+      float o[U][PL];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int j = c + k0 + sub + WPR * k;
+#pragma unroll
+        for (int d = 0; d < PL; d += 2) {
+          const float2 v = j < splits ? *reinterpret_cast<const float2*>(po + (size_t)j * D + d) : make_float2(0.f, 0.f);
+          o[k][d] = v.x;
+          o[k][d + 1] = v.y;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const float fj = __shfl_sync(FULL, f, k0 + sub + WPR * k);
+#pragma unroll
+        for (int d = 0; d < PL; ++d) num[d] += fj == 0.f ? 0.f : fj * o[k][d];
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) den += __shfl_xor_sync(FULL, den, o);
+  if (WPR > 1) {
+#pragma unroll
+    for (int d = 0; d < PL; ++d) s_num[warp][PL * lane + d] = num[d];
+    __syncthreads();
+    if (sub != 0) return;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w)
+#pragma unroll
+      for (int d = 0; d < PL; ++d) num[d] += s_num[warp + w][PL * lane + d];
+  }
+  const float inv = den > 0.f ? 1.f / den : den;
+  uint16_t* const at = out + row / Hq * out_stride + row % Hq * D + PL * lane;
+#pragma unroll
+  for (int d = 0; d < PL; d += 2) *reinterpret_cast<uint32_t*>(at + d) = pack_bf16(num[d] * inv, num[d + 1] * inv);
+}
+
+int merge8(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t st_) {
+  const long long rows = a.T * a.Hq;
+  const int per_cta = parts.splits > 4 ? 1 : MERGE8;
+  auto* kernel = D == 128 ? (parts.splits > 4 ? kv8_merge_kernel<128, MERGE8> : kv8_merge_kernel<128, 1>)
+                          : (parts.splits > 4 ? kv8_merge_kernel<64, MERGE8> : kv8_merge_kernel<64, 1>);
+  return st::launch(who, kernel, dim3((unsigned)((rows + per_cta - 1) / per_cta)), dim3(MERGE8 * 32), 0, st_, (const float*)parts.o,
+                    (const float*)parts.ml, a.cu, a.B, a.out, a.out_stride, a.Hq, parts.splits, rows);
+}
+
+template <int D, int NW, int STG>
+int attn8_launch(const Attn8& a, const Parts8& parts, cudaStream_t st_) {
+  constexpr int smem = NW * STG * (2 * PAGE * D + 8 + 4);
+  static std::atomic<uint64_t> set{0};                            // devices whose limit has been raised
+  int dev = 0;
+  if (int e = st::cuda_fail(cudaGetDevice(&dev), "st_kv8_attn: device")) return e;
+  if (dev > 63 || !(set.load() >> dev & 1)) {
+    if (int e = st::cuda_fail(cudaFuncSetAttribute(kv8_attn_kernel<D, NW, STG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                              "st_kv8_attn: shared memory attribute"))
+      return e;
+    if (dev <= 63) set.fetch_or(1ull << dev);
+  }
+  const long long ctas = (long long)a.B * a.H * ((a.Hq / a.H + 7) / 8) * parts.splits;
+  return st::launch("st_kv8_attn launch", kv8_attn_kernel<D, NW, STG>, dim3((unsigned)ctas), dim3(NW * 32), (size_t)smem, st_, a, parts,
+                    st::status_ptr());
+}
 }  // namespace
 
 extern "C" int64_t st_kv8_page_bytes(int64_t H, int64_t D) { return H * 2 * st::PAGE * D; }
@@ -465,6 +809,7 @@ int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, 
   ST_REQUIRE(nblocks > 0 && bts > 0, "%s: empty cache or block table", who);
   ST_REQUIRE(st::aligned16(q) && st::aligned16(out) && st::aligned16(kv) && qs % 8 == 0 && os % 8 == 0 && qs >= 0 && os >= 0,
              "%s: q, out and the pages must be 16-byte aligned, token strides multiples of 8", who);
+  ST_REQUIRE(((uintptr_t)exps & 1u) == 0, "%s: exponents must be 2-byte aligned", who);
   ST_REQUIRE(T * Hq < (1ll << 31) && bts < (1ll << 27), "%s: too large", who);
   a.q = (const uint16_t*)q; a.q_stride = qs; a.cu = cu; a.kv = (const uint8_t*)kv; a.exps = exps; a.nblocks = nblocks;
   a.table = bt; a.table_stride = bts; a.lens = lens; a.starts = starts; a.out = (uint16_t*)out; a.out_stride = os;
@@ -484,8 +829,17 @@ extern "C" int st_kv8_attn(const void* q, int64_t qs, int64_t B, int64_t Hq, con
   ST_REQUIRE(S >= 1 && S <= 1024, "st_kv8_attn: splits must be in [1, 1024]");
   ST_REQUIRE(S == 1 || (wo && wml && st::aligned16(wo)), "st_kv8_attn: split workspace (wo, wml) missing or unaligned");
   if (B == 0) return 0;
-  return st::launch("st_kv8_attn launch", D == 128 ? kv8_rows_kernel<128> : kv8_rows_kernel<64>, dim3((unsigned)((B * Hq + 7) / 8)), dim3(256),
-                    0, (cudaStream_t)stream, a);
+  ST_REQUIRE(st::status_ptr() != nullptr, "st_kv8_attn: no device status word");
+  const long long ctas = B * Hkv * ((Hq / Hkv + 7) / 8) * S;
+  ST_REQUIRE(ctas < (1ll << 31), "st_kv8_attn: grid too large");
+  const Parts8 parts = {wo, wml, (int)S, (int)(minpps < 1 ? 1 : minpps)};
+  const cudaStream_t st_ = (cudaStream_t)stream;
+  // An SM holds sixteen warps: four CTAs of four, or two of eight for a grid of at most two CTAs per SM
+  const bool wide = ctas <= 2ll * st::sm_count();
+  const int e = D == 128 ? (wide ? attn8_launch<128, 8, 3>(a, parts, st_) : attn8_launch<128, 4, 3>(a, parts, st_))
+                         : (wide ? attn8_launch<64, 8, 5>(a, parts, st_) : attn8_launch<64, 4, 5>(a, parts, st_));
+  if (e || S == 1) return e;
+  return merge8("st_kv8_attn merge launch", a, parts, (int)D, st_);
 }
 
 extern "C" int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
