@@ -321,80 +321,6 @@ __global__ void __launch_bounds__(256) kv8_dequant_kernel(const uint8_t* __restr
   out[1] = o[1];
 }
 
-// ------------------------------------------------------------------------------------------------ attention, plain
-// One warp per (query token, head); keys one after the other, the running maximum and sum of the softmax in fp32.
-struct Attn8 {
-  const uint16_t* q; long long q_stride;
-  const int* cu;                                   // first query of each sequence [B + 1]; nullptr: one query each
-  const uint8_t* kv; const int8_t* exps; long long nblocks;
-  const int* table; long long table_stride;
-  const int* lens; const int* starts;
-  uint16_t* out; long long out_stride;
-  float scale_log2;
-  int B, Hq, H, window;
-  long long T;
-};
-template <int D>
-__global__ void __launch_bounds__(256) kv8_rows_kernel(const Attn8 a) {
-  pdl_wait();
-  pdl_launch_dependents();
-  constexpr int PL = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const long long t = w / a.Hq;
-  if (t >= a.T) return;
-  const int hq = (int)(w % a.Hq), h = hq / (a.Hq / a.H);
-  int b = (int)t, n = 1, i = 0;
-  if (a.cu) {
-    for (b = 0; b < a.B && a.cu[b + 1] <= t; ++b) {}
-    if (b >= a.B || t < a.cu[b]) return;
-    n = a.cu[b + 1] - a.cu[b];
-    i = (int)t - a.cu[b];
-  }
-  const int pos = a.lens[b] - n + i, end = (int)min((long long)pos, a.table_stride * PAGE - 1);
-  int lo = a.starts ? max(a.starts[b], 0) : 0;
-  if (a.window > 0) lo = max(lo, pos - a.window + 1);
-  float q[PL], o[PL], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int k = 0; k < PL; ++k) {
-    q[k] = __uint_as_float((uint32_t)a.q[t * a.q_stride + (size_t)hq * D + PL * lane + k] << 16);
-    o[k] = 0.f;
-  }
-  for (int j = lo; j <= end; ++j) {
-    long long blk = a.table[b * a.table_stride + j / PAGE];
-    blk = blk < 0 ? 0 : (blk >= a.nblocks ? a.nblocks - 1 : blk);
-    const int r = j % PAGE, at = r * D + 16 * piece8<D>(r, PL * lane >> 4) + (PL * lane & 15);
-    float k[PL], v[PL];
-#pragma unroll
-    for (int kvi = 0; kvi < 2; ++kvi) {
-      const float up = pow2i(20 + page8_exp(a.exps[((size_t)blk * a.H + h) * 2 + kvi]));
-      const uint8_t* p = a.kv + page8_off<D>(blk, a.H, h, kvi) + at;
-#pragma unroll
-      for (int d = 0; d < PL; d += 2) {
-        uint32_t p01, p23;
-        codes_to_bf16((uint32_t)p[d] | (uint32_t)p[d + 1] << 8, p01, p23);
-        const float2 x = codes_value(p01, up);
-        (kvi ? v : k)[d] = x.x;
-        (kvi ? v : k)[d + 1] = x.y;
-      }
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int d = 0; d < PL; ++d) s = fmaf(q[d], k[d], s);
-#pragma unroll
-    for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(FULL, s, off);
-    s *= a.scale_log2;
-    const float top = fmaxf(m, s), f = exp2f(m - top), p = exp2f(s - top);
-    l = l * f + p;
-#pragma unroll
-    for (int d = 0; d < PL; ++d) o[d] = o[d] * f + p * v[d];
-    m = top;
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-  for (int d = 0; d < PL; d += 2)
-    *reinterpret_cast<uint32_t*>(a.out + t * a.out_stride + (size_t)hq * D + PL * lane + d) = pack_bf16(o[d] * inv, o[d + 1] * inv);
-}
 // ------------------------------------------------------------------------------------------------ attention, one token per sequence
 // Orientation.  A decode step has few query heads per KV head, so the heads of a group go on the 8-wide N side of mma.m16n8k16 and
 // tokens / dims on the 16-wide M side (groups of more than eight take a CTA per eight heads):
@@ -415,14 +341,6 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(const Attn8 a) {
 // Block-table entries and exponents come 32 pages at a time, one batch ahead.
 constexpr float RAISE8 = 8.f;
 
-struct Parts8 { float* o; float* ml; int splits, min_pages; };
-
-// q times 2^60, exactly (BF16 keeps its eight bits)
-__device__ __forceinline__ uint32_t q_up(uint32_t q) {
-  const __nv_bfloat162 c = __floats2bfloat162_rn(1152921504606846976.f, 1152921504606846976.f);
-  const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&q), c);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
 __device__ __forceinline__ float over_rows_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
@@ -712,15 +630,6 @@ __global__ void __launch_bounds__(MERGE8 * 32) kv8_merge_kernel(const float* __r
   for (int d = 0; d < PL; d += 2) *reinterpret_cast<uint32_t*>(at + d) = pack_bf16(num[d] * inv, num[d + 1] * inv);
 }
 
-int merge8(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t st_) {
-  const long long rows = a.T * a.Hq;
-  const int per_cta = parts.splits > 4 ? 1 : MERGE8;
-  auto* kernel = D == 128 ? (parts.splits > 4 ? kv8_merge_kernel<128, MERGE8> : kv8_merge_kernel<128, 1>)
-                          : (parts.splits > 4 ? kv8_merge_kernel<64, MERGE8> : kv8_merge_kernel<64, 1>);
-  return st::launch(who, kernel, dim3((unsigned)((rows + per_cta - 1) / per_cta)), dim3(MERGE8 * 32), 0, st_, (const float*)parts.o,
-                    (const float*)parts.ml, a.cu, a.B, a.out, a.out_stride, a.Hq, parts.splits, rows);
-}
-
 template <int D, int NW, int STG>
 int attn8_launch(const Attn8& a, const Parts8& parts, cudaStream_t st_) {
   constexpr int smem = NW * STG * (2 * PAGE * D + 8 + 4);
@@ -738,6 +647,17 @@ int attn8_launch(const Attn8& a, const Parts8& parts, cudaStream_t st_) {
                     st::status_ptr());
 }
 }  // namespace
+
+namespace st {
+int merge8(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t st_) {
+  const long long rows = a.T * a.Hq;
+  const int per_cta = parts.splits > 4 ? 1 : MERGE8;
+  auto* kernel = D == 128 ? (parts.splits > 4 ? kv8_merge_kernel<128, MERGE8> : kv8_merge_kernel<128, 1>)
+                          : (parts.splits > 4 ? kv8_merge_kernel<64, MERGE8> : kv8_merge_kernel<64, 1>);
+  return st::launch(who, kernel, dim3((unsigned)((rows + per_cta - 1) / per_cta)), dim3(MERGE8 * 32), 0, st_, (const float*)parts.o,
+                    (const float*)parts.ml, a.cu, a.B, a.out, a.out_stride, a.Hq, parts.splits, rows);
+}
+}  // namespace st
 
 extern "C" int64_t st_kv8_page_bytes(int64_t H, int64_t D) { return H * 2 * st::PAGE * D; }
 
@@ -795,7 +715,7 @@ extern "C" int st_kv8_dequant_blocks(const void* kv, const int8_t* exps, int64_t
                     (const uint8_t*)kv, exps, (long long)nblocks, (int)H, (const int*)blocks, (long long)n, (uint16_t*)Kd, (uint16_t*)Vd);
 }
 
-namespace {
+namespace st {
 // what both forms of the attention check and pass on
 int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
                const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens,
@@ -817,7 +737,7 @@ int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, 
   a.B = (int)B; a.Hq = (int)Hq; a.H = (int)Hkv; a.window = (int)window; a.T = T;
   return 0;
 }
-}  // namespace
+}  // namespace st
 
 extern "C" int st_kv8_attn(const void* q, int64_t qs, int64_t B, int64_t Hq, const void* kv, const int8_t* exps, int64_t nblocks,
                            int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens, const int32_t* starts,
@@ -840,19 +760,4 @@ extern "C" int st_kv8_attn(const void* q, int64_t qs, int64_t B, int64_t Hq, con
                          : (wide ? attn8_launch<64, 8, 5>(a, parts, st_) : attn8_launch<64, 4, 5>(a, parts, st_));
   if (e || S == 1) return e;
   return merge8("st_kv8_attn merge launch", a, parts, (int)D, st_);
-}
-
-extern "C" int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
-                                 const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts,
-                                 const int32_t* lens, const int32_t* starts, int64_t window, void* out, int64_t os, float* wo,
-                                 float* wml, double scale, int64_t S, void* stream) {
-  Attn8 a;
-  if (int e = attn8_args(a, "st_kv8_chunk_attn", q, qs, T, Hq, cu, B, kv, exps, nblocks, Hkv, D, bt, bts, lens, starts, window, out, os, scale))
-    return e;
-  ST_REQUIRE(S >= 1 && S <= 1024, "st_kv8_chunk_attn: splits must be in [1, 1024]");
-  ST_REQUIRE(S == 1 || (wo && wml && st::aligned16(wo)), "st_kv8_chunk_attn: split workspace (wo, wml) missing or unaligned");
-  if (T == 0 || B == 0) return 0;
-  ST_REQUIRE(cu || T == B, "st_kv8_chunk_attn: without cu every sequence has one query");
-  return st::launch("st_kv8_chunk_attn launch", D == 128 ? kv8_rows_kernel<128> : kv8_rows_kernel<64>, dim3((unsigned)((T * Hq + 7) / 8)),
-                    dim3(256), 0, (cudaStream_t)stream, a);
 }

@@ -13,7 +13,6 @@
 
 namespace st {
 constexpr int E8_MIN = -64, E8_MAX = 56;
-constexpr int MAX_D8 = 128;
 
 template <int D>
 __device__ __forceinline__ int piece8(int row, int c) {
@@ -46,4 +45,31 @@ __device__ __forceinline__ float2 codes_value(uint32_t p, float up) {      // up
   constexpr float C = 1.2676506002282294e30f;                             // 2^100
   return make_float2(__uint_as_float(p << 16) * C * up, __uint_as_float(p & 0xFFFF0000u) * C * up);
 }
+// q times 2^60, exactly (BF16 keeps its eight bits)
+__device__ __forceinline__ uint32_t q_up(uint32_t q) {
+  const __nv_bfloat162 c = __floats2bfloat162_rn(1152921504606846976.f, 1152921504606846976.f);
+  const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&q), c);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// ---- the attention's arguments
+struct Attn8 {
+  const uint16_t* q; long long q_stride;
+  const int* cu;                                   // first query of each sequence [B + 1]; nullptr: one query each
+  const uint8_t* kv; const int8_t* exps; long long nblocks;
+  const int* table; long long table_stride;
+  const int* lens; const int* starts;
+  uint16_t* out; long long out_stride;
+  float scale_log2;
+  int B, Hq, H, window;
+  long long T;
+};
+// partial results of sequences that are split: o [T, Hq, splits, D] (not normalised), ml [T, Hq, splits, 2] = (maximum, base 2; sum)
+struct Parts8 { float* o; float* ml; int splits, min_pages; };
+
+// st_kv8.cu: what both forms of the attention check and pass on; the join of the partial results
+int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
+               const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens,
+               const int32_t* starts, int64_t window, void* out, int64_t os, double scale);
+int merge8(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t stream);
 }  // namespace st

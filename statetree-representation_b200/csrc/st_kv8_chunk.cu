@@ -1,0 +1,548 @@
+// Causal attention of several query tokens per sequence over 8-bit KV pages, on the tensor cores (tcgen05).
+//
+// A row is a (query token, head) pair of one KV head's group, so a CTA's 256 rows (two accumulator tiles of 128) are 256 / G
+// consecutive tokens of one sequence, whatever G is; keys come 128 at a time (eight pages):
+//     S = Q K^T   128 x 128, A and B from shared memory            P = exp2(S * c - m) in BF16, back into S's tensor-memory columns
+//     O += P V    128 x D, A = P from tensor memory, B = V from shared memory as it lies (dims contiguous: MN-major)
+// Warps: eight of softmax (a thread owns one row, so its maximum and sum need no other thread), four that turn codes into BF16 operand
+// tiles, one that issues the MMAs.  While one tile's softmax runs, the tensor core works on the other's: S0 P0 S1 P1 ... in turn.
+// Tensor memory: S0, S1 (128 columns each; P takes the first 64 of its own), O0, O1 (D each).
+//
+// Codes reach the tensor core without a multiplication: BF16 patterns times 2^-120 (codes_split), q times 2^60, a page's key exponent in
+// the factor of its sixteen score columns, its value exponent (and 60) in the exponent of its sixteen columns of P.  The sum of the
+// probabilities takes the latter out again, per page.  All values are exact BF16 numbers, so the only roundings to fewer than 32 bits
+// are P (to BF16, 2^-9 of each probability at most) and the output.
+#include <math.h>
+
+#include <atomic>
+
+#include "../../include/statetree_b200.h"
+#include "st_host.h"
+#include "st_kv8.cuh"
+#include "st_tc.cuh"
+
+namespace {
+using namespace st;
+
+constexpr int KEYS = 128, TILE_PAGES = KEYS / PAGE, ROWS = 128;
+constexpr int W_CONV = 8, W_MMA = 12, WARPS = 13;                 // softmax warps 0 .. 7 (tile = warp / 4)
+constexpr int CRING = 4;                                          // page factors of so many key tiles are kept
+constexpr float LAZY = 8.f;                                       // a row's reference maximum is raised when a score exceeds it by this
+
+template <int D>
+struct Lay {                                                      // shared memory
+  static constexpr int HALF = 128 * 128;                          // 128 rows x 64 BF16, 128-byte swizzle
+  static constexpr int TILE = D / 64 * HALF;
+  static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, F = 6 * TILE;      // two tiles of Q, two stages of K and V
+  static constexpr int BARS = F + CRING * TILE_PAGES * 3 * 4;
+  static constexpr int NBARS = 17, SLOT = BARS + NBARS * 8;
+  // (more than half of an SM's shared memory: one CTA per SM, which holds all of its tensor memory)
+  static constexpr int BYTES = (SLOT + 16 > 120 * 1024 ? SLOT + 16 : 120 * 1024) + 1024;
+};
+
+struct Chunk8 { Attn8 a; Parts8 parts; int* status; int slots; };
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+               :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// operand whose rows (k) hold 64 contiguous values of the other dimension, 128-byte swizzle: 8-row groups 1024 B apart, the next 64
+// values `next` bytes further
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t next) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+#define ST_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
+#define ST_I4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&v)[32]) {      // (complete after tm_wait_ld)
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+               "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : ST_R4(v, 0), ST_R4(v, 4), ST_R4(v, 8), ST_R4(v, 12), ST_R4(v, 16), ST_R4(v, 20), ST_R4(v, 24), ST_R4(v, 28)
+               : "r"(addr));
+}
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&v)[32]) {                  // (v's readers stay behind the wait)
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]),
+                 "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]),
+                 "+r"(v[27]), "+r"(v[28]), "+r"(v[29])
+               :: "memory");
+  asm volatile("" : "+r"(v[30]), "+r"(v[31]) :: "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&v)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+               "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+               :: "r"(addr), ST_I4(v, 0), ST_I4(v, 4), ST_I4(v, 8), ST_I4(v, 12), ST_I4(v, 16), ST_I4(v, 20), ST_I4(v, 24), ST_I4(v, 28)
+               : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               :: "r"(addr), ST_I4(v, 0), ST_I4(v, 4), ST_I4(v, 8), ST_I4(v, 12) : "memory");
+}
+#undef ST_R4
+#undef ST_I4
+__device__ __forceinline__ float ex2(float x) {                   // 2^x, relative error below 2^-22, results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What a CTA works on; the same in all of its threads
+struct Work {
+  int b, h, split, row0, rows;                                    // rows row0 .. of the sequence's n * G
+  int first, n, pos0;                                             // first query row in q, queries, position of query 0
+  int lo0, first_tile, tiles, count0, count1;                           // key tiles of the split; of those, how many each row tile needs
+};
+
+// the sequence and 256-row tile of `slot`: sequences' tiles one after the other
+__device__ __forceinline__ bool find_work(const Chunk8& c, int G, int slot, int lane, Work& w) {
+  const Attn8& a = c.a;
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int b = b0 + lane;
+    int lo = 0, n = 0;
+    if (b < a.B) {
+      lo = a.cu ? a.cu[b] : b;
+      n = a.cu ? a.cu[b + 1] - lo : 1;
+      if (lo < 0 || n < 0 || lo + (long long)n > a.T) n = 0;      // (not inside q: no work)
+    }
+    const int mine = (int)(((long long)n * G + 2 * ROWS - 1) / (2 * ROWS));
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(FULL, sum, o);
+      if (lane >= o) sum += v;
+    }
+    const int begin = before + sum - mine;
+    const unsigned hit = __ballot_sync(FULL, slot >= begin && slot < begin + mine);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      w.b = b0 + src;
+      w.first = __shfl_sync(FULL, lo, src);
+      w.n = __shfl_sync(FULL, n, src);
+      w.row0 = (slot - __shfl_sync(FULL, begin, src)) * (2 * ROWS);
+      w.rows = min(2 * ROWS, w.n * G - w.row0);
+      return true;
+    }
+    before += __shfl_sync(FULL, sum, 31);
+  }
+  return false;
+}
+
+template <int D>
+__global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c) {
+  using L = Lay<D>;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint64_t *const qfull = bars, *const kfull = bars + 2, *const kempty = bars + 4, *const vfull = bars + 6, *const vempty = bars + 8,
+           *const sfull = bars + 10, *const pfull = bars + 12, *const ofull = bars + 14, *const drain = bars + 16;
+  uint32_t* const slot_at = reinterpret_cast<uint32_t*>(smem + L::SLOT);
+  const Attn8& a = c.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.Hq / a.H;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- what this CTA works on.  Later tiles of a sequence see more keys: they go first
+  Work w;
+  {
+    int x = blockIdx.x;
+    w.split = x % c.parts.splits;
+    x /= c.parts.splits;
+    w.h = x % a.H;
+    if (!find_work(c, G, c.slots - 1 - x / a.H, lane, w)) return;
+    const int len = a.lens[w.b], start = a.starts ? max(a.starts[w.b], 0) : 0;
+    w.pos0 = len - w.n;
+    const int first_pos = w.pos0 + w.row0 / G, last_pos = w.pos0 + (w.row0 + w.rows - 1) / G;
+    w.lo0 = start;
+    const int lo = a.window > 0 ? max(start, first_pos - a.window + 1) : start;
+    const int end = (int)min((long long)last_pos + 1, a.table_stride * PAGE);            // keys [lo, end)
+    const int t0 = lo / KEYS, t1 = end > lo ? (end - 1) / KEYS + 1 : t0;
+    const int per = (t1 - t0 + c.parts.splits - 1) / c.parts.splits;
+    w.first_tile = t0 + w.split * per;
+    w.tiles = max(0, min(t1, w.first_tile + per) - w.first_tile);
+    const int mid_pos = w.pos0 + (w.row0 + min(w.rows, ROWS) - 1) / G;                   // last position of the first row tile
+    w.count0 = mid_pos < 0 ? 0 : max(0, min(w.tiles, mid_pos / KEYS + 1 - w.first_tile));
+    w.count1 = w.rows > ROWS ? w.tiles : 0;
+  }
+  const int tiles = max(w.count0, w.count1);
+
+  if (warp == W_MMA) {
+    if (elect_one()) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(qfull + i, 4);
+        mbar_init(kfull + i, 4);
+        mbar_init(kempty + i, 1);
+        mbar_init(vfull + i, 4);
+        mbar_init(vempty + i, 1);
+        mbar_init(sfull + i, 1);
+        mbar_init(pfull + i, 4);
+        mbar_init(ofull + i, 1);
+      }
+      mbar_init(drain, 1);
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc<1>(slot_at, 512);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot_at;
+
+  if (warp < W_CONV) {
+    // ---------------------------------------------------------------- softmax: this thread's row
+    const int t = warp >> 2, my = w.row0 + t * ROWS + (warp & 3) * 32 + lane, count = t ? w.count1 : w.count0;
+    const bool live = my < w.row0 + w.rows;
+    const int token = live ? my / G : 0, head = live ? my % G : 0, hq = w.h * G + head;
+    const int pos = w.pos0 + token;
+    const int hi = live ? pos : -1, lo = a.window > 0 ? max(w.lo0, pos - a.window + 1) : w.lo0;
+    const bool any = __any_sync(FULL, live);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * D;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    if (count > 0) {
+      uint8_t* const row = smem + L::Q + t * L::TILE + ((warp & 3) * 32 + lane) * 128;
+      const uint4* const src = reinterpret_cast<const uint4*>(a.q + (long long)(w.first + token) * a.q_stride + (size_t)hq * D);
+#pragma unroll
+      for (int u = 0; u < D / 8; ++u) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (live) {
+          v = src[u];
+          v.x = q_up(v.x); v.y = q_up(v.y); v.z = q_up(v.z); v.w = q_up(v.w);
+        }
+        *reinterpret_cast<uint4*>(row + (u >> 3) * L::HALF + (((u & 7) ^ (lane & 7)) << 4)) = v;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(qfull + t);
+    }
+    for (int j = 0; j < count; ++j) {
+      if (!mbar_wait(sfull + t, (uint32_t)j & 1u)) { ok = false; break; }
+      tc_fence_after();
+      if (any) {
+        const float* const fac = reinterpret_cast<const float*>(smem + L::F) + (j % CRING) * (TILE_PAGES * 3);
+        const int k0 = (w.first_tile + j) * KEYS, l0 = lo - k0, l1 = hi - k0;                // this row sees columns l0 .. l1
+        const bool masked = __any_sync(FULL, l0 > 0 || l1 < KEYS - 1);
+        // ---- the row's maximum
+        float top = -INFINITY;
+        uint32_t v[2][32];
+        tm_ld32(ts, v[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          tm_wait_ld(v[q & 1]);
+          if (q < 3) tm_ld32(ts + 32 * (q + 1), v[(q + 1) & 1]);
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            float x[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const int col = 32 * q + 16 * p + k;
+              x[k] = __uint_as_float(v[q & 1][16 * p + k]);
+              if (masked) x[k] = col < l0 || col > l1 ? -INFINITY : x[k];
+            }
+#pragma unroll
+            for (int o = 8; o; o >>= 1)
+#pragma unroll
+              for (int k = 0; k < o; ++k) x[k] = fmaxf(x[k], x[k + o]);
+            top = fmaxf(top, x[0] * fac[2 * q + p]);
+          }
+        }
+        if (__any_sync(FULL, top > m + LAZY)) {
+          const float up = fmaxf(m, top), f = up == m ? 1.f : ex2(m - up);
+          m = up;
+          l *= f;
+          if (j > 0) {                                            // (O's product of the tile before has completed: sfull says so)
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+              tm_ld32(to + 32 * q, v[0]);
+              tm_wait_ld(v[0]);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[0][k] = __float_as_uint(__uint_as_float(v[0][k]) * f);
+              tm_st32(to + 32 * q, v[0]);
+            }
+          }
+        }
+        // ---- P, and the sum
+        const float ref = m == -INFINITY ? 0.f : m;
+        tm_ld32(ts, v[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          tm_wait_ld(v[q & 1]);
+          if (q < 3) tm_ld32(ts + 32 * (q + 1), v[(q + 1) & 1]);
+          uint32_t pk[16];
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const float by = fac[2 * q + p], add = fac[TILE_PAGES + 2 * q + p] - ref;
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+              const int col = 32 * q + 16 * p + k;
+              float x0 = __uint_as_float(v[q & 1][16 * p + k]), x1 = __uint_as_float(v[q & 1][16 * p + k + 1]);
+              x0 = fmaf(x0, by, add);
+              x1 = fmaf(x1, by, add);
+              if (masked) {
+                x0 = col < l0 || col > l1 ? -INFINITY : x0;
+                x1 = col + 1 < l0 || col + 1 > l1 ? -INFINITY : x1;
+              }
+              x0 = ex2(x0);
+              x1 = ex2(x1);
+              sum[0] += x0;
+              sum[1] += x1;
+              pk[8 * p + k / 2] = pack_bf16(x0, x1);
+            }
+            l = fmaf(sum[0] + sum[1], fac[2 * TILE_PAGES + 2 * q + p], l);
+          }
+          tm_st16(ts + 16 * q, pk);
+        }
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfull + t);
+    }
+    if (ok && count > 0) ok = mbar_wait(ofull + t, 0);
+    if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_ACC);
+    // ---- out.  (a wait that ran out leaves the rows unwritten)
+    if (ok && any) {
+      tc_fence_after();
+      const long long r = (long long)(w.first + token) * a.Hq + hq;
+      const float inv = c.parts.splits > 1 ? 1152921504606846976.f : (l > 0.f ? 1152921504606846976.f / l : l);
+      if (live && c.parts.splits > 1) {
+        float* const ml = c.parts.ml + (r * c.parts.splits + w.split) * 2;
+        ml[0] = l > 0.f || l != l ? m : -INFINITY;
+        ml[1] = l;
+      }
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t v[32];
+        if (count > 0) {
+          tm_ld32(to + 32 * q, v);
+          tm_wait_ld(v);
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
+        if (live && c.parts.splits > 1) {
+          uint4* const o = reinterpret_cast<uint4*>(c.parts.o + (r * c.parts.splits + w.split) * D + 32 * q);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+        } else if (live) {
+          uint4* const o = reinterpret_cast<uint4*>(a.out + (long long)(w.first + token) * a.out_stride + (size_t)hq * D + 32 * q);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = pack_bf16(__uint_as_float(v[8 * k + 2 * i]), __uint_as_float(v[8 * k + 2 * i + 1]));
+            o[k] = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    tc_fence_before();
+  } else if (warp < W_MMA) {
+    // ---------------------------------------------------------------- converters: codes -> operand tiles.  A lane's 16-byte piece
+    // becomes two of a tile row; eight lanes store four pieces of an even row and four of the next, so that with the swizzle they
+    // meet every bank once, and a warp reads whole rows
+    constexpr int LOADS = KEYS * D / 16 / 128, PAGES_A_LOAD = TILE_PAGES / LOADS;
+    const int cw = warp - W_CONV;
+    const int r = D == 128 ? cw * 4 + 2 * (lane >> 4) + ((lane >> 2) & 1) : (cw & 1) * 8 + (lane >> 2);
+    const int lc = D == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
+    const int sub = D == 128 ? 0 : cw >> 1;                       // page of the load
+    const uint32_t from = (uint32_t)(r * D + 16 * piece8<D>(r, lc));
+    const uint32_t to = (uint32_t)((lc >> 2) * L::HALF + r * 128), u0 = (uint32_t)((((lc & 3) * 2) ^ (r & 7)) << 4);
+    const int* const table = a.table + (long long)w.b * a.table_stride;
+    // (pages behind the last key of the tile's rows may not exist: no key of theirs is seen)
+    const int end_page = (int)min((long long)(w.pos0 + w.n - 1) / PAGE + 1, a.table_stride);
+    auto page_of = [&](int j) {                                   // lane p < 8: page p of key tile j, -1 = none
+      const int p = (w.first_tile + j) * TILE_PAGES + lane;
+      int e = -1;
+      if (lane < TILE_PAGES && j < tiles && p < end_page) {
+        e = __ldg(table + p);
+        e = e < 0 ? 0 : (e >= a.nblocks ? (int)a.nblocks - 1 : e);
+      }
+      return e;
+    };
+    auto load = [&](int pages, int kvi, uint4 (&buf)[LOADS]) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = __shfl_sync(FULL, pages, i * PAGES_A_LOAD + sub);
+        buf[i] = make_uint4(0, 0, 0, 0);
+        if (e >= 0) buf[i] = __ldg(reinterpret_cast<const uint4*>(a.kv + page8_off<D>(e, a.H, w.h, kvi) + from));
+      }
+    };
+    auto convert = [&](const uint4 (&buf)[LOADS], uint8_t* tile) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        uint32_t o[8];
+        codes_to_bf16(buf[i].x, o[0], o[1]);
+        codes_to_bf16(buf[i].y, o[2], o[3]);
+        codes_to_bf16(buf[i].z, o[4], o[5]);
+        codes_to_bf16(buf[i].w, o[6], o[7]);
+        uint8_t* const at = tile + to + (i * PAGES_A_LOAD + sub) * (PAGE * 128);
+        *reinterpret_cast<uint4*>(at + u0) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(at + (u0 ^ 16)) = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+    };
+    auto exps_of = [&](int e) -> uint32_t {
+      return e >= 0 ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(a.exps) + (size_t)e * a.H + w.h) : 0u;
+    };
+    uint4 kb[LOADS], vb[LOADS];
+    int pages = page_of(0), after = page_of(1);
+    uint32_t x = cw == 0 ? exps_of(pages) : 0u;
+    load(pages, 0, kb);
+    load(pages, 1, vb);
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      const int s = j & 1;
+      if (j > 1) ok = mbar_wait(kempty + s, (uint32_t)((j >> 1) - 1) & 1u);
+      if (!ok) break;
+      convert(kb, smem + L::K + s * L::TILE);
+      if (cw == 0 && lane < TILE_PAGES) {                         // factors of the tile's pages
+        float* const fac = reinterpret_cast<float*>(smem + L::F) + (j % CRING) * (TILE_PAGES * 3) + lane;
+        const int ek = page8_exp((int8_t)(x & 0xFF)), ev = page8_exp((int8_t)(x >> 8));
+        fac[0] = a.scale_log2 * pow2i(60 + ek);
+        fac[TILE_PAGES] = (float)(60 + ev);
+        fac[2 * TILE_PAGES] = pow2i(-60 - ev);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kfull + s);
+      pages = after;
+      load(pages, 0, kb);
+      if (cw == 0) x = exps_of(pages);
+      after = page_of(j + 2);
+      if (j > 1) ok = mbar_wait(vempty + s, (uint32_t)((j >> 1) - 1) & 1u);
+      if (!ok) break;
+      convert(vb, smem + L::V + s * L::TILE);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(vfull + s);
+      load(pages, 1, vb);
+    }
+    if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_EMPTY);
+  } else {
+    // ---------------------------------------------------------------- MMAs.  One thread's MMAs complete in the order of their issue
+    // (and a commit covers all before it): S of the next key tile may take the place of the P that the product before it reads
+    constexpr uint32_t IDESC_S = mma_idesc(128, KEYS), IDESC_O = mma_idesc(128, D) | 1u << 16;
+    const uint32_t sq = smem_addr(smem + L::Q), sk = smem_addr(smem + L::K), sv = smem_addr(smem + L::V);
+    auto scores = [&](int t, int s) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t at = (uint32_t)((k >> 2) * L::HALF);
+        mma_ss(tmem + t * 128, smem_desc_sw128(sq + t * L::TILE + at) + 2 * (k & 3), smem_desc_sw128(sk + s * L::TILE + at) + 2 * (k & 3),
+               IDESC_S, k > 0);
+      }
+    };
+    auto outputs = [&](int t, int s, bool more) {
+#pragma unroll
+      for (int k = 0; k < KEYS / 16; ++k)
+        tc_mma<1>(tmem + 256 + t * D, tmem + t * 128 + 8 * k, desc_mn(sv + s * L::TILE + k * 2048, L::HALF), IDESC_O, more || k > 0);
+    };
+    bool ok = true;
+    if (tiles > 0) {
+      ok = mbar_wait(kfull, 0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (ok && (t ? w.count1 : w.count0) > 0) {
+          ok = mbar_wait(qfull + t, 0);
+          tc_fence_after();
+          if (ok && elect_one()) {
+            scores(t, 0);
+            tc_commit(sfull + t);
+          }
+          __syncwarp();
+        }
+      if (elect_one()) tc_commit(kempty);
+      __syncwarp();
+    }
+    for (int j = 0; ok && j < tiles; ++j) {
+      const int s = j & 1, s1 = s ^ 1;
+      const bool both = j < w.count0 && j < w.count1;
+      ok = mbar_wait(vfull + s, (uint32_t)(j >> 1) & 1u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int count = t ? w.count1 : w.count0;
+        if (!ok || j >= count) continue;
+        const bool next = j + 1 < count;
+        ok = mbar_wait(pfull + t, (uint32_t)j & 1u);
+        tc_fence_after();
+        if (ok && elect_one()) {
+          outputs(t, s, j > 0);
+          if (t == 1 || !both) tc_commit(vempty + s);
+          if (!next) tc_commit(ofull + t);
+        }
+        __syncwarp();
+        if (ok && next) {
+          ok = mbar_wait(kfull + s1, (uint32_t)((j + 1) >> 1) & 1u);
+          tc_fence_after();
+          if (ok && elect_one()) {
+            scores(t, s1);
+            tc_commit(sfull + t);
+          }
+          __syncwarp();
+        }
+      }
+      if (ok && j + 1 < tiles) {
+        if (elect_one()) tc_commit(kempty + s1);
+        __syncwarp();
+      }
+    }
+    if (!ok) {                                                    // (gave up: let what was issued complete before the memory goes)
+      if (lane == 0) atomicExch(c.status, ERR_WAIT_MMA);
+      if (elect_one()) tc_commit(drain);
+      __syncwarp();
+      (void)mbar_wait(drain, 0);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == W_MMA) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, 512);
+  }
+}
+
+template <int D>
+int chunk_launch(const Chunk8& c, cudaStream_t st_) {
+  static std::atomic<uint64_t> set{0};                            // devices whose limit has been raised
+  int dev = 0;
+  if (int e = st::cuda_fail(cudaGetDevice(&dev), "st_kv8_chunk_attn: device")) return e;
+  if (dev > 63 || !(set.load() >> dev & 1)) {
+    if (int e = st::cuda_fail(cudaFuncSetAttribute(kv8_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::BYTES),
+                              "st_kv8_chunk_attn: shared memory attribute"))
+      return e;
+    if (dev <= 63) set.fetch_or(1ull << dev);
+  }
+  return st::launch("st_kv8_chunk_attn launch", kv8_chunk_kernel<D>, dim3((unsigned)((long long)c.slots * c.a.H * c.parts.splits)),
+                    dim3(WARPS * 32), (size_t)Lay<D>::BYTES, st_, c);
+}
+}  // namespace
+
+extern "C" int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
+                                 const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts,
+                                 const int32_t* lens, const int32_t* starts, int64_t window, void* out, int64_t os, float* wo,
+                                 float* wml, double scale, int64_t S, void* stream) {
+  Chunk8 c;
+  if (int e = st::attn8_args(c.a, "st_kv8_chunk_attn", q, qs, T, Hq, cu, B, kv, exps, nblocks, Hkv, D, bt, bts, lens, starts, window, out,
+                             os, scale))
+    return e;
+  ST_REQUIRE(S >= 1 && S <= 1024, "st_kv8_chunk_attn: splits must be in [1, 1024]");
+  ST_REQUIRE(S == 1 || (wo && wml && st::aligned16(wo)), "st_kv8_chunk_attn: split workspace (wo, wml) missing or unaligned");
+  if (T == 0 || B == 0) return 0;
+  ST_REQUIRE(cu || T == B, "st_kv8_chunk_attn: without cu every sequence has one query");
+  ST_REQUIRE(nblocks < (1ll << 31), "st_kv8_chunk_attn: too many pages");
+  c.parts = {wo, wml, (int)S, 1};
+  c.status = st::status_ptr();
+  ST_REQUIRE(c.status != nullptr, "st_kv8_chunk_attn: no device status word");
+  // 256-row tiles of all sequences: each may leave one unfilled
+  const long long slots = T * (Hq / Hkv) / (2 * ROWS) + B;
+  ST_REQUIRE(slots * Hkv * S < (1ll << 31), "st_kv8_chunk_attn: grid too large");
+  c.slots = (int)slots;
+  const cudaStream_t st_ = (cudaStream_t)stream;
+  const int e = D == 128 ? chunk_launch<128>(c, st_) : chunk_launch<64>(c, st_);
+  if (e || S == 1) return e;
+  return st::merge8("st_kv8_chunk_attn merge launch", c.a, c.parts, (int)D, st_);
+}
