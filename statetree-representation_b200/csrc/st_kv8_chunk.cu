@@ -25,7 +25,7 @@ namespace {
 using namespace st;
 
 constexpr int KEYS = 128, TILE_PAGES = KEYS / PAGE, ROWS = 128;
-constexpr int W_CONV = 8, W_MMA = 12, WARPS = 13;                 // softmax warps 0 .. 7 (tile = warp / 4)
+constexpr int W_CONV = 8, W_MMA = 12, WARPS = 16;                 // softmax warps 0 .. 7 (tile = warp / 4); 13 .. 15 only lend registers
 constexpr int CRING = 4;                                          // page factors of so many key tiles are kept
 constexpr float LAZY = 8.f;                                       // a row's reference maximum is raised when a score exceeds it by this
 
@@ -54,26 +54,38 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t next) {
 }
 #define ST_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
 #define ST_I4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
-__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&v)[32]) {      // (complete after tm_wait_ld)
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t* v) {            // (complete after tm_wait_ld)
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
                "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                : ST_R4(v, 0), ST_R4(v, 4), ST_R4(v, 8), ST_R4(v, 12), ST_R4(v, 16), ST_R4(v, 20), ST_R4(v, 24), ST_R4(v, 28)
                : "r"(addr));
 }
-__device__ __forceinline__ void tm_wait_ld(uint32_t (&v)[32]) {                  // (v's readers stay behind the wait)
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
-                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]),
-                 "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]),
-                 "+r"(v[27]), "+r"(v[28]), "+r"(v[29])
-               :: "memory");
-  asm volatile("" : "+r"(v[30]), "+r"(v[31]) :: "memory");
+__device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : ST_R4(v, 0), ST_R4(v, 4), ST_R4(v, 8), ST_R4(v, 12) : "r"(addr));
 }
-__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&v)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-               "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-               :: "r"(addr), ST_I4(v, 0), ST_I4(v, 4), ST_I4(v, 8), ST_I4(v, 12), ST_I4(v, 16), ST_I4(v, 20), ST_I4(v, 24), ST_I4(v, 28)
-               : "memory");
+template <int N>
+__device__ __forceinline__ void tm_wait_ld(uint32_t* v) {                        // (v's readers stay behind the wait)
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int k = 0; k < N; ++k) asm volatile("" : "+r"(v[k]));
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2f(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -81,6 +93,12 @@ __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&v)[16]) 
 }
 #undef ST_R4
 #undef ST_I4
+// registers of a warpgroup: 512 threads start with 128 each (64 K in all, the SM's); 2 x 184 + 96 + 48 = 4 x 128
+constexpr int R_SOFTMAX = 184, R_CONV = 96, R_MMA = 48;
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
 __device__ __forceinline__ float ex2(float x) {                   // 2^x, relative error below 2^-22, results below 2^-126 are 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -192,6 +210,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
   const uint32_t tmem = *slot_at;
 
   if (warp < W_CONV) {
+    regs_up<R_SOFTMAX>();
     // ---------------------------------------------------------------- softmax: this thread's row
     const int t = warp >> 2, my = w.row0 + t * ROWS + (warp & 3) * 32 + lane, count = t ? w.count1 : w.count0;
     const bool live = my < w.row0 + w.rows;
@@ -225,30 +244,26 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
       if (any) {
         const float* const fac = reinterpret_cast<const float*>(smem + L::F) + (j % CRING) * (TILE_PAGES * 3);
         const int k0 = (w.first_tile + j) * KEYS, l0 = lo - k0, l1 = hi - k0;                // this row sees columns l0 .. l1
-        const bool masked = __any_sync(FULL, l0 > 0 || l1 < KEYS - 1);
-        // ---- the row's maximum
+        // ---- the row's scores, all 128 in registers; what it does not see is -inf
+        uint32_t v[KEYS];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tm_ld32(ts + 32 * q, v + 32 * q);
+        tm_wait_ld<KEYS>(v);
+        if (__any_sync(FULL, l0 > 0 || l1 < KEYS - 1)) {
+#pragma unroll
+          for (int k = 0; k < KEYS; ++k) v[k] = k < l0 || k > l1 ? 0xFF800000u : v[k];
+        }
         float top = -INFINITY;
-        uint32_t v[2][32];
-        tm_ld32(ts, v[0]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          tm_wait_ld(v[q & 1]);
-          if (q < 3) tm_ld32(ts + 32 * (q + 1), v[(q + 1) & 1]);
+        for (int p = 0; p < TILE_PAGES; ++p) {
+          float x[16];
 #pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            float x[16];
+          for (int k = 0; k < 16; ++k) x[k] = __uint_as_float(v[16 * p + k]);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const int col = 32 * q + 16 * p + k;
-              x[k] = __uint_as_float(v[q & 1][16 * p + k]);
-              if (masked) x[k] = col < l0 || col > l1 ? -INFINITY : x[k];
-            }
+          for (int o = 8; o; o >>= 1)
 #pragma unroll
-            for (int o = 8; o; o >>= 1)
-#pragma unroll
-              for (int k = 0; k < o; ++k) x[k] = fmaxf(x[k], x[k + o]);
-            top = fmaxf(top, x[0] * fac[2 * q + p]);
-          }
+            for (int k = 0; k < o; ++k) x[k] = fmaxf(x[k], x[k + o]);
+          top = fmaxf(top, x[0] * fac[p]);
         }
         if (__any_sync(FULL, top > m + LAZY)) {
           const float up = fmaxf(m, top), f = up == m ? 1.f : ex2(m - up);
@@ -256,44 +271,39 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
           l *= f;
           if (j > 0) {                                            // (O's product of the tile before has completed: sfull says so)
 #pragma unroll
-            for (int q = 0; q < D / 32; ++q) {
-              tm_ld32(to + 32 * q, v[0]);
-              tm_wait_ld(v[0]);
+            for (int q = 0; q < D / 16; ++q) {
+              uint32_t o[16];
+              tm_ld16(to + 16 * q, o);
+              tm_wait_ld<16>(o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[0][k] = __float_as_uint(__uint_as_float(v[0][k]) * f);
-              tm_st32(to + 32 * q, v[0]);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tm_st16(to + 16 * q, o);
             }
           }
         }
         // ---- P, and the sum
         const float ref = m == -INFINITY ? 0.f : m;
-        tm_ld32(ts, v[0]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          tm_wait_ld(v[q & 1]);
-          if (q < 3) tm_ld32(ts + 32 * (q + 1), v[(q + 1) & 1]);
           uint32_t pk[16];
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
-            const float by = fac[2 * q + p], add = fac[TILE_PAGES + 2 * q + p] - ref;
-            float sum[2] = {0.f, 0.f};
+            const int pg = 2 * q + p;
+            const float add = fac[TILE_PAGES + pg] - ref;
+            const uint64_t by2 = pair2(fac[pg], fac[pg]), add2 = pair2(add, add);
+            uint64_t sum = 0;
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
-              const int col = 32 * q + 16 * p + k;
-              float x0 = __uint_as_float(v[q & 1][16 * p + k]), x1 = __uint_as_float(v[q & 1][16 * p + k + 1]);
-              x0 = fmaf(x0, by, add);
-              x1 = fmaf(x1, by, add);
-              if (masked) {
-                x0 = col < l0 || col > l1 ? -INFINITY : x0;
-                x1 = col + 1 < l0 || col + 1 > l1 ? -INFINITY : x1;
-              }
+              float x0, x1;
+              unpair2(fma2(pair2(__uint_as_float(v[16 * pg + k]), __uint_as_float(v[16 * pg + k + 1])), by2, add2), x0, x1);
               x0 = ex2(x0);
               x1 = ex2(x1);
-              sum[0] += x0;
-              sum[1] += x1;
+              sum = add2f(sum, pair2(x0, x1));
               pk[8 * p + k / 2] = pack_bf16(x0, x1);
             }
-            l = fmaf(sum[0] + sum[1], fac[2 * TILE_PAGES + 2 * q + p], l);
+            float s0, s1;
+            unpair2(sum, s0, s1);
+            l = fmaf(s0 + s1, fac[2 * TILE_PAGES + pg], l);
           }
           tm_st16(ts + 16 * q, pk);
         }
@@ -320,7 +330,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
         uint32_t v[32];
         if (count > 0) {
           tm_ld32(to + 32 * q, v);
-          tm_wait_ld(v);
+          tm_wait_ld<32>(v);
         }
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
@@ -343,6 +353,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     }
     tc_fence_before();
   } else if (warp < W_MMA) {
+    regs_down<R_CONV>();
     // ---------------------------------------------------------------- converters: codes -> operand tiles.  A lane's 16-byte piece
     // becomes two of a tile row; eight lanes store four pieces of an even row and four of the next, so that with the swizzle they
     // meet every bank once, and a warp reads whole rows
@@ -424,6 +435,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     }
     if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_EMPTY);
   } else {
+    regs_down<R_MMA>();
+    if (warp == W_MMA) {
     // ---------------------------------------------------------------- MMAs.  One thread's MMAs complete in the order of their issue
     // (and a commit covers all before it): S of the next key tile may take the place of the P that the product before it reads
     constexpr uint32_t IDESC_S = mma_idesc(128, KEYS), IDESC_O = mma_idesc(128, D) | 1u << 16;
@@ -497,6 +510,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
       (void)mbar_wait(drain, 0);
     }
     tc_fence_before();
+    }
   }
   __syncthreads();
   if (warp == W_MMA) {
