@@ -1,5 +1,5 @@
 // The host path of a module call in native code: TreeLinear products and lists of them (q / k / v, gate / up) for inputs that need
-// no conversion, and the launches of a matrix's conversion and its check.  What Python does for such a product (checks, the output
+// no conversion, the launches of a matrix's conversion and its check, and the calls of the 8-bit KV pages.  What Python does for such a product (checks, the output
 // and its views, pointer arrays, the ctypes call) takes 15 to 30 us, several times a small product's time on the GPU; this takes
 // 3 to 5.
 //
@@ -14,6 +14,7 @@
 
 #include <cstdint>
 #include <map>
+#include <optional>
 #include <stdexcept>
 #include <string>
 #include <type_traits>
@@ -37,6 +38,10 @@ struct Library {
   decltype(&st_encode_lists) lists;
   decltype(&st_dec_check) dec_check;
   decltype(&st_lists_check) lists_check;
+  decltype(&st_kv8_append) kv8_append;
+  decltype(&st_kv8_dequant_blocks) kv8_dequant;
+  decltype(&st_kv8_attn) kv8_attn;
+  decltype(&st_kv8_chunk_attn) kv8_chunk;
 };
 
 // rows of x if it can be read as it is: BF16 [..., N] on `device`, contiguous, 16-byte aligned, at least one row; else 0
@@ -78,6 +83,10 @@ Library library(const std::map<std::string, uint64_t>& address) {
   bind(lib.lists, "st_encode_lists");
   bind(lib.dec_check, "st_dec_check");
   bind(lib.lists_check, "st_lists_check");
+  bind(lib.kv8_append, "st_kv8_append");
+  bind(lib.kv8_dequant, "st_kv8_dequant_blocks");
+  bind(lib.kv8_attn, "st_kv8_attn");
+  bind(lib.kv8_chunk, "st_kv8_chunk_attn");
   return lib;
 }
 
@@ -221,6 +230,129 @@ at::Tensor check_start(const Library& lib, const at::Tensor& tree, const at::Ten
   }
   return bad;
 }
+// ---- 8-bit KV pages.  Each returns None where the call is not of the plain form (the checks in ops.py then say what is wrong with it)
+using Maybe = std::optional<at::Tensor>;
+constexpr int64_t PAGE = 16;
+
+bool flat(const at::Tensor& t, at::ScalarType type, const at::Device& device) {
+  return t.scalar_type() == type && t.device() == device && t.layout() == at::kStrided && t.is_contiguous();
+}
+// pages uint8 [blocks, H, 2, 16, D] and exps int8 [blocks, H, 2] on a GPU
+bool pages8(const at::Tensor& pages, const at::Tensor& exps) {
+  return pages.is_cuda() && pages.dim() == 5 && pages.size(2) == 2 && pages.size(3) == PAGE && (pages.size(4) == 64 || pages.size(4) == 128) &&
+         flat(pages, at::kByte, pages.device()) && flat(exps, at::kChar, pages.device()) && exps.dim() == 3 && exps.size(0) == pages.size(0) &&
+         exps.size(1) == pages.size(1) && exps.size(2) == 2;
+}
+// BF16 [N, heads, D], heads contiguous, as the kernels' 16-byte vectors need it
+bool rows8(const at::Tensor& t, int64_t D, const at::Device& device) {
+  return t.scalar_type() == at::kBFloat16 && t.device() == device && t.layout() == at::kStrided && t.dim() == 3 && t.size(2) == D &&
+         t.numel() > 0 && t.stride(2) == 1 && (t.stride(1) == D || t.size(1) == 1) && t.stride(0) % 8 == 0 && !t.is_conj() && !t.is_neg() &&
+         (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0;
+}
+bool norm8(const Maybe& w, int64_t D, const at::Device& device) {
+  return !w || (flat(*w, at::kBFloat16, device) && w->numel() == D && (reinterpret_cast<uintptr_t>(w->const_data_ptr()) & 15u) == 0);
+}
+template <typename T>
+const T* of(const Maybe& t) { return t ? reinterpret_cast<const T*>(t->const_data_ptr()) : nullptr; }
+template <typename T>
+const T* of(const at::Tensor& t) { return reinterpret_cast<const T*>(t.const_data_ptr()); }
+
+// append; returns the rotated queries (True without any)
+py::object kv8_append(const Library& lib, const at::Tensor& pages, const at::Tensor& exps, const at::Tensor& marks, const at::Tensor& bad,
+                      const at::Tensor& K, const at::Tensor& V, const at::Tensor& slots, const Maybe& positions, const Maybe& cos,
+                      const Maybe& sin, bool interleaved, const Maybe& q, const Maybe& q_norm, const Maybe& k_norm, double eps,
+                      const Maybe& q_out) {
+  if (!pages8(pages, exps)) return py::none();
+  const at::Device device = pages.device();
+  const int64_t H = pages.size(1), D = pages.size(4);
+  if (!rows8(K, D, device) || !rows8(V, D, device)) return py::none();
+  const int64_t N = K.size(0);
+  if (K.size(1) != H || V.size(0) != N || V.size(1) != H || !flat(slots, at::kLong, device) || slots.numel() != N ||
+      !flat(marks, at::kInt, device) || marks.numel() < 17 * pages.size(0) || !flat(bad, at::kInt, device) || bad.numel() < 1 ||
+      !norm8(k_norm, D, device) || !norm8(q_norm, D, device) || cos.has_value() != sin.has_value())
+    return py::none();
+  int64_t step = 0, span = 0;
+  if (cos) {
+    if (!positions || !flat(*positions, at::kLong, device) || (positions->numel() != N && positions->numel() != 1) || !flat(*cos, at::kFloat, device) ||
+        !flat(*sin, at::kFloat, device) || cos->dim() != 2 || sin->sizes() != cos->sizes() || cos->size(1) != D / 2 || cos->size(0) < 1)
+      return py::none();
+    step = positions->numel() > 1;
+    span = cos->size(0);
+  }
+  if (q && (!rows8(*q, D, device) || q->size(0) != N)) return py::none();
+  if (q_out && (!q || !rows8(*q_out, D, device) || q_out->sizes() != q->sizes())) return py::none();
+  at::Tensor out;
+  int rc;
+  {
+    py::gil_scoped_release nogil;
+    const c10::cuda::CUDAGuard guard(device);
+    if (q) out = q_out ? *q_out : at::empty(q->sizes(), q->options().requires_grad(false));
+    void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    rc = lib.kv8_append(K.const_data_ptr(), V.const_data_ptr(), K.stride(0), V.stride(0), of<int64_t>(slots), N, H, D, pages.data_ptr(),
+                        reinterpret_cast<int8_t*>(exps.data_ptr()), pages.size(0), cos ? of<int64_t>(positions) : nullptr, step,
+                        of<float>(cos), of<float>(sin), span, interleaved ? 1 : 0, of<void>(k_norm), of<void>(q), q ? q->stride(0) : 0,
+                        of<void>(q_norm), q ? q->size(1) : 0, q ? out.data_ptr() : nullptr, q ? out.stride(0) : 0, eps,
+                        reinterpret_cast<int32_t*>(marks.data_ptr()), reinterpret_cast<int32_t*>(bad.data_ptr()), stream);
+  }
+  check(lib, rc);
+  return q ? py::cast(out) : py::cast(true);
+}
+
+// attention of one query per sequence (chunk false) or of cu's rows (chunk true; cu None: one each)
+py::object kv8_attention(const Library& lib, bool chunk, const at::Tensor& pages, const at::Tensor& exps, const at::Tensor& q,
+                         const Maybe& cu, const at::Tensor& table, const at::Tensor& lens, double scale, int64_t splits,
+                         const Maybe& starts, int64_t min_pages, const Maybe& given, int64_t window) {
+  if (!pages8(pages, exps)) return py::none();
+  const at::Device device = pages.device();
+  const int64_t H = pages.size(1), D = pages.size(4);
+  if (!rows8(q, D, device) || table.dim() != 2) return py::none();
+  const int64_t T = q.size(0), Hq = q.size(1), B = table.size(0);
+  if (Hq % H || B < 1 || table.scalar_type() != at::kInt || table.device() != device || table.layout() != at::kStrided || table.stride(1) != 1 ||
+      !flat(lens, at::kInt, device) || lens.numel() != B || (starts && (!flat(*starts, at::kInt, device) || starts->numel() != B)) ||
+      splits < 1 || window < 0 || (cu ? !flat(*cu, at::kInt, device) || cu->numel() != B + 1 : T != B))
+    return py::none();
+  if (given && (!rows8(*given, D, device) || given->sizes() != q.sizes())) return py::none();
+  at::Tensor out, ws;
+  int rc;
+  {
+    py::gil_scoped_release nogil;
+    const c10::cuda::CUDAGuard guard(device);
+    out = given ? *given : at::empty(q.sizes(), q.options().requires_grad(false));
+    float *wo = nullptr, *wml = nullptr;
+    if (splits > 1) {                                             // partial results of this call alone
+      ws = at::empty({T * Hq * splits * (D + 2)}, q.options().requires_grad(false).dtype(at::kFloat));
+      wo = reinterpret_cast<float*>(ws.data_ptr());
+      wml = wo + T * Hq * splits * D;
+    }
+    void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    rc = chunk ? lib.kv8_chunk(q.const_data_ptr(), q.stride(0), T, Hq, of<int32_t>(cu), B, pages.const_data_ptr(), of<int8_t>(exps),
+                               pages.size(0), H, D, of<int32_t>(table), table.stride(0), of<int32_t>(lens), of<int32_t>(starts), window,
+                               out.data_ptr(), out.stride(0), wo, wml, scale, splits, stream)
+               : lib.kv8_attn(q.const_data_ptr(), q.stride(0), B, Hq, pages.const_data_ptr(), of<int8_t>(exps), pages.size(0), H, D,
+                              of<int32_t>(table), table.stride(0), of<int32_t>(lens), of<int32_t>(starts), window, out.data_ptr(),
+                              out.stride(0), wo, wml, scale, splits, min_pages, stream);
+  }
+  check(lib, rc);
+  return py::cast(out);
+}
+
+// listed pages (None: all) as dense BF16 [n, 16, H, D]
+py::object kv8_dense(const Library& lib, const at::Tensor& pages, const at::Tensor& exps, const Maybe& blocks) {
+  if (!pages8(pages, exps) || (blocks && (!flat(*blocks, at::kInt, pages.device()) || blocks->dim() != 1))) return py::none();
+  const int64_t H = pages.size(1), D = pages.size(4), n = blocks ? blocks->numel() : pages.size(0);
+  at::Tensor K, V;
+  int rc;
+  {
+    py::gil_scoped_release nogil;
+    const c10::cuda::CUDAGuard guard(pages.device());
+    K = at::empty({n, PAGE, H, D}, pages.options().requires_grad(false).dtype(at::kBFloat16));
+    V = at::empty_like(K);
+    rc = lib.kv8_dequant(pages.const_data_ptr(), of<int8_t>(exps), pages.size(0), H, D, of<int32_t>(blocks), n, K.data_ptr(), V.data_ptr(),
+                         c10::cuda::getCurrentCUDAStream(pages.device().index()).stream());
+  }
+  check(lib, rc);
+  return py::make_tuple(K, V);
+}
 }  // namespace
 
 PYBIND11_MODULE(_calls, m) {
@@ -232,4 +364,7 @@ PYBIND11_MODULE(_calls, m) {
   m.def("linear_list", &linear_list);
   m.def("encode", &encode);
   m.def("check_start", &check_start);
+  m.def("kv8_append", &kv8_append);
+  m.def("kv8_attention", &kv8_attention);
+  m.def("kv8_dense", &kv8_dense);
 }

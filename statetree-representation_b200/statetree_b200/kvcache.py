@@ -7,7 +7,7 @@ statetree_attention, enable) live in hf_cache.py and are re-exported here when t
 """
 import torch
 
-from .ops import kv_ext
+from .ops import calls, kv_ext
 
 PAGE = 16
 RKV = 1600
@@ -120,6 +120,12 @@ class PageStore8:
         (i, i + D/2) with interleaved=False; with k_norm (bf16 [D]) they are RMS-normalised before.  q [N, Hq, D] goes the same way
         (q_norm) into q_out, which is returned.  A page is written from row 0 on: doing that again starts it anew (its other rows
         become zero); tokens that follow raise its exponent where they need to."""
+        host = calls()                                     # one native call for inputs that need no copy
+        if host is not None:
+            done = host[0].kv8_append(host[1], self.pages, self.exps, self.marks, self.bad, K, V, slots, positions, cos, sin, interleaved, q,
+                                      q_norm, k_norm, eps, q_out)
+            if done is not None:
+                return done if q is not None else None
         K, V = _rows(K, self.D), _rows(V, self.D)
         if q is not None:
             q = _rows(q, self.D)
@@ -132,11 +138,17 @@ class PageStore8:
     def attention(self, q, block_table, lens, scale, splits=None, starts=None, min_pages=4, out=None, window=0):
         """one query token per sequence: q [B, Hq, D] bf16 -> [B, Hq, D] bf16; tokens [max(starts, lens - window), lens) take part
         (window 0: from starts on).  splits: how many CTAs share a sequence (None: by batch size and table width)"""
+        if splits is None:
+            splits = decode_splits(q.shape[0], self.H, block_table.shape[1])
+        host = calls()
+        if host is not None:
+            done = host[0].kv8_attention(host[1], False, self.pages, self.exps, q, None, block_table, lens, scale, splits, starts, min_pages,
+                                         out, window)
+            if done is not None:
+                return done
         q = _rows(q, self.D)
         if out is None:
             out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-        if splits is None:
-            splits = decode_splits(q.shape[0], self.H, block_table.shape[1])
         wo, wml = self._partials(q, splits)
         kv_ext().kv8_attn(q, self.pages, self.exps, block_table, lens, out, scale, splits, wo, wml, starts, min_pages, window)
         return out
@@ -145,11 +157,16 @@ class PageStore8:
         """causal attention of several query tokens per sequence, after their keys and values have been appended: q [T, Hq, D] bf16,
         sequence b's rows are cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1]), the last of them at position lens[b] - 1 -> [T, Hq, D];
         rows behind cu[B] of a given `out` stay as they are"""
+        if splits is None:
+            splits = 1
+        host = calls()
+        if host is not None:
+            done = host[0].kv8_attention(host[1], True, self.pages, self.exps, q, cu, block_table, lens, scale, splits, starts, 1, out, window)
+            if done is not None:
+                return done
         q = _rows(q, self.D)
         if out is None:
             out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-        if splits is None:
-            splits = 1
         wo, wml = self._partials(q, splits)
         kv_ext().kv8_chunk_attn(q, cu, self.pages, self.exps, block_table, lens, out, scale, splits, wo, wml, starts, window)
         return out
@@ -164,6 +181,11 @@ class PageStore8:
 
     def dense(self, blocks=None):
         """pages (all, or the listed block ids) as exact BF16 Kd, Vd [n, 16, H, D]"""
+        host = calls()
+        if host is not None:
+            done = host[0].kv8_dense(host[1], self.pages, self.exps, blocks)
+            if done is not None:
+                return done
         n = self.pages.shape[0] if blocks is None else blocks.numel()
         Kd = torch.empty(n, PAGE, self.H, self.D, dtype=torch.bfloat16, device=self.device)
         Vd = torch.empty_like(Kd)

@@ -122,7 +122,7 @@ def lib():
 CALLS_PATH = os.path.join(_HERE, "_calls.so")
 _CALLS = None                                           # False: there is none
 _NATIVE = ("st_gemv", "st_gemm", "st_gemv_list", "st_gemm_list", "st_last_error", "st_encode", "st_encode_lists", "st_encode_offsets",
-           "st_encode_offsets_workspace_bytes", "st_dec_check", "st_lists_check")
+           "st_encode_offsets_workspace_bytes", "st_dec_check", "st_lists_check", "st_kv8_append", "st_kv8_dequant_blocks", "st_kv8_attn", "st_kv8_chunk_attn")
 
 
 def calls():
