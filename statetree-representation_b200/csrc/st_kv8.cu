@@ -2,6 +2,7 @@
 // The page and why it is laid out so: st_kv8.cuh.
 #include <math.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/statetree_b200.h"
@@ -36,7 +37,8 @@ struct Append8 {
   const uint16_t* wq; const uint16_t* wk;
   uint16_t* q_out;
   int* marks; int* bad;
-  int N, H, Hq, q_cta;                             // q_cta: first CTA that works on queries
+  int N, H, Hq;
+  int q_cta, q_units, q_steps;                     // first CTA that works on queries; warps per token, groups of heads per warp
   float eps;
   int pairs;
 };
@@ -53,41 +55,52 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&f)[16], int at) 
 // A lane's sixteen values of a row: dims 8c .. 8c + 7 (f[0..7]) and D/2 + 8c .. (f[8..15]), c = lane % (D / 16): both partners of
 // either rotation lie in one lane.
 template <int D>
-__device__ __forceinline__ void row_norm(float (&f)[16], const uint16_t* w, float eps, int c) {
+__device__ __forceinline__ float row_rms(const float (&f)[16], float eps) {
   constexpr int LPR = D / 16;
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) ss = fmaf(f[i], f[i], ss);
 #pragma unroll
   for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
-  const float r = __frsqrt_rn(ss * (1.f / D) + eps);
+  return __frsqrt_rn(ss * (1.f / D) + eps);
+}
+template <int D>
+__device__ __forceinline__ void row_norm(float (&f)[16], const uint4 (&w)[2], float eps) {
+  const float r = row_rms<D>(f, eps);
   float g[16];
-  unpack8(*reinterpret_cast<const uint4*>(w + 8 * c), g, 0);
-  unpack8(*reinterpret_cast<const uint4*>(w + D / 2 + 8 * c), g, 8);
+  unpack8(w[0], g, 0);
+  unpack8(w[1], g, 8);
 #pragma unroll
   for (int i = 0; i < 16; ++i) f[i] = f[i] * r * g[i];
 }
 template <int D>
-__device__ __forceinline__ void row_rotate(float (&f)[16], const float* ct, const float* st, int pairs, int c) {
-  float cs[8], sn[8];
+__device__ __forceinline__ void norm_weights(uint4 (&w)[2], const uint16_t* at, int c) {
+  w[0] = *reinterpret_cast<const uint4*>(at + 8 * c);
+  w[1] = *reinterpret_cast<const uint4*>(at + D / 2 + 8 * c);
+}
+struct Turn { float cs[8], sn[8]; };               // of the lane's eight pairs
+template <int D>
+__device__ __forceinline__ void load_turn(Turn& t, const float* ct, const float* st, int pairs, int c) {
   const int p0 = pairs ? 4 * c : 8 * c, p1 = pairs ? D / 4 + 4 * c : 8 * c + 4;
-  *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(ct + p0);
-  *reinterpret_cast<float4*>(cs + 4) = *reinterpret_cast<const float4*>(ct + p1);
-  *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(st + p0);
-  *reinterpret_cast<float4*>(sn + 4) = *reinterpret_cast<const float4*>(st + p1);
+  *reinterpret_cast<float4*>(t.cs) = *reinterpret_cast<const float4*>(ct + p0);
+  *reinterpret_cast<float4*>(t.cs + 4) = *reinterpret_cast<const float4*>(ct + p1);
+  *reinterpret_cast<float4*>(t.sn) = *reinterpret_cast<const float4*>(st + p0);
+  *reinterpret_cast<float4*>(t.sn + 4) = *reinterpret_cast<const float4*>(st + p1);
+}
+__device__ __forceinline__ void row_rotate(float (&f)[16], const Turn& t, int pairs) {
   if (pairs) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {                  // pair i of the lane: f[2i], f[2i + 1]
       const float a = f[2 * i], b = f[2 * i + 1];
-      f[2 * i] = a * cs[i] - b * sn[i];
-      f[2 * i + 1] = a * sn[i] + b * cs[i];
+      f[2 * i] = a * t.cs[i] - b * t.sn[i];
+      f[2 * i + 1] = a * t.sn[i] + b * t.cs[i];
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float a = f[i], b = f[8 + i];
-      f[i] = a * cs[i] - b * sn[i];
-      f[8 + i] = a * sn[i] + b * cs[i];
+      f[i] = a * t.cs[i] - b * t.sn[i];
+      f[8 + i] = a * t.sn[i] + b * t.cs[i];
     }
   }
 }
@@ -149,33 +162,42 @@ __device__ __forceinline__ void append_unit(const Append8& a, long long page, in
   int8_t* const exp_at = a.exps + ((size_t)page * a.H + h) * 2 + kvi;
   const bool anew = rows & 1u;
   const int was = anew ? E8_MIN : page8_exp(*exp_at);
-  float f[ITER][16], top = 0.f;
-  bool odd = false;                                // (a value that is not finite)
+  float f[ITER][16];
+  uint4 w[2];
+  if (kvi == 0 && a.wk) norm_weights<D>(w, a.wk, c);
+  uint32_t most = 0;                               // bits of the largest magnitude: NaN above infinity above the finite ones
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
     unpack8(raw[i][0], f[i], 0);
     unpack8(raw[i][1], f[i], 8);
     if (kvi == 0) {
-      if (a.wk) row_norm<D>(f[i], a.wk, a.eps, c);
+      if (a.wk) row_norm<D>(f[i], w, a.eps);
       if (a.cos_t && mine[i] >= 0) {
         const long long at = table_row(a, mine[i]) * (D / 2);
-        row_rotate<D>(f[i], a.cos_t + at, a.sin_t + at, a.pairs, c);
+        Turn t;
+        load_turn<D>(t, a.cos_t + at, a.sin_t + at, a.pairs, c);
+        row_rotate(f[i], t, a.pairs);
       }
     }
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float m = fabsf(f[i][k]);
-      const bool fin = m < INFINITY;
-      odd |= !fin;
-      top = fmaxf(top, fin ? m : 0.f);
-      if (m != m) f[i][k] = 0.f;
-    }
+    for (int k = 0; k < 16; ++k) most = max(most, __float_as_uint(f[i][k]) & 0x7FFFFFFFu);
   }
+  most = __reduce_max_sync(FULL, most);
+  const bool odd = most > __float_as_uint(448.f * pow2i(E8_MAX));        // (a value that is not finite, or beyond the format)
+  float top = __uint_as_float(most);
+  if (odd) {
+    top = 0.f;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
+    for (int i = 0; i < ITER; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float m = fabsf(f[i][k]);
+        top = fmaxf(top, m < INFINITY ? m : 0.f);
+        if (m != m) f[i][k] = 0.f;
+      }
+    top = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(top)));
+  }
   const int e = max(was, exp_for(top));
-  // (a finite value beyond 448 * 2^E8_MAX is cut off there, as infinities are)
-  odd |= top > 448.f * pow2i(E8_MAX);
   const float down = pow2i(-e), up = pow2i(20 + was);
   uint8_t* const unit = a.kv + page8_off<D>(page, a.H, h, kvi);
 #pragma unroll
@@ -192,31 +214,52 @@ __device__ __forceinline__ void append_unit(const Append8& a, long long page, in
   }
   __syncwarp();                                    // (every lane has read the old exponent)
   if (lane == 0 && (anew || e != was)) *exp_at = (int8_t)e;
-  if (odd) *a.bad = 1;
+  if (odd && lane == 0) *a.bad = 1;
 }
 
-// rows [first, ..) of the queries [N * Hq, D]: a warp takes 32 / (D / 16) of them
+// A warp takes q_steps groups of 32 / (D / 16) heads of one token: its row of the tables and the norm weights are read once
 template <int D>
-__device__ __forceinline__ void rotate_queries(const Append8& a, long long first, int lane) {
-  constexpr int LPR = D / 16;
-  const long long row = first + lane / LPR;
-  const bool live = row < (long long)a.N * a.Hq;
-  const long long token = live ? row / a.Hq : 0;
-  const int h = live ? (int)(row % a.Hq) : 0, c = lane % LPR;
-  const uint16_t* const p = a.Q + token * a.qs + (size_t)h * D + 8 * c;
-  float f[16];
-  unpack8(*reinterpret_cast<const uint4*>(p), f, 0);
-  unpack8(*reinterpret_cast<const uint4*>(p + D / 2), f, 8);
-  if (a.wq) row_norm<D>(f, a.wq, a.eps, c);
+__device__ __forceinline__ void rotate_queries(const Append8& a, long long unit, int lane) {
+  constexpr int LPR = D / 16, RPI = 32 / LPR, AHEAD = 4;
+  const long long token = unit / a.q_units;
+  if (token >= a.N) return;
+  const int c = lane % LPR, h0 = (int)(unit % a.q_units) * a.q_steps * RPI, h1 = min(a.Hq, h0 + a.q_steps * RPI);
+  const uint16_t* const src = a.Q + token * a.qs + 8 * c;
+  uint16_t* const dst = a.q_out + token * a.qos + 8 * c;
+  uint4 w[2];
+  Turn t;
   if (a.cos_t) {
     const long long at = table_row(a, token) * (D / 2);
-    row_rotate<D>(f, a.cos_t + at, a.sin_t + at, a.pairs, c);
+    load_turn<D>(t, a.cos_t + at, a.sin_t + at, a.pairs, c);
   }
-  if (!live) return;
-  uint16_t* const o = a.q_out + token * a.qos + (size_t)h * D + 8 * c;
-  *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
-  *reinterpret_cast<uint4*>(o + D / 2) =
-      make_uint4(pack_bf16(f[8], f[9]), pack_bf16(f[10], f[11]), pack_bf16(f[12], f[13]), pack_bf16(f[14], f[15]));
+  if (a.wq) norm_weights<D>(w, a.wq, c);
+  for (int h = h0; h < h1; h += AHEAD * RPI) {
+    uint4 raw[AHEAD][2];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int mine = h + i * RPI + lane / LPR;
+      if (mine < h1) {
+        raw[i][0] = *reinterpret_cast<const uint4*>(src + (size_t)mine * D);
+        raw[i][1] = *reinterpret_cast<const uint4*>(src + (size_t)mine * D + D / 2);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (h + i * RPI >= h1) break;
+      const int mine = h + i * RPI + lane / LPR;
+      float f[16];
+      unpack8(raw[i][0], f, 0);
+      unpack8(raw[i][1], f, 8);
+      if (a.wq) row_norm<D>(f, w, a.eps);
+      if (a.cos_t) row_rotate(f, t, a.pairs);
+      if (mine < h1) {
+        uint4* const o = reinterpret_cast<uint4*>(dst + (size_t)mine * D);
+        o[0] = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+        *reinterpret_cast<uint4*>(dst + (size_t)mine * D + D / 2) =
+            make_uint4(pack_bf16(f[8], f[9]), pack_bf16(f[10], f[11]), pack_bf16(f[12], f[13]), pack_bf16(f[14], f[15]));
+      }
+    }
+  }
 }
 
 __device__ __forceinline__ bool slot_ok(const Append8& a, long long s) { return s >= 0 && s / PAGE < a.nblocks; }
@@ -239,8 +282,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const Append8 a) {
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, units = 2 * a.H;
   if ((int)blockIdx.x >= a.q_cta) {
-    const long long first = ((long long)((int)blockIdx.x - a.q_cta) * 8 + warp) * (512 / D);
-    if (first < (long long)a.N * a.Hq) rotate_queries<D>(a, first, lane);
+    rotate_queries<D>(a, (long long)((int)blockIdx.x - a.q_cta) * 8 + warp, lane);
     return;
   }
   if (SCAN) {
@@ -690,7 +732,11 @@ extern "C" int st_kv8_append(const void* K, const void* V, int64_t ks, int64_t v
   a.N = (int)N; a.H = (int)H; a.Hq = Q ? (int)Hq : 0; a.eps = (float)eps; a.pairs = interleaved ? 1 : 0;
   const cudaStream_t st_ = (cudaStream_t)stream;
   const long long page_ctas = scan ? (N * H * 2 + 7) / 8 : (N + st::PAGE - 1) / st::PAGE;
-  const long long per_cta = 8 * 512 / D, q_ctas = (N * a.Hq + per_cta - 1) / per_cta;
+  // queries: a warp per group of heads while that leaves SMs without one, else up to eight groups of a token
+  const int groups = (int)((a.Hq + 512 / D - 1) / (512 / D));
+  a.q_steps = (int)std::min<long long>(std::min(std::max(groups, 1), 8), std::max<long long>(1, N * groups / (16ll * st::sm_count())));
+  a.q_units = groups ? (groups + a.q_steps - 1) / a.q_steps : 0;
+  const long long q_ctas = (N * a.q_units + 7) / 8;
   ST_REQUIRE(page_ctas + q_ctas < (1ll << 31), "st_kv8_append: too large");
   a.q_cta = (int)page_ctas;
   if (!scan)
