@@ -369,14 +369,17 @@ __global__ void __launch_bounds__(256) kv8_dequant_kernel(const uint8_t* __restr
 //     S^T [16 tokens x 8 heads] = K [16 tokens x D dims] . Q^T        O^T [D dims x 8 heads] += V^T [D dims x 16 tokens] . P^T
 // The order of the k index is free as long as both operands agree on it: lane (g, t) = (lane / 4, lane % 4) takes for keys the
 // 16-byte pieces t and t + 4 of rows g and g + 8 as they lie in the page, four dims per MMA, and q in the same order; for values the
-// piece g of tokens 2t, 2t + 1, 2t + 8, 2t + 9, two dims per MMA, the codes of two tokens being paired by a byte permute.  So a page
-// goes from its codes to fragments with 1.75 (keys) and 2 (values) integer operations a code and no transposition through memory.
+// piece g of tokens 2t, 2t + 1, 2t + 8, 2t + 9, two dims per MMA, the codes of two tokens being paired by a byte permute.  So codes go
+// to fragments without a transposition through memory.
 //
-// Scales.  Codes become BF16 numbers times 2^-120 (codes_split); q carries 2^60 and P 2^(60 + exponent of the page's values), so no
-// operand or sum leaves fp32's range for values within the format's, and the page's key exponent joins the softmax scale.
-// P is rounded to BF16 (2^-9 of each probability at most, unbiased), everything else is fp32: maxima, sums, partial results.
+// Types and scales.  An e4m3 code is an FP16 number exactly, and one instruction converts two (as BF16 patterns they took 1.75
+// integer operations each, and the integer pipe, 64 lanes a cycle and SM, was the limit: 64 sequences of up to 8192 tokens 118 us).
+// q is scaled by a power of two per head so that FP16 holds its eight bits (of values down to 2^-28 of the head's largest).  The
+// exponent of a page's keys joins the softmax scale.  That of its values joins the exponent of its probabilities: with x = score +
+// exponent (base 2) the running reference M bounds x, P = 2^(x - M) <= 2^8 is rounded to FP16 (2^-12 of each at most; what is below
+// 2^-25 of the largest contribution is lost), and the sum of the probabilities takes the exponent out again, per page, in fp32.
 //
-// Softmax: a head's reference maximum m is raised when a page holds a score more than 8 above it (base 2), one vote per page.
+// A head's reference M is raised when a page holds an x more than 8 above it: one vote per page, a rescale only then.
 //
 // Work split: grid = sequences x KV heads x head blocks x splits; a CTA's pages go round-robin to its warps, each of which streams its
 // own through a private ring of bulk copies (a page of one head is contiguous, 2 * 16 * D bytes), so there is no barrier in the loop.
@@ -393,13 +396,17 @@ __device__ __forceinline__ float over_rows_sum(float v) {
   v += __shfl_xor_sync(FULL, v, 8);
   return v + __shfl_xor_sync(FULL, v, 16);
 }
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
 template <int D, int NW, int STG>
 __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 a, const Parts8 parts, int* status) {
   constexpr int PB = 2 * PAGE * D, KT = D / 16, VT = D / 16;             // bytes of a page, MMAs of its keys and of its values
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + NW * STG * PB);
-  uint32_t* const s_exp = reinterpret_cast<uint32_t*>(bars + NW * STG);
+  float2* const facs = reinterpret_cast<float2*>(bars + NW * STG);       // (softmax scale with the keys' exponent, values' exponent)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int G = a.Hq / a.H, blocks_of_heads = (G + 7) / 8;
   const int split = blockIdx.x % parts.splits;
@@ -410,7 +417,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
   const int heads = min(8, G - 8 * hb), first_head = kvh * G + 8 * hb;
   uint8_t* const ring = smem + warp * STG * PB;
   uint64_t* const bar = bars + warp * STG;
-  uint32_t* const my_exp = s_exp + warp * STG;
+  float2* const fac = facs + warp * STG;
   if (lane == 0) {
     for (int s = 0; s < STG; ++s) mbar_init(bar + s, 1);
     fence_barrier_init();
@@ -441,47 +448,69 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
   const int my_count = hi_page > my_first ? (hi_page - my_first + NW - 1) / NW : 0;
 
   const int* const my_table = a.table + (size_t)seq * a.table_stride + my_first;
-  auto entry = [&](int i) { return i + lane < my_count ? __ldg(my_table + (long long)(i + lane) * NW) : 0; };
-  auto inside = [&](int e) -> long long { return e < 0 ? 0 : (e >= a.nblocks ? a.nblocks - 1 : e); };
-  auto exps_of = [&](int e) -> uint32_t {                         // (both exponents of the page in one load)
-    return __ldg(reinterpret_cast<const uint16_t*>(a.exps) + (size_t)inside(e) * a.H + kvh);
+  auto entry = [&](int i) {
+    int e = i + lane < my_count ? __ldg(my_table + (long long)(i + lane) * NW) : 0;
+    return e < 0 ? 0 : (int)min((long long)e, a.nblocks - 1);
+  };
+  auto factors = [&](int e) {                                     // (both exponents of the page in one load)
+    const uint32_t x = __ldg(reinterpret_cast<const uint16_t*>(a.exps) + (size_t)e * a.H + kvh);
+    return make_float2(a.scale_log2 * pow2i(page8_exp((int8_t)(x & 0xFF))), (float)page8_exp((int8_t)(x >> 8)));
   };
   int now = entry(0), next = entry(32);
-  uint32_t now_x = exps_of(now), next_x = 0;
-  auto fetch = [&](int i) {                                       // this warp's i-th page -> stage i % STG (whole warp, i in order)
+  float2 now_f = factors(now), next_f = now_f;
+  const uint8_t* const head_pages = a.kv + page8_off<D>(0, a.H, kvh, 0);
+  const size_t page_step = (size_t)a.H * PB;
+  auto fetch = [&](int i, int s) {                                // this warp's i-th page -> stage s (whole warp, i in order)
     if ((i & 31) == 0 && i > 0) {
       now = next;
-      now_x = next_x;
+      now_f = next_f;
       next = entry(i + 32);
     }
-    if ((i & 31) == 16) next_x = exps_of(next);
-    const long long blk = inside(__shfl_sync(FULL, now, i & 31));
-    const uint32_t x = __shfl_sync(FULL, now_x, i & 31);
-    const int s = i % STG;
+    if ((i & 31) == 16) next_f = factors(next);
+    const int blk = __shfl_sync(FULL, now, i & 31);
+    const float2 f = make_float2(__shfl_sync(FULL, now_f.x, i & 31), __shfl_sync(FULL, now_f.y, i & 31));
     if (elect_one()) {
-      my_exp[s] = x;
+      fac[s] = f;
       mbar_expect_tx(bar + s, PB);
-      bulk_g2s(ring + s * PB, a.kv + page8_off<D>(blk, a.H, kvh, 0), PB, bar + s, stream_policy);
+      bulk_g2s(ring + s * PB, head_pages + blk * page_step, PB, bar + s, stream_policy);
     }
   };
   __syncwarp();
-  for (int i = 0; i < min(my_count, STG); ++i) fetch(i);
 #pragma unroll
-  for (int k = 0; k < KT; ++k) {                                  // columns beyond the heads are zero
-    qf[k][0] = g < heads ? q_up(qf[k][0]) : 0u;
-    qf[k][1] = g < heads ? q_up(qf[k][1]) : 0u;
+  for (int i = 0; i < STG; ++i)
+    if (i < my_count) fetch(i, i);
+  // ---- q as FP16, head g times 2^(13 - exponent of its largest); columns beyond the heads are zero
+  float qs0, qs1;                                                 // what undoes it for this lane's score columns, heads 2t, 2t + 1
+  {
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) most = max(most, max(qf[k][i] << 16 & 0x7FFF0000u, qf[k][i] & 0x7FFF0000u));
+    most = max(most, __shfl_xor_sync(FULL, most, 1));
+    most = max(most, __shfl_xor_sync(FULL, most, 2));
+    const int e = q_exp(most);
+    const float down = pow2i(-e);
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        qf[k][i] = g < heads ? pack_f16(__uint_as_float(qf[k][i] << 16) * down, __uint_as_float(qf[k][i] & 0xFFFF0000u) * down) : 0u;
+    qs0 = pow2i(__shfl_sync(FULL, e, 8 * t));
+    qs1 = pow2i(__shfl_sync(FULL, e, 8 * t + 4));
   }
   const bool head0 = 2 * t < heads, head1 = 2 * t + 1 < heads;
-  float m0 = head0 ? -INFINITY : 0.f, m1 = head1 ? -INFINITY : 0.f, l0 = 0.f, l1 = 0.f;
+  float m0 = head0 ? -INFINITY : 1e30f, m1 = head1 ? -INFINITY : 1e30f, l0 = 0.f, l1 = 0.f;     // (no head: probabilities are 0)
   float acc[VT][4];                                               // MMA j: [0], [1] dim D/8 g + 2j, [2], [3] the next; heads 2t, 2t + 1
 #pragma unroll
   for (int j = 0; j < VT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
   bool gave_up = false;
   __syncwarp();
 
-  for (int i = 0; i < my_count; ++i) {
-    const int s = i % STG, page = my_first + i * NW;
-    if (!mbar_wait(bar + s, (uint32_t)(i / STG) & 1u)) {
+  int s = 0;
+  uint32_t phase = 0;
+  for (int i = 0, page = my_first; i < my_count; ++i, page += NW) {
+    if (!mbar_wait(bar + s, phase)) {
       if (lane == 0) atomicExch(status, ERR_WAIT_FULL);
       for (int k = i + 1; k < min(my_count, i + STG); ++k)        // let the copies still in flight land
         (void)mbar_wait(bar + k % STG, (uint32_t)(k / STG) & 1u);
@@ -489,8 +518,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
       break;
     }
     const uint8_t* const pg = ring + s * PB;
-    const uint32_t x = my_exp[s];
-    const int ek = page8_exp((int8_t)(x & 0xFF)), ev = page8_exp((int8_t)(x >> 8));
+    const float2 f = fac[s];
     float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int p = 0; p < D / 64; ++p) {
@@ -498,22 +526,22 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
       const uint4 u = *reinterpret_cast<const uint4*>(at), v = *reinterpret_cast<const uint4*>(at + 8 * D);
       const uint32_t wu[4] = {u.x, u.y, u.z, u.w}, wv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t a0, a1, a2, a3;
-        codes_to_bf16(wu[k], a0, a2);
-        codes_to_bf16(wv[k], a1, a3);
-        mma_bf16_r(k & 1 ? sd : sc, a0, a1, a2, a3, qf[4 * p + k][0], qf[4 * p + k][1]);
-      }
+      for (int k = 0; k < 4; ++k)
+        mma_f16(k & 1 ? sd : sc, f16_low(wu[k]), f16_low(wv[k]), f16_high(wu[k]), f16_high(wv[k]), qf[4 * p + k][0], qf[4 * p + k][1]);
     }
-    const float c = a.scale_log2 * pow2i(60 + ek);
-    const int tok = page * PAGE + g;
-    const bool v_lo = tok >= lo && tok < len, v_hi = tok + 8 >= lo && tok + 8 < len;
-    const float x00 = v_lo && head0 ? (sc[0] + sd[0]) * c : -INFINITY, x01 = v_lo && head1 ? (sc[1] + sd[1]) * c : -INFINITY;
-    const float x10 = v_hi && head0 ? (sc[2] + sd[2]) * c : -INFINITY, x11 = v_hi && head1 ? (sc[3] + sd[3]) * c : -INFINITY;
+    const float c0 = fminf(f.x * qs0, 3e38f), c1 = fminf(f.x * qs1, 3e38f);
+    float x00 = fmaf(sc[0] + sd[0], c0, f.y), x01 = fmaf(sc[1] + sd[1], c1, f.y);
+    float x10 = fmaf(sc[2] + sd[2], c0, f.y), x11 = fmaf(sc[3] + sd[3], c1, f.y);
+    const int t0 = page * PAGE;
+    if (t0 < lo || t0 + PAGE > len) {                             // an edge page: tokens outside [lo, len)
+      const int tok = t0 + g;
+      if (tok < lo || tok >= len) x00 = x01 = -INFINITY;
+      if (tok + 8 < lo || tok + 8 >= len) x10 = x11 = -INFINITY;
+    }
     const float top0 = fmaxf(x00, x10), top1 = fmaxf(x01, x11);
     if (__any_sync(FULL, top0 > m0 + RAISE8 || top1 > m1 + RAISE8)) {
       const float n0 = fmaxf(m0, over_rows_max(top0)), n1 = fmaxf(m1, over_rows_max(top1));
-      const float f0 = n0 == m0 ? 1.f : exp2f(m0 - n0), f1 = n1 == m1 ? 1.f : exp2f(m1 - n1);
+      const float f0 = n0 == m0 ? 1.f : ex2(m0 - n0), f1 = n1 == m1 ? 1.f : ex2(m1 - n1);
       l0 *= f0;
       l1 *= f1;
 #pragma unroll
@@ -521,11 +549,10 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
       m0 = n0;
       m1 = n1;
     }
-    const float p00 = exp2f(x00 - m0), p01 = exp2f(x01 - m1), p10 = exp2f(x10 - m0), p11 = exp2f(x11 - m1);
-    l0 += p00 + p10;
-    l1 += p01 + p11;
-    const float up = pow2i(60 + ev);
-    const uint32_t b0 = movmatrix_t(pack_bf16(p00 * up, p01 * up)), b1 = movmatrix_t(pack_bf16(p10 * up, p11 * up));
+    const float p00 = ex2(x00 - m0), p01 = ex2(x01 - m1), p10 = ex2(x10 - m0), p11 = ex2(x11 - m1), out = ex2(-f.y);
+    l0 = fmaf(p00 + p10, out, l0);
+    l1 = fmaf(p01 + p11, out, l1);
+    const uint32_t b0 = movmatrix_t(pack_f16(p00, p01)), b1 = movmatrix_t(pack_f16(p10, p11));
     const uint8_t* const vp = pg + PAGE * D;
     constexpr int WORDS = D / 32;                                 // of a lane's dims of one token: D / 8 codes
     uint32_t w[4][WORDS];
@@ -544,22 +571,24 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     for (int k = 0; k < WORDS; ++k)
 #pragma unroll
       for (int d = 0; d < 2; ++d) {                               // dims 4k + 2d, 4k + 2d + 1 of the lane
-        uint32_t a0, a1, a2, a3;
-        codes_to_bf16(__byte_perm(w[0][k], w[1][k], d ? 0x7362 : 0x5140), a0, a1);
-        codes_to_bf16(__byte_perm(w[2][k], w[3][k], d ? 0x7362 : 0x5140), a2, a3);
-        mma_bf16_r(acc[2 * k + d], a0, a1, a2, a3, b0, b1);
+        const uint32_t u = __byte_perm(w[0][k], w[1][k], d ? 0x7362 : 0x5140), v = __byte_perm(w[2][k], w[3][k], d ? 0x7362 : 0x5140);
+        mma_f16(acc[2 * k + d], f16_low(u), f16_high(u), f16_low(v), f16_high(v), b0, b1);
       }
     __syncwarp();                                                 // every lane has read this stage
     if (i + STG < my_count) {
       fence_proxy_async();
-      fetch(i + STG);
+      fetch(i + STG, s);
+    }
+    if (++s == STG) {
+      s = 0;
+      phase ^= 1u;
     }
   }
   if (gave_up) { m0 = head0 ? -INFINITY : 0.f; m1 = head1 ? -INFINITY : 0.f; l0 = l1 = 0.f; }
   l0 = over_rows_sum(l0);
   l1 = over_rows_sum(l1);
 
-  // ---- the CTA's warps together.  The rings are idle now; each warp parks (O^T, m, l) of its heads there.
+  // ---- the CTA's warps together.  The rings are idle now; each warp parks (O^T, M, l) of its heads there.
   __syncthreads();
   constexpr int ROW = D + 2, PER_WARP = 8 * ROW;
   static_assert(PER_WARP * 4 <= STG * PB, "parked partials must fit in the ring");
@@ -586,11 +615,10 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     for (int w = 0; w < NW; ++w) {
       const float* const pw = park + w * PER_WARP + h * ROW;
       if (pw[D] == -INFINITY) continue;                           // a warp without pages
-      const float f = exp2f(pw[D] - top);
+      const float f = ex2(pw[D] - top);
       den += f * pw[D + 1];
       num += f * pw[d];
     }
-    num *= 1152921504606846976.f;                                 // 2^60
     const int hq = first_head + h;
     if (parts.splits == 1) {
       const __nv_bfloat16 v = __float2bfloat16_rn(den > 0.f ? num / den : den);        // (a sum that is not a number stays one)
@@ -674,7 +702,7 @@ __global__ void __launch_bounds__(MERGE8 * 32) kv8_merge_kernel(const float* __r
 
 template <int D, int NW, int STG>
 int attn8_launch(const Attn8& a, const Parts8& parts, cudaStream_t st_) {
-  constexpr int smem = NW * STG * (2 * PAGE * D + 8 + 4);
+  constexpr int smem = NW * STG * (2 * PAGE * D + 8 + 8);
   static std::atomic<uint64_t> set{0};                            // devices whose limit has been raised
   int dev = 0;
   if (int e = st::cuda_fail(cudaGetDevice(&dev), "st_kv8_attn: device")) return e;

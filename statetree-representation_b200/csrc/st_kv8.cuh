@@ -45,6 +45,31 @@ __device__ __forceinline__ float2 codes_value(uint32_t p, float up) {      // up
   constexpr float C = 1.2676506002282294e30f;                             // 2^100
   return make_float2(__uint_as_float(p << 16) * C * up, __uint_as_float(p & 0xFFFF0000u) * C * up);
 }
+// two codes -> FP16, exact: the low and the high half of a word
+__device__ __forceinline__ uint32_t f16_low(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n cvt.rn.f16x2.e4m3x2 %0, l;\n}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16_high(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n cvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// 2^x, relative error below 2^-22, results below 2^-126 are 0
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// q * 2^-e has its largest magnitude (fp32 bits `most`) in [2^13, 2^14); 0 for zeros
+__device__ __forceinline__ int q_exp(uint32_t most) { return most < 0x00800000u ? 0 : min((int)(most >> 23) - 127, 126) - 13; }
+
 // q times 2^60, exactly (BF16 keeps its eight bits)
 __device__ __forceinline__ uint32_t q_up(uint32_t q) {
   const __nv_bfloat162 c = __floats2bfloat162_rn(1152921504606846976.f, 1152921504606846976.f);

@@ -99,11 +99,6 @@ template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
-__device__ __forceinline__ float ex2(float x) {                   // 2^x, relative error below 2^-22, results below 2^-126 are 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // What a CTA works on; the same in all of its threads
 struct Work {
