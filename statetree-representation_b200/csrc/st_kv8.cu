@@ -376,16 +376,15 @@ __global__ void __launch_bounds__(256) kv8_dequant_kernel(const uint8_t* __restr
 // integer operations each, and the integer pipe, 64 lanes a cycle and SM, was the limit: 64 sequences of up to 8192 tokens 118 us).
 // q is scaled by a power of two per head so that FP16 holds its eight bits (of values down to 2^-28 of the head's largest).  The
 // exponent of a page's keys joins the softmax scale.  That of its values joins the exponent of its probabilities: with x = score +
-// exponent (base 2) the running reference M bounds x, P = 2^(x - M) <= 2^8 is rounded to FP16 (2^-12 of each at most; what is below
-// 2^-25 of the largest contribution is lost), and the sum of the probabilities takes the exponent out again, per page, in fp32.
+// exponent (base 2) and a running reference r, P = 2^(x - r) <= 2^15 is rounded to FP16 (2^-11 of each at most, and 2^-32 of the
+// largest), and the sum of the probabilities takes the exponent out again, per page, in fp32.
 //
-// A head's reference M is raised when a page holds an x more than 8 above it: one vote per page, a rescale only then.
+// A head's reference r stays between 7 and 15 below its largest x so far: it is raised when a page holds an x more than 15 above it,
+// one vote per page, a rescale only then.
 //
 // Work split: grid = sequences x KV heads x head blocks x splits; a CTA's pages go round-robin to its warps, each of which streams its
 // own through a private ring of bulk copies (a page of one head is contiguous, 2 * 16 * D bytes), so there is no barrier in the loop.
 // Block-table entries and exponents come 32 pages at a time, one batch ahead.
-constexpr float RAISE8 = 8.f;
-
 __device__ __forceinline__ float over_rows_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
@@ -540,7 +539,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     }
     const float top0 = fmaxf(x00, x10), top1 = fmaxf(x01, x11);
     if (__any_sync(FULL, top0 > m0 + RAISE8 || top1 > m1 + RAISE8)) {
-      const float n0 = fmaxf(m0, over_rows_max(top0)), n1 = fmaxf(m1, over_rows_max(top1));
+      const float n0 = fmaxf(m0, over_rows_max(top0) - UNDER8), n1 = fmaxf(m1, over_rows_max(top1) - UNDER8);
       const float f0 = n0 == m0 ? 1.f : ex2(m0 - n0), f1 = n1 == m1 ? 1.f : ex2(m1 - n1);
       l0 *= f0;
       l1 *= f1;
@@ -588,7 +587,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
   l0 = over_rows_sum(l0);
   l1 = over_rows_sum(l1);
 
-  // ---- the CTA's warps together.  The rings are idle now; each warp parks (O^T, M, l) of its heads there.
+  // ---- the CTA's warps together.  The rings are idle now; each warp parks (O^T, r, l) of its heads there.
   __syncthreads();
   constexpr int ROW = D + 2, PER_WARP = 8 * ROW;
   static_assert(PER_WARP * 4 <= STG * PB, "parked partials must fit in the ring");

@@ -70,12 +70,8 @@ __device__ __forceinline__ float ex2(float x) {
 // q * 2^-e has its largest magnitude (fp32 bits `most`) in [2^13, 2^14); 0 for zeros
 __device__ __forceinline__ int q_exp(uint32_t most) { return most < 0x00800000u ? 0 : min((int)(most >> 23) - 127, 126) - 13; }
 
-// q times 2^60, exactly (BF16 keeps its eight bits)
-__device__ __forceinline__ uint32_t q_up(uint32_t q) {
-  const __nv_bfloat162 c = __floats2bfloat162_rn(1152921504606846976.f, 1152921504606846976.f);
-  const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&q), c);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
+// the reference that probabilities are relative to (base 2, P = 2^(x - r)): between UNDER8 and RAISE8 below the largest x
+constexpr float UNDER8 = 7.f, RAISE8 = 15.f;
 
 // ---- the attention's arguments
 struct Attn8 {
@@ -89,7 +85,7 @@ struct Attn8 {
   int B, Hq, H, window;
   long long T;
 };
-// partial results of sequences that are split: o [T, Hq, splits, D] (not normalised), ml [T, Hq, splits, 2] = (maximum, base 2; sum)
+// partial results of sequences that are split: o [T, Hq, splits, D] (not normalised), ml [T, Hq, splits, 2] = (reference, base 2; sum)
 struct Parts8 { float* o; float* ml; int splits, min_pages; };
 
 // st_kv8.cu: what both forms of the attention check and pass on; the join of the partial results

@@ -2,16 +2,17 @@
 //
 // A row is a (query token, head) pair of one KV head's group, so a CTA's 256 rows (two accumulator tiles of 128) are 256 / G
 // consecutive tokens of one sequence, whatever G is; keys come 128 at a time (eight pages):
-//     S = Q K^T   128 x 128, A and B from shared memory            P = exp2(S * c - m) in BF16, back into S's tensor-memory columns
+//     S = Q K^T   128 x 128, A and B from shared memory            P = exp2(S * c - m) in FP16, back into S's tensor-memory columns
 //     O += P V    128 x D, A = P from tensor memory, B = V from shared memory as it lies (dims contiguous: MN-major)
-// Warps: eight of softmax (a thread owns one row, so its maximum and sum need no other thread), four that turn codes into BF16 operand
+// Warps: eight of softmax (a thread owns one row, so its maximum and sum need no other thread), four that turn codes into FP16 operand
 // tiles, one that issues the MMAs.  While one tile's softmax runs, the tensor core works on the other's: S0 P0 S1 P1 ... in turn.
 // Tensor memory: S0, S1 (128 columns each; P takes the first 64 of its own), O0, O1 (D each).
 //
-// Codes reach the tensor core without a multiplication: BF16 patterns times 2^-120 (codes_split), q times 2^60, a page's key exponent in
-// the factor of its sixteen score columns, its value exponent (and 60) in the exponent of its sixteen columns of P.  The sum of the
-// probabilities takes the latter out again, per page.  All values are exact BF16 numbers, so the only roundings to fewer than 32 bits
-// are P (to BF16, 2^-9 of each probability at most) and the output.
+// Types and scales as in the decode kernel: e4m3 codes are FP16 numbers (one instruction converts two; as BF16 patterns the integer
+// operations of the converters were the limit beside the softmax), a row of q is scaled by a power of two so that FP16 holds its eight
+// bits, a page's key exponent is a factor of its sixteen score columns, its value exponent joins the softmax exponent of its sixteen
+// columns of P and is taken out of the sum per page.  P is rounded to FP16 (2^-11 of each at most, and 2^-32 of the largest), everything
+// else but the output is fp32.
 #include <math.h>
 
 #include <atomic>
@@ -27,7 +28,6 @@ using namespace st;
 constexpr int KEYS = 128, TILE_PAGES = KEYS / PAGE, ROWS = 128;
 constexpr int W_CONV = 8, W_MMA = 12, WARPS = 16;                 // softmax warps 0 .. 7 (tile = warp / 4); 13 .. 15 only lend registers
 constexpr int CRING = 4;                                          // page factors of so many key tiles are kept
-constexpr float LAZY = 8.f;                                       // a row's reference maximum is raised when a score exceeds it by this
 
 template <int D>
 struct Lay {                                                      // shared memory
@@ -215,19 +215,29 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     const bool any = __any_sync(FULL, live);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * D;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, q_up = 1.f;                     // q_up undoes the scale of q
     bool ok = true;
     if (count > 0) {
       uint8_t* const row = smem + L::Q + t * L::TILE + ((warp & 3) * 32 + lane) * 128;
       const uint4* const src = reinterpret_cast<const uint4*>(a.q + (long long)(w.first + token) * a.q_stride + (size_t)hq * D);
+      uint4 u[D / 8];
+      uint32_t most = 0;
 #pragma unroll
-      for (int u = 0; u < D / 8; ++u) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live) {
-          v = src[u];
-          v.x = q_up(v.x); v.y = q_up(v.y); v.z = q_up(v.z); v.w = q_up(v.w);
-        }
-        *reinterpret_cast<uint4*>(row + (u >> 3) * L::HALF + (((u & 7) ^ (lane & 7)) << 4)) = v;
+      for (int i = 0; i < D / 8; ++i) {
+        u[i] = live ? src[i] : make_uint4(0, 0, 0, 0);
+        const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) most = max(most, max(x[k] << 16 & 0x7FFF0000u, x[k] & 0x7FFF0000u));
+      }
+      const int e = q_exp(most);
+      const float down = pow2i(-e);
+      q_up = pow2i(e);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = pack_f16(__uint_as_float(x[k] << 16) * down, __uint_as_float(x[k] & 0xFFFF0000u) * down);
+        *reinterpret_cast<uint4*>(row + (i >> 3) * L::HALF + (((i & 7) ^ (lane & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
       }
       fence_proxy_async();
       __syncwarp();
@@ -248,9 +258,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
 #pragma unroll
           for (int k = 0; k < KEYS; ++k) v[k] = k < l0 || k > l1 ? 0xFF800000u : v[k];
         }
-        float top = -INFINITY;
+        float top = -INFINITY, by[TILE_PAGES];
 #pragma unroll
         for (int p = 0; p < TILE_PAGES; ++p) {
+          by[p] = fminf(fac[p] * q_up, 3e38f);
           float x[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) x[k] = __uint_as_float(v[16 * p + k]);
@@ -258,10 +269,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
           for (int o = 8; o; o >>= 1)
 #pragma unroll
             for (int k = 0; k < o; ++k) x[k] = fmaxf(x[k], x[k + o]);
-          top = fmaxf(top, x[0] * fac[p]);
+          top = fmaxf(top, fmaf(x[0], by[p], fac[TILE_PAGES + p]));
         }
-        if (__any_sync(FULL, top > m + LAZY)) {
-          const float up = fmaxf(m, top), f = up == m ? 1.f : ex2(m - up);
+        if (__any_sync(FULL, top > m + RAISE8)) {
+          const float up = fmaxf(m, top - UNDER8), f = up == m ? 1.f : ex2(m - up);
           m = up;
           l *= f;
           if (j > 0) {                                            // (O's product of the tile before has completed: sfull says so)
@@ -285,7 +296,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
           for (int p = 0; p < 2; ++p) {
             const int pg = 2 * q + p;
             const float add = fac[TILE_PAGES + pg] - ref;
-            const uint64_t by2 = pair2(fac[pg], fac[pg]), add2 = pair2(add, add);
+            const uint64_t by2 = pair2(by[pg], by[pg]), add2 = pair2(add, add);
             uint64_t sum = 0;
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
@@ -294,7 +305,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
               x0 = ex2(x0);
               x1 = ex2(x1);
               sum = add2f(sum, pair2(x0, x1));
-              pk[8 * p + k / 2] = pack_bf16(x0, x1);
+              pk[8 * p + k / 2] = pack_f16(x0, x1);
             }
             float s0, s1;
             unpair2(sum, s0, s1);
@@ -314,7 +325,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     if (ok && any) {
       tc_fence_after();
       const long long r = (long long)(w.first + token) * a.Hq + hq;
-      const float inv = c.parts.splits > 1 ? 1152921504606846976.f : (l > 0.f ? 1152921504606846976.f / l : l);
+      const float inv = c.parts.splits > 1 ? 1.f : (l > 0.f ? 1.f / l : l);
       if (live && c.parts.splits > 1) {
         float* const ml = c.parts.ml + (r * c.parts.splits + w.split) * 2;
         ml[0] = l > 0.f || l != l ? m : -INFINITY;
@@ -382,11 +393,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     auto convert = [&](const uint4 (&buf)[LOADS], uint8_t* tile) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        uint32_t o[8];
-        codes_to_bf16(buf[i].x, o[0], o[1]);
-        codes_to_bf16(buf[i].y, o[2], o[3]);
-        codes_to_bf16(buf[i].z, o[4], o[5]);
-        codes_to_bf16(buf[i].w, o[6], o[7]);
+        const uint32_t o[8] = {f16_low(buf[i].x), f16_high(buf[i].x), f16_low(buf[i].y), f16_high(buf[i].y),
+                               f16_low(buf[i].z), f16_high(buf[i].z), f16_low(buf[i].w), f16_high(buf[i].w)};
         uint8_t* const at = tile + to + (i * PAGES_A_LOAD + sub) * (PAGE * 128);
         *reinterpret_cast<uint4*>(at + u0) = make_uint4(o[0], o[1], o[2], o[3]);
         *reinterpret_cast<uint4*>(at + (u0 ^ 16)) = make_uint4(o[4], o[5], o[6], o[7]);
@@ -409,9 +417,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
       if (cw == 0 && lane < TILE_PAGES) {                         // factors of the tile's pages
         float* const fac = reinterpret_cast<float*>(smem + L::F) + (j % CRING) * (TILE_PAGES * 3) + lane;
         const int ek = page8_exp((int8_t)(x & 0xFF)), ev = page8_exp((int8_t)(x >> 8));
-        fac[0] = a.scale_log2 * pow2i(60 + ek);
-        fac[TILE_PAGES] = (float)(60 + ev);
-        fac[2 * TILE_PAGES] = pow2i(-60 - ev);
+        fac[0] = a.scale_log2 * pow2i(ek);
+        fac[TILE_PAGES] = (float)ev;
+        fac[2 * TILE_PAGES] = pow2i(-ev);
       }
       fence_proxy_async();
       __syncwarp();
@@ -434,7 +442,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     if (warp == W_MMA) {
     // ---------------------------------------------------------------- MMAs.  One thread's MMAs complete in the order of their issue
     // (and a commit covers all before it): S of the next key tile may take the place of the P that the product before it reads
-    constexpr uint32_t IDESC_S = mma_idesc(128, KEYS), IDESC_O = mma_idesc(128, D) | 1u << 16;
+    // (mma_idesc's operands are BF16; FP16 is type 0)
+    constexpr uint32_t FP16 = ~(1u << 7 | 1u << 10), IDESC_S = mma_idesc(128, KEYS) & FP16, IDESC_O = (mma_idesc(128, D) & FP16) | 1u << 16;
     const uint32_t sq = smem_addr(smem + L::Q), sk = smem_addr(smem + L::K), sv = smem_addr(smem + L::V);
     auto scores = [&](int t, int s) {
 #pragma unroll

@@ -88,6 +88,21 @@ def _rows(t, D):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def decode_splits8(units, max_pages, sms=148):
+    """How many CTAs share a unit (sequence, KV head, eight query heads) of the 8-bit decode attention, from what the host knows: the
+    number of units and the width of the block table.  Few units: one CTA of eight warps per SM (8 units of 16K tokens 10.7 us, twice
+    as many 11.1).  More: CTAs of four warps, four to an SM, so that sequences of different lengths even out (64 units of up to 16K
+    tokens, lengths spread: two splits 43.6 us, nine 29.2; all of the full length 44.6 and 50.4).  Below eight pages per split (16,
+    64 with more units) the join costs more than it gives (128 units of 1000 tokens: one 8.4 us, four 11.2)."""
+    if units <= sms // 8:
+        want, least = sms // max(1, units), 8
+    elif units <= 128:
+        want, least = min(9, 4 * sms // units), 8 if units < 32 else 16
+    else:
+        want, least = 4 if units <= 4 * sms else 2, 64
+    return max(1, min(want, max_pages // least, 64))
+
+
 class PageStore8:
     """Pages of one attention layer in 8 bits (256 B per token and head of dimension 128; a PageStore's take 400 and are lossless):
     pages uint8 [blocks, H, 2 (keys, values), 16, D] of e4m3 codes and exps int8 [blocks, H, 2], a value being e4m3(code) * 2^exp
@@ -139,7 +154,7 @@ class PageStore8:
         """one query token per sequence: q [B, Hq, D] bf16 -> [B, Hq, D] bf16; tokens [max(starts, lens - window), lens) take part
         (window 0: from starts on).  splits: how many CTAs share a sequence (None: by batch size and table width)"""
         if splits is None:
-            splits = decode_splits(q.shape[0], self.H, block_table.shape[1])
+            splits = decode_splits8(block_table.shape[0] * self.H * -(-q.shape[1] // (8 * self.H)), block_table.shape[1])
         host = calls()
         if host is not None:
             done = host[0].kv8_attention(host[1], False, self.pages, self.exps, q, None, block_table, lens, scale, splits, starts, min_pages,
