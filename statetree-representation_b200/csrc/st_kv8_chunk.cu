@@ -42,15 +42,25 @@ struct Lay {                                                      // shared memo
 
 struct Chunk8 { Attn8 a; Parts8 parts; int* status; int slots; };
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-               :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// Shared-memory operands.  Descriptor: address / 16 and the stride of the leading dimension / 16 in the low word; in the high one the
+// stride of 8-row groups (1024 B), the version and the 128-byte swizzle, the same for all of them.  So the issuing thread keeps the low
+// words and adds to them (with whole descriptors formed at every MMA the issue took as long as the MMAs).
+//   K-major (Q, K: a row holds 64 values of the contracted dimension)   leading stride unused
+//   MN-major (V: a row, one key, holds 64 values of the other one)       the next 64 values `next` bytes further
+constexpr uint32_t DESC_HI = 64u | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_k(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4 | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t saddr, uint32_t next) { return (saddr & 0x3FFFFu) >> 4 | (next >> 4) << 16; }
+// D (+)= A B^T, A from shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}"
+               :: "r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(DESC_HI) : "memory");
 }
-// operand whose rows (k) hold 64 contiguous values of the other dimension, 128-byte swizzle: 8-row groups 1024 B apart, the next 64
-// values `next` bytes further
-__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t next) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)2 << 61);
+// the same, A from tensor memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}"
+               :: "r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(DESC_HI) : "memory");
 }
 #define ST_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
 #define ST_I4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
@@ -444,75 +454,66 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     // (and a commit covers all before it): S of the next key tile may take the place of the P that the product before it reads
     // (mma_idesc's operands are BF16; FP16 is type 0)
     constexpr uint32_t FP16 = ~(1u << 7 | 1u << 10), IDESC_S = mma_idesc(128, KEYS) & FP16, IDESC_O = (mma_idesc(128, D) & FP16) | 1u << 16;
-    const uint32_t sq = smem_addr(smem + L::Q), sk = smem_addr(smem + L::K), sv = smem_addr(smem + L::V);
-    auto scores = [&](int t, int s) {
+    // The whole loop runs in one elected thread, waits included: a warp that meets again around each step costs more than the steps
+    if (elect_one()) {
+      const uint32_t dq = desc_k(smem_addr(smem + L::Q)), dk = desc_k(smem_addr(smem + L::K)), dv = desc_mn(smem_addr(smem + L::V), L::HALF);
+      auto scores = [&](int t, int s) {
+        const uint32_t q = dq + t * (L::TILE >> 4), k = dk + s * (L::TILE >> 4);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t at = (uint32_t)((k >> 2) * L::HALF);
-        mma_ss(tmem + t * 128, smem_desc_sw128(sq + t * L::TILE + at) + 2 * (k & 3), smem_desc_sw128(sk + s * L::TILE + at) + 2 * (k & 3),
-               IDESC_S, k > 0);
-      }
-    };
-    auto outputs = [&](int t, int s, bool more) {
-#pragma unroll
-      for (int k = 0; k < KEYS / 16; ++k)
-        tc_mma<1>(tmem + 256 + t * D, tmem + t * 128 + 8 * k, desc_mn(sv + s * L::TILE + k * 2048, L::HALF), IDESC_O, more || k > 0);
-    };
-    bool ok = true;
-    if (tiles > 0) {
-      ok = mbar_wait(kfull, 0);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (ok && (t ? w.count1 : w.count0) > 0) {
-          ok = mbar_wait(qfull + t, 0);
-          tc_fence_after();
-          if (ok && elect_one()) {
-            scores(t, 0);
-            tc_commit(sfull + t);
-          }
-          __syncwarp();
+        for (int i = 0; i < D / 16; ++i) {
+          const uint32_t at = (i >> 2) * (L::HALF >> 4) + 2 * (i & 3);
+          mma_ss(tmem + t * 128, q + at, k + at, IDESC_S, i > 0);
         }
-      if (elect_one()) tc_commit(kempty);
-      __syncwarp();
-    }
-    for (int j = 0; ok && j < tiles; ++j) {
-      const int s = j & 1, s1 = s ^ 1;
-      const bool both = j < w.count0 && j < w.count1;
-      ok = mbar_wait(vfull + s, (uint32_t)(j >> 1) & 1u);
+        tc_commit(sfull + t);
+      };
+      auto outputs = [&](int t, int s, bool more) {
+        const uint32_t v = dv + s * (L::TILE >> 4);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int count = t ? w.count1 : w.count0;
-        if (!ok || j >= count) continue;
-        const bool next = j + 1 < count;
-        ok = mbar_wait(pfull + t, (uint32_t)j & 1u);
-        tc_fence_after();
-        if (ok && elect_one()) {
+        for (int i = 0; i < KEYS / 16; ++i) mma_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * i, v + i * (2048 >> 4), IDESC_O, more || i > 0);
+      };
+      bool ok = true;
+      if (tiles > 0) {
+        ok = mbar_wait(kfull, 0);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && (t ? w.count1 : w.count0) > 0) {
+            ok = mbar_wait(qfull + t, 0);
+            tc_fence_after();
+            if (ok) scores(t, 0);
+          }
+        tc_commit(kempty);
+      }
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int s = j & 1, s1 = s ^ 1;
+        const bool both = j < w.count0 && j < w.count1;
+        ok = mbar_wait(vfull + s, (uint32_t)(j >> 1) & 1u);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int count = t ? w.count1 : w.count0;
+          if (!ok || j >= count) continue;
+          ok = mbar_wait(pfull + t, (uint32_t)j & 1u);
+          if (!ok) continue;
+          tc_fence_after();
           outputs(t, s, j > 0);
           if (t == 1 || !both) tc_commit(vempty + s);
-          if (!next) tc_commit(ofull + t);
-        }
-        __syncwarp();
-        if (ok && next) {
-          ok = mbar_wait(kfull + s1, (uint32_t)((j + 1) >> 1) & 1u);
-          tc_fence_after();
-          if (ok && elect_one()) {
+          if (j + 1 < count) {
+            ok = mbar_wait(kfull + s1, (uint32_t)((j + 1) >> 1) & 1u);
+            if (!ok) continue;
+            tc_fence_after();
             scores(t, s1);
-            tc_commit(sfull + t);
+          } else {
+            tc_commit(ofull + t);
           }
-          __syncwarp();
         }
+        if (ok && j + 1 < tiles) tc_commit(kempty + s1);
       }
-      if (ok && j + 1 < tiles) {
-        if (elect_one()) tc_commit(kempty + s1);
-        __syncwarp();
+      if (!ok) {                                                  // (gave up: let what was issued complete before the memory goes)
+        atomicExch(c.status, ERR_WAIT_MMA);
+        tc_commit(drain);
+        (void)mbar_wait(drain, 0);
       }
     }
-    if (!ok) {                                                    // (gave up: let what was issued complete before the memory goes)
-      if (lane == 0) atomicExch(c.status, ERR_WAIT_MMA);
-      if (elect_one()) tc_commit(drain);
-      __syncwarp();
-      (void)mbar_wait(drain, 0);
-    }
+    __syncwarp();
     tc_fence_before();
     }
   }
