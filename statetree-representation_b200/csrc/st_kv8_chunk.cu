@@ -4,8 +4,8 @@
 // consecutive tokens of one sequence, whatever G is; keys come 128 at a time (eight pages):
 //     S = Q K^T   128 x 128, A and B from shared memory            P = exp2(S * c - m) in FP16, back into S's tensor-memory columns
 //     O += P V    128 x D, A = P from tensor memory, B = V from shared memory as it lies (dims contiguous: MN-major)
-// Warps: eight of softmax (a thread owns one row, so its maximum and sum need no other thread), four that turn codes into FP16 operand
-// tiles, one that issues the MMAs.  While one tile's softmax runs, the tensor core works on the other's: S0 P0 S1 P1 ... in turn.
+// Warps: eight of softmax (a thread owns one row, so its maximum and sum need no other thread), four that bring pages into shared memory
+// by bulk copies and turn their codes into FP16 operand tiles, one that issues the MMAs.  While one tile's softmax runs, the tensor core works on the other's: S0 P0 S1 P1 ... in turn.
 // Tensor memory: S0, S1 (128 columns each; P takes the first 64 of its own), O0, O1 (D each).
 //
 // Types and scales as in the decode kernel: e4m3 codes are FP16 numbers (one instruction converts two; as BF16 patterns the integer
@@ -33,9 +33,10 @@ template <int D>
 struct Lay {                                                      // shared memory
   static constexpr int HALF = 128 * 128;                          // 128 rows x 64 BF16, 128-byte swizzle
   static constexpr int TILE = D / 64 * HALF;
-  static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, F = 6 * TILE;      // two tiles of Q, two stages of K and V
-  static constexpr int BARS = F + CRING * TILE_PAGES * 3 * 4;
-  static constexpr int NBARS = 17, SLOT = BARS + NBARS * 8;
+  static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE;         // two tiles of Q, two stages of K and V
+  static constexpr int RAW = 6 * TILE, UNIT = PAGE * D;           // codes of one key tile: its keys, its values
+  static constexpr int F = RAW + 2 * TILE_PAGES * UNIT, BARS = F + CRING * TILE_PAGES * 3 * 4;
+  static constexpr int NBARS = 23, SLOT = BARS + NBARS * 8;
   // (more than half of an SM's shared memory: one CTA per SM, which holds all of its tensor memory)
   static constexpr int BYTES = (SLOT + 16 > 120 * 1024 ? SLOT + 16 : 120 * 1024) + 1024;
 };
@@ -158,8 +159,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  uint64_t *const qfull = bars, *const kfull = bars + 2, *const kempty = bars + 4, *const vfull = bars + 6, *const vempty = bars + 8,
-           *const sfull = bars + 10, *const pfull = bars + 12, *const ofull = bars + 14, *const drain = bars + 16;
+  uint64_t *const qfull = bars, *const kfull = bars + 2, *const vfull = bars + 4, *const sfull = bars + 6, *const pfull = bars + 8,
+           *const ofull = bars + 10, *const empty = bars + 12, *const raw = bars + 14;           // raw: [converter warp][keys, values]
+  uint64_t* const drain = bars + 22;
   uint32_t* const slot_at = reinterpret_cast<uint32_t*>(smem + L::SLOT);
   const Attn8& a = c.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.Hq / a.H;
@@ -189,19 +191,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     w.count1 = w.rows > ROWS ? w.tiles : 0;
   }
   const int tiles = max(w.count0, w.count1);
+  // (pages behind the last key of the sequence may not exist: no key of theirs is seen)
+  const int end_page = (int)min((long long)(w.pos0 + w.n - 1) / PAGE + 1, a.table_stride);
+  const uint64_t keep = policy_evict_last();                      // other row tiles of the sequence read the same pages
 
   if (warp == W_MMA) {
     if (elect_one()) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(qfull + i, 4);
         mbar_init(kfull + i, 4);
-        mbar_init(kempty + i, 1);
         mbar_init(vfull + i, 4);
-        mbar_init(vempty + i, 1);
         mbar_init(sfull + i, 1);
         mbar_init(pfull + i, 4);
         mbar_init(ofull + i, 1);
+        mbar_init(empty + i, 1);
       }
+      for (int i = 0; i < 8; ++i) mbar_init(raw + i, 1);
       mbar_init(drain, 1);
       fence_barrier_init();
     }
@@ -254,7 +259,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
       if (lane == 0) mbar_arrive(qfull + t);
     }
     for (int j = 0; j < count; ++j) {
-      if (!mbar_wait(sfull + t, (uint32_t)j & 1u)) { ok = false; break; }
+      if (!mbar_wait_look(sfull + t, (uint32_t)j & 1u)) { ok = false; break; }
       tc_fence_after();
       if (any) {
         const float* const fac = reinterpret_cast<const float*>(smem + L::F) + (j % CRING) * (TILE_PAGES * 3);
@@ -370,83 +375,113 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     tc_fence_before();
   } else if (warp < W_MMA) {
     regs_down<R_CONV>();
-    // ---------------------------------------------------------------- converters: codes -> operand tiles.  A lane's 16-byte piece
-    // becomes two of a tile row; eight lanes store four pieces of an even row and four of the next, so that with the swizzle they
-    // meet every bank once, and a warp reads whole rows
-    constexpr int LOADS = KEYS * D / 16 / 128, PAGES_A_LOAD = TILE_PAGES / LOADS;
+    // ---------------------------------------------------------------- converters: codes -> operand tiles.  A warp brings in and
+    // converts pages cw and cw + 4 of every key tile by itself: a bulk copy per page of keys or values, the next one under way as soon as
+    // this one is in registers.  (Plain loads in flight would be waited for by the proxy fence behind every tile: 1000 cycles each.)  A
+    // lane's 16-byte piece becomes two of a tile row; eight lanes read four pieces of an even row and four of the next, and store them
+    // so, which with the page's order of pieces and the tiles' swizzle meets every bank once.
+    constexpr int STEP = 512 / D, STEPS = PAGE / STEP;            // rows of a page that a warp takes at once
     const int cw = warp - W_CONV;
-    const int r = D == 128 ? cw * 4 + 2 * (lane >> 4) + ((lane >> 2) & 1) : (cw & 1) * 8 + (lane >> 2);
+    const int r = D == 128 ? 2 * (lane >> 4) + ((lane >> 2) & 1) : lane >> 2;
     const int lc = D == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
-    const int sub = D == 128 ? 0 : cw >> 1;                       // page of the load
-    const uint32_t from = (uint32_t)(r * D + 16 * piece8<D>(r, lc));
-    const uint32_t to = (uint32_t)((lc >> 2) * L::HALF + r * 128), u0 = (uint32_t)((((lc & 3) * 2) ^ (r & 7)) << 4);
+    uint8_t* const mine = smem + L::RAW + cw * (4 * L::UNIT);     // [keys, values][page cw, page cw + 4]
+    uint64_t* const my_raw = raw + 2 * cw;
+    const uint8_t* const head_pages = a.kv + page8_off<D>(0, a.H, w.h, 0);
+    const size_t page_step = (size_t)a.H * (2 * L::UNIT);
     const int* const table = a.table + (long long)w.b * a.table_stride;
-    // (pages behind the last key of the tile's rows may not exist: no key of theirs is seen)
-    const int end_page = (int)min((long long)(w.pos0 + w.n - 1) / PAGE + 1, a.table_stride);
-    auto page_of = [&](int j) {                                   // lane p < 8: page p of key tile j, -1 = none
-      const int p = (w.first_tile + j) * TILE_PAGES + lane;
-      int e = -1;
-      if (lane < TILE_PAGES && j < tiles && p < end_page) {
-        e = __ldg(table + p);
-        e = e < 0 ? 0 : (e >= a.nblocks ? (int)a.nblocks - 1 : e);
-      }
-      return e;
-    };
-    auto load = [&](int pages, int kvi, uint4 (&buf)[LOADS]) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int e = __shfl_sync(FULL, pages, i * PAGES_A_LOAD + sub);
-        buf[i] = make_uint4(0, 0, 0, 0);
-        if (e >= 0) buf[i] = __ldg(reinterpret_cast<const uint4*>(a.kv + page8_off<D>(e, a.H, w.h, kvi) + from));
-      }
-    };
-    auto convert = [&](const uint4 (&buf)[LOADS], uint8_t* tile) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const uint32_t o[8] = {f16_low(buf[i].x), f16_high(buf[i].x), f16_low(buf[i].y), f16_high(buf[i].y),
-                               f16_low(buf[i].z), f16_high(buf[i].z), f16_low(buf[i].w), f16_high(buf[i].w)};
-        uint8_t* const at = tile + to + (i * PAGES_A_LOAD + sub) * (PAGE * 128);
-        *reinterpret_cast<uint4*>(at + u0) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(at + (u0 ^ 16)) = make_uint4(o[4], o[5], o[6], o[7]);
-      }
+    // lane l holds entry and exponents of page cw + 4 (l % 2) of the sixteen key tiles' (l / 2)-th; the next sixteen are requested
+    // half way; -1 = there is no such page
+    auto entry = [&](int j) {
+      const int t = j + (lane >> 1), p = (w.first_tile + t) * TILE_PAGES + cw + 4 * (lane & 1);
+      if (t >= tiles || p >= end_page) return -1;
+      const int e = __ldg(table + p);
+      return e < 0 ? 0 : (int)min((long long)e, a.nblocks - 1);
     };
     auto exps_of = [&](int e) -> uint32_t {
       return e >= 0 ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(a.exps) + (size_t)e * a.H + w.h) : 0u;
     };
-    uint4 kb[LOADS], vb[LOADS];
-    int pages = page_of(0), after = page_of(1);
-    uint32_t x = cw == 0 ? exps_of(pages) : 0u;
-    load(pages, 0, kb);
-    load(pages, 1, vb);
+    int now = entry(0), next = -1;
+    uint32_t now_x = exps_of(now), next_x = 0;
+    auto fetch = [&](int j, int kvi, int e) {                     // e: the entries of tile j's sixteen
+      const int e0 = __shfl_sync(FULL, e, 2 * (j & 15)), e1 = __shfl_sync(FULL, e, 2 * (j & 15) + 1);
+      uint8_t* const to = mine + kvi * (2 * L::UNIT);
+      if (elect_one()) {
+        mbar_expect_tx(my_raw + kvi, (uint32_t)(((e0 >= 0) + (e1 >= 0)) * L::UNIT));
+        if (e0 >= 0) bulk_g2s(to, head_pages + e0 * page_step + kvi * L::UNIT, L::UNIT, my_raw + kvi, keep);
+        if (e1 >= 0) bulk_g2s(to + L::UNIT, head_pages + e1 * page_step + kvi * L::UNIT, L::UNIT, my_raw + kvi, keep);
+      }
+      __syncwarp();
+    };
+    if (tiles > 0) {
+      fetch(0, 0, now);
+      fetch(0, 1, now);
+    }
     bool ok = true;
-    for (int j = 0; j < tiles; ++j) {
-      const int s = j & 1;
-      if (j > 1) ok = mbar_wait(kempty + s, (uint32_t)((j >> 1) - 1) & 1u);
-      if (!ok) break;
-      convert(kb, smem + L::K + s * L::TILE);
-      if (cw == 0 && lane < TILE_PAGES) {                         // factors of the tile's pages
-        float* const fac = reinterpret_cast<float*>(smem + L::F) + (j % CRING) * (TILE_PAGES * 3) + lane;
+    for (int j = 0; ok && j < tiles; ++j) {
+      const int s = j & 1, at = 2 * (j & 15);
+      if ((j & 15) == 4) next = entry((j & ~15) + 16);
+      if ((j & 15) == 12) next_x = exps_of(next);
+      const int ahead = (j & 15) == 15 ? next : now;
+      const int have[2] = {__shfl_sync(FULL, now, at), __shfl_sync(FULL, now, at + 1)};
+      const uint32_t x0 = __shfl_sync(FULL, now_x, at), x1 = __shfl_sync(FULL, now_x, at + 1);
+      if (lane < 2) {                                             // factors of the two pages
+        float* const fac = reinterpret_cast<float*>(smem + L::F) + (j % CRING) * (TILE_PAGES * 3) + cw + 4 * lane;
+        const uint32_t x = lane ? x1 : x0;
         const int ek = page8_exp((int8_t)(x & 0xFF)), ev = page8_exp((int8_t)(x >> 8));
         fac[0] = a.scale_log2 * pow2i(ek);
         fac[TILE_PAGES] = (float)ev;
         fac[2 * TILE_PAGES] = pow2i(-ev);
       }
-      fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(kfull + s);
-      pages = after;
-      load(pages, 0, kb);
-      if (cw == 0) x = exps_of(pages);
-      after = page_of(j + 2);
-      if (j > 1) ok = mbar_wait(vempty + s, (uint32_t)((j >> 1) - 1) & 1u);
-      if (!ok) break;
-      convert(vb, smem + L::V + s * L::TILE);
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(vfull + s);
-      load(pages, 1, vb);
+#pragma unroll
+      for (int kvi = 0; kvi < 2; ++kvi) {
+        if (ok) ok = mbar_wait_look(my_raw + kvi, (uint32_t)j & 1u);
+        if (!ok) break;
+        uint4 buf[2][STEPS];
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) {
+            const int row = STEP * i + r;
+            buf[p][i] = make_uint4(0, 0, 0, 0);                   // (a page that is not there: zeros)
+            if (have[p] >= 0) buf[p][i] = *reinterpret_cast<const uint4*>(mine + (2 * kvi + p) * L::UNIT + row * D + 16 * piece8<D>(row, lc));
+          }
+        __syncwarp();
+        if (j + 1 < tiles) {
+          fence_proxy_async();
+          fetch(j + 1, kvi, ahead);
+        }
+        // K's stage is free when the scores of tile j - 2 are, V's when its products are: see the commits of the MMA loop
+        const int e = kvi ? j - 1 : j - 2;
+        if (j > 1) ok = mbar_wait_look(empty + (e & 1), (uint32_t)(e >> 1) & 1u);
+        if (!ok) break;
+        uint8_t* const tile = smem + (kvi ? L::V : L::K) + s * L::TILE + (lc >> 2) * L::HALF;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) {
+            const uint4 u = buf[p][i];
+            const uint32_t o[8] = {f16_low(u.x), f16_high(u.x), f16_low(u.y), f16_high(u.y),
+                                   f16_low(u.z), f16_high(u.z), f16_low(u.w), f16_high(u.w)};
+            const int row = (cw + 4 * p) * PAGE + STEP * i + r;
+            const uint32_t u0 = (uint32_t)((((lc & 3) * 2) ^ (row & 7)) << 4);
+            uint8_t* const to = tile + row * 128;
+            *reinterpret_cast<uint4*>(to + u0) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(to + (u0 ^ 16)) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive((kvi ? vfull : kfull) + s);
+      }
+      if ((j & 15) == 15) {
+        now = next;
+        now_x = next_x;
+      }
     }
-    if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_EMPTY);
+    if (!ok) {
+      if (lane == 0) atomicExch(c.status, ERR_WAIT_EMPTY);
+      for (int i = 0; i < 4; ++i) (void)mbar_wait(my_raw + (i >> 1), (uint32_t)i & 1u);      // (copies in flight land before the CTA ends)
+    }
   } else {
     regs_down<R_MMA>();
     if (warp == W_MMA) {
@@ -471,6 +506,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
 #pragma unroll
         for (int i = 0; i < KEYS / 16; ++i) mma_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * i, v + i * (2048 >> 4), IDESC_O, more || i > 0);
       };
+      // Three commits a key tile (each waits for the one before it): the scores of either row tile, and `empty`, behind the first
+      // product of tile j, which says that the scores of tile j and the products of tile j - 1 are done: K(j) and V(j - 1) are free
       bool ok = true;
       if (tiles > 0) {
         ok = mbar_wait(kfull, 0);
@@ -481,23 +518,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
             tc_fence_after();
             if (ok) scores(t, 0);
           }
-        tc_commit(kempty);
       }
       for (int j = 0; ok && j < tiles; ++j) {
         const int s = j & 1, s1 = s ^ 1;
-        const bool both = j < w.count0 && j < w.count1;
-        ok = mbar_wait(vfull + s, (uint32_t)(j >> 1) & 1u);
+        ok = mbar_wait_look(vfull + s, (uint32_t)(j >> 1) & 1u);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int count = t ? w.count1 : w.count0;
           if (!ok || j >= count) continue;
-          ok = mbar_wait(pfull + t, (uint32_t)j & 1u);
+          ok = mbar_wait_look(pfull + t, (uint32_t)j & 1u);
           if (!ok) continue;
           tc_fence_after();
           outputs(t, s, j > 0);
-          if (t == 1 || !both) tc_commit(vempty + s);
+          if (t == 0 || j >= w.count0) tc_commit(empty + s);
           if (j + 1 < count) {
-            ok = mbar_wait(kfull + s1, (uint32_t)((j + 1) >> 1) & 1u);
+            ok = mbar_wait_look(kfull + s1, (uint32_t)((j + 1) >> 1) & 1u);
             if (!ok) continue;
             tc_fence_after();
             scores(t, s1);
@@ -505,7 +540,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
             tc_commit(ofull + t);
           }
         }
-        if (ok && j + 1 < tiles) tc_commit(kempty + s1);
       }
       if (!ok) {                                                  // (gave up: let what was issued complete before the memory goes)
         atomicExch(c.status, ERR_WAIT_MMA);
