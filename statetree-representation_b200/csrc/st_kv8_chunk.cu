@@ -36,7 +36,7 @@ struct Lay {                                                      // shared memo
   static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE;         // two tiles of Q, two stages of K and V
   static constexpr int RAW = 6 * TILE, UNIT = PAGE * D;           // codes of one key tile: its keys, its values
   static constexpr int F = RAW + 2 * TILE_PAGES * UNIT, BARS = F + CRING * TILE_PAGES * 3 * 4;
-  static constexpr int NBARS = 23, SLOT = BARS + NBARS * 8;
+  static constexpr int NBARS = 25, SLOT = BARS + NBARS * 8;
   // (more than half of an SM's shared memory: one CTA per SM, which holds all of its tensor memory)
   static constexpr int BYTES = (SLOT + 16 > 120 * 1024 ? SLOT + 16 : 120 * 1024) + 1024;
 };
@@ -91,6 +91,11 @@ __device__ __forceinline__ void unpair2(uint64_t p, float& x, float& y) { asm("m
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ uint64_t add2f(uint64_t a, uint64_t b) {
@@ -160,8 +165,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
   uint64_t *const qfull = bars, *const kfull = bars + 2, *const vfull = bars + 4, *const sfull = bars + 6, *const pfull = bars + 8,
-           *const ofull = bars + 10, *const empty = bars + 12, *const raw = bars + 14;           // raw: [converter warp][keys, values]
-  uint64_t* const drain = bars + 22;
+           *const ofull = bars + 12, *const empty = bars + 14, *const raw = bars + 16;           // pfull: [half of the keys][row tile]
+  uint64_t* const drain = bars + 24;                              // raw: [converter warp][keys, values]
   uint32_t* const slot_at = reinterpret_cast<uint32_t*>(smem + L::SLOT);
   const Attn8& a = c.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.Hq / a.H;
@@ -203,6 +208,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
         mbar_init(vfull + i, 4);
         mbar_init(sfull + i, 1);
         mbar_init(pfull + i, 4);
+        mbar_init(pfull + 2 + i, 4);
         mbar_init(ofull + i, 1);
         mbar_init(empty + i, 1);
       }
@@ -258,7 +264,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
       __syncwarp();
       if (lane == 0) mbar_arrive(qfull + t);
     }
-    for (int j = 0; j < count; ++j) {
+    // The second row tile begins when the first has its first P: from then on each has the special function units to itself while the
+    // other's products run
+    if (t == 1 && count > 0 && w.count0 > 0) ok = mbar_wait(pfull + 2, 0);
+    for (int j = 0; ok && j < count; ++j) {
       if (!mbar_wait_look(sfull + t, (uint32_t)j & 1u)) { ok = false; break; }
       tc_fence_after();
       if (any) {
@@ -277,14 +286,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
 #pragma unroll
         for (int p = 0; p < TILE_PAGES; ++p) {
           by[p] = fminf(fac[p] * q_up, 3e38f);
-          float x[16];
+          float x = max3(__uint_as_float(v[16 * p]), __uint_as_float(v[16 * p + 1]), __uint_as_float(v[16 * p + 2]));
+          float y = max3(__uint_as_float(v[16 * p + 3]), __uint_as_float(v[16 * p + 4]), __uint_as_float(v[16 * p + 5]));
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[k] = __uint_as_float(v[16 * p + k]);
-#pragma unroll
-          for (int o = 8; o; o >>= 1)
-#pragma unroll
-            for (int k = 0; k < o; ++k) x[k] = fmaxf(x[k], x[k + o]);
-          top = fmaxf(top, fmaf(x[0], by[p], fac[TILE_PAGES + p]));
+          for (int k = 6; k < 14; k += 4) {
+            x = max3(x, __uint_as_float(v[16 * p + k]), __uint_as_float(v[16 * p + k + 1]));
+            y = max3(y, __uint_as_float(v[16 * p + k + 2]), __uint_as_float(v[16 * p + k + 3]));
+          }
+          x = max3(x, __uint_as_float(v[16 * p + 14]), __uint_as_float(v[16 * p + 15]));
+          top = fmaxf(top, fmaf(fmaxf(x, y), by[p], fac[TILE_PAGES + p]));
         }
         if (__any_sync(FULL, top > m + RAISE8)) {
           const float up = fmaxf(m, top - UNDER8), f = up == m ? 1.f : ex2(m - up);
@@ -327,12 +337,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
             l = fmaf(s0 + s1, fac[2 * TILE_PAGES + pg], l);
           }
           tm_st16(ts + 16 * q, pk);
+          if (q == 1) {                                           // the product with the first 64 keys need not wait for the others
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pfull + t);
+          }
         }
         tmem_wait_st();
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(pfull + t);
+      if (lane == 0) {
+        if (!any) mbar_arrive(pfull + t);
+        mbar_arrive(pfull + 2 + t);
+      }
     }
     if (ok && count > 0) ok = mbar_wait(ofull + t, 0);
     if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_ACC);
@@ -501,10 +520,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
         }
         tc_commit(sfull + t);
       };
-      auto outputs = [&](int t, int s, bool more) {
+      auto outputs = [&](int t, int s, int half, bool more) {
         const uint32_t v = dv + s * (L::TILE >> 4);
 #pragma unroll
-        for (int i = 0; i < KEYS / 16; ++i) mma_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * i, v + i * (2048 >> 4), IDESC_O, more || i > 0);
+        for (int k = 0; k < KEYS / 32; ++k) {
+          const int i = half * (KEYS / 32) + k;
+          mma_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * i, v + i * (2048 >> 4), IDESC_O, more || i > 0);
+        }
       };
       // Three commits a key tile (each waits for the one before it): the scores of either row tile, and `empty`, behind the first
       // product of tile j, which says that the scores of tile j and the products of tile j - 1 are done: K(j) and V(j - 1) are free
@@ -529,7 +551,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
           ok = mbar_wait_look(pfull + t, (uint32_t)j & 1u);
           if (!ok) continue;
           tc_fence_after();
-          outputs(t, s, j > 0);
+          outputs(t, s, 0, j > 0);
+          ok = mbar_wait_look(pfull + 2 + t, (uint32_t)j & 1u);
+          if (!ok) continue;
+          tc_fence_after();
+          outputs(t, s, 1, true);
           if (t == 0 || j >= w.count0) tc_commit(empty + s);
           if (j + 1 < count) {
             ok = mbar_wait_look(kfull + s1, (uint32_t)((j + 1) >> 1) & 1u);
