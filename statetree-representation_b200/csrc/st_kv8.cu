@@ -400,7 +400,9 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int D, int NW, int STG>
+// CHUNK: several queries per sequence.  The eight columns are then rows (query, head) of the sequence's n * G, each with keys of its own
+// [lo, hi], and a tile of eight of them is looked up as in the chunk kernel; else they are heads of the one query.
+template <int D, int NW, int STG, bool CHUNK>
 __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 a, const Parts8 parts, int* status) {
   constexpr int PB = 2 * PAGE * D, KT = D / 16, VT = D / 16;             // bytes of a page, MMAs of its keys and of its values
   extern __shared__ __align__(128) uint8_t smem[];
@@ -410,10 +412,28 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
   const int G = a.Hq / a.H, blocks_of_heads = (G + 7) / 8;
   const int split = blockIdx.x % parts.splits;
   int rest = blockIdx.x / parts.splits;
-  const int hb = rest % blocks_of_heads;
-  rest /= blocks_of_heads;
-  const int kvh = rest % a.H, seq = rest / a.H;
-  const int heads = min(8, G - 8 * hb), first_head = kvh * G + 8 * hb;
+  int kvh, seq, heads, first_head, first_row = 0;                 // heads: columns in use
+  Rows8 w;
+  if (CHUNK) {
+    pdl_wait();
+    pdl_launch_dependents();
+    kvh = rest % a.H;
+    if (!find_rows<8>(a, G, rest / a.H, lane, w)) return;
+    seq = w.b;
+    heads = w.rows;
+    first_head = kvh * G;
+    first_row = w.row0;
+  } else {
+    const int hb = rest % blocks_of_heads;
+    rest /= blocks_of_heads;
+    kvh = rest % a.H;
+    seq = rest / a.H;
+    heads = min(8, G - 8 * hb);
+    first_head = kvh * G + 8 * hb;
+  }
+  // column c: query (of q) and head
+  auto token_of = [&](int c) { return CHUNK ? w.first + (first_row + c) / G : seq; };
+  auto head_of = [&](int c) { return CHUNK ? first_head + (first_row + c) % G : first_head + c; };
   uint8_t* const ring = smem + warp * STG * PB;
   uint64_t* const bar = bars + warp * STG;
   float2* const fac = facs + warp * STG;
@@ -421,16 +441,21 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     for (int s = 0; s < STG; ++s) mbar_init(bar + s, 1);
     fence_barrier_init();
   }
-  const uint64_t stream_policy = policy_evict_first();
-  pdl_wait();
-  pdl_launch_dependents();
+  const uint64_t stream_policy = CHUNK ? policy_evict_last() : policy_evict_first();      // (other rows of a chunk read the same pages)
+  if (!CHUNK) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
 
-  const int len = a.lens[seq];
-  int lo = a.starts ? max(a.starts[seq], 0) : 0;
-  if (a.window > 0) lo = max(lo, len - a.window);
+  const int len = a.lens[seq], start = a.starts ? max(a.starts[seq], 0) : 0;
+  // keys [lo, end) of the columns together; column c sees [max(start, p - window + 1), p], p its query's position
+  const int p0 = CHUNK ? len - w.n + first_row / G : len - 1, p1 = CHUNK ? len - w.n + (first_row + heads - 1) / G : len - 1;
+  const int lo = a.window > 0 ? max(start, p0 - a.window + 1) : start, end = p1 + 1;
+  const int lo_all = a.window > 0 ? max(start, p1 - a.window + 1) : start, end_all = p0 + 1;      // keys that all columns see
   uint32_t qf[KT][2];
   {
-    const uint16_t* const qrow = a.q + (size_t)seq * a.q_stride + (size_t)(first_head + (g < heads ? g : 0)) * D;
+    const int c = g < heads ? g : 0;
+    const uint16_t* const qrow = a.q + (size_t)token_of(c) * a.q_stride + (size_t)head_of(c) * D;
 #pragma unroll
     for (int p = 0; p < D / 64; ++p) {
       const uint4* const at = reinterpret_cast<const uint4*>(qrow + 16 * (t + 4 * p));
@@ -440,7 +465,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     }
   }
   const int first_page = lo / PAGE;
-  const int end_page = len > lo ? (int)min((long long)(len - 1) / PAGE + 1, a.table_stride) : 0;
+  const int end_page = end > lo ? (int)min((long long)(end - 1) / PAGE + 1, a.table_stride) : 0;
   const int per_split = max(parts.min_pages, (end_page - first_page + parts.splits - 1) / parts.splits);
   const int lo_page = first_page + split * per_split, hi_page = min(end_page, lo_page + per_split);
   const int my_first = lo_page + warp;
@@ -532,10 +557,19 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     float x00 = fmaf(sc[0] + sd[0], c0, f.y), x01 = fmaf(sc[1] + sd[1], c1, f.y);
     float x10 = fmaf(sc[2] + sd[2], c0, f.y), x11 = fmaf(sc[3] + sd[3], c1, f.y);
     const int t0 = page * PAGE;
-    if (t0 < lo || t0 + PAGE > len) {                             // an edge page: tokens outside [lo, len)
+    if (t0 < lo_all || t0 + PAGE > end_all) {                     // an edge page: tokens that a column does not see
       const int tok = t0 + g;
-      if (tok < lo || tok >= len) x00 = x01 = -INFINITY;
-      if (tok + 8 < lo || tok + 8 >= len) x10 = x11 = -INFINITY;
+      if (CHUNK) {
+        const int h0 = len - w.n + (first_row + 2 * t) / G, h1 = len - w.n + (first_row + 2 * t + 1) / G;       // last key of a column
+        const int g0 = a.window > 0 ? max(start, h0 - a.window + 1) : start, g1 = a.window > 0 ? max(start, h1 - a.window + 1) : start;
+        if (tok < g0 || tok > h0) x00 = -INFINITY;
+        if (tok < g1 || tok > h1) x01 = -INFINITY;
+        if (tok + 8 < g0 || tok + 8 > h0) x10 = -INFINITY;
+        if (tok + 8 < g1 || tok + 8 > h1) x11 = -INFINITY;
+      } else {
+        if (tok < lo || tok >= end) x00 = x01 = -INFINITY;
+        if (tok + 8 < lo || tok + 8 >= end) x10 = x11 = -INFINITY;
+      }
     }
     const float top0 = fmaxf(x00, x10), top1 = fmaxf(x01, x11);
     if (__any_sync(FULL, top0 > m0 + RAISE8 || top1 > m1 + RAISE8)) {
@@ -548,7 +582,9 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
       m0 = n0;
       m1 = n1;
     }
-    const float p00 = ex2(x00 - m0), p01 = ex2(x01 - m1), p10 = ex2(x10 - m0), p11 = ex2(x11 - m1), out = ex2(-f.y);
+    // (a chunk's column may see nothing of a page, and of any: its reference is then still -inf)
+    const float r0 = CHUNK && m0 == -INFINITY ? 0.f : m0, r1 = CHUNK && m1 == -INFINITY ? 0.f : m1;
+    const float p00 = ex2(x00 - r0), p01 = ex2(x01 - r1), p10 = ex2(x10 - r0), p11 = ex2(x11 - r1), out = ex2(-f.y);
     l0 = fmaf(p00 + p10, out, l0);
     l1 = fmaf(p01 + p11, out, l1);
     const uint32_t b0 = movmatrix_t(pack_f16(p00, p01)), b1 = movmatrix_t(pack_f16(p10, p11));
@@ -618,12 +654,12 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
       den += f * pw[D + 1];
       num += f * pw[d];
     }
-    const int hq = first_head + h;
+    const int hq = head_of(h), token = token_of(h);
     if (parts.splits == 1) {
       const __nv_bfloat16 v = __float2bfloat16_rn(den > 0.f ? num / den : den);        // (a sum that is not a number stays one)
-      a.out[(size_t)seq * a.out_stride + (size_t)hq * D + d] = *reinterpret_cast<const uint16_t*>(&v);
+      a.out[(size_t)token * a.out_stride + (size_t)hq * D + d] = *reinterpret_cast<const uint16_t*>(&v);
     } else {
-      const size_t ix = ((size_t)seq * a.Hq + hq) * parts.splits + split;
+      const size_t ix = ((size_t)token * a.Hq + hq) * parts.splits + split;
       parts.o[ix * D + d] = num;
       if (d == 0) { parts.ml[ix * 2] = top; parts.ml[ix * 2 + 1] = den; }
     }
@@ -699,25 +735,37 @@ __global__ void __launch_bounds__(MERGE8 * 32) kv8_merge_kernel(const float* __r
   for (int d = 0; d < PL; d += 2) *reinterpret_cast<uint32_t*>(at + d) = pack_bf16(num[d] * inv, num[d + 1] * inv);
 }
 
-template <int D, int NW, int STG>
-int attn8_launch(const Attn8& a, const Parts8& parts, cudaStream_t st_) {
+template <int D, int NW, int STG, bool CHUNK>
+int attn8_launch(const Attn8& a, const Parts8& parts, long long ctas, cudaStream_t st_) {
   constexpr int smem = NW * STG * (2 * PAGE * D + 8 + 8);
   static std::atomic<uint64_t> set{0};                            // devices whose limit has been raised
   int dev = 0;
   if (int e = st::cuda_fail(cudaGetDevice(&dev), "st_kv8_attn: device")) return e;
   if (dev > 63 || !(set.load() >> dev & 1)) {
-    if (int e = st::cuda_fail(cudaFuncSetAttribute(kv8_attn_kernel<D, NW, STG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+    if (int e = st::cuda_fail(cudaFuncSetAttribute(kv8_attn_kernel<D, NW, STG, CHUNK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                               "st_kv8_attn: shared memory attribute"))
       return e;
     if (dev <= 63) set.fetch_or(1ull << dev);
   }
-  const long long ctas = (long long)a.B * a.H * ((a.Hq / a.H + 7) / 8) * parts.splits;
-  return st::launch("st_kv8_attn launch", kv8_attn_kernel<D, NW, STG>, dim3((unsigned)ctas), dim3(NW * 32), (size_t)smem, st_, a, parts,
-                    st::status_ptr());
+  return st::launch("st_kv8_attn launch", kv8_attn_kernel<D, NW, STG, CHUNK>, dim3((unsigned)ctas), dim3(NW * 32), (size_t)smem, st_, a,
+                    parts, st::status_ptr());
+}
+// An SM holds sixteen warps: four CTAs of four, or two of eight for a grid of at most two CTAs per SM
+template <bool CHUNK>
+int attn8_any(const Attn8& a, const Parts8& parts, int D, long long ctas, cudaStream_t st_) {
+  ST_REQUIRE(ctas < (1ll << 31), "st_kv8_attn: grid too large");
+  const bool wide = ctas <= 2ll * st::sm_count();
+  if (D == 128)
+    return wide ? attn8_launch<128, 8, 3, CHUNK>(a, parts, ctas, st_) : attn8_launch<128, 4, 3, CHUNK>(a, parts, ctas, st_);
+  return wide ? attn8_launch<64, 8, 5, CHUNK>(a, parts, ctas, st_) : attn8_launch<64, 4, 5, CHUNK>(a, parts, ctas, st_);
 }
 }  // namespace
 
 namespace st {
+int rows8_attn(const Attn8& a, const Parts8& parts, int D, cudaStream_t st_) {
+  const long long slots = a.T * (a.Hq / a.H) / 8 + a.B;
+  return attn8_any<true>(a, parts, D, slots * a.H * parts.splits, st_);
+}
 int merge8(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t st_) {
   const long long rows = a.T * a.Hq;
   const int per_cta = parts.splits > 4 ? 1 : MERGE8;
@@ -823,14 +871,9 @@ extern "C" int st_kv8_attn(const void* q, int64_t qs, int64_t B, int64_t Hq, con
   ST_REQUIRE(S == 1 || (wo && wml && st::aligned16(wo)), "st_kv8_attn: split workspace (wo, wml) missing or unaligned");
   if (B == 0) return 0;
   ST_REQUIRE(st::status_ptr() != nullptr, "st_kv8_attn: no device status word");
-  const long long ctas = B * Hkv * ((Hq / Hkv + 7) / 8) * S;
-  ST_REQUIRE(ctas < (1ll << 31), "st_kv8_attn: grid too large");
   const Parts8 parts = {wo, wml, (int)S, (int)(minpps < 1 ? 1 : minpps)};
   const cudaStream_t st_ = (cudaStream_t)stream;
-  // An SM holds sixteen warps: four CTAs of four, or two of eight for a grid of at most two CTAs per SM
-  const bool wide = ctas <= 2ll * st::sm_count();
-  const int e = D == 128 ? (wide ? attn8_launch<128, 8, 3>(a, parts, st_) : attn8_launch<128, 4, 3>(a, parts, st_))
-                         : (wide ? attn8_launch<64, 8, 5>(a, parts, st_) : attn8_launch<64, 4, 5>(a, parts, st_));
+  const int e = attn8_any<false>(a, parts, (int)D, B * Hkv * ((Hq / Hkv + 7) / 8) * S, st_);
   if (e || S == 1) return e;
   return merge8("st_kv8_attn merge launch", a, parts, (int)D, st_);
 }

@@ -88,9 +88,49 @@ struct Attn8 {
 // partial results of sequences that are split: o [T, Hq, splits, D] (not normalised), ml [T, Hq, splits, 2] = (reference, base 2; sum)
 struct Parts8 { float* o; float* ml; int splits, min_pages; };
 
+// A CTA's rows, the same in all of its threads: rows row0 .. row0 + rows - 1 of the n * G rows (query, head of the group) of sequence b,
+// whose first query is row `first` of q
+struct Rows8 { int b, row0, rows, first, n; };
+// tile `slot` of TILE rows, sequences' tiles one after the other; false: there is none
+template <int TILE>
+__device__ __forceinline__ bool find_rows(const Attn8& a, int G, int slot, int lane, Rows8& w) {
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int b = b0 + lane;
+    int lo = 0, n = 0;
+    if (b < a.B) {
+      lo = a.cu ? a.cu[b] : b;
+      n = a.cu ? a.cu[b + 1] - lo : 1;
+      if (lo < 0 || n < 0 || lo + (long long)n > a.T) n = 0;      // (not inside q: no work)
+    }
+    const int mine = (int)(((long long)n * G + TILE - 1) / TILE);
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(FULL, sum, o);
+      if (lane >= o) sum += v;
+    }
+    const int begin = before + sum - mine;
+    const unsigned hit = __ballot_sync(FULL, slot >= begin && slot < begin + mine);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      w.b = b0 + src;
+      w.first = __shfl_sync(FULL, lo, src);
+      w.n = __shfl_sync(FULL, n, src);
+      w.row0 = (slot - __shfl_sync(FULL, begin, src)) * TILE;
+      w.rows = min(TILE, w.n * G - w.row0);
+      return true;
+    }
+    before += __shfl_sync(FULL, sum, 31);
+  }
+  return false;
+}
+
 // st_kv8.cu: what both forms of the attention check and pass on; the join of the partial results
 int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
                const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens,
                const int32_t* starts, int64_t window, void* out, int64_t os, double scale);
+// chunks of few rows per sequence through the decode kernel, eight rows a CTA
+int rows8_attn(const Attn8& a, const Parts8& parts, int D, cudaStream_t stream);
 int merge8(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t stream);
 }  // namespace st

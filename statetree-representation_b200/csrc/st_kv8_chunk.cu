@@ -25,6 +25,10 @@
 namespace {
 using namespace st;
 
+// Rows per sequence up to which a chunk goes through the decode kernel (chunk_splits8 in kvcache.py states the same): its time grows with
+// every eight rows, this kernel's hardly up to 128.  32 sequences of 2000 tokens, D = 128: 16 rows 38 us there, 103 here; 32 rows 63 and
+// 74; 64 rows 119 and 75.  D = 64: 28 rows 15 and 30, 56 rows 27 and 30, 112 rows 46 and 31.
+constexpr int FEW_ROWS = 32;
 constexpr int KEYS = 128, TILE_PAGES = KEYS / PAGE, ROWS = 128;
 constexpr int W_CONV = 8, W_MMA = 12, WARPS = 16;                 // softmax warps 0 .. 7 (tile = warp / 4); 13 .. 15 only lend registers
 constexpr int CRING = 4;                                          // page factors of so many key tiles are kept
@@ -117,46 +121,10 @@ template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
 
 // What a CTA works on; the same in all of its threads
-struct Work {
-  int b, h, split, row0, rows;                                    // rows row0 .. of the sequence's n * G
-  int first, n, pos0;                                             // first query row in q, queries, position of query 0
+struct Work : Rows8 {
+  int h, split, pos0;                                             // position of query 0
   int lo0, first_tile, tiles, count0, count1;                           // key tiles of the split; of those, how many each row tile needs
 };
-
-// the sequence and 256-row tile of `slot`: sequences' tiles one after the other
-__device__ __forceinline__ bool find_work(const Chunk8& c, int G, int slot, int lane, Work& w) {
-  const Attn8& a = c.a;
-  int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int b = b0 + lane;
-    int lo = 0, n = 0;
-    if (b < a.B) {
-      lo = a.cu ? a.cu[b] : b;
-      n = a.cu ? a.cu[b + 1] - lo : 1;
-      if (lo < 0 || n < 0 || lo + (long long)n > a.T) n = 0;      // (not inside q: no work)
-    }
-    const int mine = (int)(((long long)n * G + 2 * ROWS - 1) / (2 * ROWS));
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(FULL, sum, o);
-      if (lane >= o) sum += v;
-    }
-    const int begin = before + sum - mine;
-    const unsigned hit = __ballot_sync(FULL, slot >= begin && slot < begin + mine);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      w.b = b0 + src;
-      w.first = __shfl_sync(FULL, lo, src);
-      w.n = __shfl_sync(FULL, n, src);
-      w.row0 = (slot - __shfl_sync(FULL, begin, src)) * (2 * ROWS);
-      w.rows = min(2 * ROWS, w.n * G - w.row0);
-      return true;
-    }
-    before += __shfl_sync(FULL, sum, 31);
-  }
-  return false;
-}
 
 template <int D>
 __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c) {
@@ -180,7 +148,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     w.split = x % c.parts.splits;
     x /= c.parts.splits;
     w.h = x % a.H;
-    if (!find_work(c, G, c.slots - 1 - x / a.H, lane, w)) return;
+    if (!find_rows<2 * ROWS>(a, G, c.slots - 1 - x / a.H, lane, w)) return;
     const int len = a.lens[w.b], start = a.starts ? max(a.starts[w.b], 0) : 0;
     w.pos0 = len - w.n;
     const int first_pos = w.pos0 + w.row0 / G, last_pos = w.pos0 + (w.row0 + w.rows - 1) / G;
@@ -232,7 +200,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     const bool live = my < w.row0 + w.rows;
     const int token = live ? my / G : 0, head = live ? my % G : 0, hq = w.h * G + head;
     const int pos = w.pos0 + token;
-    const int hi = live ? pos : -1, lo = a.window > 0 ? max(w.lo0, pos - a.window + 1) : w.lo0;
+    // (a row that is none sees everything: its results go nowhere, and a warp with one does not take the masked way for it)
+    const int hi = live ? pos : 0x7FFFFFFF, lo = !live ? 0 : a.window > 0 ? max(w.lo0, pos - a.window + 1) : w.lo0;
     const bool any = __any_sync(FULL, live);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * D;
@@ -618,10 +587,13 @@ extern "C" int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t H
   ST_REQUIRE(c.status != nullptr, "st_kv8_chunk_attn: no device status word");
   // 256-row tiles of all sequences: each may leave one unfilled
   const long long slots = T * (Hq / Hkv) / (2 * ROWS) + B;
-  ST_REQUIRE(slots * Hkv * S < (1ll << 31), "st_kv8_chunk_attn: grid too large");
+  ST_REQUIRE(slots * Hkv * S < (1ll << 31) && T * (Hq / Hkv) < (1ll << 31), "st_kv8_chunk_attn: grid too large");
   c.slots = (int)slots;
   const cudaStream_t st_ = (cudaStream_t)stream;
-  const int e = D == 128 ? chunk_launch<128>(c, st_) : chunk_launch<64>(c, st_);
+  // few rows per sequence: eight to a CTA through the decode kernel
+  const bool few = T * (Hq / Hkv) <= FEW_ROWS * B;
+  c.parts.min_pages = few ? 4 : 1;
+  const int e = few ? st::rows8_attn(c.a, c.parts, (int)D, st_) : D == 128 ? chunk_launch<128>(c, st_) : chunk_launch<64>(c, st_);
   if (e || S == 1) return e;
   return st::merge8("st_kv8_chunk_attn merge launch", c.a, c.parts, (int)D, st_);
 }
