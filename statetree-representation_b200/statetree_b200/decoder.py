@@ -11,6 +11,9 @@ top-k, renormalised weights, TreeExperts): under several ranks the attention sta
 split over the ranks (expert parallelism: every rank routes all tokens, computes its own experts' weighted partial
 output, and the partial outputs are all-reduced).  Every rank draws the full tensors from the same seeds and keeps its slice,
 so a tensor-parallel run computes the same function as the single-GPU one.
+
+`eight_bit_kv=True` keeps the KV cache in 8-bit pages (kvcache.PageStore8) instead of the lossless ones: a decode step then norms,
+rotates and appends through their append, and a prompt runs in one pass (prefill) over their chunk attention.
 """
 import math
 from dataclasses import dataclass
@@ -19,7 +22,7 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as Fn
 
-from .kvcache import PagedKVCache
+from .kvcache import PagedKVCache, decode_splits8
 from .linear import TreeLinear, interleave_gate_up
 from .ops import ext, kv_ext
 
@@ -61,10 +64,12 @@ class _Dense:
 
 
 class TreeDecoder:
-    def __init__(self, cfg, device, batch, max_len, compressed=True, seed=0, rank=0, world=1, group=None):
+    def __init__(self, cfg, device, batch, max_len, compressed=True, seed=0, rank=0, world=1, group=None,
+                 eight_bit_kv=False):
         self.cfg, self.dev, self.B, self.rank, self.world, self.group = cfg, torch.device(device), batch, rank, world, group
-        self.compressed = compressed
+        self.compressed, self.eight_bit_kv = compressed, eight_bit_kv
         c = cfg
+        assert compressed or not eight_bit_kv, "the BF16 control keeps its own cache"
         assert c.heads % world == 0 and c.kv_heads % world == 0 and c.inter % (64 * world) == 0 and c.vocab % (16 * world) == 0
         self.hq, self.hkv = c.heads // world, c.kv_heads // world
         self.fused_act = False
@@ -129,7 +134,8 @@ class TreeDecoder:
         self.k_buf = torch.empty(batch, self.hkv, D, dtype=torch.bfloat16, device=self.dev)
         self.tokens = torch.zeros(batch, dtype=torch.long, device=self.dev)
         if compressed:
-            self.cache = PagedKVCache(c.layers, batch, max_len, self.hkv, self.dev, pool_blocks=1 << 14)
+            self.cache = PagedKVCache(c.layers, batch, max_len, self.hkv, self.dev, pool_blocks=1 << 14, eight_bit=eight_bit_kv,
+                                      head_dim=D)
         else:
             self.kc = [torch.zeros(batch, max_len, self.hkv, D, dtype=torch.bfloat16, device=self.dev) for _ in range(c.layers)]
             self.vc = [torch.zeros_like(k) for k in self.kc]
@@ -230,6 +236,53 @@ class TreeDecoder:
             dist.all_reduce(delta, group=self.group)
         ext().add_rmsnorm(x, delta, self.norm_w, h, c.eps)
 
+    def _append8(self, layer, qkv, slots, positions, q_out):
+        """fused q/k/v rows [N, (hq + 2 hkv) D] into an 8-bit layer's pages, normed and rotated queries into q_out; the layer"""
+        q, k, v = qkv.view(qkv.shape[0], self.hq + 2 * self.hkv, self.cfg.head_dim).split([self.hq, self.hkv, self.hkv], 1)
+        layer.append(k, v, slots, positions, self.cos, self.sin, True, q, self.head_norm_w, self.head_norm_w, self.cfg.eps, q_out)
+        return layer
+
+    def prefill(self, prompt):
+        """prompt [B, P] token ids behind whatever the 8-bit cache holds, in one pass: every layer's keys and values go into the pages,
+        then its queries attend to them (causal).  Returns the logits of every sequence's last token [B, vocab]"""
+        if not self.eight_bit_kv or self.world > 1:
+            raise RuntimeError("TreeDecoder.prefill: a single-GPU decoder with eight_bit_kv=True")
+        c, E, (B, P) = self.cfg, ext(), prompt.shape
+        if B != self.B:
+            raise ValueError(f"TreeDecoder.prefill: {B} sequences, the decoder was made for {self.B}")
+        start = int(self.pos_buf.item())
+        if start + P > self.max_len:
+            raise ValueError(f"TreeDecoder.prefill: {P} tokens from position {start} exceed the cache capacity of {self.max_len} tokens")
+        N, D, cache = B * P, c.head_dim, self.cache
+        cache._stored = start                                # (decode steps count on the GPU only)
+        slots = cache.begin_chunk(B, P)
+        positions = (start + torch.arange(P, device=self.dev)).repeat(B)
+        cu = torch.arange(0, N + 1, P, dtype=torch.int32, device=self.dev)
+        x = self.embed.rows(prompt.reshape(-1))
+        h = torch.empty(N, c.hidden, dtype=torch.bfloat16, device=self.dev)
+        q = torch.empty(N, self.hq, D, dtype=torch.bfloat16, device=self.dev)
+        delta = None
+        for li, (qkv, o, gu, d) in enumerate(self.blocks):
+            E.add_rmsnorm(x, delta, self.norm_w, h, c.eps)
+            layer = self._append8(cache.layers[li], qkv(h), slots, positions, q)
+            att = layer.chunk_attention(q, cu, cache.bt32[:B], cache.lens[:B], 1.0 / math.sqrt(D))
+            E.add_rmsnorm(x, o(att.view(N, self.hq * D)), self.norm_w, h, c.eps)
+            if c.experts:
+                router, te = gu
+                delta = te(h, *E.moe_route(Fn.linear(h, router), c.top_k, True, None), None)
+                continue
+            y = gu(h)
+            if self.fused_act:                               # (16-row tiles of gate and up in turn)
+                y = y.view(N, c.inter // 16, 2, 16).transpose(1, 2).reshape(N, 2 * c.inter)
+            act = torch.empty(N, c.inter, dtype=torch.bfloat16, device=self.dev)
+            E.silu_mul(y, act)
+            delta = d(act)
+        last = torch.arange(P - 1, N, P, device=self.dev)
+        E.add_rmsnorm(x, delta, self.norm_w, h, c.eps)
+        cache.end_chunk(P)
+        self.pos_buf += P
+        return self.lm_head(h[last])
+
     def _step(self):
         """one decode step for self.tokens at position self.pos; about ten launches per layer"""
         c, B, D = self.cfg, self.B, self.cfg.head_dim
@@ -245,8 +298,11 @@ class TreeDecoder:
             else:
                 self._add_norm(x, delta, h, summed)
                 y = qkv(h)
-            if self.compressed:
-                layer = self.cache.layers[li]               # norm + rope of q and k and the append of k, v: one launch
+            if self.eight_bit_kv:                           # norm + rope of q and k and the append of k, v: one launch
+                att = self._append8(self.cache.layers[li], y, slots, self.pos_buf, qb).attention(
+                    qb, self.cache.bt32[:B], self.cache.lens[:B], scale, self.splits, None, 4)
+            elif self.compressed:
+                layer = self.cache.layers[li]
                 kv_ext().rope_append(y, self.head_norm_w, self.head_norm_w, self.cos, self.sin, self.pos_buf, qb,
                                      self.hq, self.hkv, c.eps, slots, layer.pages, layer.pool, layer.pcnt)
                 att = layer.attention(qb, self.cache.bt32[:B], self.cache.lens[:B], scale, self.splits, None, 4)
@@ -310,7 +366,9 @@ class TreeDecoder:
 
     def capture(self):
         from .kvcache import decode_splits
-        self.splits = decode_splits(self.B, self.hkv, (self.max_len + 15) // 16) if self.compressed else 1
+        pages = (self.max_len + 15) // 16
+        self.splits = (decode_splits8(self.B * self.hkv * -(-self.hq // (8 * self.hkv)), pages) if self.eight_bit_kv else
+                       decode_splits(self.B, self.hkv, pages) if self.compressed else 1)
         self.next_tok = torch.zeros(self.B, dtype=torch.long, device=self.dev)
         side = torch.cuda.Stream(self.dev)
         side.wait_stream(torch.cuda.current_stream(self.dev))      # weights and buffers were written on that stream
@@ -346,7 +404,8 @@ class TreeDecoder:
             self.lens.zero_()
 
     def run(self, prompt, n_new, collect=None, margins=None):
-        """prompt [B, P] token ids (teacher-forced one step at a time), then n_new greedy tokens -> [B, n_new].
+        """prompt [B, P] token ids (teacher-forced one step at a time, with an 8-bit cache in one pass), then n_new greedy tokens ->
+        [B, n_new].
         collect (optional list): receives the model's prediction after every prompt step (teacher-forced top-1).
         margins (optional list): receives, per generated token, the top-2 logit margin of sequence 0 that chose it."""
         start = int(self.pos_buf.item())
@@ -354,7 +413,11 @@ class TreeDecoder:
             raise ValueError(f"TreeDecoder.run: {prompt.shape[1]} prompt + {n_new} new tokens from position {start} "
                              f"exceed the cache capacity of {self.max_len} tokens")
         out = []
-        for t in range(prompt.shape[1]):
+        whole = self.eight_bit_kv and self.world == 1 and collect is None and prompt.shape[1] > 1
+        if whole:
+            self.logits.copy_(self.prefill(prompt))
+            self._pick(self.logits)
+        for t in range(0 if not whole else prompt.shape[1], prompt.shape[1]):
             self.tokens.copy_(prompt[:, t])
             self.graph.replay()
             if collect is not None:

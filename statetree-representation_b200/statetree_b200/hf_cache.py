@@ -11,13 +11,16 @@ statetree/kvcache.py (StateTreeKVLayer 35-129, StateTreeKVCache 132-177, statetr
 Positions come from a GPU-side token count (or from `cache_position` when the model passes it), buffers are static,
 so decode steps can be captured in CUDA graphs.  Left padding is supported: each sequence's first valid position is
 read once from the prefill attention mask.  Head dimension 128 only.
+
+StateTreeKVCache(..., eight_bit=True) keeps 8-bit pages instead (kvcache.PageStore8; head dimension 64 or 128): then every chunk of a
+prompt attends to the pages too, causally and from each sequence's first valid position on, and nothing is expanded.
 """
 import threading
 
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
-from .kvcache import PAGE, PageStore, decode_splits
+from .kvcache import PAGE, PageStore, PageStore8, decode_splits, decode_splits8
 
 _LAST = threading.local()          # the layer whose update() ran last on this thread; the attention function picks it up
 
@@ -38,13 +41,14 @@ class StateTreeKVLayer(CacheLayerMixin):
     def lazy_initialization(self, key_states, value_states=None):
         c = self.cache
         B, H, _, D = key_states.shape
-        if D != 128:
-            raise ValueError("StateTreeKVCache: the page format holds heads of dimension 128")
+        if D != 128 and not (c.eight_bit and D == 64):
+            raise ValueError("StateTreeKVCache: the page format holds heads of dimension 128 (8-bit pages: or 64)")
         c._allocate(B, H, key_states.device)
         self.dtype, self.device = key_states.dtype, key_states.device
         self.num_heads = H
         self.max_batch_size = self.batch_size = c.Bmax
-        self.store = PageStore(c.Bmax * c.max_pages, H, self.device, pool_blocks=c.pool_blocks)
+        self.store = (PageStore8(c.Bmax * c.max_pages, H, self.device, D) if c.eight_bit else
+                      PageStore(c.Bmax * c.max_pages, H, self.device, pool_blocks=c.pool_blocks))
         self.gpu_len = torch.zeros((), dtype=torch.long, device=self.device)     # the same count on the GPU (graphs)
         self.is_initialized = True
 
@@ -70,6 +74,10 @@ class StateTreeKVLayer(CacheLayerMixin):
         self.store.append(rows[0], rows[1], slots)
         _LAST.layer = self
         before, self.host_len = self.host_len, self.host_len + T
+        if c.eight_bit:                              # the attention function reads the pages whatever T is
+            if self.layer_idx == 0:
+                c.lens[:B].copy_((where[-1:] + 1).to(torch.int32).expand(B))
+            return key_states, value_states
         if T == 1:                                   # a decode step: the attention function reads the pages itself
             if self.layer_idx == 0:
                 c.lens[:B].copy_((where[-1:] + 1).to(torch.int32).expand(B))
@@ -105,7 +113,7 @@ class StateTreeKVLayer(CacheLayerMixin):
     def reset(self):
         self.host_len = 0
         if self.is_initialized:
-            self.store.pcnt.zero_()
+            self.store.reset()
             self.gpu_len.zero_()
         self.cache.starts_known = False
 
@@ -122,16 +130,16 @@ class StateTreeKVLayer(CacheLayerMixin):
 
 class StateTreeKVCache(Cache):
     """Lossless compressed KV cache for transformers models.  batch_size and max_cache_len fix the page tables;
-    pool_blocks sizes each layer's pool of 64-byte escape extension blocks."""
+    pool_blocks sizes each layer's pool of 64-byte escape extension blocks.  eight_bit: 8-bit pages (not lossless)."""
 
-    def __init__(self, config, batch_size=None, max_cache_len=4096, pool_blocks=None, **kwargs):
+    def __init__(self, config, batch_size=None, max_cache_len=4096, pool_blocks=None, eight_bit=False, **kwargs):
         text = config.get_text_config() if hasattr(config, "get_text_config") else config
         self.num_layers = text.num_hidden_layers
         self.num_q_heads = text.num_attention_heads
         self.num_kv_heads = getattr(text, "num_key_value_heads", None) or text.num_attention_heads
         self.max_len = int(max_cache_len)
         self.max_pages = -(-self.max_len // PAGE)
-        self.alloc_batch, self.pool_blocks = batch_size, pool_blocks
+        self.alloc_batch, self.pool_blocks, self.eight_bit = batch_size, pool_blocks, eight_bit
         self.starts_known = False
         self._allocated = False
         super().__init__(layers=[StateTreeKVLayer(self, i) for i in range(self.num_layers)])
@@ -147,7 +155,8 @@ class StateTreeKVCache(Cache):
         self.table32 = self.table64.to(torch.int32)
         self.lens = torch.zeros(n, dtype=torch.int32, device=device)
         self.starts = torch.zeros(n, dtype=torch.int32, device=device)
-        self.splits = decode_splits(n, H, self.max_pages)
+        group = -(-self.num_q_heads // max(1, H))
+        self.splits = decode_splits8(n * H * -(-group // 8), self.max_pages) if self.eight_bit else decode_splits(n, H, self.max_pages)
         if self.pool_blocks is None:
             self.pool_blocks = max(4096, n * self.max_pages * H * 4 // 8)
         self._allocated = True
@@ -161,7 +170,8 @@ class StateTreeKVCache(Cache):
             layer.check()
 
     def storage_bytes(self):
-        return sum(l.store.pages.numel() + l.store.pool.numel() * 4 for l in self.layers if l.is_initialized)
+        return sum(l.store.pages.numel() + (l.store.exps.numel() if self.eight_bit else l.store.pool.numel() * 4) for l in self.layers
+                   if l.is_initialized)
 
 
 def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, scaling=None, **kwargs):
@@ -185,6 +195,12 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
             masked = ~last_row if last_row.dtype == torch.bool else last_row < 0
             c.starts[:B].copy_(masked.sum(-1).to(torch.int32))
             c.starts_known = True
+        if c.eight_bit:                              # a chunk (its keys are in the pages already), or the first token of all
+            q = query.transpose(1, 2).reshape(B * T, Hq, D)
+            cu = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=q.device)
+            out = layer.store.chunk_attention(q, cu, c.table32[:B], c.lens[:B], float(scaling) if scaling is not None else D ** -0.5,
+                                              starts=c.starts[:B])
+            return out.view(B, T, Hq, D), None
     return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout, scaling=scaling, **kwargs)
 
 

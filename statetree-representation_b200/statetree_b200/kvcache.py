@@ -1,8 +1,8 @@
 """Paged state-tree KV cache: keys and values stored losslessly in 16-token pages of state-tree records (6400 B per
 page per KV head against 8192 B in BF16), appended on write and read by the decode attention kernel without ever
 being expanded.  PageStore holds one attention layer's pages (the tensors of the reference's statetree/kvcache.py
-StateTreeKVLayer 49-57, with its append / dense / attention calls); PagedKVCache is the static cache of the decode
-runner in this package.  The Hugging Face classes of the reference (StateTreeKVCache, StateTreeKVLayer,
+StateTreeKVLayer 49-57, with its append / dense / attention calls); PageStore8 holds them in 8 bits (no counterpart in the
+reference); PagedKVCache is the static cache of the decode runner in this package.  The Hugging Face classes of the reference (StateTreeKVCache, StateTreeKVLayer,
 statetree_attention, enable) live in hf_cache.py and are re-exported here when transformers is importable.
 """
 import torch
@@ -79,6 +79,9 @@ class PageStore:
 
     def pool_usage(self):
         return int(self.pcnt[0].item()), self.pool.shape[0]
+
+    def reset(self):
+        self.pcnt.zero_()
 
 
 def _rows(t, D):
@@ -232,14 +235,17 @@ class PageStore8:
 
 class PagedKVCache:
     """Static paged cache for a decoder: per-layer pages, one block table [B, max_pages] (sequence b owns pages
-    b * max_pages ...), a GPU-side token count so decode steps are CUDA-graph safe."""
+    b * max_pages ...), a GPU-side token count so decode steps are CUDA-graph safe.  eight_bit: the layers are PageStore8s (heads of
+    head_dim 64 or 128), which take 256 B per token and head of 128 for the 400 of the lossless pages."""
 
-    def __init__(self, num_layers, batch_size, max_cache_len, num_kv_heads, device, pool_blocks=1 << 15):
+    def __init__(self, num_layers, batch_size, max_cache_len, num_kv_heads, device, pool_blocks=1 << 15, eight_bit=False, head_dim=128):
         self.B = batch_size
         self.max_pages = (max_cache_len + PAGE - 1) // PAGE
         self.max_len = self.max_pages * PAGE
         self.device = torch.device(device)
-        self.layers = [PageStore(batch_size * self.max_pages, num_kv_heads, device, pool_blocks)
+        self.eight_bit = eight_bit
+        blocks = batch_size * self.max_pages
+        self.layers = [PageStore8(blocks, num_kv_heads, device, head_dim) if eight_bit else PageStore(blocks, num_kv_heads, device, pool_blocks)
                        for _ in range(num_layers)]
         self.bt32 = torch.arange(batch_size * self.max_pages, dtype=torch.int32, device=device).view(batch_size, -1)
         self.bt64 = self.bt32.long()
@@ -254,8 +260,7 @@ class PagedKVCache:
         if self._stored + (T if layer_idx != len(self.layers) - 1 else 0) > self.max_len:
             raise ValueError(f"PagedKVCache.update: position {self._stored + T} exceeds the capacity of "
                              f"{self.max_len} tokens")
-        cp = torch.arange(T, device=self.device) + self.cum
-        slots = (self.bt64[:B][:, cp // PAGE] * PAGE + (cp % PAGE)).reshape(-1)
+        slots = self.next_slots(B, T)
         K = key_states.transpose(1, 2).reshape(B * T, H, D)
         V = value_states.transpose(1, 2).reshape(B * T, H, D)
         self.layers[layer_idx].append(K.contiguous(), V.contiguous(), slots)
@@ -265,6 +270,23 @@ class PagedKVCache:
         elif layer_idx == 0:
             self.lens[:B] = (self.cum + T).to(torch.int32)
         return slots
+
+    def next_slots(self, B, T):
+        """slots [B * T] of the next T tokens of every sequence (sequence after sequence)"""
+        cp = torch.arange(T, device=self.device) + self.cum
+        return (self.bt64[:B][:, cp // PAGE] * PAGE + (cp % PAGE)).reshape(-1)
+
+    def begin_chunk(self, B, T):
+        """the next T tokens of every sequence, for all layers: their slots; lens counts them.  end_chunk(T) closes the chunk"""
+        if self._stored + T > self.max_len:
+            raise ValueError(f"PagedKVCache.begin_chunk: position {self._stored + T} exceeds the capacity of {self.max_len} tokens")
+        slots = self.next_slots(B, T)
+        self.lens[:B] = (self.cum + T).to(torch.int32)
+        return slots
+
+    def end_chunk(self, T):
+        self._stored += T
+        self.cum += T
 
     def begin_step(self, B):
         """decode step (one token per sequence): the slots every layer appends at, computed once; lens counts the new
@@ -285,7 +307,7 @@ class PagedKVCache:
     def attention(self, layer_idx, q, scale, splits=None):
         """decode step: q [B, Hq, 128] against everything stored in the layer (including this step's token)"""
         B = q.shape[0]
-        if splits is None:
+        if splits is None and not self.eight_bit:
             splits = decode_splits(B, self.layers[layer_idx].H, self.max_pages)
         return self.layers[layer_idx].attention(q, self.bt32[:B], self.lens[:B], scale, splits, None, 4)
 
@@ -298,7 +320,7 @@ class PagedKVCache:
         self.cum.zero_()
         self.lens.zero_()
         for layer in self.layers:
-            layer.pcnt.zero_()
+            layer.reset()
 
 
 try:                                                   # the transformers glue, under the reference's names

@@ -96,3 +96,34 @@ def test_python_calls_refuse():
     with pytest.raises(RuntimeError, match="blocks"):
         from statetree_b200.ops import kv_ext
         kv_ext().kv8_dequant_blocks(s.pages, s.exps, torch.zeros(2, dtype=torch.int64), bf(2, 16, 2, 128), bf(2, 16, 2, 128))
+
+
+def test_paged_cache_chunks():
+    """slots and lengths of whole chunks, and what does not fit"""
+    _ops()
+    from statetree_b200.kvcache import PagedKVCache, PageStore8
+    c = PagedKVCache(2, 2, 40, 3, "cpu", eight_bit=True, head_dim=64)
+    assert all(isinstance(layer, PageStore8) and layer.pages.shape == (6, 3, 2, 16, 64) for layer in c.layers)
+    assert c.begin_chunk(2, 20).tolist() == list(range(20)) + list(range(48, 68)) and c.lens.tolist() == [20, 20]
+    c.end_chunk(20)
+    assert c.begin_chunk(2, 5).tolist() == list(range(20, 25)) + list(range(68, 73)) and c.lens.tolist() == [25, 25]
+    with pytest.raises(ValueError, match="capacity"):
+        c.begin_chunk(2, 29)
+    c.layers[0].bad.fill_(1)
+    with pytest.raises(RuntimeError, match="finite"):
+        c.check()
+    c.reset()
+    c.check()
+    assert int(c.cum) == 0 and c.begin_chunk(2, 48).numel() == 96
+
+
+def test_split_rules():
+    """as many splits as the rules state, never more than pages allow"""
+    _ops()
+    from statetree_b200.kvcache import chunk_splits8, decode_splits8
+    assert decode_splits8(8, 1000) == 18 and decode_splits8(8, 63) == 7 and decode_splits8(8, 19) == 2 and decode_splits8(1, 4) == 1
+    assert decode_splits8(64, 1000) == 9 and decode_splits8(512, 512) == 4 and decode_splits8(512, 100) == 1 and decode_splits8(4096, 512) == 2
+    assert chunk_splits8(4096, 1, 8, 4, 256) == 1 and chunk_splits8(16, 1, 8, 4, 250) == 15 and chunk_splits8(4, 1, 8, 4, 250) == 9
+    for units in range(1, 700, 7):
+        for pages in (1, 2, 7, 33, 500, 5000):
+            assert 1 <= decode_splits8(units, pages) <= max(1, min(64, pages // 8))
