@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     pdl_launch_dependents();
   }
 
-  const int len = a.lens[seq], start = a.starts ? max(a.starts[seq], 0) : 0;
+  const int len = CHUNK ? w.len : a.lens[seq], start = CHUNK ? w.start : a.starts ? max(a.starts[seq], 0) : 0;
   // keys [lo, end) of the columns together; column c sees [max(start, p - window + 1), p], p its query's position
   const int p0 = CHUNK ? len - w.n + first_row / G : len - 1, p1 = CHUNK ? len - w.n + (first_row + heads - 1) / G : len - 1;
   const int lo = a.window > 0 ? max(start, p0 - a.window + 1) : start, end = p1 + 1;

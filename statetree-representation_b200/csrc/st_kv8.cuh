@@ -90,15 +90,18 @@ struct Parts8 { float* o; float* ml; int splits, min_pages; };
 
 // A CTA's rows, the same in all of its threads: rows row0 .. row0 + rows - 1 of the n * G rows (query, head of the group) of sequence b,
 // whose first query is row `first` of q
-struct Rows8 { int b, row0, rows, first, n; };
+// (and its length and first valid token, requested beside the row counts)
+struct Rows8 { int b, row0, rows, first, n, len, start; };
 // tile `slot` of TILE rows, sequences' tiles one after the other; false: there is none
 template <int TILE>
 __device__ __forceinline__ bool find_rows(const Attn8& a, int G, int slot, int lane, Rows8& w) {
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int b = b0 + lane;
-    int lo = 0, n = 0;
+    int lo = 0, n = 0, len = 0, start = 0;
     if (b < a.B) {
+      len = a.lens[b];
+      start = a.starts ? max(a.starts[b], 0) : 0;
       lo = a.cu ? a.cu[b] : b;
       n = a.cu ? a.cu[b + 1] - lo : 1;
       if (lo < 0 || n < 0 || lo + (long long)n > a.T) n = 0;      // (not inside q: no work)
@@ -117,6 +120,8 @@ __device__ __forceinline__ bool find_rows(const Attn8& a, int G, int slot, int l
       w.b = b0 + src;
       w.first = __shfl_sync(FULL, lo, src);
       w.n = __shfl_sync(FULL, n, src);
+      w.len = __shfl_sync(FULL, len, src);
+      w.start = __shfl_sync(FULL, start, src);
       w.row0 = (slot - __shfl_sync(FULL, begin, src)) * TILE;
       w.rows = min(TILE, w.n * G - w.row0);
       return true;

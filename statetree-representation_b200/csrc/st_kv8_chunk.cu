@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  uint64_t *const qfull = bars, *const kfull = bars + 2, *const vfull = bars + 4, *const sfull = bars + 6, *const pfull = bars + 8,
+  uint64_t *const kfull = bars + 2, *const vfull = bars + 4, *const sfull = bars + 6, *const pfull = bars + 8,
            *const ofull = bars + 12, *const empty = bars + 14, *const raw = bars + 16;           // pfull: [half of the keys][row tile]
   uint64_t* const drain = bars + 24;                              // raw: [converter warp][keys, values]
   uint32_t* const slot_at = reinterpret_cast<uint32_t*>(smem + L::SLOT);
@@ -149,8 +149,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     x /= c.parts.splits;
     w.h = x % a.H;
     if (!find_rows<2 * ROWS>(a, G, c.slots - 1 - x / a.H, lane, w)) return;
-    const int len = a.lens[w.b], start = a.starts ? max(a.starts[w.b], 0) : 0;
-    w.pos0 = len - w.n;
+    const int start = w.start;
+    w.pos0 = w.len - w.n;
     const int first_pos = w.pos0 + w.row0 / G, last_pos = w.pos0 + (w.row0 + w.rows - 1) / G;
     w.lo0 = start;
     const int lo = a.window > 0 ? max(start, first_pos - a.window + 1) : start;
@@ -171,7 +171,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
   if (warp == W_MMA) {
     if (elect_one()) {
       for (int i = 0; i < 2; ++i) {
-        mbar_init(qfull + i, 4);
         mbar_init(kfull + i, 4);
         mbar_init(vfull + i, 4);
         mbar_init(sfull + i, 1);
@@ -180,7 +179,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
         mbar_init(ofull + i, 1);
         mbar_init(empty + i, 1);
       }
-      for (int i = 0; i < 8; ++i) mbar_init(raw + i, 1);
       mbar_init(drain, 1);
       fence_barrier_init();
     }
@@ -188,10 +186,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     tmem_alloc<1>(slot_at, 512);
     tmem_relinquish<1>();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *slot_at;
+  // (each role has something to request before it needs the others: the rows of q, the first pages)
+  auto meet = [] {
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  };
 
   if (warp < W_CONV) {
     regs_up<R_SOFTMAX>();
@@ -203,36 +203,41 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     // (a row that is none sees everything: its results go nowhere, and a warp with one does not take the masked way for it)
     const int hi = live ? pos : 0x7FFFFFFF, lo = !live ? 0 : a.window > 0 ? max(w.lo0, pos - a.window + 1) : w.lo0;
     const bool any = __any_sync(FULL, live);
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * D;
     float m = -INFINITY, l = 0.f, q_up = 1.f;                     // q_up undoes the scale of q
     bool ok = true;
+    // ---- the warp's 32 rows of q as FP16, each times a power of two that its largest value asks for: D / 8 lanes read a row
     if (count > 0) {
-      uint8_t* const row = smem + L::Q + t * L::TILE + ((warp & 3) * 32 + lane) * 128;
-      const uint4* const src = reinterpret_cast<const uint4*>(a.q + (long long)(w.first + token) * a.q_stride + (size_t)hq * D);
-      uint4 u[D / 8];
-      uint32_t most = 0;
+      constexpr int LANES = D / 8, PER = 32 / LANES;
+      const long long mine = live ? (long long)(w.first + token) * a.q_stride + (size_t)hq * D : -1;
+      const int c = lane % LANES;
+      uint8_t* const rows = smem + L::Q + t * L::TILE + (warp & 3) * (32 * 128) + (c >> 3) * L::HALF;
+      uint4 u[LANES];
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        u[i] = live ? src[i] : make_uint4(0, 0, 0, 0);
-        const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+      for (int i = 0; i < LANES; ++i) {
+        const long long from = __shfl_sync(FULL, mine, i * PER + lane / LANES);
+        u[i] = from >= 0 ? *reinterpret_cast<const uint4*>(a.q + from + 8 * c) : make_uint4(0, 0, 0, 0);
+      }
+      int e_mine = 0;
+#pragma unroll
+      for (int i = 0; i < LANES; ++i) {
+        uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w}, most = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) most = max(most, max(x[k] << 16 & 0x7FFF0000u, x[k] & 0x7FFF0000u));
-      }
-      const int e = q_exp(most);
-      const float down = pow2i(-e);
-      q_up = pow2i(e);
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        for (int o = LANES / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(FULL, most, o));
+        const int e = q_exp(most), theirs = __shfl_sync(FULL, e, (lane % PER) * LANES);
+        if (lane / PER == i) e_mine = theirs;
+        const float down = pow2i(-e);
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = pack_f16(__uint_as_float(x[k] << 16) * down, __uint_as_float(x[k] & 0xFFFF0000u) * down);
-        *reinterpret_cast<uint4*>(row + (i >> 3) * L::HALF + (((i & 7) ^ (lane & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+        const int r = i * PER + lane / LANES;
+        *reinterpret_cast<uint4*>(rows + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
       }
+      q_up = pow2i(e_mine);
       fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(qfull + t);
     }
+    meet();
+    const uint32_t tmem = *slot_at + ((uint32_t)((warp & 3) * 32) << 16), ts = tmem + t * 128, to = tmem + 256 + t * D;
     // The second row tile begins when the first has its first P: from then on each has the special function units to itself while the
     // other's products run
     if (t == 1 && count > 0 && w.count0 > 0) ok = mbar_wait(pfull + 2, 0);
@@ -334,30 +339,53 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
         ml[0] = l > 0.f || l != l ? m : -INFINITY;
         ml[1] = l;
       }
+      if (c.parts.splits > 1) {
+        float* const o = c.parts.o + (r * c.parts.splits + w.split) * D;
 #pragma unroll
-      for (int q = 0; q < D / 32; ++q) {
-        uint32_t v[32];
-        if (count > 0) {
-          tm_ld32(to + 32 * q, v);
-          tm_wait_ld<32>(v);
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t v[32];
+          if (count > 0) {
+            tm_ld32(to + 32 * q, v);
+            tm_wait_ld<32>(v);
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
+          if (live)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) reinterpret_cast<uint4*>(o + 32 * q)[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+          __syncwarp();
         }
+      } else {
+        // the warp's rows leave through where its rows of q were (their last scores are done), D / 8 lanes a row
+        constexpr int LANES = D / 8, PER = 32 / LANES;
+        uint8_t* const rows = smem + L::Q + t * L::TILE + (warp & 3) * (32 * 2 * D);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
-        if (live && c.parts.splits > 1) {
-          uint4* const o = reinterpret_cast<uint4*>(c.parts.o + (r * c.parts.splits + w.split) * D + 32 * q);
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t v[32];
+          if (count > 0) {
+            tm_ld32(to + 32 * q, v);
+            tm_wait_ld<32>(v);
+          }
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-        } else if (live) {
-          uint4* const o = reinterpret_cast<uint4*>(a.out + (long long)(w.first + token) * a.out_stride + (size_t)hq * D + 32 * q);
+          for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             uint32_t u[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) u[i] = pack_bf16(__uint_as_float(v[8 * k + 2 * i]), __uint_as_float(v[8 * k + 2 * i + 1]));
-            o[k] = make_uint4(u[0], u[1], u[2], u[3]);
+            *reinterpret_cast<uint4*>(rows + lane * (2 * D) + (((4 * q + k) ^ (lane & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
           }
         }
         __syncwarp();
+        const long long mine = live ? (long long)(w.first + token) * a.out_stride + (size_t)hq * D : -1;
+#pragma unroll
+        for (int i = 0; i < LANES; ++i) {
+          const int row = i * PER + lane / LANES;
+          const long long out = __shfl_sync(FULL, mine, row);
+          if (out >= 0)
+            *reinterpret_cast<uint4*>(a.out + out + 8 * (lane % LANES)) =
+                *reinterpret_cast<const uint4*>(rows + row * (2 * D) + (((lane % LANES) ^ (row & 7)) << 4));
+        }
       }
     }
     tc_fence_before();
@@ -388,6 +416,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     auto exps_of = [&](int e) -> uint32_t {
       return e >= 0 ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(a.exps) + (size_t)e * a.H + w.h) : 0u;
     };
+    if (lane == 0) {
+      mbar_init(my_raw, 1);
+      mbar_init(my_raw + 1, 1);
+      fence_barrier_init();
+    }
+    __syncwarp();
     int now = entry(0), next = -1;
     uint32_t now_x = exps_of(now), next_x = 0;
     auto fetch = [&](int j, int kvi, int e) {                     // e: the entries of tile j's sixteen
@@ -404,6 +438,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
       fetch(0, 0, now);
       fetch(0, 1, now);
     }
+    meet();
     bool ok = true;
     for (int j = 0; ok && j < tiles; ++j) {
       const int s = j & 1, at = 2 * (j & 15);
@@ -477,6 +512,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     // (and a commit covers all before it): S of the next key tile may take the place of the P that the product before it reads
     // (mma_idesc's operands are BF16; FP16 is type 0)
     constexpr uint32_t FP16 = ~(1u << 7 | 1u << 10), IDESC_S = mma_idesc(128, KEYS) & FP16, IDESC_O = (mma_idesc(128, D) & FP16) | 1u << 16;
+    meet();
+    const uint32_t tmem = *slot_at;
     // The whole loop runs in one elected thread, waits included: a warp that meets again around each step costs more than the steps
     if (elect_one()) {
       const uint32_t dq = desc_k(smem_addr(smem + L::Q)), dk = desc_k(smem_addr(smem + L::K)), dv = desc_mn(smem_addr(smem + L::V), L::HALF);
@@ -505,9 +542,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           if (ok && (t ? w.count1 : w.count0) > 0) {
-            ok = mbar_wait(qfull + t, 0);
             tc_fence_after();
-            if (ok) scores(t, 0);
+            scores(t, 0);
           }
       }
       for (int j = 0; ok && j < tiles; ++j) {
@@ -544,12 +580,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     }
     __syncwarp();
     tc_fence_before();
+    } else {
+      meet();                                                     // (behind regs_down: the softmax warps wait for those registers)
     }
   }
   __syncthreads();
   if (warp == W_MMA) {
     tc_fence_after();
-    tmem_dealloc<1>(tmem, 512);
+    tmem_dealloc<1>(*slot_at, 512);
   }
 }
 
