@@ -20,8 +20,8 @@ using namespace st;
 //     new rows are rounded at e', the others again at e' if it differs from the old exponent, or cleared if row 0 is among the new
 // Which warp: the last token of the call in a page leads it.
 //   SCAN  (calls of up to SCAN_MAX tokens) a warp per (token, unit) walks the call's slots and finds out itself
-//   else  kv8_mark_kernel leaves every row's and page's last token in `marks`; a CTA takes sixteen tokens of the call, all units of
-//         the pages they lead, and clears what it read
+//   else  kv8_mark_kernel leaves every row's and page's last token in `marks`; a CTA takes sixteen tokens of the call, clears the marks
+//         of the pages they lead and writes all units of those
 // Same slot twice: the last one counts in both.  Values that are not finite are stored as the largest of their sign (infinities) or
 // as zero (NaN), and flagged in *bad.
 constexpr int SCAN_MAX = 512;
@@ -276,8 +276,9 @@ __global__ void __launch_bounds__(256) kv8_mark_kernel(const Append8 a) {
 }
 
 template <int D, bool SCAN>
-__global__ void __launch_bounds__(256) kv8_append_kernel(const Append8 a) {
-  __shared__ int s_row[8][PAGE];
+__global__ void __launch_bounds__(256, 2) kv8_append_kernel(const Append8 a) {
+  __shared__ int s_row[PAGE][PAGE];
+  __shared__ long long s_page[PAGE];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, units = 2 * a.H;
@@ -307,23 +308,31 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const Append8 a) {
     __syncwarp();
     append_unit<D>(a, page, u >> 1, u & 1, lane < PAGE ? row[lane] : -1, lane);
   } else {
-    const int i = (int)blockIdx.x * PAGE + lane;
-    const long long s = lane < PAGE && i < a.N ? a.slot[i] : -1;
-    const bool leads = slot_ok(a, s) && a.marks[a.nblocks * PAGE + s / PAGE] == i + 1;
-    unsigned left = __ballot_sync(FULL, leads);    // (the same in every warp: a mark of this CTA's pages is cleared below, behind a barrier)
-    const unsigned all = left;
-    for (; left; left &= left - 1) {
-      const long long page = __shfl_sync(FULL, s, __ffs(left) - 1) / PAGE;
-      const int tok = lane < PAGE ? a.marks[page * PAGE + lane] - 1 : -1;
-      for (int u = warp; u < units; u += 8) append_unit<D>(a, page, u >> 1, u & 1, tok, lane);
+    if (warp == 0) {
+      const int i = (int)blockIdx.x * PAGE + lane;
+      const long long s = lane < PAGE && i < a.N ? a.slot[i] : -1;
+      const bool leads = slot_ok(a, s) && a.marks[a.nblocks * PAGE + s / PAGE] == i + 1;
+      if (lane < PAGE) s_page[lane] = -1;
+      __syncwarp();
+      int n = 0;
+      for (unsigned left = __ballot_sync(FULL, leads); left; left &= left - 1, ++n) {
+        const long long page = __shfl_sync(FULL, s, __ffs(left) - 1) / PAGE;
+        if (lane < PAGE) {                         // (nobody else reads these marks: the page's other tokens do not lead it)
+          s_row[n][lane] = a.marks[page * PAGE + lane] - 1;
+          a.marks[page * PAGE + lane] = 0;
+        }
+        if (lane == 0) {
+          s_page[n] = page;
+          a.marks[a.nblocks * PAGE + page] = 0;
+        }
+      }
     }
     __syncthreads();
-    if (warp == 0)
-      for (left = all; left; left &= left - 1) {
-        const long long page = __shfl_sync(FULL, s, __ffs(left) - 1) / PAGE;
-        if (lane < PAGE) a.marks[page * PAGE + lane] = 0;
-        if (lane == PAGE) a.marks[a.nblocks * PAGE + page] = 0;
-      }
+    // (keys of all heads, then values: every warp has some of both)
+    for (int n = 0; n < PAGE && s_page[n] >= 0; ++n) {
+      const int tok = lane < PAGE ? s_row[n][lane] : -1;
+      for (int u = warp; u < units; u += 8) append_unit<D>(a, s_page[n], u < a.H ? u : u - a.H, u >= a.H, tok, lane);
+    }
   }
 }
 

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     // ---- the warp's 32 rows of q as FP16, each times a power of two that its largest value asks for: D / 8 lanes read a row
     if (count > 0) {
       constexpr int LANES = D / 8, PER = 32 / LANES;
-      const long long mine = live ? (long long)(w.first + token) * a.q_stride + (size_t)hq * D : -1;
+      const long long mine = live ? (long long)(w.first + token) * a.q_stride + (long long)hq * D : -1;
       const int c = lane % LANES;
       uint8_t* const rows = smem + L::Q + t * L::TILE + (warp & 3) * (32 * 128) + (c >> 3) * L::HALF;
       uint4 u[LANES];
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
           }
         }
         __syncwarp();
-        const long long mine = live ? (long long)(w.first + token) * a.out_stride + (size_t)hq * D : -1;
+        const long long mine = live ? (long long)(w.first + token) * a.out_stride + (long long)hq * D : -1;
 #pragma unroll
         for (int i = 0; i < LANES; ++i) {
           const int row = i * PER + lane / LANES;
