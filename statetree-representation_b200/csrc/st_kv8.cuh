@@ -3,7 +3,7 @@
 // Page: uint8 [blocks, H, 2 (K/V), 16, D] e4m3 codes and int8 exps [blocks, H, 2]; value = e4m3(code) * 2^exp, exp in [E8_MIN, E8_MAX].
 // A power of two, because the codes are floating point: a finer scale would not make them more precise, and a page whose largest value
 // grows as tokens arrive changes its exponent without rounding again (but for codes that become subnormal).  Every value has four
-// significant bits, so it is a BF16 number exactly and the tensor cores read it without a rounding of their own.
+// significant bits, so it is a BF16 number (and the code an FP16 one) exactly and the tensor cores read it without a rounding.
 //
 // At D = 128 the 16-byte pieces of a row are kept in another order (piece8): rows are 128 B apart, and both ways in which a warp of the
 // decode kernel reads a page (eight rows x four pieces for keys, four even or odd rows x two pieces for values) then touch every bank
@@ -27,9 +27,9 @@ __device__ __forceinline__ int page8_exp(int e) { return min(max(e, E8_MIN), E8_
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
 // Four codes -> their BF16 bit patterns times 2^-120: the four exponent and three mantissa bits are put at the low end of BF16's
-// exponent field and the top of its mantissa, code 0 .. 7 of an exponent (subnormal) becoming subnormals, so the value is exact
-// without a multiplication; 2^120 goes into a factor that is applied anyway.  High bytes hi = s0000eee, low bytes lo = emmm0000.
-// (The codes 0x7F and 0xFF, which no append writes, read as +-480.)
+// exponent field and the top of its mantissa, subnormal codes becoming subnormals, so the value is exact without a multiplication;
+// 2^120 goes into a factor that is applied anyway.  High bytes hi = s0000eee, low bytes lo = emmm0000.
+// (The codes 0x7F and 0xFF, not a number in e4m3, are written by no append; here they read as +-480.)
 __device__ __forceinline__ void codes_split(uint32_t w, uint32_t& lo, uint32_t& hi) {
   hi = ((w & 0x70707070u) >> 4) | (w & 0x80808080u);
   lo = (w & 0x0F0F0F0Fu) << 4;
@@ -67,8 +67,10 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// q * 2^-e has its largest magnitude (fp32 bits `most`) in [2^13, 2^14); 0 for zeros
-__device__ __forceinline__ int q_exp(uint32_t most) { return most < 0x00800000u ? 0 : min((int)(most >> 23) - 127, 126) - 13; }
+// q * 2^-e has its largest magnitude (fp32 bits `most`) in [2^13, 2^14); 0 for zeros; at least -100, so that 2^-e is a number
+__device__ __forceinline__ int q_exp(uint32_t most) {
+  return most < 0x00800000u ? 0 : max(min((int)(most >> 23) - 127, 126) - 13, -100);
+}
 
 // the reference that probabilities are relative to (base 2, P = 2^(x - r)): between UNDER8 and RAISE8 below the largest x
 constexpr float UNDER8 = 7.f, RAISE8 = 15.f;

@@ -187,8 +187,9 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
             if q.stride(-1) != 1 or q.stride(1) != D:
                 q = q.contiguous()
             scale = float(scaling) if scaling is not None else D ** -0.5
+            more = dict(window=kwargs.get("sliding_window") or 0) if c.eight_bit else {}
             out = layer.store.attention(q, c.table32[:B], c.lens[:B], scale, splits=c.splits, starts=c.starts[:B],
-                                        min_pages=4)
+                                        min_pages=4, **more)
             return out.view(B, 1, Hq, D), None
         if T > 1 and not c.starts_known and attention_mask is not None and attention_mask.dim() == 4:
             last_row = attention_mask[:, 0, -1, :]                  # the last query sees everything but the padding
@@ -199,7 +200,7 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
             q = query.transpose(1, 2).reshape(B * T, Hq, D)
             cu = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=q.device)
             out = layer.store.chunk_attention(q, cu, c.table32[:B], c.lens[:B], float(scaling) if scaling is not None else D ** -0.5,
-                                              starts=c.starts[:B])
+                                              starts=c.starts[:B], window=kwargs.get("sliding_window") or 0)
             return out.view(B, T, Hq, D), None
     return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout, scaling=scaling, **kwargs)
 

@@ -169,6 +169,8 @@ class PageStore8:
     def attention(self, q, block_table, lens, scale, splits=None, starts=None, min_pages=4, out=None, window=0):
         """one query token per sequence: q [B, Hq, D] bf16 -> [B, Hq, D] bf16; tokens [max(starts, lens - window), lens) take part
         (window 0: from starts on).  splits: how many CTAs share a sequence (None: by batch size and table width)"""
+        if q.dim() == 3 and q.shape[1] > FEW_ROWS8 * self.H:    # (many heads to a KV head: rows enough for a tile)
+            return self.chunk_attention(q, None, block_table, lens, scale, splits, starts, out, window)
         if splits is None:
             splits = decode_splits8(block_table.shape[0] * self.H * -(-q.shape[1] // (8 * self.H)), block_table.shape[1])
         host = calls()

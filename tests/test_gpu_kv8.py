@@ -375,6 +375,81 @@ def test_chunk_of_one_token_is_a_decode_step():
         _check(store.chunk_attention(q, cu, table, _ints(lens), 0.1), q, seqs, [0, 1, 2, 3], lens, 0.1)
 
 
+@pytest.mark.parametrize("size", [0.0, 1e-38, 1e-30, 1e30])
+def test_attention_of_queries_of_any_size(size):
+    """zero and tiny queries (all keys alike), huge ones"""
+    gen = _gen(17)
+    lens = [50, 33]
+    store, table, seqs = _filled(gen, lens, 1, 64, size=1e-3)
+    q = (torch.randn(70, 4, 64, generator=gen) * size).to(torch.bfloat16).to(DEV)
+    scale = 0.1 if size < 1 else 1e-28
+    _check(store.attention(q[:2], table, _ints(lens), scale), q[:2], seqs, [0, 1, 2], lens, scale)
+    for cu in ([0, 3, 5], [0, 40, 70]):
+        _check(store.chunk_attention(q[:cu[-1]], _ints(cu), table, _ints(lens), scale), q, seqs, cu, lens, scale)
+
+
+@pytest.mark.parametrize("G", [33, 64])
+def test_decode_attention_of_many_heads_to_one(G):
+    gen = _gen(G)
+    lens = [300, 1, 0, 77]
+    store, table, seqs = _filled(gen, lens, 1, 128)
+    q = _rand(gen, 4, G, 128, size=1.5).to(DEV)
+    got = store.attention(q, table, _ints(lens), 0.09)
+    assert not got[2].any()
+    _check(got, q, seqs, [0, 1, 2, 3, 4], lens, 0.09)
+
+
+def test_pages_beyond_four_gigabytes():
+    """offsets of pages and their rows that 32 bits do not hold"""
+    H, D, n = 8, 128, 40
+    blocks = (1 << 32) // (H * 2 * PAGE * D) + 20
+    gen = _gen(21)
+    store = _store(blocks, H, D)
+    last = torch.tensor([blocks - 1, 3, blocks - 7])
+    p = torch.arange(n)
+    K, V = _keys(gen, n, H, D), _rand(gen, n, H, D)
+    for a, b in ((0, 20), (20, n)):
+        store.append(K[a:b].to(DEV), V[a:b].to(DEV), (last[p[a:b] // PAGE] * PAGE + p[a:b] % PAGE).to(DEV))
+    many = torch.cat([last[:1].repeat(600) * PAGE, last[p // PAGE] * PAGE + p % PAGE])       # (a long call; the last of each slot counts)
+    store.append(torch.cat([K[:1].repeat(600, 1, 1), K]).to(DEV), torch.cat([V[:1].repeat(600, 1, 1), V]).to(DEV), many.to(DEV))
+    assert int(store.marks.abs().max()) == 0
+    ref = R.Pages(3, H, D)
+    ref.append(K.double(), V.double(), p)
+    kd, vd = store.dense(last.to(DEV))
+    assert torch.equal(kd.cpu().double(), ref.dense()[0]) and torch.equal(vd.cpu().double(), ref.dense()[1])
+    seqs = [tuple(t.flatten(0, 1)[:n] for t in ref.dense())]
+    table = last[None].to(torch.int32).to(DEV)
+    q = _rand(gen, 40, 16, D).to(DEV)
+    _check(store.attention(q[:1], table, _ints([n]), 0.1, splits=2, min_pages=1), q[:1], seqs, [0, 1], [n], 0.1)
+    for m in (3, 40):
+        _check(store.chunk_attention(q[:m], _ints([0, m]), table, _ints([n]), 0.1), q[:m], seqs, [0, m], [n], 0.1)
+
+
+def test_native_and_general_calls_agree(monkeypatch):
+    """the same bits without the native host path"""
+    gen = _gen(23)
+    lens = [90, 20]
+    store, table, _ = _filled(gen, lens, 2, 128)
+    cos, sin = (t.to(DEV) for t in _tables(128, 100))
+    K, V, q = _keys(gen, 3, 2, 128).to(DEV), _rand(gen, 3, 2, 128).to(DEV), _rand(gen, 3, 8, 128).to(DEV)
+    slots = torch.tensor([int(table[0, 5]) * PAGE + 10, int(table[1, 1]) * PAGE + 4, -1], device=DEV)
+    before = store.pages.clone(), store.exps.clone()
+
+    def calls():
+        store.pages.copy_(before[0])
+        store.exps.copy_(before[1])
+        r = store.append(K, V, slots, positions=torch.tensor([90, 20, 5], device=DEV), cos=cos, sin=sin, q=q)
+        return [r, store.pages.clone(), store.exps.clone(), store.attention(r[:2], table, _ints([91, 21]), 0.1),
+                store.attention(r[:2], table, _ints([91, 21]), 0.1, splits=3, window=7, starts=_ints([1, 2]), out=torch.zeros_like(r[:2])),
+                store.chunk_attention(r, _ints([0, 2, 3]), table, _ints([91, 21]), 0.1), *store.dense(table[0, :3].contiguous()), *store.dense()]
+
+    from statetree_b200 import kvcache
+    assert kvcache.calls() is not None
+    native = calls()
+    monkeypatch.setattr(kvcache, "calls", lambda: None)
+    assert all(torch.equal(a, b) for a, b in zip(native, calls()))
+
+
 def test_attention_strided():
     """queries inside fused rows, an output inside a larger one, a block table that is part of a wider one"""
     gen = _gen(6)
