@@ -19,12 +19,16 @@ using namespace st;
 //     e' = the smallest exponent that holds the new rows; the page's old one if that is larger and the page does not start anew
 //     new rows are rounded at e', the others again at e' if it differs from the old exponent, or cleared if row 0 is among the new
 // Which warp: the last token of the call in a page leads it.
-//   SCAN  (calls of up to SCAN_MAX tokens) a warp per (token, unit) walks the call's slots and finds out itself
-//   else  kv8_mark_kernel leaves every row's and page's last token in `marks`; a CTA takes sixteen tokens of the call, clears the marks
-//         of the pages they lead and writes all units of those
+//   SCAN  (calls of up to SCAN_MAX tokens, where the two meet: keys and values of 16, 256, 512 sequences with a token each 4.6, 9.1,
+//         17.3 us so, 7.2, 8.9, 14.9 with marks) a warp per (token, unit) walks the call's slots and finds out itself
+//   else  kv8_mark_kernel leaves every row's and page's last token in `marks`; a CTA takes up to sixteen tokens of the call, clears the
+//         marks of the pages they lead and writes all units of those (fewer tokens in shorter calls, which may lead a page each: 1024
+//         sequences 73 us with sixteen, 25 with one)
+// One token (8 KV heads, 32 query heads) 4.4 us, bound by look-ups that follow one another; 32764 tokens 179 us (755 MB), of which keys
+// and values take 84 (16 warps an SM have too little in flight beside the 64 values that a lane holds) and the queries 95 (HBM).
 // Same slot twice: the last one counts in both.  Values that are not finite are stored as the largest of their sign (infinities) or
 // as zero (NaN), and flagged in *bad.
-constexpr int SCAN_MAX = 512;
+constexpr int SCAN_MAX = 256;
 
 struct Append8 {
   const uint16_t* K; const uint16_t* V; const uint16_t* Q;
@@ -38,6 +42,7 @@ struct Append8 {
   uint16_t* q_out;
   int* marks; int* bad;
   int N, H, Hq;
+  int run;                                         // tokens of the call that a CTA looks at (without SCAN), up to sixteen
   int q_cta, q_units, q_steps;                     // first CTA that works on queries; warps per token, groups of heads per warp
   float eps;
   int pairs;
@@ -309,8 +314,8 @@ __global__ void __launch_bounds__(256, 2) kv8_append_kernel(const Append8 a) {
     append_unit<D>(a, page, u >> 1, u & 1, lane < PAGE ? row[lane] : -1, lane);
   } else {
     if (warp == 0) {
-      const int i = (int)blockIdx.x * PAGE + lane;
-      const long long s = lane < PAGE && i < a.N ? a.slot[i] : -1;
+      const int i = (int)blockIdx.x * a.run + lane;
+      const long long s = lane < a.run && i < a.N ? a.slot[i] : -1;
       const bool leads = slot_ok(a, s) && a.marks[a.nblocks * PAGE + s / PAGE] == i + 1;
       if (lane < PAGE) s_page[lane] = -1;
       __syncwarp();
@@ -394,6 +399,8 @@ __global__ void __launch_bounds__(256) kv8_dequant_kernel(const uint8_t* __restr
 // Work split: grid = sequences x KV heads x head blocks x splits; a CTA's pages go round-robin to its warps, each of which streams its
 // own through a private ring of bulk copies (a page of one head is contiguous, 2 * 16 * D bytes), so there is no barrier in the loop.
 // Block-table entries and exponents come 32 pages at a time, one batch ahead.
+// Measured (32 query heads, 8 KV heads, D = 128, in a graph): 64 sequences of up to 8192 tokens 90 us = 5.9 TB/s, one of 61003 25 us, one of
+// 1000 6.2 us.
 __device__ __forceinline__ float over_rows_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
@@ -759,7 +766,8 @@ int attn8_launch(const Attn8& a, const Parts8& parts, long long ctas, cudaStream
   return st::launch("st_kv8_attn launch", kv8_attn_kernel<D, NW, STG, CHUNK>, dim3((unsigned)ctas), dim3(NW * 32), (size_t)smem, st_, a,
                     parts, st::status_ptr());
 }
-// An SM holds sixteen warps: four CTAs of four, or two of eight for a grid of at most two CTAs per SM
+// An SM holds sixteen warps: four CTAs of four, or two of eight for a grid of at most two CTAs per SM (us with eight / four warps, 8 KV heads,
+// lengths spread: 128 CTAs, 1 x 16K 10.7 / 13.4; 256, 4 x 16K 20.9 / 24.4; 512, 16 x 16K 61.1 / 57.5, 32 x 4K 33.7 / 30.6)
 template <bool CHUNK>
 int attn8_any(const Attn8& a, const Parts8& parts, int D, long long ctas, cudaStream_t st_) {
   ST_REQUIRE(ctas < (1ll << 31), "st_kv8_attn: grid too large");
@@ -815,8 +823,10 @@ extern "C" int st_kv8_append(const void* K, const void* V, int64_t ks, int64_t v
   a.wq = (const uint16_t*)wq; a.wk = (const uint16_t*)wk; a.q_out = (uint16_t*)q_out; a.marks = marks; a.bad = bad;
   a.N = (int)N; a.H = (int)H; a.Hq = Q ? (int)Hq : 0; a.eps = (float)eps; a.pairs = interleaved ? 1 : 0;
   const cudaStream_t st_ = (cudaStream_t)stream;
-  const long long page_ctas = scan ? (N * H * 2 + 7) / 8 : (N + st::PAGE - 1) / st::PAGE;
-  // queries: a warp per group of heads while that leaves SMs without one, else up to eight groups of a token
+  a.run = (int)std::min<long long>(st::PAGE, std::max<long long>(1, N / (8ll * st::sm_count())));
+  const long long page_ctas = scan ? (N * H * 2 + 7) / 8 : (N + a.run - 1) / a.run;
+  // queries: a warp per group of heads while that leaves SMs without one, else up to eight groups of a token (the whole append, us with
+  // one / eight groups: 16 sequences 4.6 / 5.0, 2048 tokens of one 17.7 / 16.0, 4096 41.4 / 24.2)
   const int groups = (int)((a.Hq + 512 / D - 1) / (512 / D));
   a.q_steps = (int)std::min<long long>(std::min(std::max(groups, 1), 8), std::max<long long>(1, N * groups / (16ll * st::sm_count())));
   a.q_units = groups ? (groups + a.q_steps - 1) / a.q_steps : 0;

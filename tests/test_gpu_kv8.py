@@ -37,7 +37,7 @@ def _same(store, ref):
 
 # ------------------------------------------------------------------------------------------------ append
 @pytest.mark.parametrize("D,H", [(128, 1), (128, 8), (64, 3)])
-@pytest.mark.parametrize("calls", [(1,), (16,), (5, 1, 1, 20, 3), (40, 600, 1, 7), (513,)])
+@pytest.mark.parametrize("calls", [(1,), (16,), (5, 1, 1, 20, 3), (40, 600, 1, 7), (257,), (2401,)])
 def test_append_in_order(D, H, calls):
     """a sequence that grows over several calls (whole pages, parts of pages, single tokens; short and long calls)"""
     gen = _gen(sum(calls) + D + H)
@@ -58,7 +58,7 @@ def test_append_in_order(D, H, calls):
         assert torch.equal(got.cpu().double()[:3], want[[blocks - 1, 0, 0]]) and not got[3:].any()
 
 
-@pytest.mark.parametrize("n", [1, 33, 512, 700])
+@pytest.mark.parametrize("n", [1, 33, 256, 257, 700, 2500])
 def test_append_any_order(n):
     """slots in any order, padding and slots beyond the cache, the same slot several times (the last token counts), pages that do
     not start anew and pages that do"""
