@@ -13,6 +13,11 @@
 // bits, a page's key exponent is a factor of its sixteen score columns, its value exponent joins the softmax exponent of its sixteen
 // columns of P and is taken out of the sum per page.  P is rounded to FP16 (2^-11 of each at most, and 2^-32 of the largest), everything
 // else but the output is fp32.
+//
+// Measured (32 query heads, 8 KV heads, D = 128): 2048 queries behind 30000 tokens 1.02 ms = 1.0 PFLOP/s, a prompt of 4096 tokens 172 us.
+// A key tile takes 2.3 us for the 256 rows: a row tile's softmax about 2300 cycles, its MMAs and the hand-overs 1200, of which the other
+// row tile's overlap most; the MMAs by themselves 2270 cycles for both.  Shared memory is busy 2560 of its cycles (operands 192 KB,
+// conversion 128 KB).  A CTA costs about 8 us besides (look-ups, q, first pages, output).
 #include <math.h>
 
 #include <atomic>
