@@ -184,8 +184,10 @@ __device__ __forceinline__ void append_unit(const Append8& a, long long page, in
         row_rotate(f[i], t, a.pairs);
       }
     }
+    uint32_t m = 0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) most = max(most, __float_as_uint(f[i][k]) & 0x7FFFFFFFu);
+    for (int k = 0; k < 16; ++k) m = max(m, __float_as_uint(f[i][k]) & 0x7FFFFFFFu);
+    if (mine[i] >= 0) most = max(most, m);         // (norm and rotation can make NaN of a row without a token: 0 * rsqrt(0))
   }
   most = __reduce_max_sync(FULL, most);
   const bool odd = most > __float_as_uint(448.f * pow2i(E8_MAX));        // (a value that is not finite, or beyond the format)

@@ -132,7 +132,9 @@ class PageStore8:
 
     @classmethod
     def over(cls, pages, exps):
-        """a store over page tensors that exist already (another store's, or part of a larger buffer)"""
+        """a store over page tensors that exist already (another store's, or part of a larger buffer), which are zero or written by
+        append: the codes 0x7F and 0xFF, which it never writes, are no numbers and must not stand in a page that is read, masked rows
+        included"""
         self = cls.__new__(cls)
         self._take(pages, exps)
         return self

@@ -128,6 +128,25 @@ def test_append_what_the_format_cannot_hold(bad):
     store.check()
 
 
+@pytest.mark.parametrize("n", [1, 300])
+def test_append_without_an_epsilon(n):
+    """norms with eps = 0: rows of a page that no token goes to are not taken for values (0 * rsqrt(0) is not a number)"""
+    H, D = 2, 128
+    gen = _gen(n)
+    K, V = _keys(gen, n, H, D), _rand(gen, n, H, D)
+    w = (1 + 0.1 * torch.randn(D, generator=gen)).to(torch.bfloat16)
+    slots = torch.arange(n) + 2
+    store, other = _store(n // PAGE + 2, H, D), _store(n // PAGE + 2, H, D)
+    store.append(K.to(DEV), V.to(DEV), slots.to(DEV), k_norm=w.to(DEV), eps=0.0)
+    store.check()
+    other.append(K.to(DEV), V.to(DEV), slots.to(DEV), k_norm=w.to(DEV), eps=1e-30)       # (the same sum in fp32)
+    assert torch.equal(store.pages, other.pages) and torch.equal(store.exps, other.exps)
+    K[0, 1] = 0                                            # a token that is zero has no norm
+    store.append(K.to(DEV), V.to(DEV), slots.to(DEV), k_norm=w.to(DEV), eps=0.0)
+    with pytest.raises(RuntimeError, match="not finite"):
+        store.check()
+
+
 def _tables(D, span):
     inv = 1e6 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)
     ang = torch.arange(span, dtype=torch.float64)[:, None] * inv
