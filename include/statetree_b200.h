@@ -253,14 +253,18 @@ int st_kv8_dequant_blocks(const void* kv, const int8_t* exps, int64_t nblocks, i
                           void* Kd, void* Vd, void* stream);
 /* Decode attention, one query token per sequence: q, out BF16 [B, Hq, D] (16-byte aligned, token strides qs / os multiples of 8); bt
  * int32 [B, bts]; keys [max(starts, lens - window), lens) take part (starts int32 [B] or NULL, window 0: none); a sequence without
- * any gives zeros.  S splits with >= minpps pages each; wo float [B, Hq, S, D], wml float [B, Hq, S, 2] when S > 1. */
+ * any gives zeros.  S splits with >= minpps pages each; wo float [B, Hq, S, D], wml float [B, Hq, S, 2] when S > 1 and
+ * st_kv8_attn_workspace_bytes (which is what both take together) is not 0. */
 int st_kv8_attn(const void* q, int64_t qs, int64_t B, int64_t Hq, const void* kv, const int8_t* exps, int64_t nblocks, int64_t Hkv,
                 int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens, const int32_t* starts, int64_t window, void* out,
                 int64_t os, float* wo, float* wml, double scale, int64_t S, int64_t minpps, void* stream);
+/* Bytes that the partial results of S splits take: T query rows of B sequences (chunk: of st_kv8_chunk_attn); 0 where the splits join on
+ * chip (few of them, a small grid). */
+int64_t st_kv8_attn_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t S, int chunk);
 /* Causal attention of several query tokens per sequence, whose keys are in the pages already: q, out BF16 [T, Hq, D]; cu int32 [B + 1]:
  * sequence b's queries are rows cu[b] .. cu[b + 1] - 1, the last at position lens[b] - 1 (cu NULL: one each).  A query at position p
  * sees keys [max(starts, p - window + 1), p].  Rows of q behind cu[B] are left alone in out.  wo float [T, Hq, S, D], wml float [T, Hq,
- * S, 2] when S > 1. */
+ * S, 2] when S > 1 and st_kv8_attn_workspace_bytes is not 0. */
 int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
                       const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens,
                       const int32_t* starts, int64_t window, void* out, int64_t os, float* wo, float* wml, double scale, int64_t S,

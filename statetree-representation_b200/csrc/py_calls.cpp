@@ -42,6 +42,7 @@ struct Library {
   decltype(&st_kv8_dequant_blocks) kv8_dequant;
   decltype(&st_kv8_attn) kv8_attn;
   decltype(&st_kv8_chunk_attn) kv8_chunk;
+  decltype(&st_kv8_attn_workspace_bytes) kv8_workspace;
 };
 
 // rows of x if it can be read as it is: BF16 [..., N] on `device`, contiguous, 16-byte aligned, at least one row; else 0
@@ -87,6 +88,7 @@ Library library(const std::map<std::string, uint64_t>& address) {
   bind(lib.kv8_dequant, "st_kv8_dequant_blocks");
   bind(lib.kv8_attn, "st_kv8_attn");
   bind(lib.kv8_chunk, "st_kv8_chunk_attn");
+  bind(lib.kv8_workspace, "st_kv8_attn_workspace_bytes");
   return lib;
 }
 
@@ -319,8 +321,8 @@ py::object kv8_attention(const Library& lib, bool chunk, const at::Tensor& pages
     const c10::cuda::CUDAGuard guard(device);
     out = given ? *given : at::empty(q.sizes(), q.options().requires_grad(false));
     float *wo = nullptr, *wml = nullptr;
-    if (splits > 1) {                                             // partial results of this call alone
-      ws = at::empty({T * Hq * splits * (D + 2)}, q.options().requires_grad(false).dtype(at::kFloat));
+    if (const int64_t need = lib.kv8_workspace(T, B, Hq, H, D, splits, chunk)) {      // partial results of this call alone
+      ws = at::empty({need / 4}, q.options().requires_grad(false).dtype(at::kFloat));
       wo = reinterpret_cast<float*>(ws.data_ptr());
       wml = wo + T * Hq * splits * D;
     }

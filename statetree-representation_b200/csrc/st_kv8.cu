@@ -400,9 +400,10 @@ __global__ void __launch_bounds__(256) kv8_dequant_kernel(const uint8_t* __restr
 //
 // Work split: grid = sequences x KV heads x head blocks x splits; a CTA's pages go round-robin to its warps, each of which streams its
 // own through a private ring of bulk copies (a page of one head is contiguous, 2 * 16 * D bytes), so there is no barrier in the loop.
-// Block-table entries and exponents come 32 pages at a time, one batch ahead.
-// Measured (32 query heads, 8 KV heads, D = 128, in a graph): 64 sequences of up to 8192 tokens 90 us = 5.9 TB/s, one of 61003 25 us, one of
-// 1000 6.2 us.
+// Block-table entries and exponents come 32 pages at a time, one batch ahead.  The splits of a unit join through distributed shared memory,
+// as a cluster, or through memory in a second kernel (joins8).
+// Measured (32 query heads, 8 KV heads, D = 128, in a graph): 64 sequences of up to 8192 tokens 90 us = 5.9 TB/s, one of 61003 23.6 us, one
+// of 1000 5.4 us.
 __device__ __forceinline__ float over_rows_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
@@ -420,6 +421,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 
 // CHUNK: several queries per sequence.  The eight columns are then rows (query, head) of the sequence's n * G, each with keys of its own
 // [lo, hi], and a tile of eight of them is looked up as in the chunk kernel; else they are heads of the one query.
+constexpr int JOIN8 = 8;                                          // splits that one cluster joins at most
 template <int D, int NW, int STG, bool CHUNK>
 __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 a, const Parts8 parts, int* status) {
   constexpr int PB = 2 * PAGE * D, KT = D / 16, VT = D / 16;             // bytes of a page, MMAs of its keys and of its values
@@ -644,7 +646,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
   // ---- the CTA's warps together.  The rings are idle now; each warp parks (O^T, r, l) of its heads there.
   __syncthreads();
   constexpr int ROW = D + 2, PER_WARP = 8 * ROW;
-  static_assert(PER_WARP * 4 <= STG * PB, "parked partials must fit in the ring");
+  static_assert((NW + 1) * PER_WARP * 4 <= NW * STG * PB, "parked partials must fit in the rings");
   float* const park = reinterpret_cast<float*>(smem);
   float* const mine = park + warp * PER_WARP;
 #pragma unroll
@@ -658,6 +660,8 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     if (head1) *reinterpret_cast<float2*>(mine + (2 * t + 1) * ROW + D) = make_float2(m1, l1);
   }
   __syncthreads();
+  const bool joined = parts.splits > 1 && parts.o == nullptr;     // the splits of a unit are one cluster
+  float* const sum = park + NW * PER_WARP;
   for (int e = threadIdx.x; e < heads * D; e += NW * 32) {
     const int h = e / D, d = e % D;
     float top = -INFINITY;
@@ -676,12 +680,43 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     if (parts.splits == 1) {
       const __nv_bfloat16 v = __float2bfloat16_rn(den > 0.f ? num / den : den);        // (a sum that is not a number stays one)
       a.out[(size_t)token * a.out_stride + (size_t)hq * D + d] = *reinterpret_cast<const uint16_t*>(&v);
+    } else if (joined) {
+      sum[h * ROW + d] = num;
+      if (d == 0) *reinterpret_cast<float2*>(sum + h * ROW + D) = make_float2(top, den);
     } else {
       const size_t ix = ((size_t)token * a.Hq + hq) * parts.splits + split;
       parts.o[ix * D + d] = num;
       if (d == 0) { parts.ml[ix * 2] = top; parts.ml[ix * 2 + 1] = den; }
     }
   }
+  if (!joined) return;
+  // ---- every CTA of the cluster joins a share of the heads' dims, all splits' partials in flight, in the order of the splits
+  cluster_sync_all();
+  for (int e = split * NW * 32 + threadIdx.x; e < heads * D; e += parts.splits * NW * 32) {
+    const int h = e / D, d = e % D;
+    float m[JOIN8], l[JOIN8], o[JOIN8], top = -INFINITY, den = 0.f, num = 0.f;
+#pragma unroll
+    for (int j = 0; j < JOIN8; ++j)
+      if (j < parts.splits) {
+        const uint32_t at = map_to_cta(smem_addr(sum + h * ROW), (uint32_t)j);
+        m[j] = ld_cluster_f32(at + D * 4);
+        l[j] = ld_cluster_f32(at + (D + 1) * 4);
+        o[j] = ld_cluster_f32(at + d * 4);
+      }
+#pragma unroll
+    for (int j = 0; j < JOIN8; ++j)
+      if (j < parts.splits) top = fmaxf(top, m[j]);
+#pragma unroll
+    for (int j = 0; j < JOIN8; ++j)
+      if (j < parts.splits && m[j] != -INFINITY) {                // (a split without tokens weighs nothing)
+        const float f = ex2(m[j] - top);
+        den += f * l[j];
+        num += f * o[j];
+      }
+    const __nv_bfloat16 v = __float2bfloat16_rn(den > 0.f ? num / den : den);
+    a.out[(size_t)token_of(h) * a.out_stride + (size_t)head_of(h) * D + d] = *reinterpret_cast<const uint16_t*>(&v);
+  }
+  cluster_sync_all();                                             // nobody leaves while a peer still reads its partials
 }
 
 // Weighs the split partials of a (token, query head) by exp2(m_j - max m) and normalises.  Latency bounds it: WPR warps share a row
@@ -765,25 +800,53 @@ int attn8_launch(const Attn8& a, const Parts8& parts, long long ctas, cudaStream
       return e;
     if (dev <= 63) set.fetch_or(1ull << dev);
   }
-  return st::launch("st_kv8_attn launch", kv8_attn_kernel<D, NW, STG, CHUNK>, dim3((unsigned)ctas), dim3(NW * 32), (size_t)smem, st_, a,
-                    parts, st::status_ptr());
+  if (parts.splits == 1 || parts.o)
+    return st::launch("st_kv8_attn launch", kv8_attn_kernel<D, NW, STG, CHUNK>, dim3((unsigned)ctas), dim3(NW * 32), (size_t)smem, st_,
+                      a, parts, st::status_ptr());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(NW * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st_;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)parts.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = st::pdl_enabled() ? 2 : 1;
+  return st::cuda_fail(cudaLaunchKernelEx(&cfg, kv8_attn_kernel<D, NW, STG, CHUNK>, a, parts, st::status_ptr()), "st_kv8_attn launch");
 }
+// Do the splits of a unit join on chip, as a cluster?  Up to a wave of CTAs (us on chip / through memory and a second launch: 7 CTAs a unit,
+// 1 x 1000 tokens 5.6 / 6.6; 64 CTAs, 1 x 4000 7.0 / 8.1; 256, 4 x 4000 9.5 / 10.7; 512, 16 x 4000 18.5 / 19.3, 8 x 16000 32.6 / 31.2),
+// beyond it CTAs wait for their cluster's to find room (32 x 4000 with four splits 33.0 / 31.5, 64 x 8000 with eight 104 / 88).
+bool joins8(long long ctas, int64_t splits) { return splits > 1 && splits <= JOIN8 && ctas <= 4ll * st::sm_count(); }
 // An SM holds sixteen warps: four CTAs of four, or two of eight for a grid of at most two CTAs per SM (us with eight / four warps, 8 KV heads,
 // lengths spread: 128 CTAs, 1 x 16K 10.7 / 13.4; 256, 4 x 16K 20.9 / 24.4; 512, 16 x 16K 61.1 / 57.5, 32 x 4K 33.7 / 30.6)
 template <bool CHUNK>
-int attn8_any(const Attn8& a, const Parts8& parts, int D, long long ctas, cudaStream_t st_) {
-  ST_REQUIRE(ctas < (1ll << 31), "st_kv8_attn: grid too large");
+int attn8_any(const char* who, const Attn8& a, const Parts8& given, int D, long long ctas, bool joined, cudaStream_t st_) {
+  ST_REQUIRE(ctas < (1ll << 31), "%s: grid too large", who);
+  Parts8 parts = given;
+  if (joined) parts.o = parts.ml = nullptr;
   const bool wide = ctas <= 2ll * st::sm_count();
-  if (D == 128)
-    return wide ? attn8_launch<128, 8, 3, CHUNK>(a, parts, ctas, st_) : attn8_launch<128, 4, 3, CHUNK>(a, parts, ctas, st_);
-  return wide ? attn8_launch<64, 8, 5, CHUNK>(a, parts, ctas, st_) : attn8_launch<64, 4, 5, CHUNK>(a, parts, ctas, st_);
+  int e;
+  if (D == 128) e = wide ? attn8_launch<128, 8, 3, CHUNK>(a, parts, ctas, st_) : attn8_launch<128, 4, 3, CHUNK>(a, parts, ctas, st_);
+  else e = wide ? attn8_launch<64, 8, 5, CHUNK>(a, parts, ctas, st_) : attn8_launch<64, 4, 5, CHUNK>(a, parts, ctas, st_);
+  return e || joined || parts.splits == 1 ? e : merge8(who, a, parts, D, st_);
+}
+long long decode_ctas(int64_t B, int64_t Hq, int64_t Hkv, int64_t S) { return B * Hkv * ((Hq / Hkv + 7) / 8) * S; }
+bool decode_joins(int64_t B, int64_t Hq, int64_t Hkv, int64_t S) { return joins8(decode_ctas(B, Hq, Hkv, S), S); }
+// (the grid has room for a part-filled tile of every sequence; about as many as the rows or the sequences need find work)
+bool rows8_joins(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t S) {
+  return joins8(std::max(B, (T * (Hq / Hkv) + 7) / 8) * Hkv * S, S);
 }
 }  // namespace
 
 namespace st {
-int rows8_attn(const Attn8& a, const Parts8& parts, int D, cudaStream_t st_) {
+int rows8_attn(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t st_) {
   const long long slots = a.T * (a.Hq / a.H) / 8 + a.B;
-  return attn8_any<true>(a, parts, D, slots * a.H * parts.splits, st_);
+  return attn8_any<true>(who, a, parts, D, slots * a.H * parts.splits, rows8_joins(a.T, a.B, a.Hq, a.H, parts.splits), st_);
 }
 int merge8(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t st_) {
   const long long rows = a.T * a.Hq;
@@ -889,12 +952,17 @@ extern "C" int st_kv8_attn(const void* q, int64_t qs, int64_t B, int64_t Hq, con
   if (int e = attn8_args(a, "st_kv8_attn", q, qs, B, Hq, nullptr, B, kv, exps, nblocks, Hkv, D, bt, bts, lens, starts, window, out, os, scale))
     return e;
   ST_REQUIRE(S >= 1 && S <= 1024, "st_kv8_attn: splits must be in [1, 1024]");
-  ST_REQUIRE(S == 1 || (wo && wml && st::aligned16(wo)), "st_kv8_attn: split workspace (wo, wml) missing or unaligned");
+  ST_REQUIRE((wo && wml && st::aligned16(wo)) || st_kv8_attn_workspace_bytes(B, B, Hq, Hkv, D, S, 0) == 0,
+             "st_kv8_attn: split workspace (wo, wml) missing or unaligned");
   if (B == 0) return 0;
   ST_REQUIRE(st::status_ptr() != nullptr, "st_kv8_attn: no device status word");
   const Parts8 parts = {wo, wml, (int)S, (int)(minpps < 1 ? 1 : minpps)};
   const cudaStream_t st_ = (cudaStream_t)stream;
-  const int e = attn8_any<false>(a, parts, (int)D, B * Hkv * ((Hq / Hkv + 7) / 8) * S, st_);
-  if (e || S == 1) return e;
-  return merge8("st_kv8_attn merge launch", a, parts, (int)D, st_);
+  return attn8_any<false>("st_kv8_attn", a, parts, (int)D, decode_ctas(B, Hq, Hkv, S), decode_joins(B, Hq, Hkv, S), st_);
+}
+
+extern "C" int64_t st_kv8_attn_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t S, int chunk) {
+  if (T <= 0 || B <= 0 || Hkv <= 0 || S <= 1) return 0;
+  if (!chunk ? decode_joins(B, Hq, Hkv, S) : few_rows8(T, B, Hq / Hkv) && rows8_joins(T, B, Hq, Hkv, S)) return 0;
+  return T * Hq * S * (D + 2) * 4;
 }

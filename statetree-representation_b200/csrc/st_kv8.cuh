@@ -88,6 +88,7 @@ struct Attn8 {
   long long T;
 };
 // partial results of sequences that are split: o [T, Hq, splits, D] (not normalised), ml [T, Hq, splits, 2] = (reference, base 2; sum)
+// (decode kernel: o = nullptr, the splits of a unit are a cluster that joins on chip)
 struct Parts8 { float* o; float* ml; int splits, min_pages; };
 
 // A CTA's rows, the same in all of its threads: rows row0 .. row0 + rows - 1 of the n * G rows (query, head of the group) of sequence b,
@@ -137,7 +138,11 @@ __device__ __forceinline__ bool find_rows(const Attn8& a, int G, int slot, int l
 int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
                const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens,
                const int32_t* starts, int64_t window, void* out, int64_t os, double scale);
-// chunks of few rows per sequence through the decode kernel, eight rows a CTA
-int rows8_attn(const Attn8& a, const Parts8& parts, int D, cudaStream_t stream);
+// Chunks of few rows per sequence go through the decode kernel, eight rows a CTA: its time grows with every eight rows, the chunk kernel's
+// hardly up to 128.  32 sequences of 2000 tokens, D = 128, us: 16 rows 38 in the decode kernel and 103 in the other, 32 rows 63 and 74, 64
+// rows 119 and 75.  D = 64: 28 rows 15 and 30, 56 rows 27 and 30, 112 rows 46 and 31.  (chunk_splits8 in kvcache.py states the same bound.)
+constexpr int FEW_ROWS = 32;
+inline bool few_rows8(long long T, long long B, long long G) { return T * G <= FEW_ROWS * B; }
+int rows8_attn(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t stream);
 int merge8(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t stream);
 }  // namespace st

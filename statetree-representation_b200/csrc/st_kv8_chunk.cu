@@ -30,10 +30,6 @@
 namespace {
 using namespace st;
 
-// Rows per sequence up to which a chunk goes through the decode kernel (chunk_splits8 in kvcache.py states the same): its time grows with
-// every eight rows, this kernel's hardly up to 128.  32 sequences of 2000 tokens, D = 128: 16 rows 38 us there, 103 here; 32 rows 63 and
-// 74; 64 rows 119 and 75.  D = 64: 28 rows 15 and 30, 56 rows 27 and 30, 112 rows 46 and 31.
-constexpr int FEW_ROWS = 32;
 constexpr int KEYS = 128, TILE_PAGES = KEYS / PAGE, ROWS = 128;
 constexpr int W_CONV = 8, W_MMA = 12, WARPS = 16;                 // softmax warps 0 .. 7 (tile = warp / 4); 13 .. 15 only lend registers
 constexpr int CRING = 4;                                          // page factors of so many key tiles are kept
@@ -621,7 +617,8 @@ extern "C" int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t H
                              os, scale))
     return e;
   ST_REQUIRE(S >= 1 && S <= 1024, "st_kv8_chunk_attn: splits must be in [1, 1024]");
-  ST_REQUIRE(S == 1 || (wo && wml && st::aligned16(wo)), "st_kv8_chunk_attn: split workspace (wo, wml) missing or unaligned");
+  ST_REQUIRE((wo && wml && st::aligned16(wo)) || st_kv8_attn_workspace_bytes(T, B, Hq, Hkv, D, S, 1) == 0,
+             "st_kv8_chunk_attn: split workspace (wo, wml) missing or unaligned");
   if (T == 0 || B == 0) return 0;
   ST_REQUIRE(cu || T == B, "st_kv8_chunk_attn: without cu every sequence has one query");
   ST_REQUIRE(nblocks < (1ll << 31), "st_kv8_chunk_attn: too many pages");
@@ -633,10 +630,11 @@ extern "C" int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t H
   ST_REQUIRE(slots * Hkv * S < (1ll << 31) && T * (Hq / Hkv) < (1ll << 31), "st_kv8_chunk_attn: grid too large");
   c.slots = (int)slots;
   const cudaStream_t st_ = (cudaStream_t)stream;
-  // few rows per sequence: eight to a CTA through the decode kernel
-  const bool few = T * (Hq / Hkv) <= FEW_ROWS * B;
-  c.parts.min_pages = few ? 4 : 1;
-  const int e = few ? st::rows8_attn(c.a, c.parts, (int)D, st_) : D == 128 ? chunk_launch<128>(c, st_) : chunk_launch<64>(c, st_);
+  if (few_rows8(T, B, Hq / Hkv)) {
+    c.parts.min_pages = 4;
+    return st::rows8_attn("st_kv8_chunk_attn", c.a, c.parts, (int)D, st_);
+  }
+  const int e = D == 128 ? chunk_launch<128>(c, st_) : chunk_launch<64>(c, st_);
   if (e || S == 1) return e;
   return st::merge8("st_kv8_chunk_attn merge launch", c.a, c.parts, (int)D, st_);
 }

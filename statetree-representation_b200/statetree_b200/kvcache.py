@@ -7,7 +7,7 @@ statetree_attention, enable) live in hf_cache.py and are re-exported here when t
 """
 import torch
 
-from .ops import calls, kv_ext
+from .ops import calls, kv_ext, lib
 
 PAGE = 16
 RKV = 1600
@@ -93,17 +93,20 @@ def _rows(t, D):
 
 def decode_splits8(units, max_pages, sms=148):
     """How many CTAs share a unit (sequence, KV head, eight query heads) of the 8-bit decode attention, from what the host knows: the
-    number of units and the width of the block table.  Few units: one CTA of eight warps per SM (8 units of 16K tokens 10.7 us, twice
-    as many 11.1).  More: CTAs of four warps, four to an SM, so that sequences of different lengths even out (64 units of up to 16K
-    tokens, lengths spread: two splits 43.6 us, nine 29.2; all of the full length 44.6 and 50.4).  Below eight pages per split (16,
-    64 with more units) the join costs more than it gives (128 units of 1000 tokens: one 8.4 us, four 11.2)."""
+    number of units and the width of the block table.  Up to eight join on chip, as a cluster, which is a launch less; they are a power
+    of two, since other clusters leave SMs idle (64 units of 1000 tokens: two 7.0 us, three 8.3, four 7.6; 256 of 4000: three 56.3,
+    two 48.4).  Few units: eight up to 4096 tokens (8 units of 2000 tokens: 6.0 us, fifteen 7.0), one CTA of eight warps per SM beyond
+    (8 units of 16000: eighteen 11.0, eight 14.2).  More: CTAs of four warps, four to an SM, so that sequences of different lengths
+    even out (64 units of up to 16K tokens, lengths spread: two 43.6, eight 32.6; all of the full length 43.7 and 48.1).  Below 6, 8,
+    16 or 64 pages per split the join costs more than it gives (128 units of 500 tokens: one 6.0, two 7.6)."""
     if units <= sms // 8:
-        want, least = sms // max(1, units), 8
+        want, least = (8, 6) if max_pages <= 256 else (sms // max(1, units), 8)
     elif units <= 128:
-        want, least = min(9, 4 * sms // units), 8 if units < 32 else 16
+        want, least = min(8, 4 * sms // units), 8 if units < 32 else 16
     else:
         want, least = 4 if units <= 4 * sms else 2, 64
-    return max(1, min(want, max_pages // least, 64))
+    n = max(1, min(want, max_pages // least, 64))
+    return n if n > 8 else 1 << n.bit_length() - 1
 
 
 FEW_ROWS8 = 32      # rows (query, head of the group) per sequence up to which a chunk goes through the decode kernel (st_kv8_chunk.cu)
@@ -184,7 +187,7 @@ class PageStore8:
         q = _rows(q, self.D)
         if out is None:
             out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-        wo, wml = self._partials(q, splits)
+        wo, wml = self._partials(q, block_table, splits, 0)
         kv_ext().kv8_attn(q, self.pages, self.exps, block_table, lens, out, scale, splits, wo, wml, starts, min_pages, window)
         return out
 
@@ -203,16 +206,17 @@ class PageStore8:
         q = _rows(q, self.D)
         if out is None:
             out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-        wo, wml = self._partials(q, splits)
+        wo, wml = self._partials(q, block_table, splits, 1)
         kv_ext().kv8_chunk_attn(q, cu, self.pages, self.exps, block_table, lens, out, scale, splits, wo, wml, starts, window)
         return out
 
-    def _partials(self, q, splits):
-        """(wo, wml) of a call whose sequences are split: its own, from the caching allocator"""
-        if splits <= 1:
+    def _partials(self, q, block_table, splits, chunk):
+        """(wo, wml) of a call whose splits do not join on chip: its own, from the caching allocator"""
+        need = lib().st_kv8_attn_workspace_bytes(q.shape[0], block_table.shape[0], q.shape[1], self.H, self.D, splits, chunk)
+        if not need:
             return None, None
-        rows = q.shape[0] * q.shape[1] * splits
-        flat = torch.empty(rows * (self.D + 2), dtype=torch.float32, device=q.device)
+        flat = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+        rows = flat.numel() // (self.D + 2)
         return flat[:rows * self.D], flat[rows * self.D:]
 
     def dense(self, blocks=None):

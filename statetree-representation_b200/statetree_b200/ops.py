@@ -63,6 +63,7 @@ _SIGNATURES = {
     "st_kv8_append": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _vp, _vp,
                              _i64, _vp, _i64, _vp, _i64, _dbl, _vp, _vp, _vp]),
     "st_kv8_dequant_blocks": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "st_kv8_attn_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _int]),
     "st_kv8_attn": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _dbl,
                            _i64, _i64, _vp]),
     "st_kv8_chunk_attn": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64,
@@ -122,7 +123,8 @@ def lib():
 CALLS_PATH = os.path.join(_HERE, "_calls.so")
 _CALLS = None                                           # False: there is none
 _NATIVE = ("st_gemv", "st_gemm", "st_gemv_list", "st_gemm_list", "st_last_error", "st_encode", "st_encode_lists", "st_encode_offsets",
-           "st_encode_offsets_workspace_bytes", "st_dec_check", "st_lists_check", "st_kv8_append", "st_kv8_dequant_blocks", "st_kv8_attn", "st_kv8_chunk_attn")
+           "st_encode_offsets_workspace_bytes", "st_dec_check", "st_lists_check", "st_kv8_append", "st_kv8_dequant_blocks", "st_kv8_attn",
+           "st_kv8_chunk_attn", "st_kv8_attn_workspace_bytes")
 
 
 def calls():
@@ -655,7 +657,7 @@ class _KV:
                                                Vd.data_ptr(), _stream(kv)))
 
     @staticmethod
-    def _attn8(who, q, cu, kv, exps, bt, lens, out, starts, window, S, wo, wml):
+    def _attn8(who, q, cu, kv, exps, bt, lens, out, starts, window, S, wo, wml, chunk):
         H, D = _KV._pages8(who, kv, exps, q, cu, bt, lens, out, starts, wo, wml)
         _KV._rows8(who, "q", q, D)
         _KV._rows8(who, "out", out, D)
@@ -669,15 +671,16 @@ class _KV:
             raise RuntimeError(f"{who}: starts int32 [B]")
         if window < 0 or S < 1:
             raise RuntimeError(f"{who}: window / splits")
-        if S > 1 and not (wo is not None and wml is not None and wo.dtype == wml.dtype == torch.float32
-                          and wo.numel() >= q.size(0) * Hq * S * D and wml.numel() >= q.size(0) * Hq * S * 2):
+        if lib().st_kv8_attn_workspace_bytes(q.size(0), B, Hq, H, D, S, chunk) and not (
+                wo is not None and wml is not None and wo.dtype == wml.dtype == torch.float32
+                and wo.numel() >= q.size(0) * Hq * S * D and wml.numel() >= q.size(0) * Hq * S * 2):
             raise RuntimeError(f"{who}: workspace")
         return B, Hq, H, D
 
     @staticmethod
     def kv8_attn(q, kv, exps, bt, lens, out, scale, S=1, wo=None, wml=None, starts=None, minpps=1, window=0):
         """one query token per sequence, q [B, Hq, D]"""
-        B, Hq, H, D = _KV._attn8("kv8_attn", q, None, kv, exps, bt, lens, out, starts, window, S, wo, wml)
+        B, Hq, H, D = _KV._attn8("kv8_attn", q, None, kv, exps, bt, lens, out, starts, window, S, wo, wml, 0)
         if q.size(0) != B:
             raise RuntimeError("kv8_attn: one query per sequence of the block table")
         if B == 0:
@@ -691,7 +694,7 @@ class _KV:
     def kv8_chunk_attn(q, cu, kv, exps, bt, lens, out, scale, S=1, wo=None, wml=None, starts=None, window=0):
         """causal attention of the query rows cu[b] .. cu[b + 1] - 1 of every sequence b, q [T, Hq, D]"""
         who = "kv8_chunk_attn"
-        B, Hq, H, D = _KV._attn8(who, q, cu, kv, exps, bt, lens, out, starts, window, S, wo, wml)
+        B, Hq, H, D = _KV._attn8(who, q, cu, kv, exps, bt, lens, out, starts, window, S, wo, wml, 1)
         if cu is None and q.size(0) != B:
             raise RuntimeError(f"{who}: without cu every sequence has one query")
         if cu is not None and not (cu.dtype == torch.int32 and cu.is_contiguous() and cu.numel() == B + 1):

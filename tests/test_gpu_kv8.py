@@ -281,7 +281,7 @@ def _ints(v):
 
 
 @pytest.mark.parametrize("D,H,G", [(128, 8, 4), (128, 2, 1), (128, 1, 8), (64, 2, 7), (64, 3, 3), (128, 1, 16), (64, 1, 20)])
-@pytest.mark.parametrize("splits", [1, 3, None])
+@pytest.mark.parametrize("splits", [1, 3, 8, 12, None])
 def test_decode_attention(D, H, G, splits):
     lens = [1, 0, 15, 16, 17, 33, 130, 700]
     gen = _gen(D + H + G)
@@ -295,7 +295,7 @@ def test_decode_attention(D, H, G, splits):
 
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("window", [0, 1, 5, 64, 1000])
-@pytest.mark.parametrize("splits", [1, 4])
+@pytest.mark.parametrize("splits", [1, 4, 11])
 def test_decode_attention_masks(D, window, splits):
     """left padding (up to the whole sequence and beyond) and sliding windows"""
     lens, starts = [40, 40, 40, 40, 333, 333, 16], [0, 7, 39, 40, 100, 16, 50]
@@ -368,6 +368,55 @@ def test_chunk_attention_masks(D, window, splits):
     assert got is out and bool((out[cu[-1]:] == 5.0).all())
     _check(got, q, seqs, cu, lens, 0.15, starts, window)
     assert not got[cu[1]:cu[1] + 11].any() and not got[cu[2]:cu[3]].any() and not got[cu[3]:cu[3] + 5].any()
+
+
+@pytest.mark.parametrize("splits", [1, 2, 7, 12])
+@pytest.mark.parametrize("window", [0, 1, 40])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_of_few_rows(D, window, splits):
+    """chunks of a few tokens: as above, rows of one sequence that share a CTA with other tokens' and a sequence without queries"""
+    lens, new, starts = [400, 30, 130, 3, 900], [4, 0, 1, 5, 7], [0, 11, 300, 1, 5]
+    gen = _gen(D + window)
+    store, table, seqs = _filled(gen, lens, 2, D)
+    cu = [sum(new[:b]) for b in range(len(new) + 1)]
+    q = _rand(gen, cu[-1] + 2, 6, D).to(DEV)
+    out = torch.full_like(q, 5.0)
+    got = store.chunk_attention(q, _ints(cu), table, _ints(lens), 0.15, starts=_ints(starts), window=window, splits=splits, out=out)
+    assert bool((out[cu[-1]:] == 5.0).all())
+    _check(got, q, seqs, cu, lens, 0.15, starts, window)
+    assert not got[4].any() and not got[5:8].any()        # (all keys padding; positions -2, -1 and the padded 0)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("splits", [2, 5])
+def test_attention_of_more_than_a_wave(D, splits):
+    """so many sequences that their splits do not join on chip"""
+    lens = [(37 * b) % 150 for b in range(90)]
+    gen = _gen(D + splits)
+    store, table, seqs = _filled(gen, lens, 8, D)
+    q = _rand(gen, len(lens), 8, D).to(DEV)
+    got = store.attention(q, table, _ints(lens), 0.1, splits=splits, min_pages=1)
+    _check(got, q, seqs, list(range(len(lens) + 1)), lens, 0.1)
+    cu = [min(2 * b, 120) for b in range(len(lens) + 1)]
+    lens = [max(n, 2) for n in lens]
+    q = _rand(gen, 120, 16, D).to(DEV)
+    got = store.chunk_attention(q, _ints(cu), table, _ints(lens), 0.1, splits=splits)
+    mine = [(K, V) if len(K) >= 2 else None for K, V in seqs]
+    for b, s in enumerate(mine):
+        if s is not None:
+            _check(got[cu[b]:cu[b + 1]], q[cu[b]:cu[b + 1]], [s], [0, cu[b + 1] - cu[b]], [lens[b]], 0.1)
+
+
+@pytest.mark.parametrize("splits", [1, 4, 12])
+def test_attention_into_its_queries(splits):
+    gen = _gen(splits)
+    store, table, _ = _filled(gen, [300, 40], 2, 128)
+    lens, cu = _ints([300, 40]), _ints([0, 3, 5])
+    for n, call in ((2, lambda q, out: store.attention(q, table, lens, 0.1, splits=splits, min_pages=1, out=out)),
+                    (5, lambda q, out: store.chunk_attention(q, cu, table, lens, 0.1, splits=splits, out=out))):
+        q = _rand(gen, n, 8, 128).to(DEV)
+        want = call(q, None)
+        assert call(q, q) is q and torch.equal(q, want)
 
 
 def test_chunk_attention_does_not_look_ahead():

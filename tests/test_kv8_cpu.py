@@ -44,12 +44,22 @@ def test_append_refuses(kw, word):
 @pytest.mark.parametrize("chunk", [False, True])
 @pytest.mark.parametrize("kw,word", [
     (dict(D=80), b"64 or 128"), (dict(Hq=3), b"heads"), (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"),
-    (dict(window=-1), b"window"), (dict(S=0), b"splits"), (dict(S=2), b"workspace"), (dict(q=None), b"null"), (dict(blocks=0), b"empty"),
+    (dict(window=-1), b"window"), (dict(S=0), b"splits"), (dict(S=16), b"workspace"), (dict(q=None), b"null"), (dict(blocks=0), b"empty"),
     (dict(qs=4), b"multiples of 8"), (dict(q=ctypes.c_void_p(4100)), b"aligned")])
 def test_attention_refuses(chunk, kw, word):
     L = _ops().lib()
     assert _attn(L, chunk, **kw) != 0
     assert word in L.st_last_error(), L.st_last_error()
+
+
+def test_workspace_of_split_attentions():
+    """none where the splits join on chip (two to eight of them, about a wave of CTAs), else a partial row per split"""
+    ws = _ops().lib().st_kv8_attn_workspace_bytes
+    assert ws(1, 1, 32, 8, 128, 1, 0) == ws(1, 1, 32, 8, 128, 8, 0) == ws(0, 0, 32, 8, 128, 4, 1) == 0
+    assert ws(1, 1, 32, 8, 128, 9, 0) == 32 * 9 * 130 * 4
+    assert ws(64, 64, 32, 8, 64, 2, 0) == 64 * 32 * 2 * 66 * 4 and ws(32, 32, 32, 8, 64, 2, 0) == 0
+    assert ws(32, 8, 32, 8, 128, 4, 1) == 0                                     # eight sequences of four queries: 512 CTAs of eight rows
+    assert ws(100, 1, 32, 8, 128, 2, 1) == 100 * 32 * 2 * 130 * 4               # (the tensor-core kernel)
 
 
 def test_empty_calls_are_no_calls():
@@ -121,9 +131,9 @@ def test_split_rules():
     """as many splits as the rules state, never more than pages allow"""
     _ops()
     from statetree_b200.kvcache import chunk_splits8, decode_splits8
-    assert decode_splits8(8, 1000) == 18 and decode_splits8(8, 63) == 7 and decode_splits8(8, 19) == 2 and decode_splits8(1, 4) == 1
-    assert decode_splits8(64, 1000) == 9 and decode_splits8(512, 512) == 4 and decode_splits8(512, 100) == 1 and decode_splits8(4096, 512) == 2
-    assert chunk_splits8(4096, 1, 8, 4, 256) == 1 and chunk_splits8(16, 1, 8, 4, 250) == 15 and chunk_splits8(4, 1, 8, 4, 250) == 9
+    assert decode_splits8(8, 1000) == 18 and decode_splits8(8, 63) == 8 and decode_splits8(8, 19) == 2 and decode_splits8(1, 4) == 1
+    assert decode_splits8(64, 1000) == 8 and decode_splits8(512, 512) == 4 and decode_splits8(512, 100) == 1 and decode_splits8(4096, 512) == 2
+    assert chunk_splits8(4096, 1, 8, 4, 256) == 1 and chunk_splits8(16, 1, 8, 4, 250) == 15 and chunk_splits8(4, 1, 8, 4, 250) == 8
     for units in range(1, 700, 7):
         for pages in (1, 2, 7, 33, 500, 5000):
-            assert 1 <= decode_splits8(units, pages) <= max(1, min(64, pages // 8))
+            assert 1 <= decode_splits8(units, pages) <= max(1, min(64, pages // 6))
