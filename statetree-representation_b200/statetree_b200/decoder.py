@@ -250,6 +250,8 @@ class TreeDecoder:
         c, E, (B, P) = self.cfg, ext(), prompt.shape
         if B != self.B:
             raise ValueError(f"TreeDecoder.prefill: {B} sequences, the decoder was made for {self.B}")
+        if not P:
+            raise ValueError("TreeDecoder.prefill: no tokens")
         start = int(self.pos_buf.item())
         if start + P > self.max_len:
             raise ValueError(f"TreeDecoder.prefill: {P} tokens from position {start} exceed the cache capacity of {self.max_len} tokens")

@@ -192,8 +192,10 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
                                         min_pages=4, **more)
             return out.view(B, 1, Hq, D), None
         if T > 1 and not c.starts_known and attention_mask is not None and attention_mask.dim() == 4:
-            last_row = attention_mask[:, 0, -1, :]                  # the last query sees everything but the padding
-            masked = ~last_row if last_row.dtype == torch.bool else last_row < 0
+            # the last query sees everything but the padding; with a window (8-bit pages), every query that is none sees itself
+            rows = attention_mask[:, 0]
+            seen = rows.diagonal(rows.shape[2] - T, 1, 2) if c.eight_bit and kwargs.get("sliding_window") else rows[:, -1]
+            masked = ~seen if seen.dtype == torch.bool else seen < 0
             c.starts[:B].copy_(masked.sum(-1).to(torch.int32))
             c.starts_known = True
         if c.eight_bit:                              # a chunk (its keys are in the pages already), or the first token of all

@@ -82,6 +82,8 @@ def test_decoder_steps_and_prefill(batch):
         m.prefill(prompt)
     with pytest.raises(ValueError, match="sequences"):
         m.prefill(prompt[:1].expand(batch + 1, P))
+    with pytest.raises(ValueError, match="no tokens"):
+        m.prefill(prompt[:, :0])
     assert ops.device_status() == 0
 
 
@@ -108,15 +110,19 @@ def test_prefill_is_refused_without_the_cache():
 
 
 @pytest.mark.parametrize("head_dim", [64, 128])
-def test_hf_cache(head_dim):
-    """prompt in two chunks and decode steps, one sequence left-padded, against a cache-free pass whose attention quantises by pages"""
+@pytest.mark.parametrize("windows", [None, ["sliding_attention", "full_attention"], ["full_attention", "sliding_attention"]])
+@pytest.mark.parametrize("pad", [0, 5])
+def test_hf_cache(head_dim, windows, pad):
+    """prompt in two chunks (longer than the windows of the layers that have one) and decode steps, one sequence left-padded, against
+    a cache-free pass whose attention quantises by pages"""
     pytest.importorskip("transformers")
     from transformers import AttentionInterface, Qwen3Config, Qwen3ForCausalLM
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     from transformers.masking_utils import AttentionMaskInterface, sdpa_mask
     from statetree_b200.kvcache import StateTreeKVCache, enable
     cfg = Qwen3Config(vocab_size=512, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
-                      num_key_value_heads=2, head_dim=head_dim, max_position_embeddings=256, tie_word_embeddings=False)
+                      num_key_value_heads=2, head_dim=head_dim, max_position_embeddings=256, tie_word_embeddings=False,
+                      **(dict(use_sliding_window=True, sliding_window=8, layer_types=windows) if windows else {}))
     torch.manual_seed(0)
     model = Qwen3ForCausalLM(cfg).to(torch.bfloat16).cuda().eval()
 
@@ -137,7 +143,7 @@ def test_hf_cache(head_dim):
     B, P, steps = 2, 21, 6
     ids = torch.randint(0, cfg.vocab_size, (B, P + steps), device="cuda")
     mask = torch.ones(B, P + steps, dtype=torch.long, device="cuda")
-    mask[1, :5] = 0
+    mask[1, :pad] = 0
     with torch.no_grad():
         model.set_attn_implementation("kv8_plain")
         full = model(input_ids=ids, attention_mask=mask).logits.float()
