@@ -413,7 +413,8 @@ def test_attention_into_its_queries(splits):
     store, table, _ = _filled(gen, [300, 40], 2, 128)
     lens, cu = _ints([300, 40]), _ints([0, 3, 5])
     for n, call in ((2, lambda q, out: store.attention(q, table, lens, 0.1, splits=splits, min_pages=1, out=out)),
-                    (5, lambda q, out: store.chunk_attention(q, cu, table, lens, 0.1, splits=splits, out=out))):
+                    (5, lambda q, out: store.chunk_attention(q, cu, table, lens, 0.1, splits=splits, out=out)),
+                    (200, lambda q, out: store.chunk_attention(q, 40 * cu, table, lens, 0.1, splits=splits, out=out))):
         q = _rand(gen, n, 8, 128).to(DEV)
         want = call(q, None)
         assert call(q, q) is q and torch.equal(q, want)
