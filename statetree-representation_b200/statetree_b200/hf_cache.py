@@ -115,6 +115,7 @@ class StateTreeKVLayer(CacheLayerMixin):
         if self.is_initialized:
             self.store.reset()
             self.gpu_len.zero_()
+            self.cache.starts.zero_()                   # (a prompt without padding may come without a mask)
         self.cache.starts_known = False
 
     def check(self):

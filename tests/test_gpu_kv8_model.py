@@ -160,3 +160,9 @@ def test_hf_cache(head_dim, windows, pad):
         assert float((g - want).norm() / want.norm()) < REL, n
     k0, _ = cache.layers[0].dense(P)
     assert k0.shape == (B, 2, P, head_dim) and torch.isfinite(k0.float()).all()
+    # the same cache again, for a prompt without padding: as a new one
+    cache.reset()
+    with torch.no_grad():
+        one, two = (model(input_ids=ids[:, :7], past_key_values=c, use_cache=True).logits
+                    for c in (cache, StateTreeKVCache(model.config, batch_size=B, max_cache_len=P + steps + 8, eight_bit=True)))
+    assert torch.equal(one, two)
