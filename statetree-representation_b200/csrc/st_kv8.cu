@@ -14,21 +14,23 @@ using namespace st;
 
 // ------------------------------------------------------------------------------------------------ append
 // Keys (normalised and rotated on the way, in fp32, one rounding to e4m3 at the end), values, and the queries of the same tokens
-// (normalised and rotated into q_out).  A warp owns one unit (page, head, K or V) for the launch and takes every token of the call
-// that goes to the page, so nothing is added or compared between warps and the result does not depend on their order:
+// (normalised and rotated into q_out).  A warp (or two) owns one unit (page, head, K or V) for the launch and takes every token of the
+// call that goes to the page, so the result does not depend on any order:
 //     e' = the smallest exponent that holds the new rows; the page's old one if that is larger and the page does not start anew
 //     new rows are rounded at e', the others again at e' if it differs from the old exponent, or cleared if row 0 is among the new
 // Which warp: the last token of the call in a page leads it.
-//   SCAN  (calls of up to SCAN_MAX tokens, where the two meet: keys and values of 16, 256, 512 sequences with a token each 4.6, 9.1,
-//         17.3 us so, 7.2, 8.9, 14.9 with marks) a warp per (token, unit) walks the call's slots and finds out itself
+//   SCAN  (calls of up to SCAN_MAX tokens, about where the two meet: keys and values of 16, 256, 512 sequences with a token each 4.6,
+//         9.2, 17.5 us so, 8.3, 10.5, 16.4 with marks; 512 tokens of one 10.9 and 11.6) a warp per (token, unit) walks the call's slots
+//         and finds out itself
 //   else  kv8_mark_kernel leaves every row's and page's last token in `marks`; a CTA takes up to sixteen tokens of the call, clears the
 //         marks of the pages they lead and writes all units of those (fewer tokens in shorter calls, which may lead a page each: 1024
-//         sequences 73 us with sixteen, 25 with one)
-// One token (8 KV heads, 32 query heads) 4.4 us, bound by look-ups that follow one another; 32764 tokens 179 us (755 MB), of which keys
-// and values take 84 (16 warps an SM have too little in flight beside the 64 values that a lane holds) and the queries 95 (HBM).
+//         sequences 92 us with sixteen, 25 with one).  At D = 128 two warps share a unit: with half the values a lane, 24 warps find
+//         room on an SM for 16 (32764 tokens 163 us for 179, with 2 KV and 16 query heads 87 for 116; four warps a unit 171)
+// One token (8 KV heads, 32 query heads) 4.2 us, bound by look-ups that follow one another; 32764 tokens 163 us (755 MB), of which keys
+// and values take 77 (a chain of look-ups and 40 % of the issue slots) and the queries 86 (HBM).
 // Same slot twice: the last one counts in both.  Values that are not finite are stored as the largest of their sign (infinities) or
 // as zero (NaN), and flagged in *bad.
-constexpr int SCAN_MAX = 256;
+constexpr int SCAN_MAX = 384;
 
 struct Append8 {
   const uint16_t* K; const uint16_t* V; const uint16_t* Q;
@@ -144,10 +146,22 @@ __device__ __forceinline__ uint2 rescale_eight(uint2 u, float up, float down) {
   return e4m3_eight(f, down);
 }
 
-// one unit: lane r < 16 holds in `tok` the token that goes to row r, -1 = none; at least one row has a token
-template <int D>
-__device__ __forceinline__ void append_unit(const Append8& a, long long page, int h, int kvi, int tok, int lane) {
-  constexpr int LPR = D / 16, RPI = 32 / LPR, ITER = PAGE / RPI;
+// the largest of a value of each of the WPU warps that share a unit; `at` is theirs (nobody writes it again before all have read it)
+template <int WPU>
+__device__ __forceinline__ uint32_t over_warps_max(uint32_t v, uint32_t* at, int warp, int lane) {
+  if (WPU == 1) return v;
+  if (lane == 0) at[warp % WPU] = v;
+  asm volatile("bar.sync %0, %1;" :: "r"(1 + warp / WPU), "n"(32 * WPU) : "memory");
+#pragma unroll
+  for (int k = 0; k < WPU; ++k) v = max(v, at[k]);
+  return v;
+}
+// one unit: lane r < 16 holds in `tok` the token that goes to row r, -1 = none; at least one row has a token.  WPU warps share it, some
+// rows each; `share`: 2 * WPU words of theirs, others than for the unit before
+template <int D, int WPU>
+__device__ __forceinline__ void append_unit(const Append8& a, long long page, int h, int kvi, int tok, int warp, int lane, uint32_t* share) {
+  constexpr int LPR = D / 16, RPI = 32 / LPR, ITER = PAGE / RPI / WPU;
+  const int row0 = warp % WPU * (ITER * RPI);
   const unsigned rows = __ballot_sync(FULL, lane < PAGE && tok >= 0);
   const int c = lane % LPR;
   const uint16_t* const src = (kvi ? a.V : a.K) + (size_t)h * D + 8 * c;
@@ -156,7 +170,7 @@ __device__ __forceinline__ void append_unit(const Append8& a, long long page, in
   int mine[ITER];
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
-    mine[i] = __shfl_sync(FULL, tok, i * RPI + lane / LPR);
+    mine[i] = __shfl_sync(FULL, tok, row0 + i * RPI + lane / LPR);
     raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
     if (mine[i] >= 0) {
       const uint16_t* p = src + (long long)mine[i] * step;
@@ -189,7 +203,7 @@ __device__ __forceinline__ void append_unit(const Append8& a, long long page, in
     for (int k = 0; k < 16; ++k) m = max(m, __float_as_uint(f[i][k]) & 0x7FFFFFFFu);
     if (mine[i] >= 0) most = max(most, m);         // (norm and rotation can make NaN of a row without a token: 0 * rsqrt(0))
   }
-  most = __reduce_max_sync(FULL, most);
+  most = over_warps_max<WPU>(__reduce_max_sync(FULL, most), share, warp, lane);
   const bool odd = most > __float_as_uint(448.f * pow2i(E8_MAX));        // (a value that is not finite, or beyond the format)
   float top = __uint_as_float(most);
   if (odd) {
@@ -202,14 +216,14 @@ __device__ __forceinline__ void append_unit(const Append8& a, long long page, in
         top = fmaxf(top, m < INFINITY ? m : 0.f);
         if (m != m) f[i][k] = 0.f;
       }
-    top = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(top)));
+    top = __uint_as_float(over_warps_max<WPU>(__reduce_max_sync(FULL, __float_as_uint(top)), share + WPU, warp, lane));
   }
   const int e = max(was, exp_for(top));
   const float down = pow2i(-e), up = pow2i(20 + was);
   uint8_t* const unit = a.kv + page8_off<D>(page, a.H, h, kvi);
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
-    const int r = i * RPI + lane / LPR;
+    const int r = row0 + i * RPI + lane / LPR;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int d = half * (D / 2) + 8 * c;
@@ -219,15 +233,15 @@ __device__ __forceinline__ void append_unit(const Append8& a, long long page, in
       else if (e != was) *at = rescale_eight(*at, up, down);
     }
   }
-  __syncwarp();                                    // (every lane has read the old exponent)
-  if (lane == 0 && (anew || e != was)) *exp_at = (int8_t)e;
+  __syncwarp();                                    // (every lane has read the old exponent, the other warps' before they met)
+  if (lane == 0 && row0 == 0 && (anew || e != was)) *exp_at = (int8_t)e;
   if (odd && lane == 0) *a.bad = 1;
 }
 
 // A warp takes q_steps groups of 32 / (D / 16) heads of one token: its row of the tables and the norm weights are read once
-template <int D>
+template <int D, int AHEAD>
 __device__ __forceinline__ void rotate_queries(const Append8& a, long long unit, int lane) {
-  constexpr int LPR = D / 16, RPI = 32 / LPR, AHEAD = 4;
+  constexpr int LPR = D / 16, RPI = 32 / LPR;
   const long long token = unit / a.q_units;
   if (token >= a.N) return;
   const int c = lane % LPR, h0 = (int)(unit % a.q_units) * a.q_steps * RPI, h1 = min(a.Hq, h0 + a.q_steps * RPI);
@@ -283,14 +297,15 @@ __global__ void __launch_bounds__(256) kv8_mark_kernel(const Append8 a) {
 }
 
 template <int D, bool SCAN>
-__global__ void __launch_bounds__(256, 2) kv8_append_kernel(const Append8 a) {
+__global__ void __launch_bounds__(256, SCAN ? 2 : 3) kv8_append_kernel(const Append8 a) {
+  constexpr int WPU = SCAN ? 1 : D / 64;
   __shared__ int s_row[PAGE][PAGE];
   __shared__ long long s_page[PAGE];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, units = 2 * a.H;
   if ((int)blockIdx.x >= a.q_cta) {
-    rotate_queries<D>(a, (long long)((int)blockIdx.x - a.q_cta) * 8 + warp, lane);
+    rotate_queries<D, SCAN ? 4 : 2>(a, (long long)((int)blockIdx.x - a.q_cta) * 8 + warp, lane);
     return;
   }
   if (SCAN) {
@@ -313,7 +328,7 @@ __global__ void __launch_bounds__(256, 2) kv8_append_kernel(const Append8 a) {
     }
     if (__any_sync(FULL, later)) return;           // (a later token leads the page)
     __syncwarp();
-    append_unit<D>(a, page, u >> 1, u & 1, lane < PAGE ? row[lane] : -1, lane);
+    append_unit<D, WPU>(a, page, u >> 1, u & 1, lane < PAGE ? row[lane] : -1, warp, lane, nullptr);
   } else {
     if (warp == 0) {
       const int i = (int)blockIdx.x * a.run + lane;
@@ -336,9 +351,12 @@ __global__ void __launch_bounds__(256, 2) kv8_append_kernel(const Append8 a) {
     }
     __syncthreads();
     // (keys of all heads, then values: every warp has some of both)
+    __shared__ uint32_t s_share[8 / WPU][2][2 * WPU];
+    int turn = 0;
     for (int n = 0; n < PAGE && s_page[n] >= 0; ++n) {
       const int tok = lane < PAGE ? s_row[n][lane] : -1;
-      for (int u = warp; u < units; u += 8) append_unit<D>(a, s_page[n], u < a.H ? u : u - a.H, u >= a.H, tok, lane);
+      for (int u = warp / WPU; u < units; u += 8 / WPU, turn ^= 1)
+        append_unit<D, WPU>(a, s_page[n], u < a.H ? u : u - a.H, u >= a.H, tok, warp, lane, s_share[warp / WPU][turn]);
     }
   }
 }
@@ -891,7 +909,7 @@ extern "C" int st_kv8_append(const void* K, const void* V, int64_t ks, int64_t v
   a.run = (int)std::min<long long>(st::PAGE, std::max<long long>(1, N / (8ll * st::sm_count())));
   const long long page_ctas = scan ? (N * H * 2 + 7) / 8 : (N + a.run - 1) / a.run;
   // queries: a warp per group of heads while that leaves SMs without one, else up to eight groups of a token (the whole append, us with
-  // one / eight groups: 16 sequences 4.6 / 5.0, 2048 tokens of one 17.7 / 16.0, 4096 41.4 / 24.2)
+  // one / eight groups: 16 sequences 4.6 / 5.0, 2048 tokens of one 18.5 / 16.9, 4096 35.3 / 24.7)
   const int groups = (int)((a.Hq + 512 / D - 1) / (512 / D));
   a.q_steps = (int)std::min<long long>(std::min(std::max(groups, 1), 8), std::max<long long>(1, N * groups / (16ll * st::sm_count())));
   a.q_units = groups ? (groups + a.q_steps - 1) / a.q_steps : 0;

@@ -37,7 +37,7 @@ def _same(store, ref):
 
 # ------------------------------------------------------------------------------------------------ append
 @pytest.mark.parametrize("D,H", [(128, 1), (128, 8), (64, 3)])
-@pytest.mark.parametrize("calls", [(1,), (16,), (5, 1, 1, 20, 3), (40, 600, 1, 7), (257,), (2401,)])
+@pytest.mark.parametrize("calls", [(1,), (16,), (5, 1, 1, 20, 3), (40, 600, 1, 7), (385,), (2401,)])
 def test_append_in_order(D, H, calls):
     """a sequence that grows over several calls (whole pages, parts of pages, single tokens; short and long calls)"""
     gen = _gen(sum(calls) + D + H)
@@ -58,7 +58,7 @@ def test_append_in_order(D, H, calls):
         assert torch.equal(got.cpu().double()[:3], want[[blocks - 1, 0, 0]]) and not got[3:].any()
 
 
-@pytest.mark.parametrize("n", [1, 33, 256, 257, 700, 2500])
+@pytest.mark.parametrize("n", [1, 33, 384, 385, 700, 2500])
 def test_append_any_order(n):
     """slots in any order, padding and slots beyond the cache, the same slot several times (the last token counts), pages that do
     not start anew and pages that do"""
@@ -128,7 +128,33 @@ def test_append_what_the_format_cannot_hold(bad):
     store.check()
 
 
-@pytest.mark.parametrize("n", [1, 300])
+def test_append_what_the_format_cannot_hold_in_long_calls():
+    """the same in many pages of one call, in either half of them, beside the largest value and away from it"""
+    H, D, n = 3, 128, 500
+    store, ref = _store(33, H, D), R.Pages(33, H, D)
+    gen = _gen(2)
+    K, V = _keys(gen, n, H, D), _rand(gen, n, H, D)
+    y, inf = [], float("inf")
+    for X in (K, V):
+        at = torch.randint(0, n, (40,), generator=gen), torch.randint(0, H, (40,), generator=gen), torch.randint(0, D, (40,), generator=gen)
+        X[at] = torch.tensor([float("nan"), inf, -inf, 3e38])[torch.arange(40) % 4].to(torch.bfloat16)
+        Y = X.double()
+        for p in range(0, n, PAGE):                       # infinities: the largest of the block's exponent
+            for h in range(H):
+                block = Y[p:p + PAGE, h]
+                fine = torch.where(block.isfinite(), block, torch.zeros_like(block))
+                top = 448 * 2.0 ** R.exponent(float(fine.abs().max()))
+                Y[p:p + PAGE, h] = torch.where(block.isnan(), torch.zeros_like(block), block.clamp(-top, top))
+        y.append(Y)
+    slots = torch.arange(n) + PAGE
+    store.append(K.to(DEV), V.to(DEV), slots.to(DEV))
+    ref.append(y[0], y[1], slots)
+    _same(store, ref)
+    with pytest.raises(RuntimeError, match="finite"):
+        store.check()
+
+
+@pytest.mark.parametrize("n", [1, 400])
 def test_append_without_an_epsilon(n):
     """norms with eps = 0: rows of a page that no token goes to are not taken for values (0 * rsqrt(0) is not a number)"""
     H, D = 2, 128

@@ -34,7 +34,7 @@ def test_page_bytes():
     (dict(D=96), b"64 or 128"), (dict(N=-1), b"negative"), (dict(ks=260), b"multiples of 8"), (dict(K=ctypes.c_void_p(4104)), b"aligned"),
     (dict(K=None), b"null"), (dict(cos=P), b"both tables"), (dict(cos=P, sin=P, span=9), b"positions"), (dict(cos=P, sin=P, pos=P, span=0), b"positions"),
     (dict(cos=P, sin=P, pos=P, span=9, step=2), b"pos_step"), (dict(Q=P), b"queries"), (dict(Q=P, q_out=P, qs=4), b"queries"),
-    (dict(N=257), b"marks")])
+    (dict(N=385), b"marks")])
 def test_append_refuses(kw, word):
     L = _ops().lib()
     assert _append(L, **kw) != 0
