@@ -25,9 +25,10 @@ using namespace st;
 //   else  kv8_mark_kernel leaves every row's and page's last token in `marks`; a CTA takes up to sixteen tokens of the call, clears the
 //         marks of the pages they lead and writes all units of those (fewer tokens in shorter calls, which may lead a page each: 1024
 //         sequences 92 us with sixteen, 25 with one).  At D = 128 two warps share a unit: with half the values a lane, 24 warps find
-//         room on an SM for 16 (32764 tokens 163 us for 179, with 2 KV and 16 query heads 87 for 116; four warps a unit 171)
-// One token (8 KV heads, 32 query heads) 4.2 us, bound by look-ups that follow one another; 32764 tokens 163 us (755 MB), of which keys
-// and values take 77 (a chain of look-ups and 40 % of the issue slots) and the queries 86 (HBM).
+//         room on an SM for 16 (32764 tokens 163 us for 179, with 2 KV and 16 query heads 87 for 116; four warps a unit 171: before
+//         the keys' rotation became a closer one)
+// One token (8 KV heads, 32 query heads) 4.2 us, bound by look-ups that follow one another; 32764 tokens 167 us (755 MB), of which keys
+// and values take 81 (a chain of look-ups and 40 % of the issue slots) and the queries 86 (HBM).
 // Same slot twice: the last one counts in both.  Values that are not finite are stored as the largest of their sign (infinities) or
 // as zero (NaN), and flagged in *bad.
 constexpr int SCAN_MAX = 384;
@@ -71,14 +72,13 @@ __device__ __forceinline__ float row_rms(const float (&f)[16], float eps) {
   for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
   return __frsqrt_rn(ss * (1.f / D) + eps);
 }
-template <int D>
-__device__ __forceinline__ void row_norm(float (&f)[16], const uint4 (&w)[2], float eps) {
-  const float r = row_rms<D>(f, eps);
+// the row times the norm weights: exact, both are BF16
+__device__ __forceinline__ void row_weights(float (&f)[16], const uint4 (&w)[2]) {
   float g[16];
   unpack8(w[0], g, 0);
   unpack8(w[1], g, 8);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = f[i] * r * g[i];
+  for (int i = 0; i < 16; ++i) f[i] *= g[i];
 }
 template <int D>
 __device__ __forceinline__ void norm_weights(uint4 (&w)[2], const uint16_t* at, int c) {
@@ -94,21 +94,27 @@ __device__ __forceinline__ void load_turn(Turn& t, const float* ct, const float*
   *reinterpret_cast<float4*>(t.sn) = *reinterpret_cast<const float4*>(st + p0);
   *reinterpret_cast<float4*>(t.sn + 4) = *reinterpret_cast<const float4*>(st + p1);
 }
+// a * b - c * d, with the rounding of c * d taken out of the difference: 1.5 steps of the result at most, however much cancels
+__device__ __forceinline__ float diff_of_products(float a, float b, float c, float d) {
+  const float p = c * d;
+  return fmaf(a, b, -p) + fmaf(-c, d, p);
+}
+// CLOSE: for keys, so that their codes are the exact value's more often (3 x 8.4 million normalised and rotated keys: 22 codes are not, with
+// two plain roundings each 33; 32764 tokens 167 us for 163)
+template <bool CLOSE>
+__device__ __forceinline__ void rotate_pair(float& a, float& b, float cs, float sn) {
+  const float x = a, y = b;
+  a = CLOSE ? diff_of_products(x, cs, y, sn) : x * cs - y * sn;
+  b = CLOSE ? diff_of_products(x, sn, -y, cs) : x * sn + y * cs;
+}
+template <bool CLOSE>
 __device__ __forceinline__ void row_rotate(float (&f)[16], const Turn& t, int pairs) {
   if (pairs) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {                  // pair i of the lane: f[2i], f[2i + 1]
-      const float a = f[2 * i], b = f[2 * i + 1];
-      f[2 * i] = a * t.cs[i] - b * t.sn[i];
-      f[2 * i + 1] = a * t.sn[i] + b * t.cs[i];
-    }
+    for (int i = 0; i < 8; ++i) rotate_pair<CLOSE>(f[2 * i], f[2 * i + 1], t.cs[i], t.sn[i]);      // pair i of the lane
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = f[i], b = f[8 + i];
-      f[i] = a * t.cs[i] - b * t.sn[i];
-      f[8 + i] = a * t.sn[i] + b * t.cs[i];
-    }
+    for (int i = 0; i < 8; ++i) rotate_pair<CLOSE>(f[i], f[8 + i], t.cs[i], t.sn[i]);
   }
 }
 __device__ __forceinline__ long long table_row(const Append8& a, long long token) {
@@ -189,14 +195,18 @@ __device__ __forceinline__ void append_unit(const Append8& a, long long page, in
   for (int i = 0; i < ITER; ++i) {
     unpack8(raw[i][0], f[i], 0);
     unpack8(raw[i][1], f[i], 8);
-    if (kvi == 0) {
-      if (a.wk) row_norm<D>(f[i], w, a.eps);
+    if (kvi == 0) {                                // (the row's factor last: a rotation does not change it, and it rounds once)
+      const float r = a.wk ? row_rms<D>(f[i], a.eps) : 1.f;
+      if (a.wk) row_weights(f[i], w);
       if (a.cos_t && mine[i] >= 0) {
         const long long at = table_row(a, mine[i]) * (D / 2);
         Turn t;
         load_turn<D>(t, a.cos_t + at, a.sin_t + at, a.pairs, c);
-        row_rotate(f[i], t, a.pairs);
+        row_rotate<true>(f[i], t, a.pairs);
       }
+      if (a.wk)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) f[i][k] *= r;
     }
     uint32_t m = 0;
 #pragma unroll
@@ -271,8 +281,11 @@ __device__ __forceinline__ void rotate_queries(const Append8& a, long long unit,
       float f[16];
       unpack8(raw[i][0], f, 0);
       unpack8(raw[i][1], f, 8);
-      if (a.wq) row_norm<D>(f, w, a.eps);
-      if (a.cos_t) row_rotate(f, t, a.pairs);
+      const float r = a.wq ? row_rms<D>(f, a.eps) : 1.f;
+      if (a.wq) row_weights(f, w);
+      if (a.cos_t) row_rotate<false>(f, t, a.pairs);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) f[k] *= r;
       if (mine < h1) {
         uint4* const o = reinterpret_cast<uint4*>(dst + (size_t)mine * D);
         o[0] = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
