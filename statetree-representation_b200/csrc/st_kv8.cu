@@ -908,6 +908,7 @@ extern "C" int st_kv8_append(const void* K, const void* V, int64_t ks, int64_t v
   ST_REQUIRE(pos_step == 0 || pos_step == 1, "st_kv8_append: pos_step is 1, or 0 for one position of all tokens");
   ST_REQUIRE(Q == nullptr || (q_out && Hq > 0 && qs % 8 == 0 && qos % 8 == 0 && qs >= 0 && qos >= 0 && st::aligned16(Q) && st::aligned16(q_out)),
              "st_kv8_append: queries and their output must be 16-byte aligned with token strides that are multiples of 8");
+  ST_REQUIRE(Q == nullptr || N == 1 || qos >= Hq * D, "st_kv8_append: rows of the queries' output overlap");
   const bool scan = N <= SCAN_MAX;
   ST_REQUIRE(scan || marks, "st_kv8_append: calls of more than %d tokens need marks (int32 [17 * blocks], zero)", SCAN_MAX);
   ST_REQUIRE(N < (1ll << 31) - 16 && N * H < (1ll << 32) && (Q == nullptr || N * Hq < (1ll << 34)), "st_kv8_append: too large");
@@ -966,6 +967,7 @@ int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, 
   ST_REQUIRE(st::aligned16(q) && st::aligned16(out) && st::aligned16(kv) && qs % 8 == 0 && os % 8 == 0 && qs >= 0 && os >= 0,
              "%s: q, out and the pages must be 16-byte aligned, token strides multiples of 8", who);
   ST_REQUIRE(((uintptr_t)exps & 1u) == 0, "%s: exponents must be 2-byte aligned", who);
+  ST_REQUIRE(T == 1 || os >= Hq * D, "%s: rows of out overlap", who);
   ST_REQUIRE(T * Hq < (1ll << 31) && bts < (1ll << 27), "%s: too large", who);
   a.q = (const uint16_t*)q; a.q_stride = qs; a.cu = cu; a.kv = (const uint8_t*)kv; a.exps = exps; a.nblocks = nblocks;
   a.table = bt; a.table_stride = bts; a.lens = lens; a.starts = starts; a.out = (uint16_t*)out; a.out_stride = os;

@@ -52,6 +52,14 @@ def test_attention_refuses(chunk, kw, word):
     assert word in L.st_last_error(), L.st_last_error()
 
 
+def test_outputs_whose_rows_overlap_are_refused():
+    L = _ops().lib()
+    assert _attn(L, B=2, T=2, Hq=8, qs=0) != 0 and b"overlap" in L.st_last_error()
+    assert _attn(L, True, B=1, T=5, Hq=8, qs=0) != 0 and b"overlap" in L.st_last_error()
+    assert L.st_kv8_append(P, P, 256, 256, P, 2, 2, 128, P, P, 4, None, 1, None, None, 0, 1, None, P, 0, None, 4, P, 256, 1e-6, None, P, None) != 0
+    assert b"overlap" in L.st_last_error()
+
+
 def test_workspace_of_split_attentions():
     """none where the splits join on chip (two to eight of them, about a wave of CTAs), else a partial row per split"""
     ws = _ops().lib().st_kv8_attn_workspace_bytes
