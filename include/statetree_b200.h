@@ -243,7 +243,8 @@ int64_t st_kv8_page_bytes(int64_t H, int64_t D);
  * A unit's exponent (page, head, K or V) is the smallest that holds its new rows, or its old one if that is larger; the other rows are
  * then rounded again.  A page written at row 0 starts anew: rows not written in the call become zero.  Values that are not finite, or
  * beyond 448 * 2^56, are cut off there (NaN: zero) and *bad (int32) is set to 1.
- * marks: int32 [17 * nblocks], zero on entry and on exit; may be NULL for calls of up to 384 tokens. */
+ * marks: int32 [17 * nblocks], zero on entry and on exit; may be NULL for calls of up to 384 tokens.  Calls that run at the same time
+ * must go to different pages. */
 int st_kv8_append(const void* K, const void* V, int64_t ks, int64_t vs, const int64_t* slot, int64_t N, int64_t H, int64_t D, void* kv,
                   int8_t* exps, int64_t nblocks, const int64_t* pos, int64_t pos_step, const float* cos_t, const float* sin_t,
                   int64_t max_pos, int interleaved, const void* wk, const void* Q, int64_t qs, const void* wq, int64_t Hq, void* q_out,

@@ -155,7 +155,8 @@ class PageStore8:
         With cos / sin (float32 [P, D / 2]) keys are rotated at positions int64 [N] (or [1]: one for all), on pairs (2i, 2i + 1), or
         (i, i + D/2) with interleaved=False; with k_norm (bf16 [D]) they are RMS-normalised before.  q [N, Hq, D] goes the same way
         (q_norm) into q_out, which is returned.  A page is written from row 0 on: doing that again starts it anew (its other rows
-        become zero); tokens that follow raise its exponent where they need to."""
+        become zero); tokens that follow raise its exponent where they need to.  Appends that run at the same time (on two streams)
+        must go to different pages."""
         host = calls()                                     # one native call for inputs that need no copy
         if host is not None:
             done = host[0].kv8_append(host[1], self.pages, self.exps, self.marks, self.bad, K, V, slots, positions, cos, sin, interleaved, q,
