@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  uint64_t *const kfull = bars + 2, *const vfull = bars + 4, *const sfull = bars + 6, *const pfull = bars + 8,
+  uint64_t *const begin1 = bars, *const kfull = bars + 2, *const vfull = bars + 4, *const sfull = bars + 6, *const pfull = bars + 8,
            *const ofull = bars + 12, *const empty = bars + 14, *const raw = bars + 16;           // pfull: [half of the keys][row tile]
   uint64_t* const drain = bars + 24;                              // raw: [converter warp][keys, values]
   uint32_t* const slot_at = reinterpret_cast<uint32_t*>(smem + L::SLOT);
@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
         mbar_init(empty + i, 1);
       }
       mbar_init(drain, 1);
+      mbar_init(begin1, 4);
       fence_barrier_init();
     }
     __syncwarp();
@@ -240,8 +241,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     meet();
     const uint32_t tmem = *slot_at + ((uint32_t)((warp & 3) * 32) << 16), ts = tmem + t * 128, to = tmem + 256 + t * D;
     // The second row tile begins when the first has its first P: from then on each has the special function units to itself while the
-    // other's products run
-    if (t == 1 && count > 0 && w.count0 > 0) ok = mbar_wait(pfull + 2, 0);
+    // other's products run.  (A barrier of its own, which completes once: the first tile's softmax does not wait for this one's, so that
+    // it could complete a phase of `pfull` and the next before a warp here has looked)
+    if (t == 1 && count > 0 && w.count0 > 0) ok = mbar_wait(begin1, 0);
     for (int j = 0; ok && j < count; ++j) {
       if (!mbar_wait_look(sfull + t, (uint32_t)j & 1u)) { ok = false; break; }
       tc_fence_after();
@@ -326,6 +328,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
       if (lane == 0) {
         if (!any) mbar_arrive(pfull + t);
         mbar_arrive(pfull + 2 + t);
+        if (t == 0 && j == 0) mbar_arrive(begin1);
       }
     }
     if (ok && count > 0) ok = mbar_wait(ofull + t, 0);

@@ -1,0 +1,33 @@
+"""8-bit KV pages on the GPU: calls at the edges of what their descriptions allow."""
+import pytest
+import torch
+
+import kv8_ref as R
+from test_gpu_kv8 import DEV, _check, _filled, _gen, _ints, _rand
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ waits
+@pytest.mark.parametrize("D", [64, 128])
+def test_row_tiles_of_a_chunk_start_one_after_the_other(D):
+    """two full row tiles per CTA and many key tiles, over and over, beside other work on the same SMs: every wait ends and every bit
+    is the same"""
+    gen = _gen(D)
+    n = 1500
+    store, table, seqs = _filled(gen, [n], 2, D)
+    q = _rand(gen, n, 8, D).to(DEV)
+    call = lambda: store.chunk_attention(q, _ints([0, n]), table, _ints([n]), 0.1)            # noqa: E731
+    want = call()
+    rows = [0, 31, 63, 64, 127, 128, 700, n - 1]          # (of both row tiles of a CTA: 64 tokens are 256 rows)
+    for i in rows:
+        _check(want[i:i + 1], q[i:i + 1], [tuple(t[:i + 1] for t in seqs[0])], [0, 1], [i + 1], 0.1)
+    torch.cuda.synchronize()
+    side, other = torch.cuda.Stream(), torch.zeros(1 << 22, device=DEV)
+    for _ in range(25):
+        with torch.cuda.stream(side):
+            other.mul_(0.5).add_(1.0)
+        assert torch.equal(call(), want)
+    torch.cuda.synchronize()
+    from statetree_b200.ops import device_status
+    assert device_status() == 0
