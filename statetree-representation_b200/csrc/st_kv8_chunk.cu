@@ -18,6 +18,7 @@
 // A key tile takes 2.3 us for the 256 rows: a row tile's softmax about 2300 cycles, its MMAs and the hand-overs 1200, of which the other
 // row tile's overlap most; the MMAs by themselves 2270 cycles for both.  Shared memory is busy 2560 of its cycles (operands 192 KB,
 // conversion 128 KB).  A CTA costs about 8 us besides (look-ups, q, first pages, output).
+#include <float.h>
 #include <math.h>
 
 #include <atomic>
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
         float top = -INFINITY, by[TILE_PAGES];
 #pragma unroll
         for (int p = 0; p < TILE_PAGES; ++p) {
-          by[p] = fminf(fac[p] * q_up, 3e38f);
+          by[p] = fminf(fmaxf(fac[p] * q_up, FLT_MIN), 3e38f);     // (not 0: it multiplies the -inf of what the row does not see)
           float x = max3(__uint_as_float(v[16 * p]), __uint_as_float(v[16 * p + 1]), __uint_as_float(v[16 * p + 2]));
           float y = max3(__uint_as_float(v[16 * p + 3]), __uint_as_float(v[16 * p + 4]), __uint_as_float(v[16 * p + 5]));
 #pragma unroll

@@ -31,3 +31,21 @@ def test_row_tiles_of_a_chunk_start_one_after_the_other(D):
     torch.cuda.synchronize()
     from statetree_b200.ops import device_status
     assert device_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ masks
+@pytest.mark.parametrize("size,q_size,scale", [(0.0, 1e-30, 0.1), (0.0, 1e-38, 0.1), (1.0, 1.0, 1e-44), (0.0, 1.0, 1e-40)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_masked_scores_whose_factor_is_below_fp32(D, size, q_size, scale):
+    """the product of softmax scale, a page's key exponent and a query's is 0 in fp32: hidden keys still take no part"""
+    gen = _gen(D)
+    lens, new = [200, 77, 300], [200, 40, 300]
+    store, table, seqs = _filled(gen, lens, 1, D, size=size)
+    cu = [0, 200, 240, 540]
+    q = (torch.randn(540, 4, D, generator=gen) * q_size).to(torch.bfloat16).to(DEV)
+    for window, starts in ((0, None), (50, [0, 60, 131])):
+        kw = dict(starts=None if starts is None else _ints(starts), window=window)
+        got = store.chunk_attention(q, _ints(cu), table, _ints(lens), scale, **kw)
+        _check(got, q, seqs, cu, lens, scale, starts, window)
+        got = store.attention(q[:3], table, _ints(lens), scale, **kw)
+        _check(got, q[:3], seqs, [0, 1, 2, 3], lens, scale, starts, window)
