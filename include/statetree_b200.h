@@ -270,6 +270,15 @@ int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq, const in
                       const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens,
                       const int32_t* starts, int64_t window, void* out, int64_t os, float* wo, float* wml, double scale, int64_t S,
                       void* stream);
+/* The two attentions with a block table whose rows of btw entries lie bts apart (part of a wider table; bts 0: one row for all).  Keys
+ * beyond a row's pages (in all four calls) take no part. */
+int st_kv8_attn_table(const void* q, int64_t qs, int64_t B, int64_t Hq, const void* kv, const int8_t* exps, int64_t nblocks, int64_t Hkv,
+                      int64_t D, const int32_t* bt, int64_t btw, int64_t bts, const int32_t* lens, const int32_t* starts, int64_t window,
+                      void* out, int64_t os, float* wo, float* wml, double scale, int64_t S, int64_t minpps, void* stream);
+int st_kv8_chunk_attn_table(const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
+                            const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t btw, int64_t bts,
+                            const int32_t* lens, const int32_t* starts, int64_t window, void* out, int64_t os, float* wo, float* wml,
+                            double scale, int64_t S, void* stream);
 
 /* st_gemv (1 <= B <= 8) of a fused gate/up projection with the SwiGLU gate in the epilogue: the M = 2 I rows of the tree
  * are the gate and up projections interleaved in 16-row tiles (tile 2j = gate rows 16j .. 16j + 15, tile 2j + 1 = the

@@ -40,8 +40,8 @@ struct Library {
   decltype(&st_lists_check) lists_check;
   decltype(&st_kv8_append) kv8_append;
   decltype(&st_kv8_dequant_blocks) kv8_dequant;
-  decltype(&st_kv8_attn) kv8_attn;
-  decltype(&st_kv8_chunk_attn) kv8_chunk;
+  decltype(&st_kv8_attn_table) kv8_attn;
+  decltype(&st_kv8_chunk_attn_table) kv8_chunk;
   decltype(&st_kv8_attn_workspace_bytes) kv8_workspace;
 };
 
@@ -86,8 +86,8 @@ Library library(const std::map<std::string, uint64_t>& address) {
   bind(lib.lists_check, "st_lists_check");
   bind(lib.kv8_append, "st_kv8_append");
   bind(lib.kv8_dequant, "st_kv8_dequant_blocks");
-  bind(lib.kv8_attn, "st_kv8_attn");
-  bind(lib.kv8_chunk, "st_kv8_chunk_attn");
+  bind(lib.kv8_attn, "st_kv8_attn_table");
+  bind(lib.kv8_chunk, "st_kv8_chunk_attn_table");
   bind(lib.kv8_workspace, "st_kv8_attn_workspace_bytes");
   return lib;
 }
@@ -328,10 +328,10 @@ py::object kv8_attention(const Library& lib, bool chunk, const at::Tensor& pages
     }
     void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
     rc = chunk ? lib.kv8_chunk(q.const_data_ptr(), q.stride(0), T, Hq, of<int32_t>(cu), B, pages.const_data_ptr(), of<int8_t>(exps),
-                               pages.size(0), H, D, of<int32_t>(table), table.stride(0), of<int32_t>(lens), of<int32_t>(starts), window,
-                               out.data_ptr(), out.stride(0), wo, wml, scale, splits, stream)
+                               pages.size(0), H, D, of<int32_t>(table), table.size(1), table.stride(0), of<int32_t>(lens),
+                               of<int32_t>(starts), window, out.data_ptr(), out.stride(0), wo, wml, scale, splits, stream)
                : lib.kv8_attn(q.const_data_ptr(), q.stride(0), B, Hq, pages.const_data_ptr(), of<int8_t>(exps), pages.size(0), H, D,
-                              of<int32_t>(table), table.stride(0), of<int32_t>(lens), of<int32_t>(starts), window, out.data_ptr(),
+                              of<int32_t>(table), table.size(1), table.stride(0), of<int32_t>(lens), of<int32_t>(starts), window, out.data_ptr(),
                               out.stride(0), wo, wml, scale, splits, min_pages, stream);
   }
   check(lib, rc);

@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     }
   }
   const int first_page = lo / PAGE;
-  const int end_page = end > lo ? (int)min((long long)(end - 1) / PAGE + 1, a.table_stride) : 0;
+  const int end_page = end > lo ? min((end - 1) / PAGE + 1, a.table_width) : 0;
   const int per_split = max(parts.min_pages, (end_page - first_page + parts.splits - 1) / parts.splits);
   const int lo_page = first_page + split * per_split, hi_page = min(end_page, lo_page + per_split);
   const int my_first = lo_page + warp;
@@ -955,7 +955,7 @@ extern "C" int st_kv8_dequant_blocks(const void* kv, const int8_t* exps, int64_t
 namespace st {
 // what both forms of the attention check and pass on
 int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
-               const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens,
+               const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t btw, int64_t bts, const int32_t* lens,
                const int32_t* starts, int64_t window, void* out, int64_t os, double scale) {
   ST_REQUIRE(T >= 0 && B >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "%s: heads", who);
   ST_REQUIRE(D == 64 || D == 128, "%s: head dimension 64 or 128 (got %lld)", who, (long long)D);
@@ -963,14 +963,14 @@ int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, 
   ST_REQUIRE(window >= 0 && window < (1ll << 31), "%s: window", who);
   if (T == 0 || B == 0) return 0;
   ST_REQUIRE(q && kv && exps && bt && lens && out, "%s: null pointer", who);
-  ST_REQUIRE(nblocks > 0 && bts > 0, "%s: empty cache or block table", who);
+  ST_REQUIRE(nblocks > 0 && btw > 0 && bts >= 0, "%s: empty cache or block table", who);
   ST_REQUIRE(st::aligned16(q) && st::aligned16(out) && st::aligned16(kv) && qs % 8 == 0 && os % 8 == 0 && qs >= 0 && os >= 0,
              "%s: q, out and the pages must be 16-byte aligned, token strides multiples of 8", who);
   ST_REQUIRE(((uintptr_t)exps & 1u) == 0, "%s: exponents must be 2-byte aligned", who);
   ST_REQUIRE(T == 1 || os >= Hq * D, "%s: rows of out overlap", who);
-  ST_REQUIRE(T * Hq < (1ll << 31) && bts < (1ll << 27), "%s: too large", who);
+  ST_REQUIRE(T * Hq < (1ll << 31) && btw < (1ll << 27), "%s: too large", who);
   a.q = (const uint16_t*)q; a.q_stride = qs; a.cu = cu; a.kv = (const uint8_t*)kv; a.exps = exps; a.nblocks = nblocks;
-  a.table = bt; a.table_stride = bts; a.lens = lens; a.starts = starts; a.out = (uint16_t*)out; a.out_stride = os;
+  a.table = bt; a.table_stride = bts; a.table_width = (int)btw; a.lens = lens; a.starts = starts; a.out = (uint16_t*)out; a.out_stride = os;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.B = (int)B; a.Hq = (int)Hq; a.H = (int)Hkv; a.window = (int)window; a.T = T;
   return 0;
@@ -981,8 +981,16 @@ extern "C" int st_kv8_attn(const void* q, int64_t qs, int64_t B, int64_t Hq, con
                            int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens, const int32_t* starts,
                            int64_t window, void* out, int64_t os, float* wo, float* wml, double scale, int64_t S, int64_t minpps,
                            void* stream) {
+  return st_kv8_attn_table(q, qs, B, Hq, kv, exps, nblocks, Hkv, D, bt, bts, bts, lens, starts, window, out, os, wo, wml, scale, S, minpps, stream);
+}
+
+extern "C" int st_kv8_attn_table(const void* q, int64_t qs, int64_t B, int64_t Hq, const void* kv, const int8_t* exps, int64_t nblocks,
+                                 int64_t Hkv, int64_t D, const int32_t* bt, int64_t btw, int64_t bts, const int32_t* lens,
+                                 const int32_t* starts, int64_t window, void* out, int64_t os, float* wo, float* wml, double scale,
+                                 int64_t S, int64_t minpps, void* stream) {
   Attn8 a;
-  if (int e = attn8_args(a, "st_kv8_attn", q, qs, B, Hq, nullptr, B, kv, exps, nblocks, Hkv, D, bt, bts, lens, starts, window, out, os, scale))
+  if (int e = attn8_args(a, "st_kv8_attn", q, qs, B, Hq, nullptr, B, kv, exps, nblocks, Hkv, D, bt, btw, bts, lens, starts, window, out, os,
+                         scale))
     return e;
   ST_REQUIRE(S >= 1 && S <= 1024, "st_kv8_attn: splits must be in [1, 1024]");
   ST_REQUIRE((wo && wml && st::aligned16(wo)) || st_kv8_attn_workspace_bytes(B, B, Hq, Hkv, D, S, 0) == 0,

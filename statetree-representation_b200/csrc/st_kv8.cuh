@@ -80,11 +80,11 @@ struct Attn8 {
   const uint16_t* q; long long q_stride;
   const int* cu;                                   // first query of each sequence [B + 1]; nullptr: one query each
   const uint8_t* kv; const int8_t* exps; long long nblocks;
-  const int* table; long long table_stride;
+  const int* table; long long table_stride;        // rows of table_width entries
   const int* lens; const int* starts;
   uint16_t* out; long long out_stride;
   float scale_log2;
-  int B, Hq, H, window;
+  int B, Hq, H, window, table_width;
   long long T;
 };
 // partial results of sequences that are split: o [T, Hq, splits, D] (not normalised), ml [T, Hq, splits, 2] = (reference, base 2; sum)
@@ -136,7 +136,7 @@ __device__ __forceinline__ bool find_rows(const Attn8& a, int G, int slot, int l
 
 // st_kv8.cu: what both forms of the attention check and pass on; the join of the partial results
 int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
-               const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts, const int32_t* lens,
+               const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t btw, int64_t bts, const int32_t* lens,
                const int32_t* starts, int64_t window, void* out, int64_t os, double scale);
 // Chunks of few rows per sequence go through the decode kernel, eight rows a CTA: its time grows with every eight rows, the chunk kernel's
 // hardly up to 128.  32 sequences of 2000 tokens, D = 128, us: 16 rows 38 in the decode kernel and 103 in the other, 32 rows 63 and 74, 64

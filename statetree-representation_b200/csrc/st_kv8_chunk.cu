@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     const int first_pos = w.pos0 + w.row0 / G, last_pos = w.pos0 + (w.row0 + w.rows - 1) / G;
     w.lo0 = start;
     const int lo = a.window > 0 ? max(start, first_pos - a.window + 1) : start;
-    const int end = (int)min((long long)last_pos + 1, a.table_stride * PAGE);            // keys [lo, end)
+    const int end = (int)min((long long)last_pos + 1, (long long)a.table_width * PAGE);            // keys [lo, end)
     const int t0 = lo / KEYS, t1 = end > lo ? (end - 1) / KEYS + 1 : t0;
     const int per = (t1 - t0 + c.parts.splits - 1) / c.parts.splits;
     w.first_tile = t0 + w.split * per;
@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     w.count1 = w.rows > ROWS ? w.tiles : 0;
   }
   const int tiles = max(w.count0, w.count1);
-  // (pages behind the last key of the sequence may not exist: no key of theirs is seen)
-  const int end_page = (int)min((long long)(w.pos0 + w.n - 1) / PAGE + 1, a.table_stride);
+  // (pages behind the last key of the sequence, or behind its row of the table, may not exist: no key of theirs is seen)
+  const int end_page = min((w.pos0 + w.n - 1) / PAGE + 1, a.table_width);
   const uint64_t keep = policy_evict_last();                      // other row tiles of the sequence read the same pages
 
   if (warp == W_MMA) {
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     const int token = live ? my / G : 0, head = live ? my % G : 0, hq = w.h * G + head;
     const int pos = w.pos0 + token;
     // (a row that is none sees everything: its results go nowhere, and a warp with one does not take the masked way for it)
-    const int hi = live ? pos : 0x7FFFFFFF, lo = !live ? 0 : a.window > 0 ? max(w.lo0, pos - a.window + 1) : w.lo0;
+    const int hi = live ? min(pos, a.table_width * PAGE - 1) : 0x7FFFFFFF, lo = !live ? 0 : a.window > 0 ? max(w.lo0, pos - a.window + 1) : w.lo0;
     const bool any = __any_sync(FULL, live);
     float m = -INFINITY, l = 0.f, q_up = 1.f;                     // q_up undoes the scale of q
     bool ok = true;
@@ -616,9 +616,17 @@ extern "C" int st_kv8_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t H
                                  const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t bts,
                                  const int32_t* lens, const int32_t* starts, int64_t window, void* out, int64_t os, float* wo,
                                  float* wml, double scale, int64_t S, void* stream) {
+  return st_kv8_chunk_attn_table(q, qs, T, Hq, cu, B, kv, exps, nblocks, Hkv, D, bt, bts, bts, lens, starts, window, out, os, wo, wml, scale,
+                                 S, stream);
+}
+
+extern "C" int st_kv8_chunk_attn_table(const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv,
+                                       const int8_t* exps, int64_t nblocks, int64_t Hkv, int64_t D, const int32_t* bt, int64_t btw,
+                                       int64_t bts, const int32_t* lens, const int32_t* starts, int64_t window, void* out, int64_t os,
+                                       float* wo, float* wml, double scale, int64_t S, void* stream) {
   Chunk8 c;
-  if (int e = st::attn8_args(c.a, "st_kv8_chunk_attn", q, qs, T, Hq, cu, B, kv, exps, nblocks, Hkv, D, bt, bts, lens, starts, window, out,
-                             os, scale))
+  if (int e = st::attn8_args(c.a, "st_kv8_chunk_attn", q, qs, T, Hq, cu, B, kv, exps, nblocks, Hkv, D, bt, btw, bts, lens, starts, window,
+                             out, os, scale))
     return e;
   ST_REQUIRE(S >= 1 && S <= 1024, "st_kv8_chunk_attn: splits must be in [1, 1024]");
   ST_REQUIRE((wo && wml && st::aligned16(wo)) || st_kv8_attn_workspace_bytes(T, B, Hq, Hkv, D, S, 1) == 0,

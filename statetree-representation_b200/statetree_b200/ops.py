@@ -68,6 +68,10 @@ _SIGNATURES = {
                            _i64, _i64, _vp]),
     "st_kv8_chunk_attn": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64,
                                  _vp, _vp, _dbl, _i64, _vp]),
+    "st_kv8_attn_table": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp,
+                                 _dbl, _i64, _i64, _vp]),
+    "st_kv8_chunk_attn_table": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp,
+                                       _i64, _vp, _vp, _dbl, _i64, _vp]),
     "st_gemv_swiglu_supported": (_int, [_i64, _i64, _i64]),
     "st_gemv_swiglu": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "st_rope_kv_append": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _dbl, _vp, _vp, _i64,
@@ -123,8 +127,8 @@ def lib():
 CALLS_PATH = os.path.join(_HERE, "_calls.so")
 _CALLS = None                                           # False: there is none
 _NATIVE = ("st_gemv", "st_gemm", "st_gemv_list", "st_gemm_list", "st_last_error", "st_encode", "st_encode_lists", "st_encode_offsets",
-           "st_encode_offsets_workspace_bytes", "st_dec_check", "st_lists_check", "st_kv8_append", "st_kv8_dequant_blocks", "st_kv8_attn",
-           "st_kv8_chunk_attn", "st_kv8_attn_workspace_bytes")
+           "st_encode_offsets_workspace_bytes", "st_dec_check", "st_lists_check", "st_kv8_append", "st_kv8_dequant_blocks", "st_kv8_attn_table",
+           "st_kv8_chunk_attn_table", "st_kv8_attn_workspace_bytes")
 
 
 def calls():
@@ -686,9 +690,10 @@ class _KV:
         if B == 0:
             return
         with _ctx(kv):
-            _check(lib().st_kv8_attn(q.data_ptr(), q.stride(0), B, Hq, kv.data_ptr(), exps.data_ptr(), kv.size(0), H, D, bt.data_ptr(),
-                                     bt.stride(0), lens.data_ptr(), _ptr(starts), int(window), out.data_ptr(), out.stride(0), _ptr(wo),
-                                     _ptr(wml), float(scale), int(S), int(minpps), _stream(kv)))
+            _check(lib().st_kv8_attn_table(q.data_ptr(), q.stride(0), B, Hq, kv.data_ptr(), exps.data_ptr(), kv.size(0), H, D,
+                                           bt.data_ptr(), bt.size(1), bt.stride(0), lens.data_ptr(), _ptr(starts), int(window),
+                                           out.data_ptr(), out.stride(0), _ptr(wo), _ptr(wml), float(scale), int(S), int(minpps),
+                                           _stream(kv)))
 
     @staticmethod
     def kv8_chunk_attn(q, cu, kv, exps, bt, lens, out, scale, S=1, wo=None, wml=None, starts=None, window=0):
@@ -702,9 +707,10 @@ class _KV:
         if q.size(0) == 0 or B == 0:
             return
         with _ctx(kv):
-            _check(lib().st_kv8_chunk_attn(q.data_ptr(), q.stride(0), q.size(0), Hq, _ptr(cu), B, kv.data_ptr(), exps.data_ptr(),
-                                           kv.size(0), H, D, bt.data_ptr(), bt.stride(0), lens.data_ptr(), _ptr(starts), int(window),
-                                           out.data_ptr(), out.stride(0), _ptr(wo), _ptr(wml), float(scale), int(S), _stream(kv)))
+            _check(lib().st_kv8_chunk_attn_table(q.data_ptr(), q.stride(0), q.size(0), Hq, _ptr(cu), B, kv.data_ptr(), exps.data_ptr(),
+                                                 kv.size(0), H, D, bt.data_ptr(), bt.size(1), bt.stride(0), lens.data_ptr(), _ptr(starts),
+                                                 int(window), out.data_ptr(), out.stride(0), _ptr(wo), _ptr(wml), float(scale), int(S),
+                                                 _stream(kv)))
 
 
 def ext():

@@ -49,3 +49,54 @@ def test_masked_scores_whose_factor_is_below_fp32(D, size, q_size, scale):
         _check(got, q, seqs, cu, lens, scale, starts, window)
         got = store.attention(q[:3], table, _ints(lens), scale, **kw)
         _check(got, q[:3], seqs, [0, 1, 2, 3], lens, scale, starts, window)
+
+
+# ------------------------------------------------------------------------------------------------ block tables
+def _both(store, q, table, lens, cu, **kw):
+    n = table.shape[0]
+    return store.attention(q[:n], table, lens, 0.1, **kw), store.chunk_attention(q, cu, table, lens, 0.1, **kw)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("rows", [20, 300])
+def test_block_table_of_any_strides(native, rows, monkeypatch):
+    """one row whose stride is not its width, part of a wider table, one row for all sequences: the same bits"""
+    from statetree_b200 import kvcache
+    gen = _gen(rows)
+    store, table, _ = _filled(gen, [400], 2, 128)
+    if not native:
+        monkeypatch.setattr(kvcache, "calls", lambda: None)
+    q = _rand(gen, rows, 8, 128).to(DEV)
+    lens, cu = _ints([400]), _ints([0, rows])
+    want = _both(store, q, table, lens, cu)
+    line = table[0][:, None].t()
+    assert line.shape == table.shape and line.stride() == (1, 1)
+    wide = torch.cat([table + 1, table, table + 2], 1)[:, table.shape[1]:2 * table.shape[1]]
+    for other in (line, wide, table.as_strided(table.shape, (3, 1))):
+        for a, b in zip(want, _both(store, q, other, lens, cu)):
+            assert torch.equal(a, b)
+    lens, cu = _ints([400, 350, 20]), _ints([0, rows // 2, rows // 2, rows])
+    want = _both(store, q, table.repeat(3, 1), lens, cu)
+    for a, b in zip(want, _both(store, q, table.expand(3, -1), lens, cu)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("rows", [20, 300])
+def test_tokens_beyond_the_block_table(native, rows, monkeypatch):
+    """lengths that the table has no pages for: what lies behind a row of it, in a wider table or behind its end, is not looked at"""
+    from statetree_b200 import kvcache
+    gen = _gen(rows)
+    store, table, seqs = _filled(gen, [400, 400], 2, 128, table_extra=0)
+    if not native:
+        monkeypatch.setattr(kvcache, "calls", lambda: None)
+    w = table.shape[1]
+    wide = torch.cat([table.flip(1), table], 1)[:, w:]
+    q = _rand(gen, rows, 8, 128).to(DEV)
+    new = [0, rows // 2, rows]
+    for splits in (1, 3):
+        for lens in ([430, 500], [401, 400 + rows]):
+            want, got = (_both(store, q, t, _ints(lens), _ints(new), splits=splits) for t in (table, wide))
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+            _check(got[0], q[:2], seqs, [0, 1, 2], lens, 0.1)
+            _check(got[1], q, seqs, new, lens, 0.1)
