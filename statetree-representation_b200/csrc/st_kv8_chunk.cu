@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
         float top = -INFINITY, by[TILE_PAGES];
 #pragma unroll
         for (int p = 0; p < TILE_PAGES; ++p) {
-          by[p] = fminf(fmaxf(fac[p] * q_up, FLT_MIN), 3e38f);     // (not 0: it multiplies the -inf of what the row does not see)
+          by[p] = fminf(fmaf(fac[p], q_up, FLT_MIN), 3e38f);       // (not 0: it multiplies the -inf of what the row does not see)
           float x = max3(__uint_as_float(v[16 * p]), __uint_as_float(v[16 * p + 1]), __uint_as_float(v[16 * p + 2]));
           float y = max3(__uint_as_float(v[16 * p + 3]), __uint_as_float(v[16 * p + 4]), __uint_as_float(v[16 * p + 5]));
 #pragma unroll
