@@ -13,7 +13,8 @@ so decode steps can be captured in CUDA graphs.  Left padding is supported: each
 read once from the prefill attention mask.  Head dimension 128 only.
 
 StateTreeKVCache(..., eight_bit=True) keeps 8-bit pages instead (kvcache.PageStore8; head dimension 64 or 128): then every chunk of a
-prompt attends to the pages too, causally and from each sequence's first valid position on, and nothing is expanded.
+prompt attends to the pages too, causally and from each sequence's first valid position on, and nothing is expanded.  The padding may
+be longer than the first chunk.
 """
 import threading
 
@@ -117,6 +118,7 @@ class StateTreeKVLayer(CacheLayerMixin):
             self.gpu_len.zero_()
             self.cache.starts.zero_()                   # (a prompt without padding may come without a mask)
         self.cache.starts_known = False
+        self.cache.starts_at = 0
 
     def check(self):
         if self.is_initialized:
@@ -142,6 +144,7 @@ class StateTreeKVCache(Cache):
         self.max_pages = -(-self.max_len // PAGE)
         self.alloc_batch, self.pool_blocks, self.eight_bit = batch_size, pool_blocks, eight_bit
         self.starts_known = False
+        self.starts_at = 0                           # 8-bit pages: keys up to the pass whose mask has been read
         self._allocated = False
         super().__init__(layers=[StateTreeKVLayer(self, i) for i in range(self.num_layers)])
 
@@ -165,6 +168,20 @@ class StateTreeKVCache(Cache):
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None, *args, **kwargs):
         return self.layers[layer_idx].update(key_states, value_states, cache_kwargs)
 
+    def read_mask(self, mask, stored, B, T, window):
+        """the left padding of every sequence (starts) after a pass's 4-D mask over its T tokens and `stored` keys, the pass's own among
+        them"""
+        before, starts, flag = stored - T, self.starts[:B], mask.dtype == torch.bool
+        if self.starts_at != stored:                 # the first layer of the pass
+            self.starts_at = stored
+            rows = mask[:, 0]                        # the last query sees all that is none; with a window, every query that is none itself
+            rows = rows.diagonal(before, 1, 2) if window else rows[:, -1]
+            seen = (rows if flag else rows == 0).int()
+            first = torch.where(seen.any(-1), seen.argmax(-1), seen.shape[-1])
+            if window:                               # (keys before the pass: as they were, if one was no padding)
+                first = torch.where(first > 0, first + before, starts.clamp(max=before))
+            starts.copy_(first.to(torch.int32).expand(B))
+
     def check(self):
         """raise if an escape could not be stored anywhere (pool too small): the cache is never silently lossy"""
         for layer in self.layers:
@@ -176,35 +193,37 @@ class StateTreeKVCache(Cache):
 
 
 def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, scaling=None, **kwargs):
-    """the 'statetree' attention implementation: a decode step reads the compressed pages, anything else runs SDPA"""
+    """the 'statetree' attention implementation: a decode step reads the compressed pages, anything else runs SDPA (over 8-bit pages:
+    chunk attention over the pages)"""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     layer = getattr(_LAST, "layer", None)
     _LAST.layer = None
     if layer is not None and layer.layer_idx == getattr(module, "layer_idx", layer.layer_idx):
         c = layer.cache
         B, Hq, T, D = query.shape
+        window = kwargs.get("sliding_window") or 0
         if T == 1 and layer.host_len > 1:
             q = query[:, :, 0, :]
             if q.stride(-1) != 1 or q.stride(1) != D:
                 q = q.contiguous()
             scale = float(scaling) if scaling is not None else D ** -0.5
-            more = dict(window=kwargs.get("sliding_window") or 0) if c.eight_bit else {}
+            more = dict(window=window) if c.eight_bit else {}
             out = layer.store.attention(q, c.table32[:B], c.lens[:B], scale, splits=c.splits, starts=c.starts[:B],
                                         min_pages=4, **more)
             return out.view(B, 1, Hq, D), None
-        if T > 1 and not c.starts_known and attention_mask is not None and attention_mask.dim() == 4:
-            # the last query sees everything but the padding; with a window (8-bit pages), every query that is none sees itself
-            rows = attention_mask[:, 0]
-            seen = rows.diagonal(rows.shape[2] - T, 1, 2) if c.eight_bit and kwargs.get("sliding_window") else rows[:, -1]
-            masked = ~seen if seen.dtype == torch.bool else seen < 0
-            c.starts[:B].copy_(masked.sum(-1).to(torch.int32))
-            c.starts_known = True
         if c.eight_bit:                              # a chunk (its keys are in the pages already), or the first token of all
+            if attention_mask is not None and attention_mask.dim() == 4:
+                c.read_mask(attention_mask, layer.host_len, B, T, window)
             q = query.transpose(1, 2).reshape(B * T, Hq, D)
             cu = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=q.device)
             out = layer.store.chunk_attention(q, cu, c.table32[:B], c.lens[:B], float(scaling) if scaling is not None else D ** -0.5,
-                                              starts=c.starts[:B], window=kwargs.get("sliding_window") or 0)
+                                              starts=c.starts[:B], window=window)
             return out.view(B, T, Hq, D), None
+        if T > 1 and not c.starts_known and attention_mask is not None and attention_mask.dim() == 4:
+            last_row = attention_mask[:, 0, -1, :]                  # the last query sees everything but the padding
+            masked = ~last_row if last_row.dtype == torch.bool else last_row < 0
+            c.starts[:B].copy_(masked.sum(-1).to(torch.int32))
+            c.starts_known = True
     return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout, scaling=scaling, **kwargs)
 
 

@@ -100,3 +100,38 @@ def test_tokens_beyond_the_block_table(native, rows, monkeypatch):
             assert all(torch.equal(a, b) for a, b in zip(want, got))
             _check(got[0], q[:2], seqs, [0, 1, 2], lens, 0.1)
             _check(got[1], q, seqs, new, lens, 0.1)
+
+
+# ------------------------------------------------------------------------------------------------ Hugging Face cache
+@pytest.mark.parametrize("windows", [None, ["sliding_attention", "full_attention"], ["full_attention", "sliding_attention"]])
+def test_hf_cache_with_padding_longer_than_a_chunk(windows):
+    """a sequence behind 32 tokens of padding, in chunks of 16, against the same sequence by itself.  Both pass about twenty roundings
+    to BF16 in two layers (2^-8 each: 7.8e-2 at most); the pages and their exponents are the same"""
+    pytest.importorskip("transformers")
+    from transformers import Qwen3Config, Qwen3ForCausalLM
+    from statetree_b200.kvcache import StateTreeKVCache, enable
+    cfg = Qwen3Config(vocab_size=512, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=128, max_position_embeddings=256, tie_word_embeddings=False,
+                      **(dict(use_sliding_window=True, sliding_window=8, layer_types=windows) if windows else {}))
+    torch.manual_seed(0)
+    model = enable(Qwen3ForCausalLM(cfg).to(torch.bfloat16).cuda().eval())
+    P, pad, ends = 50, 32, [16, 32, 48, 50, 51, 52]
+    ids = torch.randint(0, cfg.vocab_size, (2, 52), device="cuda")
+    mask = torch.ones(2, 52, dtype=torch.long, device="cuda")
+    mask[1, :pad] = 0
+    at = torch.arange(52, device="cuda").repeat(2, 1)
+    at[1] = (at[1] - pad).clamp(min=0)
+
+    def passes(rows, first, ends):
+        cache, outs = StateTreeKVCache(model.config, batch_size=len(rows), max_cache_len=64, eight_bit=True), []
+        with torch.no_grad():
+            for a, b in zip([first] + ends, ends):
+                outs.append(model(input_ids=ids[rows, a:b], attention_mask=mask[rows, first:b], position_ids=at[rows, a:b],
+                                  past_key_values=cache, use_cache=True).logits[:, -1].float())
+        cache.check()
+        return outs
+
+    both = passes([0, 1], 0, ends)
+    for row, first in ((0, 0), (1, pad)):
+        for got, want in zip(both[2:], passes([row], first, [48, 50, 51, 52])):
+            assert float((got[row] - want[0]).norm() / want[0].norm()) < 2 * 20 * 2.0 ** -8, (row, first)

@@ -1,0 +1,103 @@
+"""The 8-bit Hugging Face cache on the CPU with a store that only takes notes: which masks its attention reads as left padding, and
+which masks and modules it refuses."""
+import types
+
+import pytest
+import torch
+
+pytest.importorskip("transformers")
+NEG = torch.finfo(torch.bfloat16).min
+
+
+class _Notes:
+    """a PageStore8's calls"""
+    def __init__(self):
+        self.calls = []
+
+    def _take(self, kind, q, starts, window):
+        self.calls.append((kind, starts.tolist(), window))
+        return torch.zeros_like(q)
+
+    def chunk_attention(self, q, cu, table, lens, scale, splits=None, starts=None, out=None, window=0):
+        return self._take("chunk", q, starts, window)
+
+    def attention(self, q, table, lens, scale, splits=None, starts=None, min_pages=4, out=None, window=0):
+        return self._take("step", q, starts, window)
+
+    def append(self, K, V, slots):
+        pass
+
+    def reset(self):
+        pass
+
+
+class _Model:
+    """layers of an attention module over one cache, fed mask by mask"""
+    def __init__(self, B, layers=2, eight_bit=True):
+        from statetree_b200.kvcache import StateTreeKVCache
+        cfg = types.SimpleNamespace(num_hidden_layers=layers, num_attention_heads=4, num_key_value_heads=2)
+        self.cache = StateTreeKVCache(cfg, batch_size=B, max_cache_len=256, eight_bit=eight_bit)
+        self.B, self.notes = B, _Notes()
+
+    def __call__(self, T, mask, windows=None, module=None, **kw):
+        """a forward pass over T tokens; a mask and a window for all layers, or a list of them"""
+        from statetree_b200.kvcache import statetree_attention
+        of = lambda x, i: x[i] if isinstance(x, list) else x                                  # noqa: E731
+        q, k = torch.zeros(self.B, 4, T, 128, dtype=torch.bfloat16), torch.zeros(self.B, 2, T, 128, dtype=torch.bfloat16)
+        for i, layer in enumerate(self.cache.layers):
+            if not layer.is_initialized:
+                layer.lazy_initialization(k, k)
+                layer.store = self.notes
+            layer.update(k, k)
+            statetree_attention(types.SimpleNamespace(layer_idx=i, **{"is_causal": True, **(module or {})}), q, k, k, of(mask, i), scaling=0.1,
+                                sliding_window=of(windows, i), **kw)
+
+    @property
+    def starts(self):
+        return self.notes.calls[-1][1]
+
+
+def _mask(pads, before, T, window=0, kind="bool"):
+    """[B, 1, T, before + T]: causal with left padding (and a window)"""
+    K = before + T
+    k, p = torch.arange(K), torch.arange(before, K)[:, None]
+    m = (k <= p) & (k >= torch.tensor(pads)[:, None, None])
+    if window:
+        m &= k > p - window
+    m = m[:, None]
+    return m if kind == "bool" else torch.zeros(m.shape, dtype=torch.bfloat16).masked_fill(~m, -float("inf") if kind == "inf" else NEG)
+
+
+@pytest.mark.parametrize("kind", ["bool", "inf", "lowest"])
+@pytest.mark.parametrize("window", [0, 5, 40])
+@pytest.mark.parametrize("pads", [[0, 3], [0, 20], [16, 33], [40, 1]])
+def test_left_padding_longer_than_a_chunk(pads, window, kind):
+    """chunks of 16: a sequence's padding may end in any of them"""
+    m, at = _Model(2), 0
+    for T in (16, 16, 16, 1, 7, 1):
+        m(T, _mask(pads, at, T, window, kind), window or None)
+        at += T
+        seen = [min(p, at) for p in pads]
+        assert m.starts == seen and m.notes.calls[-1][2] == window
+    assert [c[0] for c in m.notes.calls] == ["chunk"] * 6 + ["step"] * 2 + ["chunk"] * 2 + ["step"] * 2
+    m.cache.reset()
+    m(3, None)
+    assert m.starts == [0, 0]
+
+
+@pytest.mark.parametrize("windows", [[None, 6], [6, None]])
+def test_layers_with_and_without_a_window(windows):
+    m = _Model(2)
+    for at, T in ((0, 16), (16, 16), (32, 4)):
+        m(T, [_mask([0, 21], at, T, w or 0) for w in windows], windows)
+        assert m.starts == [0, min(21, at + T)]
+
+
+@pytest.mark.parametrize("kind", ["bool", "lowest"])
+def test_rows_of_padding_may_see_everything(kind):
+    """masks that leave no row empty let a padding token see everything"""
+    mask = _mask([0, 3], 0, 8, kind=kind)
+    mask[1, :, :3] = mask[0, 0, 7, 0]
+    m = _Model(2)
+    m(8, mask)
+    assert m.starts == [0, 3]
