@@ -14,15 +14,19 @@ read once from the prefill attention mask.  Head dimension 128 only.
 
 StateTreeKVCache(..., eight_bit=True) keeps 8-bit pages instead (kvcache.PageStore8; head dimension 64 or 128): then every chunk of a
 prompt attends to the pages too, causally and from each sequence's first valid position on, and nothing is expanded.  The padding may
-be longer than the first chunk.
+be longer than the first chunk; other masks (packed sequences, right padding) are refused.
 """
 import threading
+import weakref
 
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
 from .kvcache import PAGE, PageStore, PageStore8, decode_splits, decode_splits8
 
+HIDDEN = -1e4                      # an additive mask's values up to here hide a key (the exponential of a score is 0 then)
+ODD_MASK = "StateTreeKVCache: over 8-bit pages a mask is causal (within the layer's sliding window) with left padding"
+MASK_PART = 1 << 26                # elements of a mask that are checked at a time
 _LAST = threading.local()          # the layer whose update() ran last on this thread; the attention function picks it up
 
 
@@ -117,6 +121,7 @@ class StateTreeKVLayer(CacheLayerMixin):
             self.store.reset()
             self.gpu_len.zero_()
             self.cache.starts.zero_()                   # (a prompt without padding may come without a mask)
+            self.cache.odd_mask.zero_()
         self.cache.starts_known = False
         self.cache.starts_at = 0
 
@@ -144,7 +149,7 @@ class StateTreeKVCache(Cache):
         self.max_pages = -(-self.max_len // PAGE)
         self.alloc_batch, self.pool_blocks, self.eight_bit = batch_size, pool_blocks, eight_bit
         self.starts_known = False
-        self.starts_at = 0                           # 8-bit pages: keys up to the pass whose mask has been read
+        self.starts_at, self.masks = 0, []           # 8-bit pages: the pass whose masks have been read, and which have been checked
         self._allocated = False
         super().__init__(layers=[StateTreeKVLayer(self, i) for i in range(self.num_layers)])
 
@@ -159,6 +164,7 @@ class StateTreeKVCache(Cache):
         self.table32 = self.table64.to(torch.int32)
         self.lens = torch.zeros(n, dtype=torch.int32, device=device)
         self.starts = torch.zeros(n, dtype=torch.int32, device=device)
+        self.odd_mask = torch.zeros((), dtype=torch.bool, device=device)
         group = -(-self.num_q_heads // max(1, H))
         self.splits = decode_splits8(n * H * -(-group // 8), self.max_pages) if self.eight_bit else decode_splits(n, H, self.max_pages)
         if self.pool_blocks is None:
@@ -170,10 +176,14 @@ class StateTreeKVCache(Cache):
 
     def read_mask(self, mask, stored, B, T, window):
         """the left padding of every sequence (starts) after a pass's 4-D mask over its T tokens and `stored` keys, the pass's own among
-        them"""
+        them; ValueError for a mask that is more than causal (and windowed) with left padding, which is all that the 8-bit pages are
+        read with.  Rows of padding see nothing, or everything (in masks that leave no row empty).  The check is one wait for the GPU a
+        pass and kind of mask; a captured pass cannot wait and leaves the error to check()."""
+        if mask.dim() != 4 or mask.shape[2] != T or mask.shape[3] != stored:
+            raise ValueError(f"StateTreeKVCache: a mask of shape {tuple(mask.shape)} over {T} tokens and {stored} keys")
         before, starts, flag = stored - T, self.starts[:B], mask.dtype == torch.bool
         if self.starts_at != stored:                 # the first layer of the pass
-            self.starts_at = stored
+            self.starts_at, self.masks = stored, []
             rows = mask[:, 0]                        # the last query sees all that is none; with a window, every query that is none itself
             rows = rows.diagonal(before, 1, 2) if window else rows[:, -1]
             seen = (rows if flag else rows == 0).int()
@@ -181,11 +191,31 @@ class StateTreeKVCache(Cache):
             if window:                               # (keys before the pass: as they were, if one was no padding)
                 first = torch.where(first > 0, first + before, starts.clamp(max=before))
             starts.copy_(first.to(torch.int32).expand(B))
+        if any(m() is mask and w == window for m, w in self.masks):
+            return                                   # (the layers of a pass share their masks)
+        k, wrong = torch.arange(stored, device=mask.device), None
+        step = max(1, MASK_PART // (B * mask.shape[1] * stored))
+        for at in range(0, T, step):
+            part, p = mask[:, :, at:at + step], k[before + at:before + min(T, at + step), None]
+            want = (k <= p) & (k > p - window) if window else k <= p
+            want = (want & (k >= starts[:, None, None]))[:, None]
+            hidden, shown = (~part, part) if flag else (part <= HIDDEN, part == 0)
+            padding = (p[:, 0] < starts[:, None])[:, None]
+            bad = torch.where(padding, ~(hidden.all(-1) | shown.all(-1)), ~torch.where(want, shown, hidden).all(-1)).any()
+            wrong = bad if wrong is None else wrong | bad
+        if mask.is_cuda and torch.cuda.is_current_stream_capturing():
+            self.odd_mask |= wrong
+        elif bool(wrong):
+            raise ValueError(ODD_MASK)
+        self.masks.append((weakref.ref(mask), window))
 
     def check(self):
-        """raise if an escape could not be stored anywhere (pool too small): the cache is never silently lossy"""
+        """raise if an escape could not be stored anywhere (pool too small): the cache is never silently lossy.  8-bit pages: if values that
+        are not finite were appended, or a captured pass met a mask that read_mask refuses"""
         for layer in self.layers:
             layer.check()
+        if self._allocated and self.eight_bit and bool(self.odd_mask):
+            raise ValueError(ODD_MASK)
 
     def storage_bytes(self):
         return sum(l.store.pages.numel() + (l.store.exps.numel() if self.eight_bit else l.store.pool.numel() * 4) for l in self.layers
@@ -194,7 +224,7 @@ class StateTreeKVCache(Cache):
 
 def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, scaling=None, **kwargs):
     """the 'statetree' attention implementation: a decode step reads the compressed pages, anything else runs SDPA (over 8-bit pages:
-    chunk attention over the pages)"""
+    chunk attention over the pages, and ValueError for masks that it does not know)"""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     layer = getattr(_LAST, "layer", None)
     _LAST.layer = None
@@ -212,7 +242,7 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
                                         min_pages=4, **more)
             return out.view(B, 1, Hq, D), None
         if c.eight_bit:                              # a chunk (its keys are in the pages already), or the first token of all
-            if attention_mask is not None and attention_mask.dim() == 4:
+            if attention_mask is not None:
                 c.read_mask(attention_mask, layer.host_len, B, T, window)
             q = query.transpose(1, 2).reshape(B * T, Hq, D)
             cu = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=q.device)

@@ -135,3 +135,49 @@ def test_hf_cache_with_padding_longer_than_a_chunk(windows):
     for row, first in ((0, 0), (1, pad)):
         for got, want in zip(both[2:], passes([row], first, [48, 50, 51, 52])):
             assert float((got[row] - want[0]).norm() / want[0].norm()) < 2 * 20 * 2.0 ** -8, (row, first)
+
+
+def test_hf_cache_masks_in_a_captured_pass():
+    """a captured chunk reads its mask's padding when it is replayed; a mask that an eager pass refuses shows in check()"""
+    pytest.importorskip("transformers")
+    import types
+    from statetree_b200.kvcache import StateTreeKVCache, statetree_attention
+    B, T = 2, 24
+    cfg = types.SimpleNamespace(num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2)
+    cache = StateTreeKVCache(cfg, batch_size=B, max_cache_len=64, eight_bit=True)
+    gen = _gen(1)
+    q, k, v = (_rand(gen, B, h, T, 128).to(DEV) for h in (4, 2, 2))
+    at = torch.arange(T, device=DEV)
+    plain = lambda pads: ((at <= at[:, None]) & (at >= _ints(pads)[:, None, None]))[:, None]  # noqa: E731
+    mask = plain([0, 0])
+
+    def step():
+        outs = []
+        for i in range(2):
+            cache.update(k, v, i)
+            outs.append(statetree_attention(types.SimpleNamespace(layer_idx=i), q, k, v, mask, scaling=0.1)[0])
+        return outs
+
+    step()
+    cache.reset()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for pads in ([0, 5], [3, 0]):
+        mask.copy_(plain(pads))
+        cache.reset()
+        graph.replay()
+        got = [o.clone() for o in outs]
+        cache.check()
+        cache.reset()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+    mask[0, 0, 20, 7] = False                              # one hidden key
+    cache.reset()
+    graph.replay()
+    with pytest.raises(ValueError, match="mask"):
+        cache.check()
+    cache.reset()
+    cache.check()
+    with pytest.raises(ValueError, match="mask"):
+        step()

@@ -101,3 +101,73 @@ def test_rows_of_padding_may_see_everything(kind):
     m = _Model(2)
     m(8, mask)
     assert m.starts == [0, 3]
+
+
+def _packed():
+    m = _mask([0, 0], 0, 8)
+    m[:, :, 3:, :3] = False
+    return m
+
+
+def _right():
+    return _mask([0, 0], 0, 8) & torch.tensor([[1] * 8, [1] * 6 + [0, 0]], dtype=torch.bool)[:, None, None]
+
+
+def _prefix():
+    m = _mask([0, 0], 0, 8)
+    m[:, :, :4, :4] = True
+    return m
+
+
+def _holes():
+    m = _mask([0, 0], 0, 8)
+    m[1, 0, 7, 4] = False
+    return m
+
+
+def _heads():
+    m = _mask([0, 0], 0, 8).repeat(1, 4, 1, 1)
+    m[1, 2, 7, 4] = False
+    return m
+
+
+@pytest.mark.parametrize("make", [_packed, _right, _prefix, _holes, _heads])
+@pytest.mark.parametrize("kind", [torch.bool, torch.float32])
+def test_other_masks_are_refused(make, kind):
+    """packed sequences, right padding, a prefix that sees ahead, single hidden keys, heads of their own"""
+    mask = make()
+    if kind != torch.bool:
+        mask = torch.zeros(mask.shape).masked_fill(~mask, -float("inf"))
+    with pytest.raises(ValueError, match="mask"):
+        _Model(2)(8, mask)
+
+
+@pytest.mark.parametrize("row", [0, 1, 70, 129, 130, 199])
+def test_a_mask_is_checked_in_all_its_rows(row, monkeypatch):
+    """large masks are gone through some rows at a time"""
+    from statetree_b200 import hf_cache
+    monkeypatch.setattr(hf_cache, "MASK_PART", 65 * 200 * 2)
+    mask = _mask([0, 0], 0, 200)
+    _Model(2)(200, mask)
+    mask[1, 0, row, row] = False
+    with pytest.raises(ValueError, match="mask"):
+        _Model(2)(200, mask)
+
+
+def test_more_masks_are_refused():
+    bias = torch.zeros(2, 1, 8, 8).masked_fill(~_mask([0, 0], 0, 8), -float("inf"))
+    bias[0, 0, 5, 2] = -0.5                                # a bias, not a mask
+    nan = bias.clone()
+    nan[0, 0, 5, 2] = float("nan")
+    for mask in (bias, nan, _mask([0, 0], 0, 8, 4), _mask([0, 0], 0, 8)[:, 0], torch.ones(2, 8)):
+        with pytest.raises(ValueError, match="mask"):
+            _Model(2)(8, mask)
+    with pytest.raises(ValueError, match="mask"):          # a window that the mask has not
+        _Model(2)(8, _mask([0, 0], 0, 8), 4)
+    m = _Model(2)                                          # only the second layer's, and only in a later pass
+    m(8, _mask([0, 2], 0, 8))
+    m(8, _mask([0, 2], 8, 8))
+    late = _mask([0, 2], 16, 8)
+    late[0, 0, 7, 9] = False
+    with pytest.raises(ValueError, match="mask"):
+        m(8, [_mask([0, 2], 16, 8), late])
