@@ -14,7 +14,8 @@ read once from the prefill attention mask.  Head dimension 128 only.
 
 StateTreeKVCache(..., eight_bit=True) keeps 8-bit pages instead (kvcache.PageStore8; head dimension 64 or 128): then every chunk of a
 prompt attends to the pages too, causally and from each sequence's first valid position on, and nothing is expanded.  The padding may
-be longer than the first chunk; other masks (packed sequences, right padding) are refused.
+be longer than the first chunk; masks and modules that ask for anything else (packed sequences, right padding, softcaps, sinks,
+dropout) are refused.
 """
 import threading
 import weakref
@@ -224,7 +225,7 @@ class StateTreeKVCache(Cache):
 
 def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, scaling=None, **kwargs):
     """the 'statetree' attention implementation: a decode step reads the compressed pages, anything else runs SDPA (over 8-bit pages:
-    chunk attention over the pages, and ValueError for masks that it does not know)"""
+    chunk attention over the pages, and ValueError for what that does not compute)"""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     layer = getattr(_LAST, "layer", None)
     _LAST.layer = None
@@ -232,6 +233,8 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
         c = layer.cache
         B, Hq, T, D = query.shape
         window = kwargs.get("sliding_window") or 0
+        if c.eight_bit:
+            _refuse_other_attention(dropout, kwargs)
         if T == 1 and layer.host_len > 1:
             q = query[:, :, 0, :]
             if q.stride(-1) != 1 or q.stride(1) != D:
@@ -244,6 +247,8 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
         if c.eight_bit:                              # a chunk (its keys are in the pages already), or the first token of all
             if attention_mask is not None:
                 c.read_mask(attention_mask, layer.host_len, B, T, window)
+            elif T > 1 and not _causal(module, kwargs):
+                raise ValueError("StateTreeKVCache: attention over 8-bit pages is causal")
             q = query.transpose(1, 2).reshape(B * T, Hq, D)
             cu = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=q.device)
             out = layer.store.chunk_attention(q, cu, c.table32[:B], c.lens[:B], float(scaling) if scaling is not None else D ** -0.5,
@@ -255,6 +260,17 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
             c.starts[:B].copy_(masked.sum(-1).to(torch.int32))
             c.starts_known = True
     return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout, scaling=scaling, **kwargs)
+
+
+def _causal(module, kwargs):
+    given = kwargs.get("is_causal")
+    return getattr(module, "is_causal", True) if given is None else given
+
+
+def _refuse_other_attention(dropout, kwargs):
+    for name, given in (("dropout", dropout > 0), ("softcap", kwargs.get("softcap") is not None), ("s_aux", kwargs.get("s_aux") is not None)):
+        if given:
+            raise ValueError(f"StateTreeKVCache: attention over 8-bit pages has no {name}")
 
 
 def enable(model):

@@ -171,3 +171,23 @@ def test_more_masks_are_refused():
     late[0, 0, 7, 9] = False
     with pytest.raises(ValueError, match="mask"):
         m(8, [_mask([0, 2], 16, 8), late])
+
+
+@pytest.mark.parametrize("T", [4, 1])
+@pytest.mark.parametrize("kw", [dict(softcap=30.0), dict(s_aux=torch.zeros(4)), dict(dropout=0.1)])
+def test_attention_of_another_kind_is_refused(T, kw):
+    m = _Model(1)
+    m(3, None)
+    with pytest.raises(ValueError, match=next(iter(kw))):
+        m(T, None, **kw)
+    _Model(1)(4, None, softcap=None, s_aux=None, dropout=0.0)
+
+
+def test_attention_that_is_not_causal_is_refused():
+    for ways in (dict(is_causal=False), dict(module=dict(is_causal=False)), dict(module=dict(is_causal=False), is_causal=None)):
+        with pytest.raises(ValueError, match="causal"):
+            _Model(1)(4, None, **ways)
+        _Model(1)(4, _mask([0], 0, 4), **ways)             # (the mask says what is seen)
+        m = _Model(1)
+        m(4, None)
+        m(1, None, **ways)                                 # one token sees everything either way
