@@ -10,12 +10,11 @@ statetree/kvcache.py (StateTreeKVLayer 35-129, StateTreeKVCache 132-177, statetr
 
 Positions come from a GPU-side token count (or from `cache_position` when the model passes it), buffers are static,
 so decode steps can be captured in CUDA graphs.  Left padding is supported: each sequence's first valid position is
-read once from the prefill attention mask.  Head dimension 128 only.
+read from the attention masks of the prompt.  Head dimension 128 only.
 
 StateTreeKVCache(..., eight_bit=True) keeps 8-bit pages instead (kvcache.PageStore8; head dimension 64 or 128): then every chunk of a
-prompt attends to the pages too, causally and from each sequence's first valid position on, and nothing is expanded.  The padding may
-be longer than the first chunk; masks and modules that ask for anything else (packed sequences, right padding, softcaps, sinks,
-dropout) are refused.
+prompt attends to the pages too, causally and from each sequence's first valid position on, and nothing is expanded.  Masks and
+modules that ask for anything else (packed sequences, right padding, softcaps, sinks, dropout) are refused.
 """
 import threading
 import weakref
@@ -150,7 +149,7 @@ class StateTreeKVCache(Cache):
         self.max_pages = -(-self.max_len // PAGE)
         self.alloc_batch, self.pool_blocks, self.eight_bit = batch_size, pool_blocks, eight_bit
         self.starts_known = False
-        self.starts_at, self.masks = 0, []           # 8-bit pages: the pass whose masks have been read, and which have been checked
+        self.starts_at, self.masks = 0, []           # the pass whose mask has been read; 8-bit pages: its masks that have been checked
         self._allocated = False
         super().__init__(layers=[StateTreeKVLayer(self, i) for i in range(self.num_layers)])
 
@@ -254,10 +253,13 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
             out = layer.store.chunk_attention(q, cu, c.table32[:B], c.lens[:B], float(scaling) if scaling is not None else D ** -0.5,
                                               starts=c.starts[:B], window=window)
             return out.view(B, T, Hq, D), None
-        if T > 1 and not c.starts_known and attention_mask is not None and attention_mask.dim() == 4:
+        if T > 1 and attention_mask is not None and attention_mask.dim() == 4 and c.starts_at != layer.host_len:
+            c.starts_at = layer.host_len                            # the first layer of the pass
             last_row = attention_mask[:, 0, -1, :]                  # the last query sees everything but the padding
-            masked = ~last_row if last_row.dtype == torch.bool else last_row < 0
-            c.starts[:B].copy_(masked.sum(-1).to(torch.int32))
+            masked = (~last_row if last_row.dtype == torch.bool else last_row < 0).sum(-1).to(torch.int32)
+            if c.starts_known:                                      # (padding may go on behind an earlier chunk that was nothing else)
+                masked = torch.where(c.starts[:B] >= layer.host_len - T, masked, c.starts[:B])
+            c.starts[:B].copy_(masked)
             c.starts_known = True
     return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout, scaling=scaling, **kwargs)
 

@@ -1,5 +1,5 @@
-"""The 8-bit Hugging Face cache on the CPU with a store that only takes notes: which masks its attention reads as left padding, and
-which masks and modules it refuses."""
+"""The Hugging Face cache on the CPU with a store that only takes notes: which masks its attention reads as left padding, and
+which masks and modules it refuses over 8-bit pages."""
 import types
 
 import pytest
@@ -27,6 +27,9 @@ class _Notes:
     def append(self, K, V, slots):
         pass
 
+    def dense(self):
+        return torch.zeros(2, 2 * 16, 16, 2, 128, dtype=torch.bfloat16)
+
     def reset(self):
         pass
 
@@ -43,14 +46,14 @@ class _Model:
         """a forward pass over T tokens; a mask and a window for all layers, or a list of them"""
         from statetree_b200.kvcache import statetree_attention
         of = lambda x, i: x[i] if isinstance(x, list) else x                                  # noqa: E731
-        q, k = torch.zeros(self.B, 4, T, 128, dtype=torch.bfloat16), torch.zeros(self.B, 2, T, 128, dtype=torch.bfloat16)
+        q, k = (torch.zeros(self.B, h, T, 128, dtype=torch.bfloat16) for h in (4 if self.cache.eight_bit else 2, 2))
         for i, layer in enumerate(self.cache.layers):
             if not layer.is_initialized:
                 layer.lazy_initialization(k, k)
                 layer.store = self.notes
-            layer.update(k, k)
-            statetree_attention(types.SimpleNamespace(layer_idx=i, **{"is_causal": True, **(module or {})}), q, k, k, of(mask, i), scaling=0.1,
-                                sliding_window=of(windows, i), **kw)
+            keys, values = layer.update(k, k)
+            attends = types.SimpleNamespace(layer_idx=i, **{"is_causal": True, **(module or {})})
+            statetree_attention(attends, q, keys, values, of(mask, i), scaling=0.1, sliding_window=of(windows, i), **kw)
 
     @property
     def starts(self):
@@ -91,6 +94,18 @@ def test_layers_with_and_without_a_window(windows):
     for at, T in ((0, 16), (16, 16), (32, 4)):
         m(T, [_mask([0, 21], at, T, w or 0) for w in windows], windows)
         assert m.starts == [0, min(21, at + T)]
+
+
+@pytest.mark.parametrize("kind", ["bool", "inf"])
+@pytest.mark.parametrize("pads", [[0, 3], [0, 20], [16, 33], [40, 1]])
+def test_left_padding_of_the_lossless_cache(pads, kind):
+    """decode steps begin behind the padding there too"""
+    m, at = _Model(2, eight_bit=False), 0
+    for T in (16, 16, 16, 1, 7, 1):
+        m(T, _mask(pads, at, T, 0, kind))
+        at += T
+        assert m.cache.starts.tolist() == [min(p, at) for p in pads]
+    assert m.notes.calls == [("step", pads, 0)] * 4
 
 
 @pytest.mark.parametrize("kind", ["bool", "lowest"])
