@@ -181,3 +181,99 @@ def test_hf_cache_masks_in_a_captured_pass():
     cache.check()
     with pytest.raises(ValueError, match="mask"):
         step()
+
+
+# ------------------------------------------------------------------------------------------------ precision
+def _close(q, seqs, cu, lens, scale, got):
+    """the kernels' own bound, per value: probabilities rounded to FP16 (2^-11 of each at most, or, where that is subnormal, 2^-32 of the
+    largest times its page's largest value, at most twice the largest of all values), the output rounded to BF16 (2^-8), scores summed
+    in fp32 over D products (each sum off by at most D 2^-24 of its absolute sum, twice since the reference is subtracted; the factors
+    and the difference four roundings more), sums over the keys (2^-24 each), the exponential (2^-21 with its argument's rounding)"""
+    got = got.cpu().double()
+    for b, (K, V) in enumerate(seqs):
+        n, L, D = cu[b + 1] - cu[b], lens[b], q.shape[-1]
+        out, mag, wide = R.attend(q[cu[b]:cu[b + 1]].cpu().double(), K, V, list(range(L - n, L)), scale)
+        rel = 2.0 ** -11 + 2 * (D + 4) * 2.0 ** -24 * wide[..., None] + L * 2.0 ** -24 + 2.0 ** -21
+        near = mag * rel * 1.01 + L * 2.0 ** -31 * float(V.abs().max())
+        off = (got[cu[b]:cu[b + 1]] - out).abs()
+        assert bool((off <= near + 2.0 ** -8 * (out.abs() + near)).all()), (b, float((off / (near + 2.0 ** -8 * out.abs())).max()))
+
+
+def _opposed(gen, n, H, D, spread):
+    """keys of which two share the weight almost evenly, their values opposed, the others far below: the output is a difference of two
+    probabilities, in which a rounding of either shows"""
+    K, V = torch.zeros(n, H, D), torch.zeros(n, H, D)
+    K[:, :, 0] = -24.0
+    K[:2, :, 0] = 0.0
+    K[:2, :, 1:9] = torch.randn(2, H, 8, generator=gen) * spread
+    V[0], V[1] = 1.0, -1.0
+    V[2:] = torch.randn(n - 2, H, D, generator=gen)
+    return K, V
+
+
+@pytest.mark.parametrize("D,H,G", [(128, 2, 4), (64, 1, 7)])
+@pytest.mark.parametrize("spread", [0.02, 0.2])
+def test_probabilities_have_eleven_bits(D, H, G, spread):
+    gen = _gen(D)
+    n, new = 150, 70
+    store, table, _ = _filled(gen, [n], H, D)
+    K, V = _opposed(gen, n, H, D, spread)
+    p = torch.arange(n)
+    store.append(K.to(torch.bfloat16).to(DEV), V.to(torch.bfloat16).to(DEV), (table[0].cpu()[p // 16] * 16 + p % 16).to(DEV))
+    seqs = [tuple(t.cpu().double().flatten(0, 1)[:n] for t in store.dense(table[0, :-(-n // 16)].contiguous()))]
+    q = torch.randn(new, H * G, D, generator=gen)
+    q[:, :, 0] = 1.0
+    q = q.to(torch.bfloat16).to(DEV)
+    for rows, splits in ((1, 1), (1, 3), (4, 1), (4, 2), (new, 1), (new, 2)):
+        got = store.chunk_attention(q[:rows], _ints([0, rows]), table, _ints([n]), 1.0, splits=splits)
+        _close(q[:rows], seqs, [0, rows], [n], 1.0, got)
+    _close(q[:1], seqs, [0, 1], [n], 1.0, store.attention(q[:1], table, _ints([n]), 1.0, splits=2, min_pages=1))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("splits", [1, 3, 11])
+def test_precision_of_random_scores(D, splits):
+    gen = _gen(splits)
+    lens, cu = [300, 33, 700], [0, 60, 63, 200]
+    store, table, seqs = _filled(gen, lens, 2, D)
+    q = _rand(gen, 200, 8, D, size=1.5).to(DEV)
+    _close(q, seqs, cu, lens, D ** -0.5, store.chunk_attention(q, _ints(cu), table, _ints(lens), D ** -0.5, splits=splits))
+    got = store.attention(q[:3], table, _ints(lens), D ** -0.5, splits=splits, min_pages=1)
+    _close(q[:3], seqs, [0, 1, 2, 3], lens, D ** -0.5, got)
+    few = [0, 4, 5, 9]
+    got = store.chunk_attention(q[:9], _ints(few), table, _ints(lens), D ** -0.5, splits=splits)
+    _close(q[:9], seqs, few, lens, D ** -0.5, got)
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_both_host_paths_refuse_the_same(monkeypatch):
+    """what a call of wrong form is told does not depend on the native host path"""
+    from statetree_b200 import kvcache
+    store = kvcache.PageStore8(4, 2, DEV)
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=DEV)                         # noqa: E731
+    f32 = lambda *s: torch.zeros(*s, device=DEV)                                              # noqa: E731
+    K, slots = bf(3, 2, 128), torch.zeros(3, dtype=torch.int64, device=DEV)
+    table, lens, q = torch.zeros(3, 4, dtype=torch.int32, device=DEV), _ints([0, 0, 0]), bf(3, 4, 128)
+    calls = [(store.append, dict(K=K, V=K, slots=slots), bad) for bad in (
+        dict(K=bf(3, 2, 64)), dict(K=bf(3, 1, 128), V=bf(3, 1, 128)), dict(V=bf(2, 2, 128)), dict(K=f32(3, 2, 128)), dict(slots=slots[:2]),
+        dict(slots=slots.int()), dict(slots=slots.cpu()), dict(V=K.cpu()), dict(cos=f32(9, 64)), dict(cos=f32(9, 64), sin=f32(9, 64)),
+        dict(cos=f32(9, 32), sin=f32(9, 32), positions=slots), dict(cos=f32(9, 64), sin=f32(9, 64), positions=slots[:2]),
+        dict(k_norm=bf(64)), dict(q=bf(2, 4, 128)), dict(q=q, q_out=bf(3, 5, 128)), dict(q=q, q_out=bf(3, 1, 128).expand(3, 4, 128)))]
+    one = dict(q=q, block_table=table, lens=lens, scale=0.1)
+    calls += [(store.attention, one, bad) for bad in (
+        dict(q=bf(3, 3, 128)), dict(q=bf(2, 4, 128)), dict(lens=lens.long()), dict(lens=lens[:2]), dict(block_table=table.long()),
+        dict(block_table=table[:, :0]), dict(block_table=table.repeat(1, 2)[:, ::2]), dict(starts=lens[:1]), dict(window=-1), dict(splits=0),
+        dict(out=bf(3, 2, 128)), dict(q=q.float()), dict(scale=0.0), dict(scale=float("nan")), dict(splits=2000), dict(lens=lens.cpu()))]
+    calls += [(store.chunk_attention, dict(one, cu=_ints([0, 1, 2, 3])), bad) for bad in (
+        dict(cu=lens), dict(cu=_ints([0, 1, 2, 3]).long()), dict(cu=None, q=bf(5, 4, 128)), dict(splits=0), dict(window=-1))]
+    said = []
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(kvcache, "calls", lambda: None)
+        said.append([])
+        for call, good, bad in calls:
+            with pytest.raises(RuntimeError) as e:
+                call(**{**good, **bad})
+            said[-1].append(str(e.value))
+    assert said[0] == said[1]
+    torch.cuda.synchronize()
