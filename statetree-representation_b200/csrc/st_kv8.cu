@@ -1,5 +1,6 @@
 // KV pages in 8 bits on sm_100a: append (rotation and quantisation on the way), read-back, and attention over the pages.
 // The page and why it is laid out so: st_kv8.cuh.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -575,7 +576,8 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
     qs1 = pow2i(__shfl_sync(FULL, e, 8 * t + 4));
   }
   const bool head0 = 2 * t < heads, head1 = 2 * t + 1 < heads;
-  float m0 = head0 ? -INFINITY : 1e30f, m1 = head1 ? -INFINITY : 1e30f, l0 = 0.f, l1 = 0.f;     // (no head: probabilities are 0)
+  // (a reference is finite from the start: what is hidden, or below fp32, then is 0 and not -inf - -inf; no head: probabilities are 0)
+  float m0 = head0 ? -FLT_MAX : 1e30f, m1 = head1 ? -FLT_MAX : 1e30f, l0 = 0.f, l1 = 0.f;
   float acc[VT][4];                                               // MMA j: [0], [1] dim D/8 g + 2j, [2], [3] the next; heads 2t, 2t + 1
 #pragma unroll
   for (int j = 0; j < VT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
@@ -633,9 +635,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
       m0 = n0;
       m1 = n1;
     }
-    // (a chunk's column may see nothing of a page, and of any: its reference is then still -inf)
-    const float r0 = CHUNK && m0 == -INFINITY ? 0.f : m0, r1 = CHUNK && m1 == -INFINITY ? 0.f : m1;
-    const float p00 = ex2(x00 - r0), p01 = ex2(x01 - r1), p10 = ex2(x10 - r0), p11 = ex2(x11 - r1), out = ex2(-f.y);
+    const float p00 = ex2(x00 - m0), p01 = ex2(x01 - m1), p10 = ex2(x10 - m0), p11 = ex2(x11 - m1), out = ex2(-f.y);
     l0 = fmaf(p00 + p10, out, l0);
     l1 = fmaf(p01 + p11, out, l1);
     const uint32_t b0 = movmatrix_t(pack_f16(p00, p01)), b1 = movmatrix_t(pack_f16(p10, p11));
@@ -670,9 +670,11 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
       phase ^= 1u;
     }
   }
-  if (gave_up) { m0 = head0 ? -INFINITY : 0.f; m1 = head1 ? -INFINITY : 0.f; l0 = l1 = 0.f; }
+  if (gave_up) { m0 = m1 = -FLT_MAX; l0 = l1 = 0.f; }
   l0 = over_rows_sum(l0);
   l1 = over_rows_sum(l1);
+  if (m0 == -FLT_MAX && l0 == 0.f) m0 = -INFINITY;                // nothing seen (a sum that is not a number stays one)
+  if (m1 == -FLT_MAX && l1 == 0.f) m1 = -INFINITY;
 
   // ---- the CTA's warps together.  The rings are idle now; each warp parks (O^T, r, l) of its heads there.
   __syncthreads();
@@ -702,7 +704,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) kv8_attn_kernel(const Attn8 
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float* const pw = park + w * PER_WARP + h * ROW;
-      if (pw[D] == -INFINITY) continue;                           // a warp without pages
+      if (pw[D] == -INFINITY) continue;                           // a warp that saw nothing
       const float f = ex2(pw[D] - top);
       den += f * pw[D + 1];
       num += f * pw[d];

@@ -277,3 +277,47 @@ def test_both_host_paths_refuse_the_same(monkeypatch):
             said[-1].append(str(e.value))
     assert said[0] == said[1]
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------ scores beyond fp32
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("splits", [1, 2, 3])
+def test_scores_below_fp32(D, splits):
+    """finite queries and keys whose product no fp32 number holds, far below all others: those keys weigh nothing, wherever they stand"""
+    gen = _gen(D)
+    n, H = 200, 1
+    store, table, _ = _filled(gen, [n], H, D)
+    for lows in ([0], [0, 1, 2], [3], [2, 12], list(range(12))):                             # pages of such keys
+        K, V = torch.zeros(n, H, D), _rand(gen, n, H, D)
+        for p in lows:
+            K[p * 16:(p + 1) * 16] = -1e3
+        at = torch.arange(n)
+        slots = table[0].cpu()[at // 16] * 16 + at % 16
+        store.append(K.to(torch.bfloat16).to(DEV), V.to(DEV), slots.to(DEV))
+        seqs = [tuple(t.cpu().double().flatten(0, 1)[:n] for t in store.dense(table[0, :-(-n // 16)].contiguous()))]
+        q = torch.full((80, 4, D), 3e38, dtype=torch.bfloat16, device=DEV)
+        _check(store.attention(q[:1], table, _ints([n]), 0.1, splits=splits, min_pages=1), q[:1], seqs, [0, 1], [n], 0.1)
+        for rows in (1, 3, 80):
+            # (rows all of whose keys are such: no answer in fp32)
+            rows = min(rows, n - 16 * (max(lows) + 1) + 16) if len(lows) < 12 else 1
+            got = store.chunk_attention(q[:rows], _ints([0, rows]), table, _ints([n]), 0.1, splits=splits)
+            _check(got, q[:rows], seqs, [0, rows], [n], 0.1)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("splits", [1, 3, 12])
+def test_queries_that_are_no_numbers(splits, bad):
+    """give outputs that are none, and leave every other row and head as it is"""
+    gen = _gen(splits)
+    lens, H = [300, 70, 0], 2
+    store, table, _ = _filled(gen, lens, H, 128)
+    for cu in (None, [0, 5, 8, 8], [0, 200, 270, 270]):
+        q = _rand(gen, cu[-1] if cu else 3, 8, 128).to(DEV)
+        call = lambda q: (store.attention(q, table, _ints(lens), 0.1, splits=splits, min_pages=1) if cu is None else      # noqa: E731
+                          store.chunk_attention(q, _ints(cu), table, _ints(lens), 0.1, splits=splits))
+        want = call(q)
+        q[1, 5, 17] = bad
+        got = call(q)
+        assert bool(got[1, 5].isnan().all())
+        got[1, 5] = want[1, 5]
+        assert torch.equal(got, want)
