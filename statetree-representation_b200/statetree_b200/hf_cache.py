@@ -69,6 +69,8 @@ class StateTreeKVLayer(CacheLayerMixin):
         B, H, T, D = key_states.shape
         where = opts.get("cache_position") if isinstance(opts, dict) else None
         if where is None:
+            if self.host_len + T > c.max_pages * PAGE:      # (beyond it the page lookup would leave the table)
+                raise ValueError(f"StateTreeKVCache: {T} tokens behind {self.host_len} exceed the capacity of {c.max_pages * PAGE}")
             where = self.gpu_len + torch.arange(T, device=self.device)
         self.gpu_len.copy_(where[-1] + 1)
         slots = (c.table64[:B].index_select(1, where // PAGE) * PAGE + where % PAGE).reshape(-1)

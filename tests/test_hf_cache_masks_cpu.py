@@ -206,3 +206,16 @@ def test_attention_that_is_not_causal_is_refused():
         m = _Model(1)
         m(4, None)
         m(1, None, **ways)                                 # one token sees everything either way
+
+
+@pytest.mark.parametrize("eight_bit", [True, False])
+def test_tokens_beyond_the_capacity_are_refused(eight_bit):
+    m = _Model(2, eight_bit=eight_bit)
+    m(250, None)
+    m(6, _mask([0, 0], 250, 6))
+    for T in (1, 3):
+        with pytest.raises(ValueError, match="capacity"):
+            m(T, None)
+    m.cache.reset()
+    with pytest.raises(ValueError, match="capacity"):
+        m(257, None)
