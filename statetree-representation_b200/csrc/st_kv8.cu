@@ -434,8 +434,8 @@ __global__ void __launch_bounds__(256) kv8_dequant_kernel(const uint8_t* __restr
 // own through a private ring of bulk copies (a page of one head is contiguous, 2 * 16 * D bytes), so there is no barrier in the loop.
 // Block-table entries and exponents come 32 pages at a time, one batch ahead.  The splits of a unit join through distributed shared memory,
 // as a cluster, or through memory in a second kernel (joins8).
-// Measured (32 query heads, 8 KV heads, D = 128, in a graph): 64 sequences of up to 8192 tokens 90 us = 5.9 TB/s, one of 61003 23.6 us, one
-// of 1000 5.4 us.
+// Measured (32 query heads, 8 KV heads, D = 128, in a graph): 64 sequences of up to 8192 tokens 90 us = 5.9 TB/s, one of 61003 23.0 us, one
+// of 1000 5.0-5.4 us.
 __device__ __forceinline__ float over_rows_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
   v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));

@@ -140,7 +140,8 @@ int attn8_args(Attn8& a, const char* who, const void* q, int64_t qs, int64_t T, 
                const int32_t* starts, int64_t window, void* out, int64_t os, double scale);
 // Chunks of few rows per sequence go through the decode kernel, eight rows a CTA: its time grows with every eight rows, the chunk kernel's
 // hardly up to 128.  32 sequences of 2000 tokens, D = 128, us: 16 rows 38 in the decode kernel and 103 in the other, 32 rows 63 and 74, 64
-// rows 119 and 75.  D = 64: 28 rows 15 and 30, 56 rows 27 and 30, 112 rows 46 and 31.  (chunk_splits8 in kvcache.py states the same bound.)
+// rows 119 and 75.  D = 64: 28 rows 15 and 30, 56 rows 27 and 30, 112 rows 46 and 31.  By the mean over the sequences, which is what the host
+// knows: a batch of decode tokens with one long chunk is faster as two calls.  (chunk_splits8 in kvcache.py states the same bound.)
 constexpr int FEW_ROWS = 32;
 inline bool few_rows8(long long T, long long B, long long G) { return T * G <= FEW_ROWS * B; }
 int rows8_attn(const char* who, const Attn8& a, const Parts8& parts, int D, cudaStream_t stream);

@@ -5,7 +5,8 @@
 //     S = Q K^T   128 x 128, A and B from shared memory            P = exp2(S * c - m) in FP16, back into S's tensor-memory columns
 //     O += P V    128 x D, A = P from tensor memory, B = V from shared memory as it lies (dims contiguous: MN-major)
 // Warps: eight of softmax (a thread owns one row, so its maximum and sum need no other thread), four that bring pages into shared memory
-// by bulk copies and turn their codes into FP16 operand tiles, one that issues the MMAs.  While one tile's softmax runs, the tensor core works on the other's: S0 P0 S1 P1 ... in turn.
+// by bulk copies and turn their codes into FP16 operand tiles, one that issues the MMAs.  While one tile's softmax
+// runs, the tensor core works on the other's: S0 P0 S1 P1 ... in turn.
 // Tensor memory: S0, S1 (128 columns each; P takes the first 64 of its own), O0, O1 (D each).
 //
 // Types and scales as in the decode kernel: e4m3 codes are FP16 numbers (one instruction converts two; as BF16 patterns the integer
@@ -14,7 +15,7 @@
 // columns of P and is taken out of the sum per page.  P is rounded to FP16 (2^-11 of each at most, and 2^-32 of the largest), everything
 // else but the output is fp32.
 //
-// Measured (32 query heads, 8 KV heads, D = 128): 2048 queries behind 30000 tokens 1.02 ms = 1.0 PFLOP/s, a prompt of 4096 tokens 172 us.
+// Measured (32 query heads, 8 KV heads, D = 128): 2048 queries behind 30000 tokens 1.00-1.05 ms = 1.0 PFLOP/s, a prompt of 4096 tokens 172 us.
 // A key tile takes 2.3 us for the 256 rows: a row tile's softmax about 2300 cycles, its MMAs and the hand-overs 1200, of which the other
 // row tile's overlap most; the MMAs by themselves 2270 cycles for both.  Shared memory is busy 2560 of its cycles (operands 192 KB,
 // conversion 128 KB).  A CTA costs about 8 us besides (look-ups, q, first pages, output).
@@ -37,7 +38,7 @@ constexpr int CRING = 4;                                          // page factor
 
 template <int D>
 struct Lay {                                                      // shared memory
-  static constexpr int HALF = 128 * 128;                          // 128 rows x 64 BF16, 128-byte swizzle
+  static constexpr int HALF = 128 * 128;                          // 128 rows x 64 FP16, 128-byte swizzle
   static constexpr int TILE = D / 64 * HALF;
   static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE;         // two tiles of Q, two stages of K and V
   static constexpr int RAW = 6 * TILE, UNIT = PAGE * D;           // codes of one key tile: its keys, its values
