@@ -272,7 +272,7 @@ def _causal(module, kwargs):
 
 
 def _refuse_other_attention(dropout, kwargs):
-    for name, given in (("dropout", dropout > 0), ("softcap", kwargs.get("softcap") is not None), ("s_aux", kwargs.get("s_aux") is not None)):
+    for name, given in (("dropout", dropout), ("softcap", kwargs.get("softcap")), ("s_aux", kwargs.get("s_aux") is not None)):
         if given:
             raise ValueError(f"StateTreeKVCache: attention over 8-bit pages has no {name}")
 

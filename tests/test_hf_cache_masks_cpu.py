@@ -195,7 +195,8 @@ def test_attention_of_another_kind_is_refused(T, kw):
     m(3, None)
     with pytest.raises(ValueError, match=next(iter(kw))):
         m(T, None, **kw)
-    _Model(1)(4, None, softcap=None, s_aux=None, dropout=0.0)
+    for off in (dict(softcap=None, s_aux=None, dropout=0.0), dict(softcap=0.0, dropout=None)):
+        _Model(1)(4, None, **off)
 
 
 def test_attention_that_is_not_causal_is_refused():
