@@ -14,7 +14,8 @@ read from the attention masks of the prompt.  Head dimension 128 only.
 
 StateTreeKVCache(..., eight_bit=True) keeps 8-bit pages instead (kvcache.PageStore8; head dimension 64 or 128): then every chunk of a
 prompt attends to the pages too, causally and from each sequence's first valid position on, and nothing is expanded.  Masks and
-modules that ask for anything else (packed sequences, right padding, softcaps, sinks, dropout) are refused.
+modules that ask for anything else (packed sequences, right padding, softcaps, sinks, dropout) are refused: reset() the
+cache then, since the keys of the refused pass have been appended.  Decode steps read no mask, in either cache.
 """
 import threading
 import weakref
