@@ -300,6 +300,18 @@ int st_rope_kv_append(const void* qkv, int64_t row_stride, const void* wq, const
                       int64_t hkv, double eps, const int64_t* slot, void* kv, int64_t nblocks, uint32_t* pool, int64_t P,
                       int32_t* pool_cnt, void* stream);
 
+/* Rotary positions of N tokens' queries [N, Hq, D] and keys [N, Hk, D] (either may have no heads): the pairs of the values offset ..
+ * offset + part - 1 of every head, (2i, 2i + 1) of them (interleaved) or (i, i + part / 2), become (a c - b s, a s + b c) with the float32
+ * cos / sin [span, part / 2] of the token's position positions[i * positions_step] (clamped to the table; positions_step 0: one for
+ * all); inverse: s of the other sign, which is also the gradient.  The other values of a head pass through.  With wq / wk (of the
+ * values' type, [D], or NULL) heads are RMS-normalised before.  type: 0 BF16, 1 FP16, 2 float32; fp32 arithmetic, one rounding.  Strides
+ * in values, of a token and of a head (a head's values are contiguous); an output may be its input.  No counterpart in the reference
+ * (its models' own modules rotate). */
+int st_rotate(const void* q, int64_t q_token, int64_t q_head, int64_t Hq, const void* k, int64_t k_token, int64_t k_head, int64_t Hk,
+              int64_t N, int64_t D, int type, const int64_t* positions, int positions_step, const float* cos_t, const float* sin_t,
+              int64_t span, int64_t part, int64_t offset, int interleaved, int inverse, const void* wq, const void* wk, double eps,
+              void* q_out, int64_t qo_token, int64_t qo_head, void* k_out, int64_t ko_token, int64_t ko_head, void* stream);
+
 /* ---- tensor-parallel exchange over NVLink peer memory -------------------------------------------------------------- *
  * No counterpart in the reference: it has no communication code (under vLLM each rank runs the reference's kernels on
  * its shard and vLLM all-reduces the outputs of the row-parallel o / down projections with NCCL).  These entry points

@@ -1,5 +1,5 @@
 // The host path of a module call in native code: TreeLinear products and lists of them (q / k / v, gate / up) for inputs that need
-// no conversion, the launches of a matrix's conversion and its check, and the calls of the 8-bit KV pages.  What Python does for such a product (checks, the output
+// no conversion, the launches of a matrix's conversion and its check, the calls of the 8-bit KV pages and the rotation.  What Python does for such a product (checks, the output
 // and its views, pointer arrays, the ctypes call) takes 15 to 30 us, several times a small product's time on the GPU; this takes
 // 3 to 5.
 //
@@ -43,6 +43,7 @@ struct Library {
   decltype(&st_kv8_attn_table) kv8_attn;
   decltype(&st_kv8_chunk_attn_table) kv8_chunk;
   decltype(&st_kv8_attn_workspace_bytes) kv8_workspace;
+  decltype(&st_rotate) rotate;
 };
 
 // rows of x if it can be read as it is: BF16 [..., N] on `device`, contiguous, 16-byte aligned, at least one row; else 0
@@ -89,6 +90,7 @@ Library library(const std::map<std::string, uint64_t>& address) {
   bind(lib.kv8_attn, "st_kv8_attn_table");
   bind(lib.kv8_chunk, "st_kv8_chunk_attn_table");
   bind(lib.kv8_workspace, "st_kv8_attn_workspace_bytes");
+  bind(lib.rotate, "st_rotate");
   return lib;
 }
 
@@ -355,6 +357,40 @@ py::object kv8_dense(const Library& lib, const at::Tensor& pages, const at::Tens
   check(lib, rc);
   return py::make_tuple(K, V);
 }
+
+// ---- rotary positions: q [N, Hq, D] and k [N, Hk, D] (or None) into new tensors; (q, k) or None
+py::object rotate(const Library& lib, const at::Tensor& q, const Maybe& k, const at::Tensor& positions, const at::Tensor& cos,
+                  const at::Tensor& sin, bool interleaved, int64_t offset, bool inverse, const Maybe& wq, const Maybe& wk, double eps) {
+  if (!q.is_cuda() || q.dim() != 3) return py::none();
+  const at::Device device = q.device();
+  const auto type = q.scalar_type();
+  const int code = type == at::kBFloat16 ? 0 : type == at::kHalf ? 1 : type == at::kFloat ? 2 : -1;
+  const int64_t N = q.size(0), D = q.size(2);
+  auto rows = [&](const at::Tensor& t) {
+    return t.dim() == 3 && t.scalar_type() == type && t.device() == device && t.layout() == at::kStrided && t.size(0) == N && t.size(2) == D &&
+           t.numel() > 0 && t.stride(2) == 1 && !t.is_conj() && !t.is_neg();
+  };
+  auto norm = [&](const Maybe& w) { return !w || (flat(*w, type, device) && w->dim() == 1 && w->numel() == D); };
+  if (code < 0 || !rows(q) || (k && !rows(*k)) || !norm(wq) || !norm(wk) || !flat(positions, at::kLong, device) ||
+      (positions.numel() != N && positions.numel() != 1) || !flat(cos, at::kFloat, device) || !flat(sin, at::kFloat, device) || cos.dim() != 2 ||
+      sin.sizes() != cos.sizes() || cos.size(0) < 1 || offset < 0 || offset + 2 * cos.size(1) > D)
+    return py::none();
+  at::Tensor yq, yk;
+  int rc;
+  {
+    py::gil_scoped_release nogil;
+    const c10::cuda::CUDAGuard guard(device);
+    yq = at::empty(q.sizes(), q.options().requires_grad(false));
+    if (k) yk = at::empty(k->sizes(), yq.options());
+    rc = lib.rotate(q.const_data_ptr(), q.stride(0), q.stride(1), q.size(1), of<void>(k), k ? k->stride(0) : 0, k ? k->stride(1) : 0,
+                    k ? k->size(1) : 0, N, D, code, of<int64_t>(positions), positions.numel() > 1, of<float>(cos), of<float>(sin),
+                    cos.size(0), 2 * cos.size(1), offset, interleaved, inverse, of<void>(wq), of<void>(wk), eps, yq.data_ptr(), yq.stride(0),
+                    yq.stride(1), k ? yk.data_ptr() : nullptr, k ? yk.stride(0) : 0, k ? yk.stride(1) : 0,
+                    c10::cuda::getCurrentCUDAStream(device.index()).stream());
+  }
+  check(lib, rc);
+  return k ? py::object(py::make_tuple(yq, yk)) : py::cast(yq);
+}
 }  // namespace
 
 PYBIND11_MODULE(_calls, m) {
@@ -369,4 +405,5 @@ PYBIND11_MODULE(_calls, m) {
   m.def("kv8_append", &kv8_append);
   m.def("kv8_attention", &kv8_attention);
   m.def("kv8_dense", &kv8_dense);
+  m.def("rotate", &rotate);
 }

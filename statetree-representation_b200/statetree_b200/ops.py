@@ -76,6 +76,8 @@ _SIGNATURES = {
     "st_gemv_swiglu": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "st_rope_kv_append": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _dbl, _vp, _vp, _i64,
                                  _vp, _i64, _vp, _vp]),
+    "st_rotate": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _i64, _i64, _i64, _int, _int,
+                         _vp, _vp, _dbl, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
     "st_moe_align": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
     "st_moe_tensor_map_bytes": (_i64, []),
     "st_moe_tensor_maps": (_int, [_vp, _i64, _i64, _i64, _vp, _vp]),
@@ -128,7 +130,7 @@ CALLS_PATH = os.path.join(_HERE, "_calls.so")
 _CALLS = None                                           # False: there is none
 _NATIVE = ("st_gemv", "st_gemm", "st_gemv_list", "st_gemm_list", "st_last_error", "st_encode", "st_encode_lists", "st_encode_offsets",
            "st_encode_offsets_workspace_bytes", "st_dec_check", "st_lists_check", "st_kv8_append", "st_kv8_dequant_blocks", "st_kv8_attn_table",
-           "st_kv8_chunk_attn_table", "st_kv8_attn_workspace_bytes")
+           "st_kv8_chunk_attn_table", "st_kv8_attn_workspace_bytes", "st_rotate")
 
 
 def calls():
@@ -481,6 +483,76 @@ class _Weights:
         S, I2 = gu.shape
         with _ctx(gu):
             _check(lib().st_silu_mul(_ptr(gu), _ptr(act), S, I2 // 2, _stream(gu)))
+
+
+    ROTATED = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+    @staticmethod
+    def _apart(a, b):
+        """do the rows [N, heads, D] of a and b have no value in common: memory of their own, or heads beside one another in the same rows"""
+        size = a.element_size()
+        extent = lambda t: sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1                          # noqa: E731
+        row = lambda t: (t.shape[1] - 1) * t.stride(1) + (t.shape[2] - 1) * t.stride(2) + 1                   # noqa: E731
+        if a.numel() == 0 or b.numel() == 0:
+            return True
+        gap = (b.data_ptr() - a.data_ptr()) // size
+        if gap >= extent(a) or -gap >= extent(b):
+            return True
+        step = a.stride(0)
+        if a.element_size() != b.element_size() or step != b.stride(0) or step == 0 or (b.data_ptr() - a.data_ptr()) % size:
+            return False
+        return gap % step >= row(a) and step - gap % step >= row(b)
+
+    @staticmethod
+    def rotate(q, k, positions, cos, sin, interleaved, offset, inverse, wq, wk, eps, q_out, k_out):
+        """q [N, Hq, D] and k [N, Hk, D] (or None) rotated into q_out and k_out"""
+        who = "rotate"
+        D = q.size(2) if q.dim() == 3 else 0
+        given = [(t, o, w) for t, o, w in ((q, q_out, wq), (k, k_out, wk)) if t is not None]
+        if not q.is_cuda:
+            raise RuntimeError("statetree_b200: the kernels take CUDA tensors only (no CPU path)")
+        for t, o, w in given:
+            if not (t.dim() == 3 and t.dtype in _Weights.ROTATED and t.dtype == q.dtype and t.shape[::2] == q.shape[::2] and D > 0):
+                raise RuntimeError(f"{who}: q and k of one type (BF16, FP16 or float32), [N, heads, {D or 'D'}]")
+            if t.numel() and t.stride(2) != 1 and D > 1:
+                raise RuntimeError(f"{who}: the values of a head must be contiguous")
+            if not (o.shape == t.shape and o.dtype == t.dtype and (o.numel() == 0 or o.stride(2) == 1 or D == 1)):
+                raise RuntimeError(f"{who}: an output of the input's shape and type, the values of a head contiguous")
+            if w is not None and not (w.dtype == t.dtype and w.shape == (D,) and w.is_contiguous()):
+                raise RuntimeError(f"{who}: norm weights of the values' type [{D}]")
+        N = q.size(0)
+        if not (cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and cos.is_contiguous()
+                and sin.is_contiguous() and cos.size(0) > 0):
+            raise RuntimeError(f"{who}: cos and sin float32 [positions, pairs]")
+        part = 2 * cos.size(1)
+        if offset < 0 or offset + part > D:
+            raise RuntimeError(f"{who}: values {offset} to {offset + part} of heads of {D}")
+        if not (positions.dtype == torch.int64 and positions.is_contiguous() and positions.numel() in (1, N)):
+            raise RuntimeError(f"{who}: positions int64 [N] or [1]")
+        for t in (k, positions, cos, sin, wq, wk, q_out, k_out):
+            if t is not None and t.device != q.device:
+                raise RuntimeError(f"{who}: a tensor on {t.device}, q on {q.device}")
+        outs = [o for _, o, _ in given]
+        for i, (t, o, _) in enumerate(given):
+            same = o.data_ptr() == t.data_ptr() and o.stride() == t.stride()
+            if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())) or (o.size(1) > 1 and o.stride(1) < D) or (
+                    o.size(0) > 1 and o.stride(0) < (o.size(1) - 1) * o.stride(1) + D):
+                raise RuntimeError(f"{who}: an output whose values overlap")
+            for j, (x, _, _) in enumerate(given):
+                if not (same if i == j else False) and not _Weights._apart(o, x):
+                    raise RuntimeError(f"{who}: an output is its own input or lies apart from the inputs")
+        if len(outs) == 2 and not _Weights._apart(*outs):
+            raise RuntimeError(f"{who}: the outputs overlap")
+        if N == 0:
+            return
+        a = []
+        for t, o in ((q, q_out), (k, k_out)):
+            a.append((None, 0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1), t.size(1)))
+            a.append((None, 0, 0) if t is None else (o.data_ptr(), o.stride(0), o.stride(1)))
+        with _ctx(q):
+            _check(lib().st_rotate(*a[0], *a[2], N, D, _Weights.ROTATED[q.dtype], positions.data_ptr(), int(positions.numel() > 1),
+                                   cos.data_ptr(), sin.data_ptr(), cos.size(0), part, int(offset), 1 if interleaved else 0,
+                                   1 if inverse else 0, _ptr(wq), _ptr(wk), float(eps), *a[1], *a[3], _stream(q)))
 
 
 class _KV:
