@@ -1,5 +1,5 @@
 // The host path of a module call in native code: TreeLinear products and lists of them (q / k / v, gate / up) for inputs that need
-// no conversion, the launches of a matrix's conversion and its check, the calls of the 8-bit KV pages and the rotation.  What Python does for such a product (checks, the output
+// no conversion, the launches of a matrix's conversion and its check, the calls of the 8-bit KV pages, the chunk attention and the rotation.  What Python does for such a product (checks, the output
 // and its views, pointer arrays, the ctypes call) takes 15 to 30 us, several times a small product's time on the GPU; this takes
 // 3 to 5.
 //
@@ -44,6 +44,7 @@ struct Library {
   decltype(&st_kv8_chunk_attn_table) kv8_chunk;
   decltype(&st_kv8_attn_workspace_bytes) kv8_workspace;
   decltype(&st_rotate) rotate;
+  decltype(&st_kv_chunk_attn) kv_chunk;
 };
 
 // rows of x if it can be read as it is: BF16 [..., N] on `device`, contiguous, 16-byte aligned, at least one row; else 0
@@ -91,6 +92,7 @@ Library library(const std::map<std::string, uint64_t>& address) {
   bind(lib.kv8_chunk, "st_kv8_chunk_attn_table");
   bind(lib.kv8_workspace, "st_kv8_attn_workspace_bytes");
   bind(lib.rotate, "st_rotate");
+  bind(lib.kv_chunk, "st_kv_chunk_attn");
   return lib;
 }
 
@@ -358,6 +360,43 @@ py::object kv8_dense(const Library& lib, const at::Tensor& pages, const at::Tens
   return py::make_tuple(K, V);
 }
 
+// ---- lossless KV pages: attention of cu's rows (None: one query per sequence), pages uint8 [blocks, H, 2, 2, 1600], pool int32 [P, 16]
+py::object kv_chunk_attention(const Library& lib, const at::Tensor& pages, const at::Tensor& pool, const at::Tensor& q, const Maybe& cu,
+                              const at::Tensor& table, const at::Tensor& lens, double scale, int64_t splits, const Maybe& starts,
+                              const Maybe& given, int64_t window) {
+  constexpr int64_t D = 128;
+  const at::Device device = pages.device();
+  if (!pages.is_cuda() || pages.dim() != 5 || pages.size(2) != 2 || pages.size(3) != 2 || pages.size(4) != 1600 || !flat(pages, at::kByte, device) ||
+      !flat(pool, at::kInt, device) || pool.dim() != 2 || pool.size(1) != 16 || !rows8(q, D, device) || table.dim() != 2)
+    return py::none();
+  const int64_t H = pages.size(1), T = q.size(0), Hq = q.size(1), B = table.size(0);
+  if (H < 1 || Hq % H || B < 1 || table.scalar_type() != at::kInt || table.device() != device || table.layout() != at::kStrided ||
+      table.stride(1) != 1 || !flat(lens, at::kInt, device) || lens.numel() != B ||
+      (starts && (!flat(*starts, at::kInt, device) || starts->numel() != B)) || splits < 1 || window < 0 ||
+      (cu ? !flat(*cu, at::kInt, device) || cu->numel() != B + 1 : T != B))
+    return py::none();
+  if (given && (!rows8(*given, D, device) || given->sizes() != q.sizes())) return py::none();
+  at::Tensor out, ws;
+  int rc;
+  {
+    py::gil_scoped_release nogil;
+    const c10::cuda::CUDAGuard guard(device);
+    out = given ? *given : at::empty(q.sizes(), q.options().requires_grad(false));
+    float *wo = nullptr, *wml = nullptr;
+    if (splits > 1) {                                             // partial results of this call alone
+      ws = at::empty({T * Hq * splits * (D + 2)}, q.options().requires_grad(false).dtype(at::kFloat));
+      wo = reinterpret_cast<float*>(ws.data_ptr());
+      wml = wo + T * Hq * splits * D;
+    }
+    rc = lib.kv_chunk(q.const_data_ptr(), q.stride(0), T, Hq, of<int32_t>(cu), B, pages.const_data_ptr(), pages.size(0), H,
+                      of<uint32_t>(pool), pool.size(0), of<int32_t>(table), table.size(1), table.stride(0), of<int32_t>(lens),
+                      of<int32_t>(starts), window, out.data_ptr(), out.stride(0), wo, wml, scale, splits,
+                      c10::cuda::getCurrentCUDAStream(device.index()).stream());
+  }
+  check(lib, rc);
+  return py::cast(out);
+}
+
 // ---- rotary positions: q [N, Hq, D] and k [N, Hk, D] (or None) into new tensors; (q, k) or None
 py::object rotate(const Library& lib, const at::Tensor& q, const Maybe& k, const at::Tensor& positions, const at::Tensor& cos,
                   const at::Tensor& sin, bool interleaved, int64_t offset, bool inverse, const Maybe& wq, const Maybe& wk, double eps) {
@@ -406,4 +445,5 @@ PYBIND11_MODULE(_calls, m) {
   m.def("kv8_attention", &kv8_attention);
   m.def("kv8_dense", &kv8_dense);
   m.def("rotate", &rotate);
+  m.def("kv_chunk_attention", &kv_chunk_attention);
 }

@@ -1,0 +1,63 @@
+// The lossless KV page to its readers (st_kv.cu: decode attention; st_kv_chunk.cu: attention of chunks).  A page of one KV head is 6400 bytes:
+// keys, then values, each two units of 1600 bytes (dims 0 .. 63 and 64 .. 127), each a record of 16 tokens and its escapes.
+#pragma once
+#include "st_common.cuh"
+
+namespace st {
+constexpr int PAGE_BYTES = 4 * RKV;
+
+// exact bits of one element of a decoded record; the entry is the same in every lane, so the register it lands in is
+// warp-uniform and only the lane that owns the element takes the (single) branch
+__device__ __forceinline__ void put_exact(uint32_t (&R)[4][4], uint32_t entry, int lane) {
+  const int row = (int)((entry >> 6) & 15u), col = (int)(entry & 63u);
+  if (lane != (row & 7) * 4 + ((col & 7) >> 1)) return;
+  const uint32_t sh = 16u * (uint32_t)(col & 1), keep = ~(0xFFFFu << sh), val = (entry >> 16) << sh;
+  switch ((col >> 4) * 4 + (row >> 3) + 2 * ((col >> 3) & 1)) {
+#define ST_PUT(i) case i: R[(i) >> 2][(i) & 3] = (R[(i) >> 2][(i) & 3] & keep) | val; break;
+    ST_PUT(0) ST_PUT(1) ST_PUT(2) ST_PUT(3) ST_PUT(4) ST_PUT(5) ST_PUT(6) ST_PUT(7)
+    ST_PUT(8) ST_PUT(9) ST_PUT(10) ST_PUT(11) ST_PUT(12) ST_PUT(13) ST_PUT(14) ST_PUT(15)
+#undef ST_PUT
+  }
+}
+
+// exact values of a unit's escapes (in-record slots, then the pool chain) put into its decoded fragments
+__device__ __forceinline__ void unit_escapes(const uint8_t* unit, uint32_t head, const uint32_t* pool, int pool_blocks,
+                                             int lane, uint32_t (&R)[4][4]) {
+  if ((head & 31u) == 0u) return;
+  const uint32_t* slot = reinterpret_cast<const uint32_t*>(unit + REC + 4);
+  const int used = min((int)(head & 15u), NSLOT);
+  for (int i = 0; i < used; ++i) put_exact(R, slot[i], lane);
+  if (head & 16u) {
+    int blk = (int)(head >> 8);
+    for (int hops = 0; blk >= 0 && blk < pool_blocks && hops < 4096; ++hops) {
+      const uint32_t w0 = __ldg(pool + (size_t)blk * 16);
+      const int n = min((int)(w0 & 0xFFu), XSLOT);
+      for (int i = 0; i < n; ++i) put_exact(R, __ldg(pool + (size_t)blk * 16 + 1 + i), lane);
+      blk = (int)(w0 >> 8) - 1;
+    }
+  }
+}
+// the two units (dims 0..63, 64..127) of a page's keys or values in shared memory -> the lane's fragment registers.  Both
+// are decoded before the first escape is looked at: two independent chains instead of one
+__device__ __forceinline__ void units_to_frag(const uint8_t* unit, const uint32_t* pool, int pool_blocks, int lane,
+                                              uint32_t (&R)[2][4][4]) {
+  const uint32_t h0 = *reinterpret_cast<const uint32_t*>(unit + REC), h1 = *reinterpret_cast<const uint32_t*>(unit + RKV + REC);
+  const RecRegs r0 = load_rec_shared(unit, lane), r1 = load_rec_shared(unit + RKV, lane);
+  decode_frag(r0, R[0]);
+  decode_frag(r1, R[1]);
+  if (((h0 | h1) & 31u) == 0u) return;
+  unit_escapes(unit, h0, pool, pool_blocks, lane, R[0]);
+  unit_escapes(unit + RKV, h1, pool, pool_blocks, lane, R[1]);
+}
+
+__device__ __forceinline__ float max_over_rows(float v) {        // lanes that differ in g (bits 2..4) hold other tokens
+  v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
+  return fmaxf(v, __shfl_xor_sync(FULL, v, 16));
+}
+__device__ __forceinline__ float sum_over_rows(float v) {
+  v += __shfl_xor_sync(FULL, v, 4);
+  v += __shfl_xor_sync(FULL, v, 8);
+  return v + __shfl_xor_sync(FULL, v, 16);
+}
+}  // namespace st

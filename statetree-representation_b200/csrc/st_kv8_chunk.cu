@@ -26,166 +26,47 @@
 
 #include "../../include/statetree_b200.h"
 #include "st_host.h"
-#include "st_kv8.cuh"
-#include "st_tc.cuh"
+#include "st_chunk_tc.cuh"
 
 namespace {
 using namespace st;
 
-constexpr int KEYS = 128, TILE_PAGES = KEYS / PAGE, ROWS = 128;
-constexpr int W_CONV = 8, W_MMA = 12, WARPS = 16;                 // softmax warps 0 .. 7 (tile = warp / 4); 13 .. 15 only lend registers
 constexpr int CRING = 4;                                          // page factors of so many key tiles are kept
 
 template <int D>
-struct Lay {                                                      // shared memory
-  static constexpr int HALF = 128 * 128;                          // 128 rows x 64 FP16, 128-byte swizzle
-  static constexpr int TILE = D / 64 * HALF;
-  static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE;         // two tiles of Q, two stages of K and V
-  static constexpr int RAW = 6 * TILE, UNIT = PAGE * D;           // codes of one key tile: its keys, its values
+struct Lay : Tiles<D> {                                           // shared memory
+  static constexpr int RAW = Tiles<D>::END, UNIT = PAGE * D;      // codes of one key tile: its keys, its values
   static constexpr int F = RAW + 2 * TILE_PAGES * UNIT, BARS = F + CRING * TILE_PAGES * 3 * 4;
-  static constexpr int NBARS = 25, SLOT = BARS + NBARS * 8;
+  static constexpr int NBARS = ChunkBars::COUNT + 8, SLOT = BARS + NBARS * 8;
   // (more than half of an SM's shared memory: one CTA per SM, which holds all of its tensor memory)
   static constexpr int BYTES = (SLOT + 16 > 120 * 1024 ? SLOT + 16 : 120 * 1024) + 1024;
 };
 
 struct Chunk8 { Attn8 a; Parts8 parts; int* status; int slots; };
 
-// Shared-memory operands.  Descriptor: address / 16 and the stride of the leading dimension / 16 in the low word; in the high one the
-// stride of 8-row groups (1024 B), the version and the 128-byte swizzle, the same for all of them.  So the issuing thread keeps the low
-// words and adds to them (with whole descriptors formed at every MMA the issue took as long as the MMAs).
-//   K-major (Q, K: a row holds 64 values of the contracted dimension)   leading stride unused
-//   MN-major (V: a row, one key, holds 64 values of the other one)       the next 64 values `next` bytes further
-constexpr uint32_t DESC_HI = 64u | 1u << 14 | 2u << 29;
-__device__ __forceinline__ uint32_t desc_k(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4 | 1u << 16; }
-__device__ __forceinline__ uint32_t desc_mn(uint32_t saddr, uint32_t next) { return (saddr & 0x3FFFFu) >> 4 | (next >> 4) << 16; }
-// D (+)= A B^T, A from shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
-  asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}"
-               :: "r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(DESC_HI) : "memory");
-}
-// the same, A from tensor memory
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
-  asm volatile("{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}"
-               :: "r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(DESC_HI) : "memory");
-}
-#define ST_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
-#define ST_I4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
-__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t* v) {            // (complete after tm_wait_ld)
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-               "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-               : ST_R4(v, 0), ST_R4(v, 4), ST_R4(v, 8), ST_R4(v, 12), ST_R4(v, 16), ST_R4(v, 20), ST_R4(v, 24), ST_R4(v, 28)
-               : "r"(addr));
-}
-__device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t* v) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-               : ST_R4(v, 0), ST_R4(v, 4), ST_R4(v, 8), ST_R4(v, 12) : "r"(addr));
-}
-template <int N>
-__device__ __forceinline__ void tm_wait_ld(uint32_t* v) {                        // (v's readers stay behind the wait)
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int k = 0; k < N; ++k) asm volatile("" : "+r"(v[k]));
-}
-// two fp32 operations in one instruction
-__device__ __forceinline__ uint64_t pair2(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpair2(uint64_t p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2f(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&v)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-               :: "r"(addr), ST_I4(v, 0), ST_I4(v, 4), ST_I4(v, 8), ST_I4(v, 12) : "memory");
-}
-#undef ST_R4
-#undef ST_I4
-// registers of a warpgroup: 512 threads start with 128 each (64 K in all, the SM's); 2 x 184 + 96 + 48 = 4 x 128
-constexpr int R_SOFTMAX = 184, R_CONV = 96, R_MMA = 48;
-template <int N>
-__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
-
-// What a CTA works on; the same in all of its threads
-struct Work : Rows8 {
-  int h, split, pos0;                                             // position of query 0
-  int lo0, first_tile, tiles, count0, count1;                           // key tiles of the split; of those, how many each row tile needs
-};
-
 template <int D>
 __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c) {
   using L = Lay<D>;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  uint64_t *const begin1 = bars, *const kfull = bars + 2, *const vfull = bars + 4, *const sfull = bars + 6, *const pfull = bars + 8,
-           *const ofull = bars + 12, *const empty = bars + 14, *const raw = bars + 16;           // pfull: [half of the keys][row tile]
-  uint64_t* const drain = bars + 24;                              // raw: [converter warp][keys, values]
+  const ChunkBars b(reinterpret_cast<uint64_t*>(smem + L::BARS));
+  uint64_t *const begin1 = b.begin1, *const kfull = b.kfull, *const vfull = b.vfull, *const sfull = b.sfull, *const pfull = b.pfull,
+           *const ofull = b.ofull, *const empty = b.empty, *const raw = b.rest;                  // raw: [converter warp][keys, values]
   uint32_t* const slot_at = reinterpret_cast<uint32_t*>(smem + L::SLOT);
   const Attn8& a = c.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.Hq / a.H;
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- what this CTA works on.  Later tiles of a sequence see more keys: they go first
   Work w;
-  {
-    int x = blockIdx.x;
-    w.split = x % c.parts.splits;
-    x /= c.parts.splits;
-    w.h = x % a.H;
-    if (!find_rows<2 * ROWS>(a, G, c.slots - 1 - x / a.H, lane, w)) return;
-    const int start = w.start;
-    w.pos0 = w.len - w.n;
-    const int first_pos = w.pos0 + w.row0 / G, last_pos = w.pos0 + (w.row0 + w.rows - 1) / G;
-    w.lo0 = start;
-    const int lo = a.window > 0 ? max(start, first_pos - a.window + 1) : start;
-    const int end = (int)min((long long)last_pos + 1, (long long)a.table_width * PAGE);            // keys [lo, end)
-    const int t0 = lo / KEYS, t1 = end > lo ? (end - 1) / KEYS + 1 : t0;
-    const int per = (t1 - t0 + c.parts.splits - 1) / c.parts.splits;
-    w.first_tile = t0 + w.split * per;
-    w.tiles = max(0, min(t1, w.first_tile + per) - w.first_tile);
-    const int mid_pos = w.pos0 + (w.row0 + min(w.rows, ROWS) - 1) / G;                   // last position of the first row tile
-    w.count0 = mid_pos < 0 ? 0 : max(0, min(w.tiles, mid_pos / KEYS + 1 - w.first_tile));
-    w.count1 = w.rows > ROWS ? w.tiles : 0;
-  }
+  if (!chunk_work(a, c.parts.splits, c.slots, G, lane, w)) return;
   const int tiles = max(w.count0, w.count1);
   // (pages behind the last key of the sequence, or behind its row of the table, may not exist: no key of theirs is seen)
   const int end_page = min((w.pos0 + w.n - 1) / PAGE + 1, a.table_width);
   const uint64_t keep = policy_evict_last();                      // other row tiles of the sequence read the same pages
 
   if (warp == W_MMA) {
-    if (elect_one()) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(kfull + i, 4);
-        mbar_init(vfull + i, 4);
-        mbar_init(sfull + i, 1);
-        mbar_init(pfull + i, 4);
-        mbar_init(pfull + 2 + i, 4);
-        mbar_init(ofull + i, 1);
-        mbar_init(empty + i, 1);
-      }
-      mbar_init(drain, 1);
-      mbar_init(begin1, 4);
-      fence_barrier_init();
-    }
+    if (elect_one()) b.init();
     __syncwarp();
     tmem_alloc<1>(slot_at, 512);
     tmem_relinquish<1>();
@@ -336,64 +217,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     if (ok && count > 0) ok = mbar_wait(ofull + t, 0);
     if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_ACC);
     // ---- out.  (a wait that ran out leaves the rows unwritten)
-    if (ok && any) {
-      tc_fence_after();
-      const long long r = (long long)(w.first + token) * a.Hq + hq;
-      const float inv = c.parts.splits > 1 ? 1.f : (l > 0.f ? 1.f / l : l);
-      if (live && c.parts.splits > 1) {
-        float* const ml = c.parts.ml + (r * c.parts.splits + w.split) * 2;
-        ml[0] = l > 0.f || l != l ? m : -INFINITY;
-        ml[1] = l;
-      }
-      if (c.parts.splits > 1) {
-        float* const o = c.parts.o + (r * c.parts.splits + w.split) * D;
-#pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t v[32];
-          if (count > 0) {
-            tm_ld32(to + 32 * q, v);
-            tm_wait_ld<32>(v);
-          }
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
-          if (live)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) reinterpret_cast<uint4*>(o + 32 * q)[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-          __syncwarp();
-        }
-      } else {
-        // the warp's rows leave through where its rows of q were (their last scores are done), D / 8 lanes a row
-        constexpr int LANES = D / 8, PER = 32 / LANES;
-        uint8_t* const rows = smem + L::Q + t * L::TILE + (warp & 3) * (32 * 2 * D);
-#pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t v[32];
-          if (count > 0) {
-            tm_ld32(to + 32 * q, v);
-            tm_wait_ld<32>(v);
-          }
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t u[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] = pack_bf16(__uint_as_float(v[8 * k + 2 * i]), __uint_as_float(v[8 * k + 2 * i + 1]));
-            *reinterpret_cast<uint4*>(rows + lane * (2 * D) + (((4 * q + k) ^ (lane & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
-          }
-        }
-        __syncwarp();
-        const long long mine = live ? (long long)(w.first + token) * a.out_stride + (long long)hq * D : -1;
-#pragma unroll
-        for (int i = 0; i < LANES; ++i) {
-          const int row = i * PER + lane / LANES;
-          const long long out = __shfl_sync(FULL, mine, row);
-          if (out >= 0)
-            *reinterpret_cast<uint4*>(a.out + out + 8 * (lane % LANES)) =
-                *reinterpret_cast<const uint4*>(rows + row * (2 * D) + (((lane % LANES) ^ (row & 7)) << 4));
-        }
-      }
-    }
+    if (ok && any) chunk_store<D>(a, c.parts, w, smem, t, warp, lane, live, token, hq, count, to, m, l);
     tc_fence_before();
   } else if (warp < W_MMA) {
     regs_down<R_CONV>();
@@ -514,76 +338,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
   } else {
     regs_down<R_MMA>();
     if (warp == W_MMA) {
-    // ---------------------------------------------------------------- MMAs.  One thread's MMAs complete in the order of their issue
-    // (and a commit covers all before it): S of the next key tile may take the place of the P that the product before it reads
-    // (mma_idesc's operands are BF16; FP16 is type 0)
+    // ---------------------------------------------------------------- MMAs (mma_idesc's operands are BF16; FP16 is type 0)
     constexpr uint32_t FP16 = ~(1u << 7 | 1u << 10), IDESC_S = mma_idesc(128, KEYS) & FP16, IDESC_O = (mma_idesc(128, D) & FP16) | 1u << 16;
     meet();
     const uint32_t tmem = *slot_at;
-    // The whole loop runs in one elected thread, waits included: a warp that meets again around each step costs more than the steps
-    if (elect_one()) {
-      const uint32_t dq = desc_k(smem_addr(smem + L::Q)), dk = desc_k(smem_addr(smem + L::K)), dv = desc_mn(smem_addr(smem + L::V), L::HALF);
-      auto scores = [&](int t, int s) {
-        const uint32_t q = dq + t * (L::TILE >> 4), k = dk + s * (L::TILE >> 4);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint32_t at = (i >> 2) * (L::HALF >> 4) + 2 * (i & 3);
-          mma_ss(tmem + t * 128, q + at, k + at, IDESC_S, i > 0);
-        }
-        tc_commit(sfull + t);
-      };
-      auto outputs = [&](int t, int s, int half, bool more) {
-        const uint32_t v = dv + s * (L::TILE >> 4);
-#pragma unroll
-        for (int k = 0; k < KEYS / 32; ++k) {
-          const int i = half * (KEYS / 32) + k;
-          mma_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * i, v + i * (2048 >> 4), IDESC_O, more || i > 0);
-        }
-      };
-      // Three commits a key tile (each waits for the one before it): the scores of either row tile, and `empty`, behind the first
-      // product of tile j, which says that the scores of tile j and the products of tile j - 1 are done: K(j) and V(j - 1) are free
-      bool ok = true;
-      if (tiles > 0) {
-        ok = mbar_wait(kfull, 0);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (ok && (t ? w.count1 : w.count0) > 0) {
-            tc_fence_after();
-            scores(t, 0);
-          }
-      }
-      for (int j = 0; ok && j < tiles; ++j) {
-        const int s = j & 1, s1 = s ^ 1;
-        ok = mbar_wait_look(vfull + s, (uint32_t)(j >> 1) & 1u);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int count = t ? w.count1 : w.count0;
-          if (!ok || j >= count) continue;
-          ok = mbar_wait_look(pfull + t, (uint32_t)j & 1u);
-          if (!ok) continue;
-          tc_fence_after();
-          outputs(t, s, 0, j > 0);
-          ok = mbar_wait_look(pfull + 2 + t, (uint32_t)j & 1u);
-          if (!ok) continue;
-          tc_fence_after();
-          outputs(t, s, 1, true);
-          if (t == 0 || j >= w.count0) tc_commit(empty + s);
-          if (j + 1 < count) {
-            ok = mbar_wait_look(kfull + s1, (uint32_t)((j + 1) >> 1) & 1u);
-            if (!ok) continue;
-            tc_fence_after();
-            scores(t, s1);
-          } else {
-            tc_commit(ofull + t);
-          }
-        }
-      }
-      if (!ok) {                                                  // (gave up: let what was issued complete before the memory goes)
-        atomicExch(c.status, ERR_WAIT_MMA);
-        tc_commit(drain);
-        (void)mbar_wait(drain, 0);
-      }
-    }
+    if (elect_one()) issue_mmas<D, IDESC_S, IDESC_O>(smem, b, tmem, tiles, w.count0, w.count1, c.status);
     __syncwarp();
     tc_fence_before();
     } else {

@@ -29,11 +29,25 @@ class PageStore:
     """pages of one attention layer: uint8 [blocks, H, 2, 2, 1600], escape pool int32 [P, 16], pool counter int32 [2]"""
 
     def __init__(self, num_blocks, num_kv_heads, device, pool_blocks=1 << 15):
-        self.H = num_kv_heads
-        self.device = torch.device(device)
-        self.pages = torch.zeros(num_blocks, num_kv_heads, 2, 2, RKV, dtype=torch.uint8, device=device)
-        self.pool = torch.zeros(pool_blocks, 16, dtype=torch.int32, device=device)
-        self.pcnt = torch.zeros(2, dtype=torch.int32, device=device)
+        self._take(torch.zeros(num_blocks, num_kv_heads, 2, 2, RKV, dtype=torch.uint8, device=device),
+                   torch.zeros(pool_blocks, 16, dtype=torch.int32, device=device), torch.zeros(2, dtype=torch.int32, device=device))
+
+    @classmethod
+    def over(cls, pages, pool, pcnt=None):
+        """a store over tensors that exist already (another store's, part of a larger buffer, pages that were saved).  pcnt: the pool's
+        counter, for appends; None: every block of the pool counts as taken"""
+        self = cls.__new__(cls)
+        kv_ext()._pages("PageStore", pages, pool, pcnt)
+        if pcnt is None:
+            pcnt = torch.tensor([pool.shape[0], 0], dtype=torch.int32, device=pages.device)
+        if pcnt.dtype != torch.int32 or pcnt.numel() != 2:
+            raise RuntimeError("PageStore: pool counter int32 [2]")
+        self._take(pages, pool, pcnt)
+        return self
+
+    def _take(self, pages, pool, pcnt):
+        self.H, self.device = pages.shape[1], pages.device
+        self.pages, self.pool, self.pcnt = pages, pool, pcnt
         self._wo = self._wml = None                        # split partials: grown, never freed (a captured graph may write
         self._retired = []                                 # into the ones it was given)
 
@@ -59,6 +73,27 @@ class PageStore:
                 self._wml = torch.empty(1, dtype=torch.float32, device=q.device)
         kv_ext().attn(q, self.pages, self.pool, block_table, lens, out, self._wo, self._wml, scale, splits, starts,
                       min_pages)
+        return out
+
+    def chunk_attention(self, q, cu, block_table, lens, scale, splits=None, starts=None, out=None, window=0):
+        """causal attention of several query tokens per sequence, after their keys and values have been appended: q [T, Hq, 128] bf16,
+        sequence b's rows are cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1]; None: one each), the last of them at position lens[b] - 1 ->
+        [T, Hq, 128].  A query at position p sees tokens [max(starts, p - window + 1), p] (window 0: from starts on), one that sees none
+        gives zeros; rows behind cu[B] of a given `out` stay as they are.  splits: how many CTAs share a sequence (None: by the sizes)"""
+        if splits is None:
+            splits = chunk_splits(q.shape[0], block_table.shape[0], self.H, q.shape[1] // self.H, block_table.shape[1])
+        host = calls()
+        if host is not None:
+            done = host[0].kv_chunk_attention(host[1], self.pages, self.pool, q, cu, block_table, lens, scale, splits, starts, out, window)
+            if done is not None:
+                return done
+        q = _rows(q, 128)
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        need = lib().st_kv_chunk_attn_workspace_bytes(q.shape[0], q.shape[1], splits) // 4
+        flat = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+        wo, wml = (flat[:need // 130 * 128], flat[need // 130 * 128:]) if need else (None, None)
+        kv_ext().chunk_attn(q, cu, self.pages, self.pool, block_table, lens, out, scale, splits, wo, wml, starts, window)
         return out
 
     def dense(self, blocks=None):
@@ -119,6 +154,16 @@ def chunk_splits8(tokens, seqs, kv_heads, group, max_pages, sms=148):
     rows = -(-tokens * group // seqs)                       # of a sequence, on the mean
     if rows <= FEW_ROWS8:
         return decode_splits8(kv_heads * seqs * -(-rows // 8), max_pages, sms)
+    return max(1, min(sms // (kv_heads * seqs * -(-rows // 256)), max_pages // 16, 64))
+
+
+def chunk_splits(tokens, seqs, kv_heads, group, max_pages, sms=148):
+    """How many CTAs share a sequence of the chunk attention over lossless pages, from what the host knows (st_kv_chunk.cu)"""
+    seqs = max(1, seqs)
+    rows = -(-tokens * group // seqs)                       # of a sequence, on the mean
+    if rows <= FEW_ROWS8:
+        units = seqs * kv_heads * -(-rows // 16)
+        return max(1, min(2 * sms // max(1, units), max_pages // 8, 64))
     return max(1, min(sms // (kv_heads * seqs * -(-rows // 256)), max_pages // 16, 64))
 
 

@@ -76,6 +76,9 @@ _SIGNATURES = {
     "st_gemv_swiglu": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "st_rope_kv_append": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _dbl, _vp, _vp, _i64,
                                  _vp, _i64, _vp, _vp]),
+    "st_kv_chunk_attn_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "st_kv_chunk_attn": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp,
+                                _vp, _dbl, _i64, _vp]),
     "st_rotate": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _i64, _i64, _i64, _int, _int,
                          _vp, _vp, _dbl, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
     "st_moe_align": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
@@ -130,7 +133,7 @@ CALLS_PATH = os.path.join(_HERE, "_calls.so")
 _CALLS = None                                           # False: there is none
 _NATIVE = ("st_gemv", "st_gemm", "st_gemv_list", "st_gemm_list", "st_last_error", "st_encode", "st_encode_lists", "st_encode_offsets",
            "st_encode_offsets_workspace_bytes", "st_dec_check", "st_lists_check", "st_kv8_append", "st_kv8_dequant_blocks", "st_kv8_attn_table",
-           "st_kv8_chunk_attn_table", "st_kv8_attn_workspace_bytes", "st_rotate")
+           "st_kv8_chunk_attn_table", "st_kv8_attn_workspace_bytes", "st_rotate", "st_kv_chunk_attn")
 
 
 def calls():
@@ -648,6 +651,54 @@ class _KV:
             _check(lib().st_kv_attn(_ptr(q), q.stride(0), B, Hq, _ptr(kv), kv.size(0), Hkv, _ptr(pool), pool.size(0),
                                     _ptr(bt), bt.stride(0), _ptr(lens), _ptr(starts), _ptr(out), out.stride(0),
                                     _ptr(wo), _ptr(wml), float(scale), int(S), int(minpps), _stream(q)))
+
+    @staticmethod
+    def _pages(who, kv, pool, *others):
+        """KV heads of the pages kv uint8 [blocks, H, 2, 2, 1600] with their escape pool int32 [P, 16]; `others` lie on their device"""
+        if not (kv.dtype == torch.uint8 and kv.dim() == 5 and kv.shape[2:] == (2, 2, 1600) and kv.is_contiguous()):
+            raise RuntimeError(f"{who}: cache uint8 [blocks, H, 2, 2, 1600]")
+        if not (pool.dtype == torch.int32 and pool.dim() == 2 and pool.size(1) == 16 and pool.is_contiguous()):
+            raise RuntimeError(f"{who}: pool int32 [P, 16]")
+        for t in (pool, *others):
+            if t is not None and t.device != kv.device:
+                raise RuntimeError(f"{who}: a tensor on {t.device}, the cache on {kv.device}")
+        return kv.shape[1]
+
+    @staticmethod
+    def chunk_attn(q, cu, kv, pool, bt, lens, out, scale, S=1, wo=None, wml=None, starts=None, window=0):
+        """causal attention of the query rows cu[b] .. cu[b + 1] - 1 of every sequence b, q [T, Hq, 128], over the lossless pages"""
+        who = "kv_chunk_attn"
+        H = _KV._pages(who, kv, pool, q, cu, bt, lens, out, starts, wo, wml)
+        _KV._rows8(who, "q", q, 128)
+        _KV._rows8(who, "out", out, 128)
+        T, B, Hq = q.size(0), bt.size(0), q.size(1)
+        if Hq % H or Hq == 0 or out.shape != q.shape:
+            raise RuntimeError(f"{who}: q and out [tokens, a multiple of {H} heads, 128]")
+        _KV._table(who, bt, lens, starts)
+        if window < 0 or S < 1:
+            raise RuntimeError(f"{who}: window / splits")
+        if cu is None and T != B:
+            raise RuntimeError(f"{who}: without cu every sequence has one query")
+        if cu is not None and not (cu.dtype == torch.int32 and cu.is_contiguous() and cu.numel() == B + 1):
+            raise RuntimeError(f"{who}: cu int32 [B + 1]")
+        if S > 1 and not (wo is not None and wml is not None and wo.dtype == wml.dtype == torch.float32 and wo.is_contiguous()
+                          and wml.is_contiguous() and wo.numel() >= T * Hq * S * 128 and wml.numel() >= T * Hq * S * 2):
+            raise RuntimeError(f"{who}: workspace")
+        if T == 0 or B == 0:
+            return
+        with _ctx(kv):
+            _check(lib().st_kv_chunk_attn(q.data_ptr(), q.stride(0), T, Hq, _ptr(cu), B, kv.data_ptr(), kv.size(0), H, pool.data_ptr(),
+                                          pool.size(0), bt.data_ptr(), bt.size(1), bt.stride(0), lens.data_ptr(), _ptr(starts), int(window),
+                                          out.data_ptr(), out.stride(0), _ptr(wo), _ptr(wml), float(scale), int(S), _stream(q)))
+
+    @staticmethod
+    def _table(who, bt, lens, starts):
+        B = bt.size(0)
+        if not (bt.dtype == torch.int32 and bt.dim() == 2 and (bt.stride(1) == 1 or bt.size(1) == 1) and lens.dtype == torch.int32
+                and lens.is_contiguous() and lens.numel() == B):
+            raise RuntimeError(f"{who}: block table int32 [B, pages], lens int32 [B]")
+        if starts is not None and not (starts.dtype == torch.int32 and starts.is_contiguous() and starts.numel() == B):
+            raise RuntimeError(f"{who}: starts int32 [B]")
 
     # ---- pages in 8 bits (no counterpart in the reference)
     @staticmethod
