@@ -6,7 +6,7 @@
 
 namespace st {
 constexpr int KEYS = 128, TILE_PAGES = KEYS / PAGE, ROWS = 128;
-constexpr int W_CONV = 8, W_MMA = 12, WARPS = 16;                 // softmax warps 0 .. 7 (tile = warp / 4); 13 .. 15 only lend registers
+constexpr int W_CONV = 8;                                         // softmax warps 0 .. 7 (tile = warp / 4), converter warps from here
 
 // Shared memory: the operand tiles, 64 values of a row in 128 bytes with the 128-byte swizzle
 template <int D>
@@ -82,8 +82,6 @@ __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&v)[16]) 
 }
 #undef ST_R4
 #undef ST_I4
-// registers of a warpgroup: 512 threads start with 128 each (64 K in all, the SM's); 2 x 184 + 96 + 48 = 4 x 128
-constexpr int R_SOFTMAX = 184, R_CONV = 96, R_MMA = 48;
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
 template <int N>
@@ -128,10 +126,10 @@ struct ChunkBars {
   static constexpr int COUNT = 17;
   __device__ explicit ChunkBars(uint64_t* b)
       : begin1(b), kfull(b + 2), vfull(b + 4), sfull(b + 6), pfull(b + 8), ofull(b + 12), empty(b + 14), drain(b + 16), rest(b + 17) {}
-  __device__ void init() const {                                  // one thread; 4: an arrival per converter or softmax warp
+  __device__ void init(int converters) const {                    // one thread; an arrival per converter warp, or per softmax warp of a row tile
     for (int i = 0; i < 2; ++i) {
-      mbar_init(kfull + i, 4);
-      mbar_init(vfull + i, 4);
+      mbar_init(kfull + i, converters);
+      mbar_init(vfull + i, converters);
       mbar_init(sfull + i, 1);
       mbar_init(pfull + i, 4);
       mbar_init(pfull + 2 + i, 4);

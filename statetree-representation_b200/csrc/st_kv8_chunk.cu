@@ -31,6 +31,9 @@
 namespace {
 using namespace st;
 
+constexpr int W_MMA = 12, WARPS = 16;                             // (four converter warps; 13 .. 15 only lend registers)
+// registers of a warpgroup: 512 threads start with 128 each (64 K in all, the SM's); 2 x 184 + 96 + 48 = 4 x 128
+constexpr int R_SOFTMAX = 184, R_CONV = 96, R_MMA = 48;
 constexpr int CRING = 4;                                          // page factors of so many key tiles are kept
 
 template <int D>
@@ -66,7 +69,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
   const uint64_t keep = policy_evict_last();                      // other row tiles of the sequence read the same pages
 
   if (warp == W_MMA) {
-    if (elect_one()) b.init();
+    if (elect_one()) b.init(W_MMA - W_CONV);
     __syncwarp();
     tmem_alloc<1>(slot_at, 512);
     tmem_relinquish<1>();

@@ -22,6 +22,11 @@
 namespace {
 using namespace st;
 
+// Warps of kv_chunk_kernel: eight of softmax, eight converters (a page of a key tile each), one that issues the MMAs, three producers
+constexpr int W_MMA = W_CONV + TILE_PAGES, W_FETCH = W_MMA + 1, WARPS = W_MMA + 4, FETCHERS = WARPS - W_FETCH;
+// registers of a warpgroup: 640 threads start with 96 each; 2 x 160 + 2 x 56 + 48 = 5 x 96
+constexpr int R_START = 96, R_SOFTMAX = 160, R_CONV = 56, R_MMA = 48;
+static_assert(2 * R_SOFTMAX + 2 * R_CONV + R_MMA <= 5 * R_START, "what the warpgroups take up is what the block starts with");
 struct Pool { const uint32_t* at; int blocks; };
 struct ChunkArgs { Attn8 a; Parts8 parts; Pool pool; int* status; int slots; };
 
@@ -30,22 +35,32 @@ constexpr float RAISE = 8.f;
 
 // ------------------------------------------------------------------------------------------------ many rows
 // The division of the work, the hand-overs and the products are those of the attention over 8-bit pages (st_chunk_tc.cuh); what differs:
-// there is no factor per page, and the converter warps decode records.  A warp brings in pages cw and cw + 4 of every key tile, their keys and
-// then their values, by bulk copies of 3200 bytes into two slots of its own, each requested again as soon as its records are in registers.
-// Decoded, a record is four mma A fragments: four stmatrix put it into the swizzled tile.  Its escapes are written over the tile, a lane an
+// there is no factor per page, and the converter warps decode records.  A warp takes one page of every key tile, its keys and then its values,
+// from a slot of its own, which producer warps fill by bulk copies of 3200 bytes as soon as the records before are in registers (an issue
+// takes some 270 cycles: one warp for all sixteen of a key tile would be the limit).  Decoded, a record is four mma A fragments: four stmatrix put it into the swizzled tile.  Its escapes are written over the tile, a lane an
 // entry (patching the fragments instead takes a serial step an entry).
 struct LayX : Tiles<HD> {
-  static constexpr int RAW = Tiles<HD>::END, SLOT_BYTES = 2 * RKV;                                 // [converter warp][page cw, page cw + 4]
-  static constexpr int BARS = RAW + 8 * SLOT_BYTES, NBARS = ChunkBars::COUNT + 8, SLOT = BARS + NBARS * 8;
+  static constexpr int RAW = Tiles<HD>::END, SLOT_BYTES = 2 * RKV;                                 // a slot per page of a key tile
+  static constexpr int BARS = RAW + 8 * SLOT_BYTES, NBARS = ChunkBars::COUNT + 16, SLOT = BARS + NBARS * 8;
   static constexpr int BYTES = SLOT + 16 + 1024;
 };
 
-// a unit's entries over its tile: lane's `entry` if `live`.  The same element twice: the later entry stands
-__device__ __forceinline__ void put_entries(uint8_t* tile, uint32_t entry, bool live, int lane) {
-  const unsigned same = __match_any_sync(FULL, live ? entry & 1023u : 1024u + lane);
-  if (!live || (same >> lane) != 1u) return;
-  const int row = (int)((entry >> 6) & 15u), col = (int)(entry & 63u);
-  *reinterpret_cast<uint16_t*>(tile + row * 128 + ((((col >> 3) ^ (row & 7)) << 4) | (col & 7) * 2)) = (uint16_t)(entry >> 16);
+// entries of a page's two units over their tile, half a warp for each unit: those that are listed (in the order of the lanes), in rows that
+// are wanted (`seen`).  They ascend unless a row has been appended again in place: then one after the other, so that the later entry of an
+// element stands
+__device__ __forceinline__ void put_entries(uint8_t* tile, uint32_t entry, bool listed, bool seen, int lane) {
+  const int row = (int)((entry >> 6) & 15u), col = (int)(entry & 63u), at = lane & 15;
+  uint16_t* const to = reinterpret_cast<uint16_t*>(tile + (lane >> 4) * LayX::HALF + row * 128 + ((((col >> 3) ^ (row & 7)) << 4) | (col & 7) * 2));
+  const uint32_t key = listed ? entry & 1023u : 1024u, before = __shfl_up_sync(FULL, key, 1, 16);
+  const bool live = listed && seen;
+  if (!__any_sync(FULL, listed && at > 0 && before != 1024u && key <= before)) {
+    if (live) *to = (uint16_t)(entry >> 16);
+    return;
+  }
+  for (int i = 0; i < 16; ++i) {
+    if (at == i && live) *to = (uint16_t)(entry >> 16);
+    __syncwarp();
+  }
 }
 
 __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs c) {
@@ -54,7 +69,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   const ChunkBars b(reinterpret_cast<uint64_t*>(smem + L::BARS));
-  uint64_t* const raw = b.rest;                                   // [converter warp][slot]
+  uint64_t *const raw = b.rest, *const rempty = raw + 8;           // of every slot: filled, in registers
   uint32_t* const slot_at = reinterpret_cast<uint32_t*>(smem + L::SLOT);
   const Attn8& a = c.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.Hq / a.H;
@@ -68,7 +83,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
   const uint64_t keep = policy_evict_last();                      // other row tiles of the sequence read the same pages
 
   if (warp == W_MMA) {
-    if (elect_one()) b.init();
+    if (elect_one()) b.init(W_MMA - W_CONV);
     __syncwarp();
     tmem_alloc<1>(slot_at, 512);
     tmem_relinquish<1>();
@@ -200,136 +215,85 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
     regs_down<R_CONV>();
     // ---------------------------------------------------------------- converters: records -> operand tiles
     const int cw = warp - W_CONV;
-    uint8_t* const mine = smem + L::RAW + cw * (2 * L::SLOT_BYTES);
-    uint64_t* const my_raw = raw + 2 * cw;
-    const uint8_t* const head_pages = a.kv + (size_t)w.h * PAGE_BYTES;
-    const size_t page_step = (size_t)a.H * PAGE_BYTES;
-    const int* const table = a.table + (long long)w.b * a.table_stride;
-    // lane l holds the entry of page cw + 4 (l % 2) of the sixteen key tiles' (l / 2)-th; the next sixteen are requested half way; -1 =
-    // there is no such page
-    auto entry = [&](int j) {
-      const int t = j + (lane >> 1), p = (w.first_tile + t) * TILE_PAGES + cw + 4 * (lane & 1);
-      if (t >= tiles || p >= end_page) return -1;
-      const int e = __ldg(table + p);
-      return e < 0 ? 0 : (int)min((long long)e, a.nblocks - 1);
-    };
-    if (lane == 0) {
-      mbar_init(my_raw, 1);
-      mbar_init(my_raw + 1, 1);
-      fence_barrier_init();
-    }
-    __syncwarp();
-    int now = entry(0), next = -1;
-    auto fetch = [&](int p, int kvi, int e) {                     // page p (0, 1) of a tile, its keys or values
-      if (elect_one()) {
-        mbar_expect_tx(my_raw + p, e >= 0 ? (uint32_t)L::SLOT_BYTES : 0u);
-        if (e >= 0) bulk_g2s(mine + p * L::SLOT_BYTES, head_pages + e * page_step + kvi * L::SLOT_BYTES, L::SLOT_BYTES, my_raw + p, keep);
-      }
-      __syncwarp();
-    };
-    if (tiles > 0) {
-      fetch(0, 0, __shfl_sync(FULL, now, 0));
-      fetch(1, 0, __shfl_sync(FULL, now, 1));
-    }
+    const uint8_t* const unit = smem + L::RAW + cw * L::SLOT_BYTES;
     meet();
     // where this lane's rows of the four 8 x 8 blocks of a k-step go: row lane % 16, columns 8 (lane / 16) on
     const int at_row = (lane & 15) * 128, at_col = lane >> 4;
-    int asked = 2;                                                // fetches under way or done (of 4 a tile), for the way out
     bool ok = true;
     for (int j = 0; ok && j < tiles; ++j) {
-      const int s = j & 1, at = 2 * (j & 15);
-      if ((j & 15) == 4) next = entry((j & ~15) + 16);
-      const int ahead = (j & 15) == 15 ? next : now;
-      const int have[2] = {__shfl_sync(FULL, now, at), __shfl_sync(FULL, now, at + 1)};
-      const int then[2] = {__shfl_sync(FULL, ahead, (at + 2) & 31), __shfl_sync(FULL, ahead, (at + 3) & 31)};
+      const int s = j & 1;
 #pragma unroll
       for (int kvi = 0; kvi < 2; ++kvi) {
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          if (ok) ok = mbar_wait_look(my_raw + p, (uint32_t)kvi);  // (two phases a tile)
-          if (!ok) break;
-          const uint8_t* const unit = mine + p * L::SLOT_BYTES;
-          uint32_t A[2][4][4], head[2] = {0u, 0u}, ent[2];
-          if (have[p] >= 0) {
-            RecRegs r[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              r[h] = load_rec_shared(unit + h * RKV, lane);
-              head[h] = *reinterpret_cast<const uint32_t*>(unit + h * RKV + REC);
-              ent[h] = *reinterpret_cast<const uint32_t*>(unit + h * RKV + REC + 4 + 4 * min(lane, NSLOT - 1));
-            }
-            __syncwarp();
-            if (kvi == 0 || j + 1 < tiles) {
-              fence_proxy_async();
-              fetch(p, kvi ^ 1, kvi ? then[p] : have[p]);
-              ++asked;
-            }
-            decode_frag(r[0], A[0]);
-            decode_frag(r[1], A[1]);
-          } else {                                                // (a page that is not there: zeros)
-            if (kvi == 0 || j + 1 < tiles) {
-              fetch(p, kvi ^ 1, kvi ? then[p] : have[p]);
-              ++asked;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) A[i >> 4][(i >> 2) & 3][i & 3] = 0u;
-          }
-          const int first = (w.first_tile + j) * KEYS + (cw + 4 * p) * PAGE;                  // position of the page's first token
-          const bool edge = kvi && (first < w.start || first + PAGE > w.len);
-          if (edge) {
-            const int pos = first + (lane >> 2);
-            const bool x0 = pos >= w.start && pos < w.len, x8 = pos + 8 >= w.start && pos + 8 < w.len;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) A[i >> 4][(i >> 2) & 3][i & 3] = ((i & 1) ? x8 : x0) ? A[i >> 4][(i >> 2) & 3][i & 3] : 0u;
-          }
-          // K's stage is free when the scores of tile j - 2 are, V's when its products are: see the commits of the MMA loop
-          const int e = kvi ? j - 1 : j - 2;
-          if (p == 0 && j > 1) ok = mbar_wait_look(b.empty + (e & 1), (uint32_t)(e >> 1) & 1u);
-          if (!ok) break;
-          uint8_t* const tile = smem + (kvi ? L::V : L::K) + s * L::TILE + (cw + 4 * p) * (PAGE * 128);
+        ok = mbar_wait_look(raw + cw, (uint32_t)kvi);            // (two phases a tile)
+        if (!ok) break;
+        const bool there = (w.first_tile + j) * TILE_PAGES + cw < end_page;
+        uint32_t A[2][4][4], heads = 0u, head = 0u, ent = 0u, word = 0u;       // head, ent, word: of the lane's unit, lane / 16
+        if (there) {
+          RecRegs r[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t to = smem_addr(tile + h * L::HALF + at_row);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) stmatrix_x4(to + (((2 * i + at_col) ^ (lane & 7)) << 4), A[h][i][0], A[h][i][1], A[h][i][2], A[h][i][3]);
+            r[h] = load_rec_shared(unit + h * RKV, lane);
+            heads |= *reinterpret_cast<const uint32_t*>(unit + h * RKV + REC);
           }
-          if (((head[0] | head[1]) & 31u) != 0u) {                // (the same in every lane)
-            __syncwarp();
-            auto seen = [&](uint32_t entry) {
-              const int pos = first + (int)((entry >> 6) & 15u);
-              return !edge || (pos >= w.start && pos < w.len);
-            };
+          const uint8_t* const tail = unit + (lane >> 4) * RKV + REC;
+          head = *reinterpret_cast<const uint32_t*>(tail);
+          ent = *reinterpret_cast<const uint32_t*>(tail + 4 + 4 * min(lane & 15, NSLOT - 1));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(rempty + cw);
+          if ((head & 16u) && (int)(head >> 8) < c.pool.blocks)  // (requested here, looked at behind the decoding)
+            word = __ldg(c.pool.at + (size_t)(head >> 8) * 16 + (lane & 15));
+          decode_frag(r[0], A[0]);
+          decode_frag(r[1], A[1]);
+        } else {                                                // (a page that is not there: zeros)
+          if (lane == 0) mbar_arrive(rempty + cw);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if ((head[h] & 31u) == 0u) continue;
-              put_entries(tile + h * L::HALF, ent[h], lane < (int)min(head[h] & 15u, (uint32_t)NSLOT) && seen(ent[h]), lane);
-              if (head[h] & 16u) {
-                int blk = (int)(head[h] >> 8);
-                for (int hops = 0; blk >= 0 && blk < c.pool.blocks && hops < 4096; ++hops) {
-                  const uint32_t word = __ldg(c.pool.at + (size_t)blk * 16 + (lane & 15)), w0 = __shfl_sync(FULL, word, 0);
-                  __syncwarp();
-                  put_entries(tile + h * L::HALF, word, lane > 0 && lane <= (int)min(w0 & 0xFFu, (uint32_t)XSLOT) && seen(word), lane);
-                  blk = (int)(w0 >> 8) - 1;
-                }
-              }
+          for (int i = 0; i < 32; ++i) A[i >> 4][(i >> 2) & 3][i & 3] = 0u;
+        }
+        const int first = (w.first_tile + j) * KEYS + cw * PAGE;                  // position of the page's first token
+        const bool edge = kvi && (first < w.start || first + PAGE > w.len);
+        if (edge) {
+          const int pos = first + (lane >> 2);
+          const bool x0 = pos >= w.start && pos < w.len, x8 = pos + 8 >= w.start && pos + 8 < w.len;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) A[i >> 4][(i >> 2) & 3][i & 3] = ((i & 1) ? x8 : x0) ? A[i >> 4][(i >> 2) & 3][i & 3] : 0u;
+        }
+        // K's stage is free when the scores of tile j - 2 are, V's when its products are: see the commits of the MMA loop
+        const int e = kvi ? j - 1 : j - 2;
+        if (j > 1) ok = mbar_wait_look(b.empty + (e & 1), (uint32_t)(e >> 1) & 1u);
+        if (!ok) break;
+        uint8_t* const tile = smem + (kvi ? L::V : L::K) + s * L::TILE + cw * (PAGE * 128);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t to = smem_addr(tile + h * L::HALF + at_row);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) stmatrix_x4(to + (((2 * i + at_col) ^ (lane & 7)) << 4), A[h][i][0], A[h][i][1], A[h][i][2], A[h][i][3]);
+        }
+        if ((heads & 31u) != 0u) {                              // (the same in every lane)
+          __syncwarp();
+          auto seen = [&](uint32_t entry) {
+            const int pos = first + (int)((entry >> 6) & 15u);
+            return !edge || (pos >= w.start && pos < w.len);
+          };
+          put_entries(tile, ent, (lane & 15) < (int)min(head & 15u, (uint32_t)NSLOT), seen(ent), lane);
+          if (heads & 16u) {
+            int blk = (head & 16u) ? (int)(head >> 8) : -1;
+            for (int hops = 0; hops < 4096; ++hops) {
+              const bool more = blk >= 0 && blk < c.pool.blocks;
+              if (!__any_sync(FULL, more)) break;
+              const uint32_t w0 = __shfl_sync(FULL, word, 0, 16);
+              __syncwarp();                                       // (entries before these stand already)
+              put_entries(tile, word, more && (lane & 15) > 0 && (lane & 15) <= (int)min(w0 & 0xFFu, (uint32_t)XSLOT), seen(word), lane);
+              blk = more ? (int)(w0 >> 8) - 1 : -1;
+              if (blk >= 0 && blk < c.pool.blocks) word = __ldg(c.pool.at + (size_t)blk * 16 + (lane & 15));
             }
           }
         }
-        if (!ok) break;
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive((kvi ? b.vfull : b.kfull) + s);
       }
-      if ((j & 15) == 15) now = next;
     }
-    if (!ok) {
-      if (lane == 0) atomicExch(c.status, ERR_WAIT_EMPTY);
-      // copies in flight land before the CTA ends: the last fetch of either slot (its phases: two a tile)
-      for (int p = 0; p < 2; ++p) {
-        const int done = (asked - p + 1) / 2;                     // fetches into slot p
-        (void)mbar_wait(my_raw + p, (uint32_t)(done - 1) & 1u);
-      }
-    }
+    if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_EMPTY);
   } else {
     regs_down<R_MMA>();
     if (warp == W_MMA) {
@@ -340,7 +304,55 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
       __syncwarp();
       tc_fence_before();
     } else {
-      meet();                                                     // (behind regs_down: the softmax warps wait for those registers)
+      // -------------------------------------------------------------- producers: pages -> slots, a key tile's keys, then its values; warp f
+      // brings pages f, f + 3, f + 6 of the eight
+      const int f = warp - W_FETCH;
+      const uint8_t* const head_pages = a.kv + (size_t)w.h * PAGE_BYTES;
+      const size_t page_step = (size_t)a.H * PAGE_BYTES;
+      const int* const table = a.table + (long long)w.b * a.table_stride;
+      // lane l holds the entry of page l % 8 of the (l / 8)-th of four key tiles; -1 = there is no such page
+      auto entry = [&](int j) {
+        const int t = j + (lane >> 3), p = (w.first_tile + t) * TILE_PAGES + (lane & 7);
+        if (t >= tiles || p >= end_page) return -1;
+        const int e = __ldg(table + p);
+        return e < 0 ? 0 : (int)min((long long)e, a.nblocks - 1);
+      };
+      if (lane < 8 && lane % FETCHERS == f) {
+        mbar_init(raw + lane, 1);
+        mbar_init(rempty + lane, 1);
+        fence_barrier_init();
+      }
+      __syncwarp();
+      int now = entry(0), next = -1;
+      auto fetch = [&](int i, int kvi, int e) {                   // keys or values of page i of a tile
+        if (elect_one()) {
+          mbar_expect_tx(raw + i, e >= 0 ? (uint32_t)L::SLOT_BYTES : 0u);
+          if (e >= 0) bulk_g2s(smem + L::RAW + i * L::SLOT_BYTES, head_pages + e * page_step + kvi * L::SLOT_BYTES, L::SLOT_BYTES, raw + i, keep);
+        }
+        __syncwarp();
+      };
+      if (tiles > 0)
+        for (int i = f; i < 8; i += FETCHERS) fetch(i, 0, __shfl_sync(FULL, now, i));
+      meet();
+      bool ok = true;
+      for (int j = 0; ok && j < tiles; ++j) {
+        if ((j & 3) == 0) next = entry(j + 4);
+#pragma unroll 1
+        for (int kvi = j == 0; ok && kvi < 2; ++kvi) {
+          const int n = 2 * j + kvi;                              // fetches into every slot before this round
+          int i = f;
+          for (; i < 8; i += FETCHERS) {
+            ok = mbar_wait_look(rempty + i, (uint32_t)(n - 1) & 1u);
+            if (!ok) break;
+            fetch(i, kvi, __shfl_sync(FULL, now, 8 * (j & 3) + i));
+          }
+          if (!ok) {                                              // copies in flight land before the CTA ends: the last of every slot
+            if (lane == 0) atomicExch(c.status, ERR_WAIT_EMPTY);
+            for (int k = f; k < 8; k += FETCHERS) (void)mbar_wait(raw + k, (uint32_t)(k < i ? n : n - 1) & 1u);
+          }
+        }
+        if ((j & 3) == 3) now = next;
+      }
     }
   }
   __syncthreads();
