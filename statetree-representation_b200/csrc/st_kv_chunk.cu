@@ -45,20 +45,19 @@ struct LayX : Tiles<HD> {
   static constexpr int BYTES = SLOT + 16 + 1024;
 };
 
-// entries of a page's two units over their tile, half a warp for each unit: those that are listed (in the order of the lanes), in rows that
-// are wanted (`seen`).  They ascend unless a row has been appended again in place: then one after the other, so that the later entry of an
-// element stands
-__device__ __forceinline__ void put_entries(uint8_t* tile, uint32_t entry, bool listed, bool seen, int lane) {
-  const int row = (int)((entry >> 6) & 15u), col = (int)(entry & 63u), at = lane & 15;
+// A list of entries of a page's two units, half a warp for each unit, `listed` of them.  They ascend unless a row has been appended again in
+// place: does one not?
+__device__ __forceinline__ bool out_of_order(uint32_t entry, bool listed, int lane) {
+  const uint32_t key = listed ? entry & 1023u : 0u, before = __shfl_up_sync(FULL, key, 1, 16);
+  return __any_sync(FULL, listed && (lane & 15) > 0 && key <= before);
+}
+// the entries over the units' tile; `one_by_one`: so that the later entry of an element stands
+__device__ __forceinline__ void put_entries(uint8_t* tile, uint32_t entry, bool wanted, bool one_by_one, int lane) {
+  const int row = (int)((entry >> 6) & 15u), col = (int)(entry & 63u);
   uint16_t* const to = reinterpret_cast<uint16_t*>(tile + (lane >> 4) * LayX::HALF + row * 128 + ((((col >> 3) ^ (row & 7)) << 4) | (col & 7) * 2));
-  const uint32_t key = listed ? entry & 1023u : 1024u, before = __shfl_up_sync(FULL, key, 1, 16);
-  const bool live = listed && seen;
-  if (!__any_sync(FULL, listed && at > 0 && before != 1024u && key <= before)) {
-    if (live) *to = (uint16_t)(entry >> 16);
-    return;
-  }
-  for (int i = 0; i < 16; ++i) {
-    if (at == i && live) *to = (uint16_t)(entry >> 16);
+#pragma unroll 1
+  for (int i = one_by_one ? 0 : 15; i < 16; ++i) {
+    if (wanted && (!one_by_one || (lane & 15) == i)) *to = (uint16_t)(entry >> 16);
     __syncwarp();
   }
 }
@@ -222,12 +221,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
     bool ok = true;
     for (int j = 0; ok && j < tiles; ++j) {
       const int s = j & 1;
-#pragma unroll
+#pragma unroll 1                                                  // (twice the code costs more, in instruction fetches, than it saves)
       for (int kvi = 0; kvi < 2; ++kvi) {
         ok = mbar_wait_look(raw + cw, (uint32_t)kvi);            // (two phases a tile)
         if (!ok) break;
         const bool there = (w.first_tile + j) * TILE_PAGES + cw < end_page;
         uint32_t A[2][4][4], heads = 0u, head = 0u, ent = 0u, word = 0u;       // head, ent, word: of the lane's unit, lane / 16
+        bool listed = false, odd = false;
         if (there) {
           RecRegs r[2];
 #pragma unroll
@@ -240,6 +240,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
           ent = *reinterpret_cast<const uint32_t*>(tail + 4 + 4 * min(lane & 15, NSLOT - 1));
           __syncwarp();
           if (lane == 0) mbar_arrive(rempty + cw);
+          listed = (lane & 15) < (int)min(head & 15u, (uint32_t)NSLOT);
+          odd = out_of_order(ent, listed, lane);
           if ((head & 16u) && (int)(head >> 8) < c.pool.blocks)  // (requested here, looked at behind the decoding)
             word = __ldg(c.pool.at + (size_t)(head >> 8) * 16 + (lane & 15));
           decode_frag(r[0], A[0]);
@@ -270,22 +272,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
         }
         if ((heads & 31u) != 0u) {                              // (the same in every lane)
           __syncwarp();
-          auto seen = [&](uint32_t entry) {
-            const int pos = first + (int)((entry >> 6) & 15u);
-            return !edge || (pos >= w.start && pos < w.len);
-          };
-          put_entries(tile, ent, (lane & 15) < (int)min(head & 15u, (uint32_t)NSLOT), seen(ent), lane);
-          if (heads & 16u) {
-            int blk = (head & 16u) ? (int)(head >> 8) : -1;
-            for (int hops = 0; hops < 4096; ++hops) {
-              const bool more = blk >= 0 && blk < c.pool.blocks;
-              if (!__any_sync(FULL, more)) break;
-              const uint32_t w0 = __shfl_sync(FULL, word, 0, 16);
-              __syncwarp();                                       // (entries before these stand already)
-              put_entries(tile, word, more && (lane & 15) > 0 && (lane & 15) <= (int)min(w0 & 0xFFu, (uint32_t)XSLOT), seen(word), lane);
-              blk = more ? (int)(w0 >> 8) - 1 : -1;
-              if (blk >= 0 && blk < c.pool.blocks) word = __ldg(c.pool.at + (size_t)blk * 16 + (lane & 15));
-            }
+          int blk = (head & 16u) ? (int)(head >> 8) : -1;
+#pragma unroll 1
+          for (int hops = 0; hops < 4096; ++hops) {
+            const int pos = first + (int)((ent >> 6) & 15u);
+            put_entries(tile, ent, listed && (!edge || (pos >= w.start && pos < w.len)), odd, lane);
+            const bool more = blk >= 0 && blk < c.pool.blocks;
+            if ((heads & 16u) == 0u || !__any_sync(FULL, more)) break;
+            if (hops > 0 && more) word = __ldg(c.pool.at + (size_t)blk * 16 + (lane & 15));
+            const uint32_t w0 = __shfl_sync(FULL, word, 0, 16);
+            ent = word;
+            listed = more && (lane & 15) > 0 && (lane & 15) <= (int)min(w0 & 0xFFu, (uint32_t)XSLOT);
+            odd = out_of_order(ent, listed, lane);
+            blk = more ? (int)(w0 >> 8) - 1 : -1;
           }
         }
         fence_proxy_async();
@@ -632,9 +631,9 @@ extern "C" int st_kv_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq
     const bool two = T * G > 8 * B;
     const long long ctas = ctas_of(two ? 16 : 8);
     ST_REQUIRE(ctas < (1ll << 31), "%s: grid too large", who);
-    const bool wide = ctas <= 2ll * st::sm_count();
-    e = two ? (wide ? rows_launch<8, 2>(c, ctas, st_) : rows_launch<4, 2>(c, ctas, st_))
-            : (wide ? rows_launch<8, 1>(c, ctas, st_) : rows_launch<4, 1>(c, ctas, st_));
+    // (an SM holds sixteen warps of eight rows, as CTAs of four or two of eight, or twelve of sixteen rows: three CTAs of four, one of eight)
+    e = two ? (ctas <= st::sm_count() ? rows_launch<8, 2>(c, ctas, st_) : rows_launch<4, 2>(c, ctas, st_))
+            : (ctas <= 2ll * st::sm_count() ? rows_launch<8, 1>(c, ctas, st_) : rows_launch<4, 1>(c, ctas, st_));
   } else {
     static std::atomic<uint64_t> set{0};
     const long long ctas = ctas_of(2 * ROWS);
