@@ -96,13 +96,14 @@ struct Work : Rows8 {
   int h, split, pos0;                                             // position of query 0
   int lo0, first_tile, tiles, count0, count1;                     // key tiles of the split; of those, how many each row tile needs
 };
-// false: the CTA has no rows.  Later tiles of a sequence see more keys: they go first
+// false: the CTA has no rows.  Later tiles (of TILE rows) of a sequence see more keys: they go first
+template <int TILE>
 __device__ __forceinline__ bool chunk_work(const Attn8& a, int splits, int slots, int G, int lane, Work& w) {
   int x = blockIdx.x;
   w.split = x % splits;
   x /= splits;
   w.h = x % a.H;
-  if (!find_rows<2 * ROWS>(a, G, slots - 1 - x / a.H, lane, w)) return false;
+  if (!find_rows<TILE>(a, G, slots - 1 - x / a.H, lane, w)) return false;
   const int start = w.start;
   w.pos0 = w.len - w.n;
   const int first_pos = w.pos0 + w.row0 / G, last_pos = w.pos0 + (w.row0 + w.rows - 1) / G;

@@ -16,6 +16,7 @@ namespace st {
 constexpr int REC = 1552;          // bytes per weight record
 constexpr int RKV = 1600;          // bytes per KV record (record + header + 11 escape slots)
 constexpr int PAGE = 16;           // tokens per KV page
+constexpr int PAGE_BYTES = 4 * RKV;   // of one KV head: keys, then values, each a unit per half of the head
 constexpr int HD = 128;            // head dimension of the KV kernels
 constexpr int NSLOT = 11;          // in-record escape slots of a KV record
 constexpr int XSLOT = 15;          // escape slots of a pool extension block

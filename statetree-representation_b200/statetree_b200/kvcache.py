@@ -161,10 +161,8 @@ def chunk_splits(tokens, seqs, kv_heads, group, max_pages, sms=148):
     """How many CTAs share a sequence of the chunk attention over lossless pages, from what the host knows (st_kv_chunk.cu)"""
     seqs = max(1, seqs)
     rows = -(-tokens * group // seqs)                       # of a sequence, on the mean
-    if rows <= FEW_ROWS8:
-        units = seqs * kv_heads * -(-rows // 16)
-        return max(1, min(2 * sms // max(1, units), max_pages // 8, 64))
-    return max(1, min(sms // (kv_heads * seqs * -(-rows // 256)), max_pages // 16, 64))
+    ctas = kv_heads * seqs * -(-rows // (32 if rows <= 32 else 256))
+    return max(1, min(sms // max(1, ctas), max_pages // 16, 64))
 
 
 class PageStore8:
