@@ -21,11 +21,15 @@ namespace {
 using namespace st;
 
 constexpr int FEW = 32;                            // rows of a CTA of the narrow form, and per sequence (on the mean) up to which it is taken
-// Warps of kv_chunk_kernel: eight of softmax, eight converters (a page of a key tile each), one that issues the MMAs, three producers
-constexpr int W_MMA = W_CONV + TILE_PAGES, W_FETCH = W_MMA + 1, WARPS = W_MMA + 4, FETCHERS = WARPS - W_FETCH;
-// registers of a warpgroup: 640 threads start with 96 each; 2 x 160 + 2 x 64 + 32 = 5 x 96
-constexpr int R_START = 96, R_SOFTMAX = 160, R_CONV = 64, R_MMA = 32;
-static_assert(2 * R_SOFTMAX + 2 * R_CONV + R_MMA <= 5 * R_START, "what the warpgroups take up is what the block starts with");
+// Warps of kv_chunk_kernel: of softmax, of conversion (a page of a key tile each; NARROW: its keys or its values), one that issues the MMAs, three
+// producers.  Registers of a warpgroup: what they take up together is at most what the block starts with, a multiple of 8 a thread
+template <bool NARROW>
+struct Roles {
+  static constexpr int CONV = NARROW ? 4 : 8, CONVERTERS = NARROW ? 2 * TILE_PAGES : TILE_PAGES;
+  static constexpr int MMA = CONV + CONVERTERS, FETCH = MMA + 1, WARPS = MMA + 4, FETCHERS = WARPS - FETCH, GROUPS = WARPS / 4;
+  static constexpr int R_START = 65536 / (WARPS * 32) / 8 * 8, R_SOFTMAX = NARROW ? 112 : 160, R_CONV = NARROW ? 80 : 64, R_MMA = 32;
+  static_assert(CONV / 4 * R_SOFTMAX + CONVERTERS / 4 * R_CONV + R_MMA <= GROUPS * R_START, "more registers than there are");
+};
 struct Pool { const uint32_t* at; int blocks; };
 struct ChunkArgs { Attn8 a; Parts8 parts; Pool pool; int* status; int slots; };
 
@@ -182,9 +186,10 @@ __device__ __forceinline__ void narrow_store(const Attn8& a, const Parts8& parts
 }
 
 template <bool NARROW>
-__global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs c) {
+__global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs c) {
   constexpr int D = HD, COLS = NARROW ? 32 : KEYS, SETS = NARROW ? 2 : 1;
   using L = LayX;
+  using R = Roles<NARROW>;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   const ChunkBars b(reinterpret_cast<uint64_t*>(smem + L::BARS));
@@ -201,8 +206,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
   const int end_page = min((w.pos0 + w.n - 1) / PAGE + 1, a.table_width);
   const uint64_t keep = policy_evict_last();                      // other row tiles of the sequence read the same pages
 
-  if (warp == W_MMA) {
-    if (elect_one()) b.init(W_MMA - W_CONV);
+  if (warp == R::MMA) {
+    if (elect_one()) b.init(TILE_PAGES);
     __syncwarp();
     tmem_alloc<1>(slot_at, 512);
     tmem_relinquish<1>();
@@ -214,8 +219,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
     tc_fence_after();
   };
 
-  if (warp < W_CONV) {
-    regs_up<R_SOFTMAX>();
+  if (warp < R::CONV) {
+    if (R::R_SOFTMAX > R::R_START) regs_up<R::R_SOFTMAX>();
     // ---------------------------------------------------------------- softmax: this thread's row
     const int t = warp >> 2, count = t ? w.count1 : w.count0, my = w.row0 + (NARROW ? lane : t * ROWS + (warp & 3) * 32 + lane);
     const bool live = my < w.row0 + w.rows;
@@ -335,21 +340,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
     if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_ACC);
     // ---- out.  (a wait that ran out leaves the rows unwritten)
     if (NARROW) {
-      if (t == 0) narrow_store(a, c.parts, w, smem, warp, lane, ok, count, to, m, l);
+      narrow_store(a, c.parts, w, smem, warp, lane, ok, count, to, m, l);
     } else if (ok && any) {
       chunk_store<D>(a, c.parts, w, smem, t, warp, lane, live, token, hq, count, to, m, l);
     }
     tc_fence_before();
-  } else if (warp < W_MMA) {
-    regs_down<R_CONV>();
+  } else if (warp < R::MMA) {
+    if (R::R_CONV < R::R_START) regs_down<R::R_CONV>();
     // ---------------------------------------------------------------- converters: records -> operand tiles
-    const int cw = warp - W_CONV;
+    const int cw = (warp - R::CONV) % TILE_PAGES, only = (warp - R::CONV) / TILE_PAGES;
     meet();
     bool ok = true;
     for (int j = 0; ok && j < tiles; ++j) {
       const int s = j & 1;
 #pragma unroll 1                                                  // (twice the code costs more, in instruction fetches, than it saves)
-      for (int kvi = 0; kvi < 2; ++kvi) {
+      for (int kvi = NARROW ? only : 0; kvi < (NARROW ? only + 1 : 2); ++kvi) {
         const int n = 2 * j + kvi, set = n % SETS;                // the n-th fetch of this page's
         ok = mbar_wait_look(raw + 8 * set + cw, (uint32_t)(n / SETS) & 1u);
         if (!ok) break;
@@ -386,8 +391,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
     }
     if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_EMPTY);
   } else {
-    regs_down<R_MMA>();
-    if (warp == W_MMA) {
+    regs_down<R::R_MMA>();
+    if (warp == R::MMA) {
       // -------------------------------------------------------------- MMAs.  V is read as it lies (dims contiguous: MN-major)
       meet();
       if (elect_one())
@@ -397,7 +402,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
     } else {
       // -------------------------------------------------------------- producers: pages -> slots, a key tile's keys, then its values; warp f
       // brings pages f, f + 3, f + 6 of the eight
-      const int f = warp - W_FETCH;
+      const int f = warp - R::FETCH, FETCHERS = R::FETCHERS;
       const uint8_t* const head_pages = a.kv + (size_t)w.h * PAGE_BYTES;
       const size_t page_step = (size_t)a.H * PAGE_BYTES;
       const int* const table = a.table + (long long)w.b * a.table_stride;
@@ -450,19 +455,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_chunk_kernel(const ChunkArgs
     }
   }
   __syncthreads();
-  if (warp == W_MMA) {
+  if (warp == R::MMA) {
     tc_fence_after();
     tmem_dealloc<1>(*slot_at, 512);
   }
 }
 
 template <typename Kernel>
-int opt_in(Kernel* kernel, int bytes, std::atomic<uint64_t>& set) {
+int opt_in(Kernel* kernel, int bytes, int regs, std::atomic<uint64_t>& set) {
   int dev = 0;                                                    // (set: devices whose limit has been raised)
   if (int e = st::cuda_fail(cudaGetDevice(&dev), "st_kv_chunk_attn: device")) return e;
   if (dev <= 63 && (set.load() >> dev & 1)) return 0;
   if (int e = st::cuda_fail(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "st_kv_chunk_attn: shared memory attribute"))
     return e;
+  cudaFuncAttributes has;                                         // (with fewer registers a warpgroup would wait for its share for good)
+  if (int e = st::cuda_fail(cudaFuncGetAttributes(&has, kernel), "st_kv_chunk_attn: attributes")) return e;
+  ST_REQUIRE(has.numRegs == regs, "st_kv_chunk_attn: compiled to %d registers, not %d", has.numRegs, regs);
   if (dev <= 63) set.fetch_or(1ull << dev);
   return 0;
 }
@@ -471,8 +479,8 @@ int chunk_launch(ChunkArgs& c, long long ctas, cudaStream_t st_) {
   static std::atomic<uint64_t> set{0};
   ST_REQUIRE(ctas < (1ll << 31), "st_kv_chunk_attn: grid too large");
   c.slots = (int)(ctas / c.a.H / c.parts.splits);
-  if (int e = opt_in(kv_chunk_kernel<NARROW>, LayX::BYTES, set)) return e;
-  return st::launch("st_kv_chunk_attn launch", kv_chunk_kernel<NARROW>, dim3((unsigned)ctas), dim3(WARPS * 32), (size_t)LayX::BYTES, st_, c);
+  if (int e = opt_in(kv_chunk_kernel<NARROW>, LayX::BYTES, Roles<NARROW>::R_START, set)) return e;
+  return st::launch("st_kv_chunk_attn launch", kv_chunk_kernel<NARROW>, dim3((unsigned)ctas), dim3(Roles<NARROW>::WARPS * 32), (size_t)LayX::BYTES, st_, c);
 }
 }  // namespace
 
