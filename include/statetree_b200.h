@@ -300,6 +300,16 @@ int st_rope_kv_append(const void* qkv, int64_t row_stride, const void* wq, const
                       int64_t hkv, double eps, const int64_t* slot, void* kv, int64_t nblocks, uint32_t* pool, int64_t P,
                       int32_t* pool_cnt, void* stream);
 
+/* Products with an epilogue: Y [B, M] BF16 = act(X W^T + bias) + res, from the fp32 sums, rounded once.  act: 0 none, 1 ReLU, 2 SiLU, 3 GELU,
+ * 4 GELU by tanh, 5 SwiGLU: W's M rows are gate and up in 16-row tiles in turn (as for st_gemv_swiglu; bias too) and Y is [B, M / 2], silu(gate)
+ * * up.  bias BF16 [M] or NULL; res BF16 of Y's shape, rows res_stride apart (8-byte aligned, a multiple of 4), or NULL, may be Y.  Y must not
+ * overlap X.  st_gemv_epilogue: 1 <= B <= 32, workspace as for st_gemv, SwiGLU where st_gemv_swiglu_supported says so; st_gemm_epilogue:
+ * any B, M a multiple of 16 (SwiGLU: of 32), no workspace.  No counterpart in the reference (its linears add the bias in a step of its own). */
+int st_gemv_epilogue(const void* tree, const int32_t* eo, const uint32_t* eb, const uint32_t* el, const void* X, void* Y, const void* bias,
+                     int act, const void* res, int64_t res_stride, int64_t B, int64_t M, int64_t N, void* ws, int64_t ws_bytes, void* stream);
+int st_gemm_epilogue(const void* tree, const int32_t* eo, const uint32_t* el, const void* X, void* Y, const void* bias, int act,
+                     const void* res, int64_t res_stride, int64_t B, int64_t M, int64_t N, void* stream);
+
 /* Causal attention of several query tokens per sequence over the lossless pages, whose keys and values have been appended already
  * (st_kv_append): q, out BF16 [T, Hq, 128] (16-byte aligned, token strides qs / os multiples of 8); cu int32 [B + 1]: sequence b's queries
  * are rows cu[b] .. cu[b + 1] - 1, the last at position lens[b] - 1 (cu NULL: one each).  A query at position p sees keys

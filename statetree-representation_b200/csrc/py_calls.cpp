@@ -45,6 +45,8 @@ struct Library {
   decltype(&st_kv8_attn_workspace_bytes) kv8_workspace;
   decltype(&st_rotate) rotate;
   decltype(&st_kv_chunk_attn) kv_chunk;
+  decltype(&st_gemv_epilogue) gemv_epilogue;
+  decltype(&st_gemm_epilogue) gemm_epilogue;
 };
 
 // rows of x if it can be read as it is: BF16 [..., N] on `device`, contiguous, 16-byte aligned, at least one row; else 0
@@ -93,6 +95,8 @@ Library library(const std::map<std::string, uint64_t>& address) {
   bind(lib.kv8_workspace, "st_kv8_attn_workspace_bytes");
   bind(lib.rotate, "st_rotate");
   bind(lib.kv_chunk, "st_kv_chunk_attn");
+  bind(lib.gemv_epilogue, "st_gemv_epilogue");
+  bind(lib.gemm_epilogue, "st_gemm_epilogue");
   return lib;
 }
 
@@ -360,6 +364,31 @@ py::object kv8_dense(const Library& lib, const at::Tensor& pages, const at::Tens
   return py::make_tuple(K, V);
 }
 
+// ---- act(x W^T + bias) + residual for one tree; the residual contiguous.  ws: the GEMV's
+py::object fused(const Library& lib, bool use_gemm, const at::Tensor& tree, const at::Tensor& eo, const at::Tensor& el, const at::Tensor& eb,
+                 const at::Tensor& x, const at::Tensor& ws, const Maybe& bias, int act, const Maybe& residual) {
+  const int64_t M = tree.size(0) * 16, N = tree.size(1) * 64, B = plain_rows(x, N, tree.device()), width = act == 5 ? M / 2 : M;
+  const at::Device device = tree.device();
+  if (B == 0 || !on(device, eo, el, eb) || (bias && (!flat(*bias, at::kBFloat16, device) || bias->numel() != M)) ||
+      (residual && (plain_rows(*residual, width, device) != B || residual->dim() != x.dim())))
+    return py::none();
+  at::Tensor y;
+  int rc;
+  {
+    py::gil_scoped_release nogil;
+    const c10::cuda::CUDAGuard guard(device);
+    y = at::empty(out_sizes(x, width), x.options().requires_grad(false));
+    void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    rc = use_gemm ? lib.gemm_epilogue(tree.const_data_ptr(), of<int32_t>(eo), of<uint32_t>(el), x.const_data_ptr(), y.data_ptr(), of<void>(bias), act,
+                                      of<void>(residual), width, B, M, N, stream)
+                  : lib.gemv_epilogue(tree.const_data_ptr(), of<int32_t>(eo), of<uint32_t>(eb), of<uint32_t>(el), x.const_data_ptr(), y.data_ptr(),
+                                      of<void>(bias), act, of<void>(residual), width, B, M, N, ws.data_ptr(),
+                                      ws.numel() * (int64_t)ws.element_size(), stream);
+  }
+  check(lib, rc);
+  return py::cast(y);
+}
+
 // ---- lossless KV pages: attention of cu's rows (None: one query per sequence), pages uint8 [blocks, H, 2, 2, 1600], pool int32 [P, 16]
 py::object kv_chunk_attention(const Library& lib, const at::Tensor& pages, const at::Tensor& pool, const at::Tensor& q, const Maybe& cu,
                               const at::Tensor& table, const at::Tensor& lens, double scale, int64_t splits, const Maybe& starts,
@@ -445,5 +474,6 @@ PYBIND11_MODULE(_calls, m) {
   m.def("kv8_attention", &kv8_attention);
   m.def("kv8_dense", &kv8_dense);
   m.def("rotate", &rotate);
+  m.def("fused", &fused);
   m.def("kv_chunk_attention", &kv_chunk_attention);
 }

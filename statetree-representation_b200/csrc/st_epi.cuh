@@ -1,0 +1,105 @@
+// The epilogue of a product y = act(x W^T + bias) + residual, applied to fp32 sums before the one rounding to BF16.  Shared by the GEMV
+// (st_gemv.cu) and the two tcgen05 kernels (st_gemm.cu, st_gemm_pair.cu), whose plain forms are compiled without it.
+//   EPI_SWIGLU: W's rows are gate and up in 16-row tiles in turn; row j of the result is silu(gate_j) * up_j
+#pragma once
+#include "st_common.cuh"
+
+namespace st {
+constexpr int EPI_NONE = 0, EPI_RELU = 1, EPI_SILU = 2, EPI_GELU = 3, EPI_GELU_TANH = 4, EPI_SWIGLU = 5;
+
+struct Epi {
+  const uint16_t* bias;                            // BF16 [M] or nullptr
+  const uint16_t* res; long long res_stride;       // BF16 [B][M, swiglu: M / 2] or nullptr; may be the output
+  int act;
+  long long rows;                                  // of the result (its row stride): M, or M / 2
+};
+
+// st_gemm.cu, st_gemv.cu: what both entry points check
+int epi_args(Epi& e, const char* who, const void* bias, int act, const void* res, int64_t res_stride, int64_t M);
+
+#ifdef __CUDACC__
+// (__expf: relative error below 2^-21 where it matters here, under the rounding to BF16; beyond its range the quotients go to 0 or z)
+__device__ __forceinline__ float epi_silu(float z) { return z / (1.f + __expf(-z)); }
+__device__ __forceinline__ float epi_act(int act, float z) {
+  switch (act) {                                   // (the same for the whole launch)
+    case EPI_RELU: return z < 0.f ? 0.f : z;
+    case EPI_SILU: return epi_silu(z);
+    case EPI_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case EPI_GELU_TANH: return z / (1.f + __expf(-1.5957691216057308f * z * __fmaf_rn(0.044715f * z, z, 1.f)));      // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
+  }
+  return z;
+}
+__device__ __forceinline__ float epi_value(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ uint16_t epi_round(float v) {
+  const __nv_bfloat16 h = __float2bfloat16_rn(v);
+  return *reinterpret_cast<const uint16_t*>(&h);
+}
+
+// Sixteen token columns of a warp's 32 rows, lane = row, as tensor memory hands them out.  `left` of the columns exist, `valid` of the rows
+// (a multiple of 16); y, res: this warp's first result row of the first column, columns `rows` / `res_stride` values apart.  Lanes pair up,
+// even ones on column c and odd on c + 1 with two rows each, so that a store writes 4 bytes a lane, 64 a column; under EPI_SWIGLU lane l
+// and l + 16 (gate and up of a row) pair up the same way.  The residual's words are requested before the first store (they may be the same memory), from L2:
+// the threads here have not waited for the kernel before themselves, so that a line of theirs in L1 may be older than its writes.
+__device__ __forceinline__ void epi_store16(const Epi& e, const uint32_t (&v)[16], float bias, int left, int valid, uint16_t* y, const uint16_t* res) {
+  const int lane = threadIdx.x & 31;
+  if (e.act == EPI_SWIGLU) {
+    const int hi = lane >> 4, row = lane & 15;
+    uint16_t r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = res && valid == 32 && 2 * j + hi < left ? __ldcg(res + (size_t)(2 * j + hi) * e.res_stride + row) : (uint16_t)0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float z0 = __uint_as_float(v[2 * j]) + bias, z1 = __uint_as_float(v[2 * j + 1]) + bias;
+      const float got = __shfl_xor_sync(FULL, hi ? z0 : z1, 16);
+      const float x = epi_silu(hi ? got : z0) * (hi ? z1 : got) + epi_value(r[j]);
+      if (valid == 32 && 2 * j + hi < left) y[(size_t)(2 * j + hi) * e.rows + row] = epi_round(x);
+    }
+    return;
+  }
+  const int odd = lane & 1, row = lane & ~1;
+  uint32_t r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    r[j] = res && row < valid && 2 * j + odd < left ? __ldcg(reinterpret_cast<const uint32_t*>(res + (size_t)(2 * j + odd) * e.res_stride + row)) : 0u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float z0 = epi_act(e.act, __uint_as_float(v[2 * j]) + bias), z1 = epi_act(e.act, __uint_as_float(v[2 * j + 1]) + bias);
+    const float got = __shfl_xor_sync(FULL, odd ? z0 : z1, 1);
+    const float x0 = (odd ? got : z0) + __uint_as_float(r[j] << 16), x1 = (odd ? z1 : got) + __uint_as_float(r[j] & 0xFFFF0000u);
+    if (row < valid && 2 * j + odd < left) *reinterpret_cast<uint32_t*>(y + (size_t)(2 * j + odd) * e.rows + row) = pack_bf16(x0, x1);
+  }
+}
+
+// Four rows 4 lane .. 4 lane + 3 of a 128-row block in one token column (a warp a column).  bias: of these rows; y, res: the block's first
+// result row of the column; valid: rows of the block that exist.  `word`: epi_fetch4's
+__device__ __forceinline__ uint2 epi_fetch4(const Epi& e, int valid, const uint16_t* res) {
+  const int lane = threadIdx.x & 31;
+  if (!res || 4 * lane >= valid) return make_uint2(0u, 0u);
+  return __ldcg(reinterpret_cast<const uint2*>(res + (e.act == EPI_SWIGLU ? (lane >> 3) * 16 + (lane & 3) * 4 : 4 * lane)));
+}
+__device__ __forceinline__ void epi_store4(const Epi& e, float4 z, const float (&bias)[4], int valid, uint16_t* y, uint2 word) {
+  const int lane = threadIdx.x & 31;
+  z.x += bias[0]; z.y += bias[1]; z.z += bias[2]; z.w += bias[3];
+  int at = 4 * lane;
+  bool mine = at < valid;
+  if (e.act == EPI_SWIGLU) {                       // lane ^ 4 holds the same rows of the other projection
+    float4 up;
+    up.x = __shfl_xor_sync(FULL, z.x, 4); up.y = __shfl_xor_sync(FULL, z.y, 4); up.z = __shfl_xor_sync(FULL, z.z, 4); up.w = __shfl_xor_sync(FULL, z.w, 4);
+    z.x = epi_silu(z.x) * up.x; z.y = epi_silu(z.y) * up.y; z.z = epi_silu(z.z) * up.z; z.w = epi_silu(z.w) * up.w;
+    mine = mine && !(lane & 4);
+    at = (lane >> 3) * 16 + (lane & 3) * 4;
+  } else {
+    z.x = epi_act(e.act, z.x); z.y = epi_act(e.act, z.y); z.z = epi_act(e.act, z.z); z.w = epi_act(e.act, z.w);
+  }
+  if (!mine) return;
+  *reinterpret_cast<uint2*>(y + at) = make_uint2(pack_bf16(z.x + __uint_as_float(word.x << 16), z.y + __uint_as_float(word.x & 0xFFFF0000u)),
+                                                 pack_bf16(z.z + __uint_as_float(word.y << 16), z.w + __uint_as_float(word.y & 0xFFFF0000u)));
+}
+__device__ __forceinline__ void epi_bias4(const Epi& e, long long row0, int valid, float (&bias)[4]) {
+  const int lane = threadIdx.x & 31;
+  const bool has = e.bias && 4 * lane < valid;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) bias[k] = has ? epi_value(__ldg(e.bias + row0 + 4 * lane + k)) : 0.f;
+}
+#endif
+}  // namespace st

@@ -66,7 +66,7 @@ template <int DG> constexpr int gemm_threads() { return (DG * NDEC + 3) * 32; }
 // the rank).  After its main loop every CTA parks its fp32 accumulator tile in its own shared memory; after a cluster
 // barrier CTA j adds the KS tiles for its share of the token columns through distributed shared memory, in rank
 // order (bit-identical from run to run), and stores BF16.  No partial sums travel through global memory.
-template <int DG, bool GROUPED>
+template <int DG, bool GROUPED, bool EPI>
 __global__ void __launch_bounds__(gemm_threads<DG>(), DG == 1 ? 2 : 1)
 gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ WMaps wmaps) {
   constexpr int NDW = DG * NDEC;                                              // decode warps
@@ -239,7 +239,8 @@ gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
     const uint32_t my_a = tmem_a + ((uint32_t)(rec * 16) << 16);
     const uint8_t* const my_raw = rawring + rec * (PAIR * REC);
     const int* const my_eo = eo + (size_t)(lrb * 8 + rec) * a.NG + k0;
-    const int last = a.NG - k0;                                    // records of this row tile from k0 on
+    // records of this row tile from k0 on (EPI: none of a row tile beyond the matrix, which the map fills with zeros)
+    const int last = !EPI || (lrb * 8 + rec) * 16 < a.M ? a.NG - k0 : 0;
     // The two records of a pair are neighbours in memory order, so their escapes are one run of the list.  It is fetched
     // one pair ahead: the list offsets come 32 pairs at a time (lane l holds those of pair eo_base + l) and the first 32
     // entries of the next pair are requested before this pair is decoded, so no global-load latency sits between the
@@ -328,12 +329,20 @@ gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
     tc_fence_after();
     const int q4 = warp & 3, cg = warp >> 2;                     // TMEM lane quadrant, column share of the warp
     float* stg = reinterpret_cast<float*>(smem);                 // [NT][128] fp32, over the (now idle) rings
+    // EPI: rows of this warp's 32 that exist, its row's bias
+    const int row0 = lrb * 128 + q4 * 32, valid = EPI ? (int)min(32ll, max(0ll, a.M - row0)) : 32;
+    const float bias = EPI && a.epi.bias && lane < valid ? epi_value(__ldg(a.epi.bias + row0 + lane)) : 0.f;
     for (int c0 = cg * 16; c0 < nmma; c0 += (NDW / 4) * 16) {
       uint32_t v[16];
       tmem_ld16(tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)c0, v);
       if (!GROUPED && a.KS > 1) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) stg[(size_t)(c0 + j) * 128 + q4 * 32 + lane] = __uint_as_float(v[j]);
+      } else if (EPI) {
+        const size_t tok = (size_t)(tok0 + c0);
+        const int out0 = a.epi.act == EPI_SWIGLU ? row0 >> 1 : row0;
+        epi_store16(a.epi, v, bias, acc_ok ? ncol - c0 : 0, valid, Yp + tok * a.epi.rows + out0,
+                    a.epi.res ? a.epi.res + tok * a.epi.res_stride + out0 : nullptr);
       } else {
         // whole k range: this lane holds row q4 * 32 + lane of 16 token columns.  Lanes pair up (even: column j, odd:
         // column j + 1, two rows each) so that a store instruction writes 4 bytes per lane, 64 bytes per column
@@ -366,6 +375,9 @@ gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
       // -------------------------------------------------------------- epilogue 2: add the KS tiles, rank order
       const int c_lo = (int)((long long)ncol * ks / a.KS), c_end = (int)((long long)ncol * (ks + 1) / a.KS);
       const uint32_t mine = smem_addr(smem);
+      const int valid = EPI ? (int)min(128ll, a.M - (long long)lrb * 128) : 128, out0 = EPI && a.epi.act == EPI_SWIGLU ? lrb * 64 : lrb * 128;
+      float bias[4] = {0.f, 0.f, 0.f, 0.f};
+      if (EPI) epi_bias4(a.epi, (long long)lrb * 128, valid, bias);
       // CPP columns per pass, every partial tile's float4 requested before the first add: distributed-shared-memory
       // reads have a long latency, so the loads of a pass must all be in flight together
       constexpr int CPP = DG;                                    // (DG = 2 has up to twice the columns; DG = 1 takes 63 registers of the 88 it may)
@@ -377,6 +389,12 @@ gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
           for (int p = 0; p < 8; ++p)
             if (p < a.KS && c + h * NDW < c_end)
               v[h][p] = ld_cluster_f4(map_to_cta(mine + (uint32_t)(((c + h * NDW) * 128 + 4 * lane) * 4), (uint32_t)p));
+        uint2 word[CPP];
+        if (EPI)
+#pragma unroll
+          for (int h = 0; h < CPP; ++h)
+            word[h] = a.epi.res && c + h * NDW < c_end ? epi_fetch4(a.epi, valid, a.epi.res + (size_t)(tok0 + c + h * NDW) * a.epi.res_stride + out0)
+                                                       : make_uint2(0u, 0u);
 #pragma unroll
         for (int h = 0; h < CPP; ++h) {
           const int cc = c + h * NDW;
@@ -385,6 +403,10 @@ gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
 #pragma unroll
           for (int p = 0; p < 8; ++p)
             if (p < a.KS) { sum.x += v[h][p].x; sum.y += v[h][p].y; sum.z += v[h][p].z; sum.w += v[h][p].w; }
+          if (EPI) {
+            epi_store4(a.epi, sum, bias, valid, Yp + (size_t)(tok0 + cc) * a.epi.rows + out0, word[h]);
+            continue;
+          }
           const size_t o = (size_t)(tok0 + cc) * Mp + lrb * 128 + 4 * lane;
           uint2 packed;
           packed.x = pack_bf16(sum.x, sum.y);
@@ -427,13 +449,13 @@ struct GemmPlan {
   size_t smem;
 };
 
-template <int DG, bool GROUPED>
+template <int DG, bool GROUPED, bool EPI = false>
 int gemm_attr() {                                                // once per device: opt in to the large dynamic shared memory
   static bool set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !set[dev]) {
-    if (int e = st::cuda_fail(cudaFuncSetAttribute(gemm_kernel<DG, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (int e = st::cuda_fail(cudaFuncSetAttribute(gemm_kernel<DG, GROUPED, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    DG == 1 ? 113 * 1024 : 220 * 1024), "st_gemm: shared memory attribute"))
       return e;
     set[dev] = true;
@@ -465,7 +487,7 @@ long long resident_ctas(int ks, size_t smem, int sms) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (gemm_attr<DG, false>() != 0 || cudaOccupancyMaxActiveClusters(&n, gemm_kernel<DG, false>, &cfg) != cudaSuccess || n <= 0) {
+    if (gemm_attr<DG, false>() != 0 || cudaOccupancyMaxActiveClusters(&n, gemm_kernel<DG, false, false>, &cfg) != cudaSuccess || n <= 0) {
       (void)cudaGetLastError();
       n = sms / ks;                                              // no answer (no device): assume perfect packing
     }
@@ -571,9 +593,9 @@ GemmPlan gemm_plan(long long M, int NG, long long B, double& us) {
   return p;
 }
 
-template <int DG, bool GROUPED>
+template <int DG, bool GROUPED, bool EPI = false>
 int gemm_launch(const GemmPlan& p, const GemmArgs& a, const CUtensorMap& xmap, const WMaps& wmaps, cudaStream_t stream) {
-  if (int e = gemm_attr<DG, GROUPED>()) return e;
+  if (int e = gemm_attr<DG, GROUPED, EPI>()) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.RB * p.TT * p.KS));
   cfg.blockDim = dim3(gemm_threads<DG>());
@@ -588,7 +610,7 @@ int gemm_launch(const GemmPlan& p, const GemmArgs& a, const CUtensorMap& xmap, c
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = st::pdl_enabled() ? 2 : 1;
-  return st::cuda_fail(cudaLaunchKernelEx(&cfg, gemm_kernel<DG, GROUPED>, a, xmap, wmaps),
+  return st::cuda_fail(cudaLaunchKernelEx(&cfg, gemm_kernel<DG, GROUPED, EPI>, a, xmap, wmaps),
                        GROUPED ? "st_moe_group_gemm launch" : "st_gemm launch");
 }
 void plan_args(GemmArgs& a, const GemmPlan& p) {
@@ -600,7 +622,7 @@ void plan_args(GemmArgs& a, const GemmPlan& p) {
 int dense_gemm(GemmArgs& a, const WMaps& wmaps, const void* X, const char* who, cudaStream_t stream) {
   ST_REQUIRE(a.M / 128 * 8 * ((a.B + NT_MAX - 1) / NT_MAX) < (1ll << 31), "%s: grid too large", who);
   double us;
-  const GemmPlan plan = gemm_plan(a.M, a.NG, a.B, us);
+  const GemmPlan plan = gemm_plan((a.M + 127) / 128 * 128, a.NG, a.B, us);      // (an epilogue's last row block may be part-filled)
   // More than 128 tokens: CTA pairs where they are expected to be the faster ones.  Measured, us, this kernel / CTA pairs:
   //   2048 x 2048   at 300 tokens 11.2 / 10.1, 321 11.1 / 12.7        4096 x 4096   at 300 17.5 / 20.2, 321 19.0 / 20.4
   //   4608 x 3584   at 321 18.2 / 22.3, 900 32.4 / 29.7               4096 x 12288  at 300 32.3 / 42.1
@@ -618,6 +640,7 @@ int dense_gemm(GemmArgs& a, const WMaps& wmaps, const void* X, const char* who, 
   GemmPlan p = plan;
   auto go = [&] {
     plan_args(a, p);
+    if (a.fused) return p.DG == 1 ? gemm_launch<1, false, true>(p, a, xmap, wmaps, stream) : gemm_launch<2, false, true>(p, a, xmap, wmaps, stream);
     return p.DG == 1 ? gemm_launch<1, false>(p, a, xmap, wmaps, stream) : gemm_launch<2, false>(p, a, xmap, wmaps, stream);
   };
   a.rb0 = 0;
@@ -686,6 +709,37 @@ extern "C" int st_gemm(const void* tree, const int32_t* eo, const uint32_t* el, 
   ST_REQUIRE(a.status != nullptr, "st_gemm: no device status word");
   a.M = M; a.B = (int)B; a.NG = (int)(N / 64);
   return dense_gemm(a, wmaps, X, "st_gemm", (cudaStream_t)stream);
+}
+
+// ---------------------------------------------------------------------------------------------- with an epilogue
+int st::epi_args(Epi& e, const char* who, const void* bias, int act, const void* res, int64_t res_stride, int64_t M) {
+  ST_REQUIRE(act >= EPI_NONE && act <= EPI_SWIGLU, "%s: activation 0 to 5 (got %d)", who, act);
+  ST_REQUIRE(act != EPI_SWIGLU || M % 32 == 0, "%s: SwiGLU needs M %% 32 == 0 (got %lld)", who, (long long)M);
+  e.rows = act == EPI_SWIGLU ? M / 2 : M;
+  ST_REQUIRE(!res || (res_stride >= e.rows && res_stride % 4 == 0 && ((uintptr_t)res & 7u) == 0),
+             "%s: residual rows must be 8-byte aligned and at least as long as the result's", who);
+  e.bias = (const uint16_t*)bias; e.res = (const uint16_t*)res; e.res_stride = res_stride; e.act = act;
+  return 0;
+}
+
+extern "C" int st_gemm_epilogue(const void* tree, const int32_t* eo, const uint32_t* el, const void* X, void* Y, const void* bias, int act,
+                                const void* res, int64_t res_stride, int64_t B, int64_t M, int64_t N, void* stream) {
+  const char* who = "st_gemm_epilogue";
+  ST_REQUIRE(M > 0 && N > 0 && M % 16 == 0 && N % 64 == 0 && M < (1ll << 31), "%s: M %% 16 and N %% 64 must be 0 (got %lld x %lld)", who, (long long)M,
+             (long long)N);
+  ST_REQUIRE(B >= 1 && B < (1ll << 24), "%s: batch out of range", who);
+  ST_REQUIRE(tree && eo && el && X && Y, "%s: null pointer", who);
+  ST_REQUIRE(st::aligned16(tree) && st::aligned16(X) && ((uintptr_t)Y & 7u) == 0, "%s: tree and X must be 16-byte aligned, Y 8-byte", who);
+  GemmArgs a = {};
+  if (int e = st::epi_args(a.epi, who, bias, act, res, res_stride, M)) return e;
+  WMaps wmaps;
+  memset(&wmaps, 0, sizeof(wmaps));
+  if (int e = make_wmap(&wmaps.m[0], tree, M, N, who)) return e;
+  a.eo = eo; a.el = el; a.Y = (uint16_t*)Y; a.fused = 1;
+  a.status = st::status_ptr();
+  ST_REQUIRE(a.status != nullptr, "%s: no device status word", who);
+  a.M = M; a.B = (int)B; a.NG = (int)(N / 64);
+  return dense_gemm(a, wmaps, X, who, (cudaStream_t)stream);
 }
 
 // ---------------------------------------------------------------------------------------------- list of matrices

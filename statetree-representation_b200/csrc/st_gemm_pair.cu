@@ -94,9 +94,28 @@ __device__ __forceinline__ void store_unit(uint32_t acc, int c0, int NT, int nco
   }
 }
 
+// The same with an epilogue: a chunk is read and finished at a time.  row0: this warp's first row of the matrix
+__device__ __forceinline__ void store_unit_epi(const GemmArgs& a, uint32_t acc, int c0, int NT, int ncol, int tok0, int row0, uint32_t accfree) {
+  const int lane = threadIdx.x & 31, valid = (int)min(32ll, max(0ll, a.M - row0)), out0 = a.epi.act == EPI_SWIGLU ? row0 >> 1 : row0;
+  const float bias = a.epi.bias && lane < valid ? epi_value(__ldg(a.epi.bias + row0 + lane)) : 0.f;
+#pragma unroll 1
+  for (; c0 < NT; c0 += CSTEP) {
+    uint32_t v[16];
+    tmem_ld16(acc + (uint32_t)c0, v);
+    if (c0 + CSTEP >= NT) {                                      // this warp has read its share: the next unit may accumulate
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(accfree);
+    }
+    const size_t tok = (size_t)(tok0 + c0);
+    epi_store16(a.epi, v, bias, ncol - c0, valid, a.Y + tok * a.epi.rows + out0, a.epi.res ? a.epi.res + tok * a.epi.res_stride + out0 : nullptr);
+  }
+}
+
 // *Slot parity.*  An mbarrier tells only its current phase from the previous one, so a waiter must never be two phases away.
 // The two decode groups alternate pairs of k-tiles, counted over all units of the cluster, so every A slot and record slot
 // belongs to one group (whose own program order guarantees that): both counts are even.
+template <bool EPI>
 __global__ void __launch_bounds__(THREADS, 1)
 pair_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ WMaps wmaps) {
   extern __shared__ uint8_t smem_raw[];
@@ -291,7 +310,8 @@ pair_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
       if (unit != e_unit) {
         const Rows rw = rows_of(unit);
         e_unit = unit;
-        e_live = rw.rb < a.RB;                                   // (beyond an odd number of row blocks: zero records)
+        // (beyond an odd number of row blocks, with an epilogue beyond the matrix's last row tile: zero records)
+        e_live = rw.rb < a.RB && (!EPI || (rw.lrb * 8 + rec) * 16 < a.M);
         el = a.nlist > 0 ? a.lel[rw.m] : a.el;
         my_eo = (a.nlist > 0 ? a.leo[rw.m] : a.eo) + (size_t)(rw.lrb * 8 + rec) * a.NG + k0;
         load_offsets(i);
@@ -328,6 +348,10 @@ pair_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
 #pragma unroll
           for (int j = 0; j < 16; ++j) stg[(size_t)(c0 + j) * 128 + q4 * 32 + lane] = __uint_as_float(v[j]);
         }
+        return true;
+      }
+      if (EPI) {
+        store_unit_epi(a, my_acc, cg * 16, NT, ncol, tok0, rw.lrb * 128 + q4 * 32, map_to_cta(smem_addr(accfree), first_rank));
         return true;
       }
       const size_t at = (size_t)tok0 * Mp + (size_t)rw.lrb * 128 + q4 * 32;
@@ -413,6 +437,10 @@ pair_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
       const int ncol = rw.rb < a.RB ? min(NT, a.B - tok0) : 0;
       const int c_lo = (int)((long long)ncol * ks / a.KS), c_end = (int)((long long)ncol * (ks + 1) / a.KS);
       const uint32_t mine = smem_addr(smem);
+      const int valid = EPI ? (int)min(128ll, max(0ll, a.M - (long long)rw.lrb * 128)) : 128;
+      const int out0 = EPI && a.epi.act == EPI_SWIGLU ? rw.lrb * 64 : rw.lrb * 128;
+      float bias[4] = {0.f, 0.f, 0.f, 0.f};
+      if (EPI) epi_bias4(a.epi, (long long)rw.lrb * 128, valid, bias);
       // CPP columns per pass, every partial tile's float4 requested before the first add: distributed-shared-memory reads
       // have a long latency, so the loads of a pass must all be in flight together
       constexpr int CPP = 4;
@@ -427,6 +455,12 @@ pair_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
               v[h][p] = p == ks ? *reinterpret_cast<const float4*>(smem + at)
                                 : ld_cluster_f4(map_to_cta(mine + at, (uint32_t)(2 * p + half)));
             }
+        uint2 word[CPP];
+        if (EPI)
+#pragma unroll
+          for (int h = 0; h < CPP; ++h)
+            word[h] = a.epi.res && c + h * NDW < c_end ? epi_fetch4(a.epi, valid, a.epi.res + (size_t)(tok0 + c + h * NDW) * a.epi.res_stride + out0)
+                                                       : make_uint2(0u, 0u);
 #pragma unroll
         for (int h = 0; h < CPP; ++h) {
           const int cc = c + h * NDW;
@@ -435,6 +469,10 @@ pair_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
 #pragma unroll
           for (int p = 1; p < 4; ++p)
             if (p < a.KS) { sum.x += v[h][p].x; sum.y += v[h][p].y; sum.z += v[h][p].z; sum.w += v[h][p].w; }
+          if (EPI) {
+            epi_store4(a.epi, sum, bias, valid, Yp + (size_t)(tok0 + cc) * a.epi.rows + out0, word[h]);
+            continue;
+          }
           const size_t o = (size_t)(tok0 + cc) * Mp + (size_t)rw.lrb * 128 + 4 * lane;
           uint2 packed;
           packed.x = pack_bf16(sum.x, sum.y);
@@ -454,12 +492,13 @@ pair_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
 }
 
 // ------------------------------------------------------------------------------------------------ host side
+template <bool EPI>
 int set_attr() {                                                 // once per device: opt in to the large dynamic shared memory
   static bool set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !set[dev]) {
-    if (int e = st::cuda_fail(cudaFuncSetAttribute(pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+    if (int e = st::cuda_fail(cudaFuncSetAttribute(pair_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
                               "st_gemm: shared memory attribute"))
       return e;
     set[dev] = true;
@@ -487,7 +526,7 @@ int resident_clusters(int ks, int sms) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (set_attr() != 0 || cudaOccupancyMaxActiveClusters(&n, pair_kernel, &cfg) != cudaSuccess || n <= 0) {
+    if (set_attr<false>() != 0 || cudaOccupancyMaxActiveClusters(&n, pair_kernel<false>, &cfg) != cudaSuccess || n <= 0) {
       (void)cudaGetLastError();
       n = sms / (2 * ks);                                        // no answer (no device): assume perfect packing
     }
@@ -617,19 +656,19 @@ int launch(const PairPlan& p, GemmArgs& a, int tile0, int tile1, int KS, const C
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = st::pdl_enabled() ? 2 : 1;
-  return st::cuda_fail(cudaLaunchKernelEx(&cfg, pair_kernel, a, xmap, wmaps), "st_gemm launch");
+  return st::cuda_fail(cudaLaunchKernelEx(&cfg, a.fused ? pair_kernel<true> : pair_kernel<false>, a, xmap, wmaps), "st_gemm launch");
 }
 }  // namespace
 
 int st::pair_gemm(GemmArgs& a, const WMaps& wmaps, const void* X, const char* who, double us, cudaStream_t stream) {
   double mine;
-  const PairPlan p = make_plan(a.M, a.NG, a.B, mine);
+  const PairPlan p = make_plan((a.M + 127) / 128 * 128, a.NG, a.B, mine);
   if (mine >= us) return -1;
   ST_REQUIRE((a.M / 256 + 1) * (long long)p.TT * 8 < (1ll << 31), "%s: grid too large", who);
-  if (int e = set_attr()) return e;
+  if (int e = a.fused ? set_attr<true>() : set_attr<false>()) return e;
   CUtensorMap xmap;
   if (int e = make_xmap(&xmap, X, a.B, (long long)a.NG * 64, p.box, who)) return e;
-  a.NT = p.NT; a.TT = p.TT; a.n1 = p.n1; a.box = p.box; a.RB = (int)(a.M / 128);
+  a.NT = p.NT; a.TT = p.TT; a.n1 = p.n1; a.box = p.box; a.RB = (int)((a.M + 127) / 128);
   a.astages = p.astages; a.xstages = p.xstages; a.rstages = p.rstages; a.bar_off = p.bar_off; a.tmem_cols = TMEM_COLS;
   const int units = (a.RB + 1) / 2 * p.TT;
   if (p.tile1 > 0)

@@ -32,6 +32,7 @@
 
 #include <mutex>
 
+#include "st_epi.cuh"
 #include "st_host.h"
 
 
@@ -42,10 +43,10 @@ constexpr int CW = 8;                     // consumer warps = records per unit
 constexpr int UNIT_BYTES = CW * REC;      // 12416
 constexpr int SIDE_BYTES = 64;            // escape block of a unit
 constexpr int XROW = CW * 128 + 16;       // bytes per staged activation row (512 columns + pad: conflict-free ldmatrix)
-constexpr int MODE_DENSE = 0, MODE_SLOT = 1, MODE_GROUP = 2, MODE_LIST = 3, MODE_AR = 4, MODE_NORM = 5;
+constexpr int MODE_DENSE = 0, MODE_SLOT = 1, MODE_GROUP = 2, MODE_LIST = 3, MODE_AR = 4, MODE_NORM = 5, MODE_EPI = 6;   // EPI: dense with an epilogue
 constexpr int FIN_CAP = 32;               // MODE_AR: tiles a CTA may have delivered and not yet summed over the ranks
 __host__ __device__ constexpr bool one_matrix(int mode) {
-  return mode == MODE_DENSE || mode == MODE_LIST || mode == MODE_AR || mode == MODE_NORM;
+  return mode == MODE_DENSE || mode == MODE_LIST || mode == MODE_AR || mode == MODE_NORM || mode == MODE_EPI;
 }
 constexpr int MAXL = 4;                   // matrices in one MODE_LIST launch
 constexpr uint32_t EMPTY_SLOT = 0xFFFFFFFFu;  // what every word of the workspace holds between launches
@@ -75,6 +76,7 @@ struct GemvArgs {
   int nprob, maxcover, stages, fill, stage_bytes, nxrows, xwhole, xw_stride, xw_bytes;
   int act;                                // dense mode: rows are gate / up tiles in turn, the reducer stores silu(gate) * up
   ListTab lt;
+  Epi epi;                                // MODE_EPI
   const uint16_t* delta; const uint16_t* nw; uint16_t* xout; float eps;   // MODE_NORM: X = RMSNorm(X + delta) * nw
   uint8_t* peer[MAX_RANKS];               // MODE_AR: communication buffer of every rank (peer[rank] is the own one)
   int rank, world;
@@ -452,6 +454,18 @@ __global__ void __launch_bounds__((CW + 2) * 32, NT <= 2 ? 2 : 1) gemv_kernel(co
     };
     for (; cur.valid(); cur.advance(a, cur.run_len(a))) {      // one hand-over per run of units of a tile
       const int buf = nf % NRED;
+      // MODE_EPI: the tile's bias and residual are on their way while its sums are being formed
+      float bias[EL / 32];
+      uint16_t resw[EL / 32];
+      if (MODE == MODE_EPI) {
+        const size_t row0 = (size_t)cur.tile * 16, out0 = a.act ? (size_t)(cur.tile >> 1) * 16 : row0;
+#pragma unroll
+        for (int k = 0; k < EL / 32; ++k) {
+          const int n = (lane + 32 * k) >> 4, r = (lane + 32 * k) & 15;
+          bias[k] = a.epi.bias ? epi_value(__ldg(a.epi.bias + row0 + r)) : 0.f;
+          resw[k] = a.epi.res && n < a.B ? __ldcg(a.epi.res + (size_t)n * a.epi.res_stride + out0 + r) : (uint16_t)0;
+        }
+      }
       if (!mbar_wait(done + buf, (uint32_t)(nf / NRED) & 1u)) {
         if (lane == 0) atomicExch(a.status, ERR_WAIT_FULL);
         return;
@@ -503,6 +517,7 @@ __global__ void __launch_bounds__((CW + 2) * 32, NT <= 2 ? 2 : 1) gemv_kernel(co
                 deliver(cur.tile, k, v);
               } else {
                 const int r = (lane + 32 * k) & 15;
+                if (MODE == MODE_EPI) v = epi_act(a.epi.act, v + bias[k]) + epi_value(resw[k]);
                 const __nv_bfloat16 hv = __float2bfloat16_rn(v);
                 Yp[orow[k] * Mp + row0 + r] = *reinterpret_cast<const uint16_t*>(&hv);
                 if (Yfp) Yfp[orow[k] * Mp + row0 + r] = v;
@@ -517,6 +532,14 @@ __global__ void __launch_bounds__((CW + 2) * 32, NT <= 2 ? 2 : 1) gemv_kernel(co
 #pragma unroll
         for (int k = 0; k < EL / 32; ++k)
           if (orow[k] >= 0) deliver(cur.tile, k, sum[k]);
+      } else if (MODE == MODE_EPI && a.act) {                   // SwiGLU as below, rounded once
+#pragma unroll
+        for (int k = 0; k < EL / 32; ++k) {
+          const float z = sum[k] + bias[k];
+          if ((cur.tile & 1) == 0) gate[k] = z;
+          else if (orow[k] >= 0)
+            a.Y[orow[k] * (a.M >> 1) + (size_t)(cur.tile >> 1) * 16 + ((lane + 32 * k) & 15)] = epi_round(epi_silu(gate[k]) * z + epi_value(resw[k]));
+        }
       } else if ((MODE == MODE_DENSE || MODE == MODE_NORM) && a.act) {
         // SwiGLU epilogue: tiles 2j and 2j + 1 hold rows 16j .. 16j + 15 of the gate and of the up projection; the host
         // only allows this when every CTA owns whole tiles in pairs, so the gate tile is always the one just before.
@@ -540,6 +563,7 @@ __global__ void __launch_bounds__((CW + 2) * 32, NT <= 2 ? 2 : 1) gemv_kernel(co
         for (int k = 0; k < EL / 32; ++k) {
           const int r = (lane + 32 * k) & 15;
           if (orow[k] >= 0) {
+            if (MODE == MODE_EPI) sum[k] = epi_act(a.epi.act, sum[k] + bias[k]) + epi_value(resw[k]);
             const __nv_bfloat16 hv = __float2bfloat16_rn(sum[k]);
             Yp[orow[k] * Mp + row0 + r] = *reinterpret_cast<const uint16_t*>(&hv);
             if (Yfp) Yfp[orow[k] * Mp + row0 + r] = sum[k];
@@ -976,6 +1000,25 @@ extern "C" int st_gemv(const void* tree, const int32_t* eo, const uint32_t* eb, 
                        void* Y, float* Yf32, int64_t B, int64_t M, int64_t N, void* ws, int64_t ws_bytes, int32_t* cnt,
                        void* stream) {
   return dense_gemv("st_gemv", tree, eo, eb, el, X, Y, Yf32, B, M, N, ws, ws_bytes, cnt, 0, (cudaStream_t)stream);
+}
+
+extern "C" int st_gemv_epilogue(const void* tree, const int32_t* eo, const uint32_t* eb, const uint32_t* el, const void* X, void* Y,
+                                const void* bias, int act, const void* res, int64_t res_stride, int64_t B, int64_t M, int64_t N, void* ws,
+                                int64_t ws_bytes, void* stream) {
+  const char* who = "st_gemv_epilogue";
+  if (int e = shape_checks(who, M, N, B)) return e;
+  ST_REQUIRE(tree && eo && eb && el && X && Y, "%s: null pointer", who);
+  ST_REQUIRE(st::aligned16(tree) && st::aligned16(eb) && st::aligned16(X), "%s: tree, eb and X must be 16-byte aligned", who);
+  ST_REQUIRE(act != EPI_SWIGLU || B <= 8, "%s: SwiGLU up to 8 rows", who);
+  GemvArgs a = {};
+  if (int e = st::epi_args(a.epi, who, bias, act, res, res_stride, M)) return e;
+  a.tree = (const uint8_t*)tree; a.eo = eo; a.eb = eb; a.el = el;
+  a.X = (const uint16_t*)X; a.Y = (uint16_t*)Y; a.ws = (float*)ws;
+  a.M = M; a.N = N; a.B = (int)B; a.E = 1; a.xdiv = 1; a.act = act == EPI_SWIGLU;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (B <= 8) return launch<1, MODE_EPI>(a, 1, (int)B, ws_bytes, s, who);
+  if (B <= 16) return launch<2, MODE_EPI>(a, 1, (int)B, ws_bytes, s, who);
+  return launch<4, MODE_EPI>(a, 1, (int)B, ws_bytes, s, who);
 }
 
 extern "C" int st_gemv_swiglu_supported(int64_t M, int64_t N, int64_t B) {

@@ -4,6 +4,7 @@
 #include <cuda.h>
 
 #include "st_common.cuh"
+#include "st_epi.cuh"
 #include "st_host.h"
 
 namespace st {
@@ -29,6 +30,7 @@ struct GemmArgs {
   int nlist; int rbend[MAXL_GEMM];            // first row block after each member in the concatenation
   const int* leo[MAXL_GEMM]; const uint32_t* lel[MAXL_GEMM]; uint16_t* lY[MAXL_GEMM]; float* lYf[MAXL_GEMM];
   long long lM[MAXL_GEMM];
+  int fused; Epi epi;                         // one matrix with an epilogue: a kernel of its own, whose last row block may be part-filled
 };
 struct WMaps { CUtensorMap m[MAXL_GEMM]; };   // weight tensor maps: one, or one per member of a list
 

@@ -17,7 +17,7 @@ import torch
 import torch.nn as nn
 
 from . import format as F
-from .ops import _raw_stream, built, calls, ext, on_device
+from .ops import _raw_stream, built, calls, ext, lib, on_device
 
 # activation rows up to which the GEMV kernel runs (<= 32).  The four projections of a 4096 / 12288 layer in a graph, us with
 # the GEMV / the tcgen05 GEMM: 8 rows 57 / 72, 16 rows 68 / 72, 20 rows 125 / 72 (beyond 16 the GEMV holds one CTA per SM)
@@ -81,6 +81,17 @@ class _DevState:
             if len(self._need) < 4096:
                 self._need[(M, N, B)] = need
         return self.get_ws(need)
+
+    def swiglu_gemv(self, M, N, B):
+        """does the GEMV take the shape with its SwiGLU epilogue (a grid of whole pairs of tiles)"""
+        key = ("swiglu", M, N, B)
+        known = self._need.get(key)
+        if known is None:
+            with on_device(self.device.index):
+                known = bool(lib().st_gemv_swiglu_supported(M, N, B))
+            if len(self._need) < 4096:
+                self._need[key] = known
+        return known
 
     def get_scratch(self, nbytes):
         if self.scratch.numel() * 4 < nbytes:
@@ -503,6 +514,75 @@ def swiglu(self, x):
 
 
 TreeLinear.swiglu = swiglu
+
+
+def _span(t):
+    """the addresses [first, last) between which a tensor's values lie"""
+    at = t.data_ptr()
+    return at, at + t.element_size() * (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0)
+
+
+def fused(self, x, activation=None, residual=None, out=None):
+    """activation(x W^T + bias) + residual in one launch, from the fp32 sums, rounded to BF16 once (forward rounds the product before it adds
+    the bias).  x as for forward: any leading shape (any number of rows), float type and device.  activation: None, "relu", "silu",
+    "gelu", "gelu_tanh", or "swiglu" for a layer built from interleave_gate_up(gate, up) (its bias in that order too): silu(gate) * up, half
+    as many columns.  residual: BF16 of the result's shape, on the layer's device.  out: a contiguous BF16 result, which may be the residual
+    itself (the residual stream is then added to in place), else apart from x and residual.  Inference only: no gradients, as forward."""
+    home, M, N = self._buffers["tree"].device, self.out_features, self.in_features
+    if activation not in ext().ACTIVATIONS:
+        raise ValueError(f"TreeLinear.fused: activation {activation!r}; there are {', '.join(map(repr, ext().ACTIVATIONS))}")
+    act, width = ext().ACTIVATIONS[activation], M // 2 if activation == "swiglu" else M
+    if activation == "swiglu" and M % 32:
+        raise ValueError(f"TreeLinear.fused: swiglu needs pairs of 16-row tiles, the layer has {M} rows")
+    if home.type != "cuda":
+        raise RuntimeError("statetree_b200: the kernels take CUDA tensors only (no CPU path); move the layer to a GPU")
+    if not x.shape or x.shape[-1] != N:
+        raise RuntimeError(f"statetree_b200: the layer takes inputs of {N} columns, got {tuple(x.shape)}")
+    shape, B = (*x.shape[:-1], width), x.shape[:-1].numel()
+    E = ext()
+    st = _state(home)
+    ws, use_gemm = st.scratch, True
+    if 1 <= B <= min(GEMV_MAX, 32) and (activation != "swiglu" or (B <= 8 and st.swiglu_gemv(M, N, B))):
+        ws, use_gemm = st.gemv_ws(M, N, B), False
+    tables = self._tables or self.tables()
+    host = calls() if out is None and B else None
+    if host is not None:                                # one native call for inputs that need no conversion
+        done = host[0].fused(host[1], use_gemm, self._buffers["tree"], tables[0], tables[1], tables[2], x, ws, self.bias, act, residual)
+        if done is not None:
+            return done
+    for name, t in (("residual", residual), ("out", out)):
+        if t is not None and (t.dtype != torch.bfloat16 or t.device != home or t.shape != shape):
+            raise RuntimeError(f"TreeLinear.fused: {name} BF16 {list(shape)} on {home}, got {t.dtype} {list(t.shape)} on {t.device}")
+    acts = _rows_2d(x if x.device == home else x.to(home), N)
+    given = out
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=home)
+    elif not out.is_contiguous() or out.data_ptr() % 8:
+        raise RuntimeError("TreeLinear.fused: out must be contiguous and 8-byte aligned")
+    apart = lambda a, b: a[0] >= b[1] or b[0] >= a[1]                      # noqa: E731
+    if given is not None and not (apart(_span(out), _span(acts)) and (residual is None or apart(_span(out), _span(residual)) or (
+            residual.data_ptr() == out.data_ptr() and residual.stride() == out.stride()))):
+        raise RuntimeError("TreeLinear.fused: out overlaps x, or the residual without being it")
+    res = None
+    if residual is not None and B:
+        res = residual.reshape(B, width)
+        if res.stride(1) != 1 or (B > 1 and res.stride(0) < width) or res.stride(0) % 4 or res.data_ptr() % 8:
+            res = res.clone(memory_format=torch.contiguous_format)
+        elif B == 1:
+            res = res.as_strided((1, width), (width, 1))
+    if B:
+        bias = self.bias
+        with on_device(home.index):
+            if use_gemm:
+                E.gemm_epilogue(self._buffers["tree"], tables[0], tables[1], acts, out.view(B, width), bias, act, res)
+            else:
+                E.gemv_epilogue(self._buffers["tree"], tables[0], tables[2], tables[1], acts, out.view(B, width), bias, act, res, ws)
+    if given is not None or (x.dtype == torch.bfloat16 and x.device == home):
+        return out
+    return out.to(device=x.device, dtype=x.dtype)
+
+
+TreeLinear.fused = fused
 
 
 def forward_list(layers, x):

@@ -76,6 +76,8 @@ _SIGNATURES = {
     "st_gemv_swiglu": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "st_rope_kv_append": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _dbl, _vp, _vp, _i64,
                                  _vp, _i64, _vp, _vp]),
+    "st_gemv_epilogue": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "st_gemm_epilogue": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _i64, _vp]),
     "st_kv_chunk_attn_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "st_kv_chunk_attn": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp,
                                 _vp, _dbl, _i64, _vp]),
@@ -133,7 +135,8 @@ CALLS_PATH = os.path.join(_HERE, "_calls.so")
 _CALLS = None                                           # False: there is none
 _NATIVE = ("st_gemv", "st_gemm", "st_gemv_list", "st_gemm_list", "st_last_error", "st_encode", "st_encode_lists", "st_encode_offsets",
            "st_encode_offsets_workspace_bytes", "st_dec_check", "st_lists_check", "st_kv8_append", "st_kv8_dequant_blocks", "st_kv8_attn_table",
-           "st_kv8_chunk_attn_table", "st_kv8_attn_workspace_bytes", "st_rotate", "st_kv_chunk_attn")
+           "st_kv8_chunk_attn_table", "st_kv8_attn_workspace_bytes", "st_rotate", "st_kv_chunk_attn", "st_gemv_epilogue",
+           "st_gemm_epilogue")
 
 
 def calls():
@@ -487,6 +490,23 @@ class _Weights:
         with _ctx(gu):
             _check(lib().st_silu_mul(_ptr(gu), _ptr(act), S, I2 // 2, _stream(gu)))
 
+
+    ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "swiglu": 5}
+
+    @staticmethod
+    def gemv_epilogue(T, EO, EB, EL, X, Y, bias, act, res, WS):
+        """Y = act(X W^T + bias) + res, up to 32 rows; act: a value of ACTIVATIONS, res rows at any stride"""
+        with _ctx(T):
+            _check(lib().st_gemv_epilogue(_ptr(T), _ptr(EO), _ptr(EB), _ptr(EL), _ptr(X), _ptr(Y), _ptr(bias), act, _ptr(res),
+                                          0 if res is None else res.stride(0), X.shape[0], T.shape[0] * 16, X.shape[1], _ptr(WS),
+                                          WS.numel() * WS.element_size(), _stream(T)))
+
+    @staticmethod
+    def gemm_epilogue(T, EO, EL, X, Y, bias, act, res):
+        """the same for any number of rows (tcgen05)"""
+        with _ctx(T):
+            _check(lib().st_gemm_epilogue(_ptr(T), _ptr(EO), _ptr(EL), _ptr(X), _ptr(Y), _ptr(bias), act, _ptr(res),
+                                          0 if res is None else res.stride(0), X.shape[0], T.shape[0] * 16, X.shape[1], _stream(T)))
 
     ROTATED = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
