@@ -14,6 +14,10 @@ so a tensor-parallel run computes the same function as the single-GPU one.
 
 `eight_bit_kv=True` keeps the KV cache in 8-bit pages (kvcache.PageStore8) instead of the lossless ones: a decode step then norms,
 rotates and appends through their append, and a prompt runs in one pass (prefill) over their chunk attention.
+
+`whole_prompts=True` runs prompts in one pass over the lossless pages too: q/k/v rows are normed and rotated (rotary.rotate), appended, and
+the queries attend to the pages (PageStore.chunk_attention); the o and down projections add the residual stream in their epilogue, and
+SwiGLU is the gate/up projection's (TreeLinear.fused).  Decode steps stay as they are.
 """
 import math
 from dataclasses import dataclass
@@ -25,6 +29,7 @@ import torch.nn.functional as Fn
 from .kvcache import PagedKVCache, decode_splits8
 from .linear import TreeLinear, interleave_gate_up
 from .ops import ext, kv_ext
+from .rotary import rotate
 
 
 def _flash():
@@ -65,11 +70,13 @@ class _Dense:
 
 class TreeDecoder:
     def __init__(self, cfg, device, batch, max_len, compressed=True, seed=0, rank=0, world=1, group=None,
-                 eight_bit_kv=False):
+                 eight_bit_kv=False, whole_prompts=False):
         self.cfg, self.dev, self.B, self.rank, self.world, self.group = cfg, torch.device(device), batch, rank, world, group
         self.compressed, self.eight_bit_kv = compressed, eight_bit_kv
+        self.whole_prompts = eight_bit_kv or whole_prompts
         c = cfg
-        assert compressed or not eight_bit_kv, "the BF16 control keeps its own cache"
+        assert compressed or not self.whole_prompts, "the BF16 control keeps its own cache"
+        assert not whole_prompts or eight_bit_kv or c.head_dim == 128, "the lossless pages hold heads of dimension 128"
         assert c.heads % world == 0 and c.kv_heads % world == 0 and c.inter % (64 * world) == 0 and c.vocab % (16 * world) == 0
         self.hq, self.hkv = c.heads // world, c.kv_heads // world
         self.fused_act = False
@@ -243,10 +250,10 @@ class TreeDecoder:
         return layer
 
     def prefill(self, prompt):
-        """prompt [B, P] token ids behind whatever the 8-bit cache holds, in one pass: every layer's keys and values go into the pages,
+        """prompt [B, P] token ids behind whatever the cache holds, in one pass: every layer's keys and values go into the pages,
         then its queries attend to them (causal).  Returns the logits of every sequence's last token [B, vocab]"""
-        if not self.eight_bit_kv or self.world > 1:
-            raise RuntimeError("TreeDecoder.prefill: a single-GPU decoder with eight_bit_kv=True")
+        if not self.whole_prompts or self.world > 1:
+            raise RuntimeError("TreeDecoder.prefill: a single-GPU decoder with eight_bit_kv=True or whole_prompts=True")
         c, E, (B, P) = self.cfg, ext(), prompt.shape
         if B != self.B:
             raise ValueError(f"TreeDecoder.prefill: {B} sequences, the decoder was made for {self.B}")
@@ -265,6 +272,9 @@ class TreeDecoder:
         q = torch.empty(N, self.hq, D, dtype=torch.bfloat16, device=self.dev)
         delta = None
         for li, (qkv, o, gu, d) in enumerate(self.blocks):
+            if not self.eight_bit_kv:
+                delta = self._prefill_block(li, x, delta, h, slots, positions, cu)
+                continue
             E.add_rmsnorm(x, delta, self.norm_w, h, c.eps)
             layer = self._append8(cache.layers[li], qkv(h), slots, positions, q)
             att = layer.chunk_attention(q, cu, cache.bt32[:B], cache.lens[:B], 1.0 / math.sqrt(D))
@@ -284,6 +294,29 @@ class TreeDecoder:
         cache.end_chunk(P)
         self.pos_buf += P
         return self.lm_head(h[last])
+
+    def _prefill_block(self, li, x, delta, h, slots, positions, cu):
+        """layer li of a prompt pass over the lossless pages: x (the residual stream, after the experts' `delta` of the layer before, if
+        any) is added to in place; returns this layer's experts' output, which the next norm adds, or None"""
+        c, E, (N, D), layer = self.cfg, ext(), (x.shape[0], self.cfg.head_dim), self.cache.layers[li]
+        qkv, o, gu, d = self.blocks[li]
+        E.add_rmsnorm(x, delta, self.norm_w, h, c.eps)
+        q, k, v = qkv.fused(h).view(N, self.hq + 2 * self.hkv, D).split([self.hq, self.hkv, self.hkv], 1)
+        q, k = rotate(q, k, positions, self.cos, self.sin, q_norm=self.head_norm_w, k_norm=self.head_norm_w, eps=c.eps)
+        layer.append(k, v, slots)
+        att = layer.chunk_attention(q, cu, self.cache.bt32[:self.B], self.cache.lens[:self.B], 1.0 / math.sqrt(D))
+        o.fused(att.view(N, self.hq * D), residual=x, out=x)
+        E.add_rmsnorm(x, None, self.norm_w, h, c.eps)
+        if c.experts:
+            router, te = gu
+            return te(h, *E.moe_route(Fn.linear(h, router), c.top_k, True, None), None)
+        if self.fused_act:                                   # (16-row tiles of gate and up in turn)
+            act = gu.fused(h, "swiglu")
+        else:
+            act = torch.empty(N, c.inter, dtype=torch.bfloat16, device=self.dev)
+            E.silu_mul(gu.fused(h), act)
+        d.fused(act, residual=x, out=x)
+        return None
 
     def _step(self):
         """one decode step for self.tokens at position self.pos; about ten launches per layer"""
@@ -406,7 +439,7 @@ class TreeDecoder:
             self.lens.zero_()
 
     def run(self, prompt, n_new, collect=None, margins=None):
-        """prompt [B, P] token ids (teacher-forced one step at a time, with an 8-bit cache in one pass), then n_new greedy tokens ->
+        """prompt [B, P] token ids (teacher-forced one step at a time; with an 8-bit cache or whole_prompts in one pass), then n_new greedy tokens ->
         [B, n_new].
         collect (optional list): receives the model's prediction after every prompt step (teacher-forced top-1).
         margins (optional list): receives, per generated token, the top-2 logit margin of sequence 0 that chose it."""
@@ -415,7 +448,7 @@ class TreeDecoder:
             raise ValueError(f"TreeDecoder.run: {prompt.shape[1]} prompt + {n_new} new tokens from position {start} "
                              f"exceed the cache capacity of {self.max_len} tokens")
         out = []
-        whole = self.eight_bit_kv and self.world == 1 and collect is None and prompt.shape[1] > 1
+        whole = self.whole_prompts and self.world == 1 and collect is None and prompt.shape[1] > 1
         if whole:
             self.logits.copy_(self.prefill(prompt))
             self._pick(self.logits)

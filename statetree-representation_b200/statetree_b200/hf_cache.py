@@ -16,6 +16,10 @@ StateTreeKVCache(..., eight_bit=True) keeps 8-bit pages instead (kvcache.PageSto
 prompt attends to the pages too, causally and from each sequence's first valid position on, and nothing is expanded.  Masks and
 modules that ask for anything else (packed sequences, right padding, softcaps, sinks, dropout) are refused: reset() the
 cache then, since the keys of the refused pass have been appended.  Decode steps read no mask, in either cache.
+
+StateTreeKVCache(..., paged_prompts=True) does the same over the lossless pages (kvcache.PageStore.chunk_attention): a chunk of a prompt
+attends to the pages, which are no longer expanded to BF16 for it, sliding windows hold in decode steps too, and the same masks and
+modules are refused.
 """
 import threading
 import weakref
@@ -26,7 +30,7 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 from .kvcache import PAGE, PageStore, PageStore8, decode_splits, decode_splits8
 
 HIDDEN = -1e4                      # an additive mask's values up to here hide a key (the exponential of a score is 0 then)
-ODD_MASK = "StateTreeKVCache: over 8-bit pages a mask is causal (within the layer's sliding window) with left padding"
+ODD_MASK = "StateTreeKVCache: with eight_bit or paged_prompts a mask is causal (within the layer's sliding window) with left padding"
 MASK_PART = 1 << 26                # elements of a mask that are checked at a time
 _LAST = threading.local()          # the layer whose update() ran last on this thread; the attention function picks it up
 
@@ -82,7 +86,7 @@ class StateTreeKVLayer(CacheLayerMixin):
         self.store.append(rows[0], rows[1], slots)
         _LAST.layer = self
         before, self.host_len = self.host_len, self.host_len + T
-        if c.eight_bit:                              # the attention function reads the pages whatever T is
+        if c.paged:                                  # the attention function reads the pages whatever T is
             if self.layer_idx == 0:
                 c.lens[:B].copy_((where[-1:] + 1).to(torch.int32).expand(B))
             return key_states, value_states
@@ -141,16 +145,17 @@ class StateTreeKVLayer(CacheLayerMixin):
 
 class StateTreeKVCache(Cache):
     """Lossless compressed KV cache for transformers models.  batch_size and max_cache_len fix the page tables;
-    pool_blocks sizes each layer's pool of 64-byte escape extension blocks.  eight_bit: 8-bit pages (not lossless)."""
+    pool_blocks sizes each layer's pool of 64-byte escape extension blocks.  eight_bit: 8-bit pages (not lossless).  paged_prompts: chunks of
+    a prompt attend to the (lossless) pages."""
 
-    def __init__(self, config, batch_size=None, max_cache_len=4096, pool_blocks=None, eight_bit=False, **kwargs):
+    def __init__(self, config, batch_size=None, max_cache_len=4096, pool_blocks=None, eight_bit=False, paged_prompts=False, **kwargs):
         text = config.get_text_config() if hasattr(config, "get_text_config") else config
         self.num_layers = text.num_hidden_layers
         self.num_q_heads = text.num_attention_heads
         self.num_kv_heads = getattr(text, "num_key_value_heads", None) or text.num_attention_heads
         self.max_len = int(max_cache_len)
         self.max_pages = -(-self.max_len // PAGE)
-        self.alloc_batch, self.pool_blocks, self.eight_bit = batch_size, pool_blocks, eight_bit
+        self.alloc_batch, self.pool_blocks, self.eight_bit, self.paged = batch_size, pool_blocks, eight_bit, eight_bit or paged_prompts
         self.starts_known = False
         self.starts_at, self.masks = 0, []           # the pass whose mask has been read; 8-bit pages: its masks that have been checked
         self._allocated = False
@@ -180,7 +185,7 @@ class StateTreeKVCache(Cache):
     def read_mask(self, mask, stored, B, T, window):
         """the left padding of every sequence (starts) after a pass's 4-D mask over its T tokens and `stored` keys, the pass's own among
         them; ValueError for a mask that is more than causal (and windowed) with left padding, which is all that the 8-bit pages are
-        read with.  Rows of padding see nothing, or everything (in masks that leave no row empty).  The check is one wait for the GPU a
+        read with (and the lossless ones with paged_prompts).  Rows of padding see nothing, or everything (in masks that leave no row empty).  The check is one wait for the GPU a
         pass and kind of mask; a captured pass cannot wait and leaves the error to check()."""
         if mask.dim() != 4 or mask.shape[2] != T or mask.shape[3] != stored:
             raise ValueError(f"StateTreeKVCache: a mask of shape {tuple(mask.shape)} over {T} tokens and {stored} keys")
@@ -217,7 +222,7 @@ class StateTreeKVCache(Cache):
         are not finite were appended, or a captured pass met a mask that read_mask refuses"""
         for layer in self.layers:
             layer.check()
-        if self._allocated and self.eight_bit and bool(self.odd_mask):
+        if self._allocated and self.paged and bool(self.odd_mask):
             raise ValueError(ODD_MASK)
 
     def storage_bytes(self):
@@ -226,8 +231,8 @@ class StateTreeKVCache(Cache):
 
 
 def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, scaling=None, **kwargs):
-    """the 'statetree' attention implementation: a decode step reads the compressed pages, anything else runs SDPA (over 8-bit pages:
-    chunk attention over the pages, and ValueError for what that does not compute)"""
+    """the 'statetree' attention implementation: a decode step reads the compressed pages, anything else runs SDPA (over 8-bit pages, and
+    with paged_prompts: chunk attention over the pages, and ValueError for what that does not compute)"""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     layer = getattr(_LAST, "layer", None)
     _LAST.layer = None
@@ -235,7 +240,7 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
         c = layer.cache
         B, Hq, T, D = query.shape
         window = kwargs.get("sliding_window") or 0
-        if c.eight_bit:
+        if c.paged:
             _refuse_other_attention(dropout, kwargs)
         if T == 1 and layer.host_len > 1:
             q = query[:, :, 0, :]
@@ -243,14 +248,17 @@ def statetree_attention(module, query, key, value, attention_mask, dropout=0.0, 
                 q = q.contiguous()
             scale = float(scaling) if scaling is not None else D ** -0.5
             more = dict(window=window) if c.eight_bit else {}
-            out = layer.store.attention(q, c.table32[:B], c.lens[:B], scale, splits=c.splits, starts=c.starts[:B],
-                                        min_pages=4, **more)
+            if c.paged and window and not c.eight_bit:  # (the lossless pages' decode attention has no window)
+                out = layer.store.chunk_attention(q, None, c.table32[:B], c.lens[:B], scale, starts=c.starts[:B], window=window)
+            else:
+                out = layer.store.attention(q, c.table32[:B], c.lens[:B], scale, splits=c.splits, starts=c.starts[:B],
+                                            min_pages=4, **more)
             return out.view(B, 1, Hq, D), None
-        if c.eight_bit:                              # a chunk (its keys are in the pages already), or the first token of all
+        if c.paged:                                  # a chunk (its keys are in the pages already), or the first token of all
             if attention_mask is not None:
                 c.read_mask(attention_mask, layer.host_len, B, T, window)
             elif T > 1 and not _causal(module, kwargs):
-                raise ValueError("StateTreeKVCache: attention over 8-bit pages is causal")
+                raise ValueError("StateTreeKVCache: attention over the pages is causal")
             q = query.transpose(1, 2).reshape(B * T, Hq, D)
             cu = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=q.device)
             out = layer.store.chunk_attention(q, cu, c.table32[:B], c.lens[:B], float(scaling) if scaling is not None else D ** -0.5,
@@ -275,7 +283,7 @@ def _causal(module, kwargs):
 def _refuse_other_attention(dropout, kwargs):
     for name, given in (("dropout", dropout), ("softcap", kwargs.get("softcap")), ("s_aux", kwargs.get("s_aux") is not None)):
         if given:
-            raise ValueError(f"StateTreeKVCache: attention over 8-bit pages has no {name}")
+            raise ValueError(f"StateTreeKVCache: attention over the pages has no {name}")
 
 
 def enable(model):

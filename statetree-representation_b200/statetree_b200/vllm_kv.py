@@ -2,7 +2,7 @@
 need vLLM itself: the page specification, the decode split contract, the per-process escape pool with its delayed
 exhaustion check, the view of a vLLM layer cache as pages, and a `PageBackend` that performs the three data-path
 calls of the backend (write at a slot mapping with recycling, decode attention over the pages, exact decode of cached
-prefix pages for a paged prefill kernel).  The vLLM-facing classes (AttentionBackend / metadata builder / impl) are
+prefix pages for a paged prefill kernel), and the attention of new tokens over the pages themselves (prefill).  The vLLM-facing classes (AttentionBackend / metadata builder / impl) are
 thin wrappers over these; they are not built here because this image ships vLLM 0.22, whose v1 attention interface
 differs ("vLLM 0.32 absent"): `register()` reports that instead of installing anything.
 """
@@ -10,7 +10,7 @@ import os
 
 import torch
 
-from .kvcache import decode_splits as _splits_for_pages
+from .kvcache import PageStore, decode_splits as _splits_for_pages
 from .ops import kv_ext
 
 PAGE, RKV, HD = 16, 1600, 128
@@ -134,6 +134,17 @@ class PageBackend:
         self.kx.attn(query.view(n, self.num_heads, HD), page_view(kv_cache, self.num_kv_heads), self.shared.pool,
                      block_table[:n], seq_lens[:n], out.view(n, self.num_heads, HD), self.shared.wo, self.shared.wml,
                      self.scale, splits, None, MIN_PAGES_PER_SPLIT)
+        return out
+
+    def prefill(self, query, kv_cache, block_table, cu, seq_lens, out, splits=None, window=0):
+        """requests with new tokens (a prompt, a chunk of one behind cached context, speculative tokens), after write(): causal attention of
+        query rows cu[r] .. cu[r + 1] - 1 of every request r (cu int32 [requests + 1]), the last of them token seq_lens[r] - 1, straight from
+        the pages into out; rows behind cu[-1] (padding) stay as they are.  Nothing is decoded to memory (cached_pages is the way for
+        another attention kernel)"""
+        n, requests = query.shape[0], cu.numel() - 1
+        store = PageStore.over(page_view(kv_cache, self.num_kv_heads), self.shared.pool, self.shared.cnt)
+        store.chunk_attention(query.view(n, self.num_heads, HD), cu, block_table[:requests], seq_lens[:requests], self.scale, splits=splits,
+                              out=out.view(n, self.num_heads, HD), window=window)
         return out
 
     def cached_pages(self, kv_cache, blocks):
