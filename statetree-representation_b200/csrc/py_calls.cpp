@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/version.h>
 
@@ -426,10 +427,11 @@ py::object kv_chunk_attention(const Library& lib, const at::Tensor& pages, const
   return py::cast(out);
 }
 
-// ---- rotary positions: q [N, Hq, D] and k [N, Hk, D] (or None) into new tensors; (q, k) or None
-py::object rotate(const Library& lib, const at::Tensor& q, const Maybe& k, const at::Tensor& positions, const at::Tensor& cos,
-                  const at::Tensor& sin, bool interleaved, int64_t offset, bool inverse, const Maybe& wq, const Maybe& wk, double eps) {
-  if (!q.is_cuda() || q.dim() != 3) return py::none();
+// ---- rotary positions: q [N, Hq, D] and k [N, Hk, D] (or none) into new tensors; false where the call is not of the plain form
+bool rotate_into(const Library& lib, const at::Tensor& q, const Maybe& k, const at::Tensor& positions, const at::Tensor& cos,
+                 const at::Tensor& sin, bool interleaved, int64_t offset, bool inverse, const Maybe& wq, const Maybe& wk, double eps,
+                 at::Tensor& yq, at::Tensor& yk) {
+  if (!q.is_cuda() || q.dim() != 3) return false;
   const at::Device device = q.device();
   const auto type = q.scalar_type();
   const int code = type == at::kBFloat16 ? 0 : type == at::kHalf ? 1 : type == at::kFloat ? 2 : -1;
@@ -442,22 +444,74 @@ py::object rotate(const Library& lib, const at::Tensor& q, const Maybe& k, const
   if (code < 0 || !rows(q) || (k && !rows(*k)) || !norm(wq) || !norm(wk) || !flat(positions, at::kLong, device) ||
       (positions.numel() != N && positions.numel() != 1) || !flat(cos, at::kFloat, device) || !flat(sin, at::kFloat, device) || cos.dim() != 2 ||
       sin.sizes() != cos.sizes() || cos.size(0) < 1 || offset < 0 || offset + 2 * cos.size(1) > D)
-    return py::none();
+    return false;
+  const c10::cuda::CUDAGuard guard(device);
+  yq = at::empty(q.sizes(), q.options().requires_grad(false));
+  if (k) yk = at::empty(k->sizes(), yq.options());
+  const int rc = lib.rotate(q.const_data_ptr(), q.stride(0), q.stride(1), q.size(1), of<void>(k), k ? k->stride(0) : 0, k ? k->stride(1) : 0,
+                            k ? k->size(1) : 0, N, D, code, of<int64_t>(positions), positions.numel() > 1, of<float>(cos), of<float>(sin),
+                            cos.size(0), 2 * cos.size(1), offset, interleaved, inverse, of<void>(wq), of<void>(wk), eps, yq.data_ptr(),
+                            yq.stride(0), yq.stride(1), k ? yk.data_ptr() : nullptr, k ? yk.stride(0) : 0, k ? yk.stride(1) : 0,
+                            c10::cuda::getCurrentCUDAStream(device.index()).stream());
+  check(lib, rc);
+  return true;
+}
+
+// (q, k), or q without k, or None
+py::object rotate(const Library& lib, const at::Tensor& q, const Maybe& k, const at::Tensor& positions, const at::Tensor& cos,
+                  const at::Tensor& sin, bool interleaved, int64_t offset, bool inverse, const Maybe& wq, const Maybe& wk, double eps) {
   at::Tensor yq, yk;
-  int rc;
   {
     py::gil_scoped_release nogil;
-    const c10::cuda::CUDAGuard guard(device);
-    yq = at::empty(q.sizes(), q.options().requires_grad(false));
-    if (k) yk = at::empty(k->sizes(), yq.options());
-    rc = lib.rotate(q.const_data_ptr(), q.stride(0), q.stride(1), q.size(1), of<void>(k), k ? k->stride(0) : 0, k ? k->stride(1) : 0,
-                    k ? k->size(1) : 0, N, D, code, of<int64_t>(positions), positions.numel() > 1, of<float>(cos), of<float>(sin),
-                    cos.size(0), 2 * cos.size(1), offset, interleaved, inverse, of<void>(wq), of<void>(wk), eps, yq.data_ptr(), yq.stride(0),
-                    yq.stride(1), k ? yk.data_ptr() : nullptr, k ? yk.stride(0) : 0, k ? yk.stride(1) : 0,
-                    c10::cuda::getCurrentCUDAStream(device.index()).stream());
+    if (!rotate_into(lib, q, k, positions, cos, sin, interleaved, offset, inverse, wq, wk, eps, yq, yk)) yq = at::Tensor();
   }
-  check(lib, rc);
+  if (!yq.defined()) return py::none();
   return k ? py::object(py::make_tuple(yq, yk)) : py::cast(yq);
+}
+
+// the same with gradients to q and k: the rotation by the opposite angles
+struct RotateGrad : torch::autograd::Function<RotateGrad> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
+                                                const at::Tensor& positions, const at::Tensor& cos, const at::Tensor& sin, int64_t lib,
+                                                bool interleaved, int64_t offset, bool inverse) {
+    ctx->save_for_backward({positions, cos, sin});
+    ctx->saved_data["lib"] = lib;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["offset"] = offset;
+    ctx->saved_data["inverse"] = inverse;
+    at::Tensor yq, yk;
+    TORCH_CHECK(rotate_into(*reinterpret_cast<const Library*>(lib), q, k, positions, cos, sin, interleaved, offset, inverse, {}, {}, 0.0, yq, yk),
+                "rotate: a gradient of another type or device than its output's");
+    return {yq, yk};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    for (at::Tensor& g : grads)
+      if (g.stride(2) != 1) g = g.contiguous();
+    auto back = RotateGrad::apply(grads[0], grads[1], saved[0], saved[1], saved[2], ctx->saved_data["lib"].toInt(),
+                                  ctx->saved_data["interleaved"].toBool(), ctx->saved_data["offset"].toInt(), !ctx->saved_data["inverse"].toBool());
+    return {back[0], back[1], {}, {}, {}, {}, {}, {}, {}};
+  }
+};
+py::object rotate_grad(const Library& lib, const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions, const at::Tensor& cos,
+                       const at::Tensor& sin, bool interleaved, int64_t offset, bool inverse) {
+  if (q.dim() != 3 || k.dim() != 3 || q.numel() == 0 || k.numel() == 0 || q.size(2) < 2 || q.stride(2) != 1 || k.stride(2) != 1 || !q.is_cuda() ||
+      k.device() != q.device() || k.scalar_type() != q.scalar_type() || k.size(0) != q.size(0) || k.size(2) != q.size(2) ||
+      positions.device() != q.device() || cos.device() != q.device() || sin.device() != q.device() || cos.requires_grad() || sin.requires_grad())
+    return py::none();
+  // (what the kernel takes is looked at before the function is recorded: a refusal takes the general path, which says what is wrong)
+  const auto type = q.scalar_type();
+  if ((type != at::kBFloat16 && type != at::kHalf && type != at::kFloat) || !flat(positions, at::kLong, q.device()) ||
+      (positions.numel() != q.size(0) && positions.numel() != 1) || !flat(cos, at::kFloat, q.device()) || !flat(sin, at::kFloat, q.device()) ||
+      cos.dim() != 2 || sin.sizes() != cos.sizes() || cos.size(0) < 1 || offset < 0 || offset + 2 * cos.size(1) > q.size(2) || q.is_conj() ||
+      q.is_neg() || k.is_conj() || k.is_neg() || q.layout() != at::kStrided || k.layout() != at::kStrided)
+    return py::none();
+  torch::autograd::variable_list y;
+  {
+    py::gil_scoped_release nogil;
+    y = RotateGrad::apply(q, k, positions, cos, sin, reinterpret_cast<int64_t>(&lib), interleaved, offset, inverse);
+  }
+  return py::make_tuple(y[0], y[1]);
 }
 }  // namespace
 
@@ -474,6 +528,7 @@ PYBIND11_MODULE(_calls, m) {
   m.def("kv8_attention", &kv8_attention);
   m.def("kv8_dense", &kv8_dense);
   m.def("rotate", &rotate);
+  m.def("rotate_grad", &rotate_grad);              // (the library object lives as long as the process: ops.py keeps it)
   m.def("fused", &fused);
   m.def("kv_chunk_attention", &kv_chunk_attention);
 }

@@ -5,6 +5,9 @@
 // Bound by HBM: every value is read once and written once.  A lane owns VEC pairs (two 16-byte vectors) of a head, so that a pair
 // never crosses lanes in either layout and the norm needs one reduction over the head's lanes; a warp walks the heads of ONE token, whose
 // cosines and sines stay in registers.  Few tokens: the heads of a token are dealt to several warps.
+// Measured, us in a graph (BF16, heads of 128): 32764 tokens of 32 + 8 heads 111 = 6.1 TB/s (a copy of as many bytes 105), with norms 121;
+// 8190 tokens of 16 + 16 heads 26.7 (copy 24.7); 1261 tokens of 64 heads of 80, 32 of them rotated, 8.5; one token 2.9.  Two heads in flight
+// and 24 warps an SM; with norms one and 32 (two and 24: 129; the weights in registers 143; four in flight and 16 warps 159).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -75,9 +78,9 @@ __device__ __forceinline__ long long place(const RotArgs& a, long long n) {
 constexpr int THREADS = 256;
 
 template <typename T, bool PAIRS, bool NORM>
-__global__ void __launch_bounds__(THREADS) rotate_kernel(const RotArgs a) {
+__global__ void __launch_bounds__(THREADS, NORM ? 4 : 3) rotate_kernel(const RotArgs a) {
   constexpr int VEC = 16 / sizeof(T);              // pairs of a lane = values of one of its two vectors
-  constexpr int U = 2;                             // heads whose loads are in flight together
+  constexpr int U = NORM ? 1 : 2;                  // heads whose loads are in flight together
   const int lane = threadIdx.x & 31;
   const long long w = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
   const long long n = w / a.parts;
@@ -89,6 +92,7 @@ __global__ void __launch_bounds__(THREADS) rotate_kernel(const RotArgs a) {
   const int p0 = (int)((long long)passes * part / a.parts), p1 = (int)((long long)passes * (part + 1) / a.parts);
   // this lane's two vectors of every head
   const int s0 = li * VEC, half = a.part / 2;
+  const float inv_d = 1.f / (float)a.D;
   const bool here = 2 * s0 < a.D, rot = s0 < half;
   int d0, d1;
   if (rot) {
@@ -146,8 +150,8 @@ __global__ void __launch_bounds__(THREADS) rotate_kernel(const RotArgs a) {
         for (int k = 0; k < 2 * VEC; ++k) ss = __fmaf_rn(f[k], f[k], ss);
         for (int o = a.lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
         const T* const wt = reinterpret_cast<const T*>(a.s[kv].w);
-        if (h >= 0 && wt) {
-          const float r = rsqrtf(ss / (float)a.D + a.eps);
+        if (h >= 0 && wt) {                        // (from L1: held in registers they cost a quarter of the resident warps)
+          const float r = rsqrtf(ss * inv_d + a.eps);
           float g[2 * VEC];
           unpack<T>(__ldg(reinterpret_cast<const uint4*>(wt + d0)), g);
           unpack<T>(second ? __ldg(reinterpret_cast<const uint4*>(wt + d1)) : make_uint4(0, 0, 0, 0), g + VEC);
@@ -227,9 +231,9 @@ int rotate_launch(RotArgs& a, bool pairs, cudaStream_t st_) {
   }
   a.lanes = 1;
   while (a.lanes * 2 * VEC < a.D) a.lanes *= 2;
-  // a token's heads are dealt to more warps while that leaves the GPU's warps (64 an SM) idle
+  // a token's heads are dealt to more warps while the GPU's (some 32 an SM fit) are not all at work
   const int passes = (total + 32 / a.lanes - 1) / (32 / a.lanes);
-  const long long want = 64ll * st::sm_count() / a.N;
+  const long long want = 32ll * st::sm_count() / a.N;
   a.parts = (int)(want < 1 ? 1 : want > passes ? passes : want);
   const long long blocks = (a.N * a.parts + THREADS / 32 - 1) / (THREADS / 32);
   ST_REQUIRE(blocks < (1ll << 31), "st_rotate: too many tokens");

@@ -114,6 +114,11 @@ def rotate(q, k, positions, cos, sin, interleaved=True, offset=0, q_norm=None, k
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_norm, k_norm)):
         if q_norm is not None or k_norm is not None or out is not None:
             raise RuntimeError("rotate: gradients flow through the rotation alone (without norms and given outputs)")
+        host = calls() if k is not None else None
+        if host is not None:                                # (the same function in native code)
+            done = host[0].rotate_grad(host[1], q, k, positions, cos, sin, interleaved, offset, inverse)
+            if done is not None:
+                return done
         if k is None:
             return _Rotate.apply(q, q[:, :0], positions, cos, sin, interleaved, offset, inverse)[0], None
         return _Rotate.apply(q, k, positions, cos, sin, interleaved, offset, inverse)
