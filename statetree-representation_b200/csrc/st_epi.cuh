@@ -29,6 +29,14 @@ __device__ __forceinline__ float epi_act(int act, float z) {
   }
   return z;
 }
+// the same of sixteen values, one branch for all
+__device__ __forceinline__ void epi_act16(int act, float (&z)[16]) {
+  switch (act) {
+#define ST_ACT(A) case A: _Pragma("unroll") for (int k = 0; k < 16; ++k) z[k] = epi_act(A, z[k]); break;
+    ST_ACT(EPI_RELU) ST_ACT(EPI_SILU) ST_ACT(EPI_GELU) ST_ACT(EPI_GELU_TANH)
+#undef ST_ACT
+  }
+}
 __device__ __forceinline__ float epi_value(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ uint16_t epi_round(float v) {
   const __nv_bfloat16 h = __float2bfloat16_rn(v);
@@ -38,35 +46,52 @@ __device__ __forceinline__ uint16_t epi_round(float v) {
 // Sixteen token columns of a warp's 32 rows, lane = row, as tensor memory hands them out.  `left` of the columns exist, `valid` of the rows
 // (a multiple of 16); y, res: this warp's first result row of the first column, columns `rows` / `res_stride` values apart.  Lanes pair up,
 // even ones on column c and odd on c + 1 with two rows each, so that a store writes 4 bytes a lane, 64 a column; under EPI_SWIGLU lane l
-// and l + 16 (gate and up of a row) pair up the same way.  The residual's words are requested before the first store (they may be the same memory), from L2:
-// the threads here have not waited for the kernel before themselves, so that a line of theirs in L1 may be older than its writes.
-__device__ __forceinline__ void epi_store16(const Epi& e, const uint32_t (&v)[16], float bias, int left, int valid, uint16_t* y, const uint16_t* res) {
+// and l + 16 (gate and up of a row) pair up the same way.  The residual's words are fetched by a call of their own, so that they can be
+// requested a chunk ahead, and before the first store (they may be the same memory); from L2: the threads here have not waited for the
+// kernel before themselves, so that a line of theirs in L1 may be older than its writes.
+__device__ __forceinline__ void epi_fetch16(const Epi& e, int left, int valid, const uint16_t* res, uint32_t (&r)[8]) {
   const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = 0u;
+  if (!e.res) return;
   if (e.act == EPI_SWIGLU) {
     const int hi = lane >> 4, row = lane & 15;
-    uint16_t r[8];
+    if (valid == 32)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = res && valid == 32 && 2 * j + hi < left ? __ldcg(res + (size_t)(2 * j + hi) * e.res_stride + row) : (uint16_t)0;
+      for (int j = 0; j < 8; ++j)
+        if (2 * j + hi < left) r[j] = (uint32_t)__ldcg(res + (size_t)(2 * j + hi) * e.res_stride + row);
+  } else {
+    const int odd = lane & 1, row = lane & ~1;
+    if (row < valid)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (2 * j + odd < left) r[j] = __ldcg(reinterpret_cast<const uint32_t*>(res + (size_t)(2 * j + odd) * e.res_stride + row));
+  }
+}
+__device__ __forceinline__ void epi_store16(const Epi& e, const uint32_t (&v)[16], float bias, int left, int valid, uint16_t* y, const uint32_t (&r)[8]) {
+  const int lane = threadIdx.x & 31;
+  float z[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) z[k] = __uint_as_float(v[k]) + bias;
+  if (e.act == EPI_SWIGLU) {
+    const int hi = lane >> 4;
+    uint16_t* const p = y + (size_t)hi * e.rows + (lane & 15);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float z0 = __uint_as_float(v[2 * j]) + bias, z1 = __uint_as_float(v[2 * j + 1]) + bias;
-      const float got = __shfl_xor_sync(FULL, hi ? z0 : z1, 16);
-      const float x = epi_silu(hi ? got : z0) * (hi ? z1 : got) + epi_value(r[j]);
-      if (valid == 32 && 2 * j + hi < left) y[(size_t)(2 * j + hi) * e.rows + row] = epi_round(x);
+      const float got = __shfl_xor_sync(FULL, hi ? z[2 * j] : z[2 * j + 1], 16);
+      const float x = epi_silu(hi ? got : z[2 * j]) * (hi ? z[2 * j + 1] : got) + __uint_as_float(r[j] << 16);
+      if (valid == 32 && 2 * j + hi < left) p[(size_t)(2 * j) * e.rows] = epi_round(x);
     }
     return;
   }
+  epi_act16(e.act, z);
   const int odd = lane & 1, row = lane & ~1;
-  uint32_t r[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    r[j] = res && row < valid && 2 * j + odd < left ? __ldcg(reinterpret_cast<const uint32_t*>(res + (size_t)(2 * j + odd) * e.res_stride + row)) : 0u;
+  uint16_t* const p = y + (size_t)odd * e.rows + row;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float z0 = epi_act(e.act, __uint_as_float(v[2 * j]) + bias), z1 = epi_act(e.act, __uint_as_float(v[2 * j + 1]) + bias);
-    const float got = __shfl_xor_sync(FULL, odd ? z0 : z1, 1);
-    const float x0 = (odd ? got : z0) + __uint_as_float(r[j] << 16), x1 = (odd ? z1 : got) + __uint_as_float(r[j] & 0xFFFF0000u);
-    if (row < valid && 2 * j + odd < left) *reinterpret_cast<uint32_t*>(y + (size_t)(2 * j + odd) * e.rows + row) = pack_bf16(x0, x1);
+    const float got = __shfl_xor_sync(FULL, odd ? z[2 * j] : z[2 * j + 1], 1);
+    const float x0 = (odd ? got : z[2 * j]) + __uint_as_float(r[j] << 16), x1 = (odd ? z[2 * j + 1] : got) + __uint_as_float(r[j] & 0xFFFF0000u);
+    if (row < valid && 2 * j + odd < left) *reinterpret_cast<uint32_t*>(p + (size_t)(2 * j) * e.rows) = pack_bf16(x0, x1);
   }
 }
 

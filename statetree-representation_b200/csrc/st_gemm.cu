@@ -332,6 +332,7 @@ gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
     // EPI: rows of this warp's 32 that exist, its row's bias
     const int row0 = lrb * 128 + q4 * 32, valid = EPI ? (int)min(32ll, max(0ll, a.M - row0)) : 32;
     const float bias = EPI && a.epi.bias && lane < valid ? epi_value(__ldg(a.epi.bias + row0 + lane)) : 0.f;
+    const int out0 = EPI && a.epi.act == EPI_SWIGLU ? row0 >> 1 : row0;
     for (int c0 = cg * 16; c0 < nmma; c0 += (NDW / 4) * 16) {
       uint32_t v[16];
       tmem_ld16(tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)c0, v);
@@ -339,10 +340,9 @@ gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap xmap, const __
 #pragma unroll
         for (int j = 0; j < 16; ++j) stg[(size_t)(c0 + j) * 128 + q4 * 32 + lane] = __uint_as_float(v[j]);
       } else if (EPI) {
-        const size_t tok = (size_t)(tok0 + c0);
-        const int out0 = a.epi.act == EPI_SWIGLU ? row0 >> 1 : row0;
-        epi_store16(a.epi, v, bias, acc_ok ? ncol - c0 : 0, valid, Yp + tok * a.epi.rows + out0,
-                    a.epi.res ? a.epi.res + tok * a.epi.res_stride + out0 : nullptr);
+        uint32_t words[8];
+        epi_fetch16(a.epi, ncol - c0, valid, a.epi.res + (size_t)(tok0 + c0) * a.epi.res_stride + out0, words);
+        epi_store16(a.epi, v, bias, acc_ok ? ncol - c0 : 0, valid, Yp + (size_t)(tok0 + c0) * a.epi.rows + out0, words);
       } else {
         // whole k range: this lane holds row q4 * 32 + lane of 16 token columns.  Lanes pair up (even: column j, odd:
         // column j + 1, two rows each) so that a store instruction writes 4 bytes per lane, 64 bytes per column

@@ -98,6 +98,10 @@ __device__ __forceinline__ void store_unit(uint32_t acc, int c0, int NT, int nco
 __device__ __forceinline__ void store_unit_epi(const GemmArgs& a, uint32_t acc, int c0, int NT, int ncol, int tok0, int row0, uint32_t accfree) {
   const int lane = threadIdx.x & 31, valid = (int)min(32ll, max(0ll, a.M - row0)), out0 = a.epi.act == EPI_SWIGLU ? row0 >> 1 : row0;
   const float bias = a.epi.bias && lane < valid ? epi_value(__ldg(a.epi.bias + row0 + lane)) : 0.f;
+  const uint16_t* res = a.epi.res + (size_t)(tok0 + c0) * a.epi.res_stride + out0;
+  uint16_t* y = a.Y + (size_t)(tok0 + c0) * a.epi.rows + out0;
+  uint32_t words[8], next[8];
+  epi_fetch16(a.epi, ncol - c0, valid, res, words);
 #pragma unroll 1
   for (; c0 < NT; c0 += CSTEP) {
     uint32_t v[16];
@@ -107,8 +111,12 @@ __device__ __forceinline__ void store_unit_epi(const GemmArgs& a, uint32_t acc, 
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(accfree);
     }
-    const size_t tok = (size_t)(tok0 + c0);
-    epi_store16(a.epi, v, bias, ncol - c0, valid, a.Y + tok * a.epi.rows + out0, a.epi.res ? a.epi.res + tok * a.epi.res_stride + out0 : nullptr);
+    res += (size_t)CSTEP * a.epi.res_stride;
+    epi_fetch16(a.epi, ncol - c0 - CSTEP, valid, res, next);     // (a chunk ahead)
+    epi_store16(a.epi, v, bias, ncol - c0, valid, y, words);
+    y += (size_t)CSTEP * a.epi.rows;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) words[j] = next[j];
   }
 }
 
