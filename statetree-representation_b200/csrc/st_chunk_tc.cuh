@@ -145,9 +145,11 @@ struct ChunkBars {
 
 // The MMAs of a CTA's two row tiles (of `count0` and `count1` key tiles).  One thread's MMAs complete in the order of their issue (and a
 // commit covers all before it): S of the next key tile may take the place of the P that the product before it reads.
-// The whole loop runs in one elected thread, waits included: a warp that meets again around each step costs more than the steps
+// The whole loop runs in one elected thread, waits included: a warp that meets again around each step costs more than the steps.
+// qfull: a barrier per row tile that says its q is in shared memory (nullptr: it is)
 template <int D, uint32_t IDESC_S, uint32_t IDESC_O>
-__device__ __forceinline__ void issue_mmas(uint8_t* const smem, const ChunkBars& b, uint32_t tmem, int tiles, int count0, int count1, int* status) {
+__device__ __forceinline__ void issue_mmas(uint8_t* const smem, const ChunkBars& b, uint32_t tmem, int tiles, int count0, int count1, int* status,
+                                           uint64_t* qfull = nullptr) {
   const uint32_t dq = desc_k(smem_addr(smem + Tiles<D>::Q)), dk = desc_k(smem_addr(smem + Tiles<D>::K)), dv = desc_mn(smem_addr(smem + Tiles<D>::V), Tiles<D>::HALF);
   auto scores = [&](int t, int s) {
     const uint32_t q = dq + t * (Tiles<D>::TILE >> 4), k = dk + s * (Tiles<D>::TILE >> 4);
@@ -173,7 +175,7 @@ __device__ __forceinline__ void issue_mmas(uint8_t* const smem, const ChunkBars&
     ok = mbar_wait(b.kfull, 0);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
-      if (ok && (t ? count1 : count0) > 0) {
+      if (ok && (t ? count1 : count0) > 0 && (!qfull || (ok = mbar_wait(qfull + t, 0)))) {
         tc_fence_after();
         scores(t, 0);
       }
@@ -210,6 +212,16 @@ __device__ __forceinline__ void issue_mmas(uint8_t* const smem, const ChunkBars&
     (void)mbar_wait(b.drain, 0);
   }
 }
+// Walks rows (query, head of the group) of a sequence in steps, without a division a step; and without a shuffle: shuffles between loads wait
+// for them (sixteen rows of q took 7000 cycles to ask for, one after the other)
+struct RowWalk {
+  int token, head, G;
+  __device__ RowWalk(int row, int group) : token(row / group), head(row % group), G(group) {}
+  __device__ __forceinline__ void step(int rows) {
+    head += rows;
+    while (head >= G) { head -= G; ++token; }
+  }
+};
 // A softmax warp's rows leave: this lane's row of O (tensor memory `to`, key tiles seen: count) over its sum l, or, of a split, as it is
 // with (reference m, l).  The whole warp calls
 template <int D>
@@ -243,7 +255,7 @@ __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts,
     // the warp's rows leave through where its rows of q were (their last scores are done), D / 8 lanes a row
     constexpr int LANES = D / 8, PER = 32 / LANES;
     uint8_t* const rows = smem + Tiles<D>::Q + t * Tiles<D>::TILE + (warp & 3) * (32 * 2 * D);
-#pragma unroll
+#pragma unroll 1                                                  // (code that runs once: what it costs is to be fetched)
     for (int q = 0; q < D / 32; ++q) {
       uint32_t v[32];
       if (count > 0) {
@@ -261,15 +273,14 @@ __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts,
       }
     }
     __syncwarp();
-    const long long mine = live ? (long long)(w.first + token) * a.out_stride + (long long)hq * D : -1;
-#pragma unroll
-    for (int i = 0; i < LANES; ++i) {
-      const int row = i * PER + lane / LANES;
-      const long long out = __shfl_sync(FULL, mine, row);
-      if (out >= 0)
-        *reinterpret_cast<uint4*>(a.out + out + 8 * (lane % LANES)) =
+    int row = lane / LANES;
+    const int at = t * ROWS + (warp & 3) * 32 + row, G = a.Hq / a.H;
+    RowWalk to_row(w.row0 + at, G);
+#pragma unroll 4
+    for (int i = 0; i < LANES; ++i, row += PER, to_row.step(PER))
+      if (at + i * PER < w.rows)
+        *reinterpret_cast<uint4*>(a.out + (long long)(w.first + to_row.token) * a.out_stride + (w.h * G + to_row.head) * D + 8 * (lane % LANES)) =
             *reinterpret_cast<const uint4*>(rows + row * (2 * D) + (((lane % LANES) ^ (row & 7)) << 4));
-    }
   }
 }
 }  // namespace st

@@ -125,7 +125,7 @@ __device__ __forceinline__ void page_edge(uint32_t (&A)[2][4][4], int first, int
 // its keys are decoded: these pages are read once, from memory, not by many CTAs from L2.
 struct LayX : Tiles<HD> {
   static constexpr int RAW = Tiles<HD>::END, SLOT_BYTES = 2 * RKV;                                 // a slot per page of a key tile
-  static constexpr int BARS = RAW + 8 * SLOT_BYTES, NBARS = ChunkBars::COUNT + 32, SLOT = BARS + NBARS * 8;
+  static constexpr int BARS = RAW + 8 * SLOT_BYTES, NBARS = ChunkBars::COUNT + 34, SLOT = BARS + NBARS * 8;
   static constexpr int BYTES = SLOT + 16 + 1024;
   static __device__ __forceinline__ int slot(int set, int page) { return (set ? Q + TILE : RAW) + page * SLOT_BYTES; }
 };
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   const ChunkBars b(reinterpret_cast<uint64_t*>(smem + L::BARS));
-  uint64_t *const raw = b.rest, *const rempty = raw + 8 * SETS;    // [set][page] of every slot: filled, in registers
+  uint64_t *const qfull = b.rest, *const raw = qfull + 2, *const rempty = raw + 8 * SETS;      // raw, rempty: [set][page], of every slot: filled, in registers
   uint32_t* const slot_at = reinterpret_cast<uint32_t*>(smem + L::SLOT);
   const Attn8& a = c.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.Hq / a.H;
@@ -207,12 +207,16 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
   const uint64_t keep = policy_evict_last();                      // other row tiles of the sequence read the same pages
 
   if (warp == R::MMA) {
-    if (elect_one()) b.init(TILE_PAGES);
+    if (elect_one()) {
+      mbar_init(qfull, 4);
+      mbar_init(qfull + 1, 4);
+      b.init(TILE_PAGES);
+    }
     __syncwarp();
     tmem_alloc<1>(slot_at, 512);
     tmem_relinquish<1>();
   }
-  // (each role has something to request before it needs the others: the rows of q, the first pages)
+  // (the first pages are requested before the roles meet; q, which takes its time, is nobody's but the MMAs' to wait for)
   auto meet = [] {
     tc_fence_before();
     __syncthreads();
@@ -231,25 +235,29 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
     const bool any = __any_sync(FULL, live);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    // ---- the warp's 32 rows of q: sixteen lanes read a row
+    meet();
+    // ---- the warp's 32 rows of q: sixteen lanes read a row (rows that are none: the last one again)
     if (count > 0) {
-      const long long mine = live ? (long long)(w.first + token) * a.q_stride + (long long)hq * D : -1;
-      const int col = lane & 15;
-      uint8_t* const rows = smem + L::Q + t * L::TILE + (warp & 3) * (32 * 128) + (col >> 3) * L::HALF;
+      const int last = w.row0 + w.rows - 1, col = lane & 15;
+      int row = my - lane + (lane >> 4);
+      RowWalk at(min(row, last), G);
       uint4 u[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const long long from = __shfl_sync(FULL, mine, 2 * i + (lane >> 4));
-        u[i] = from >= 0 ? *reinterpret_cast<const uint4*>(a.q + from + 8 * col) : make_uint4(0, 0, 0, 0);
+        u[i] = *reinterpret_cast<const uint4*>(a.q + (long long)(w.first + at.token) * a.q_stride + (w.h * G + at.head) * D + 8 * col);
+        row += 2;
+        at.step(row <= last ? 2 : 0);
       }
+      uint8_t* const rows = smem + L::Q + t * L::TILE + (warp & 3) * (32 * 128) + (col >> 3) * L::HALF;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = 2 * i + (lane >> 4);
         *reinterpret_cast<uint4*>(rows + r * 128 + (((col & 7) ^ (r & 7)) << 4)) = u[i];
       }
       fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(qfull + t);
     }
-    meet();
     const uint32_t tmem = *slot_at + ((uint32_t)((warp & 3) * 32) << 16), ts = tmem + t * 128, to = tmem + 256 + t * D;
     // The second row tile begins when the first has its first P: from then on each has the special function units to itself while the
     // other's products run.  (A barrier of its own, which completes once: the first tile's softmax does not wait for this one's, so that
@@ -396,7 +404,7 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
       // -------------------------------------------------------------- MMAs.  V is read as it lies (dims contiguous: MN-major)
       meet();
       if (elect_one())
-        issue_mmas<D, mma_idesc(128, KEYS), mma_idesc(128, D) | 1u << 16>(smem, b, *slot_at, tiles, w.count0, w.count1, c.status);
+        issue_mmas<D, mma_idesc(128, KEYS), mma_idesc(128, D) | 1u << 16>(smem, b, *slot_at, tiles, w.count0, w.count1, c.status, qfull);
       __syncwarp();
       tc_fence_before();
     } else {
