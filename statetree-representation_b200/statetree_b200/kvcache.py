@@ -158,11 +158,18 @@ def chunk_splits8(tokens, seqs, kv_heads, group, max_pages, sms=148):
 
 
 def chunk_splits(tokens, seqs, kv_heads, group, max_pages, sms=148):
-    """How many CTAs share a sequence of the chunk attention over lossless pages, from what the host knows (st_kv_chunk.cu)"""
+    """How many CTAs share a sequence of the chunk attention over lossless pages, from what the host knows.  A CTA takes an SM: 32 rows for
+    sequences of at most as many on the mean, else 256 (st_kv_chunk.cu).  Split while that leaves SMs idle, down to 256 keys, and if the
+    steps of 128 keys that it saves (some 2 us each) are worth the join (a launch, and every row's partial results through memory: 512
+    queries of a prompt 21 us, in two splits 27; behind 4000 tokens 95 and 66)."""
     seqs = max(1, seqs)
     rows = -(-tokens * group // seqs)                       # of a sequence, on the mean
     ctas = kv_heads * seqs * -(-rows // (32 if rows <= 32 else 256))
-    return max(1, min(sms // max(1, ctas), max_pages // 16, 64))
+    n = min(sms // max(1, ctas), max_pages // 16, 64)
+    if n < 2:
+        return 1
+    steps = (16 * max_pages - tokens // (2 * seqs)) / 128
+    return n if 2.0 * steps * (1 - 1 / n) > 5 + 3e-4 * tokens * group * kv_heads * n else 1
 
 
 class PageStore8:

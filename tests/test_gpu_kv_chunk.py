@@ -137,6 +137,39 @@ def test_escapes_and_chains(new):
     assert torch.equal(out[0].view(4, 2, D)[:, 0], flat.V[0][0]) and torch.equal(out[0].view(4, 2, D)[:, 1], flat.V[0][0])
 
 
+@pytest.mark.parametrize("new", [4, 90])
+@pytest.mark.parametrize("tiny", [3, 14, 40])
+def test_rows_that_were_appended_again(new, tiny):
+    """a row rewritten in place leaves its old escapes in the list, before the new ones of the same elements: the attention reads what the
+    pages decode to (tiny escapes a row and half: in the unit's slots, beyond them, and in chains)"""
+    s = Setup(8, 2, [new], [200], seed=14)
+    i = torch.arange(200, device="cuda")
+    slots = s.table[0].long()[i // PAGE] * PAGE + i % PAGE
+    K, V = kv_values(200, 2, 5, dead=False)
+    for t in (K, V):
+        t[:, :, :tiny] = (t[:, :, :tiny].float() * 1e-7).to(torch.bfloat16)
+    s.store.append(K, V, slots)
+    again = torch.tensor([17, 18, 37, 190, 199], device="cuda")             # (not the first of their pages)
+    for times in range(2):
+        for t in (K, V):
+            t[again] = (t[again].float() * -1.5).to(torch.bfloat16)
+        for j in again.tolist():
+            s.store.append(K[j:j + 1], V[j:j + 1], slots[j:j + 1])
+    s.store.check()
+    Kd, Vd = s.store.dense()
+    Kd, Vd = Kd.view(-1, 2, D)[slots], Vd.view(-1, 2, D)[slots]
+    assert torch.equal(Kd, K) and torch.equal(Vd, V)
+    s.K, s.V = [Kd], [Vd]
+    for splits in (1, 3):
+        s.check(s.call(splits=splits))
+    one = Setup(8, 2, [1], [1], seed=15)                                    # one key: its value comes back exactly
+    one.store, one.table, one.l32 = s.store, (slots[199:200] // PAGE).int()[None], torch.tensor([16], dtype=torch.int32, device="cuda")
+    start = torch.tensor([int(slots[199] % PAGE)], dtype=torch.int32, device="cuda")
+    one.l32 = start + 1
+    out = one.store.chunk_attention(one.q, one.cu, one.table, one.l32, one.scale, starts=start)
+    assert torch.equal(out[0].view(2, 4, D), V[199][:, None].expand(2, 4, D))
+
+
 @pytest.mark.parametrize("new", [3, 70])
 @pytest.mark.parametrize("junk", [float("nan"), float("inf"), -float("inf"), 3e38])
 def test_values_in_masked_places(new, junk):
