@@ -315,14 +315,15 @@ int st_gemm_epilogue(const void* tree, const int32_t* eo, const uint32_t* el, co
  * are rows cu[b] .. cu[b + 1] - 1, the last at position lens[b] - 1 (cu NULL: one each).  A query at position p sees keys
  * [max(starts, p - window + 1), p] (starts int32 [B] or NULL; window 0: from starts on); one that sees none gives zeros.  bt int32: rows
  * of btw entries, bts apart (0: one row for all); keys beyond a row's pages take no part.  Rows of q behind cu[B] are left alone in
- * out.  S splits of every sequence; wo float [T, Hq, S, 128] and wml float [T, Hq, S, 2] when S > 1
+ * out.  S splits of every unit (a tile of 256 rows, or of 32 where sequences have at most as many on the mean, and a KV head) but the
+ * first `whole`, which are the last tiles of the last sequences; wo float [T, Hq, S, 128] and wml float [T, Hq, S, 2] when S > 1
  * (st_kv_chunk_attn_workspace_bytes is what both take).  Any number of query heads per KV head.  No counterpart in the reference,
  * whose backend decodes cached pages into BF16 ones for a library kernel (statetree/vllm_kv.py:208-225). */
 int64_t st_kv_chunk_attn_workspace_bytes(int64_t T, int64_t Hq, int64_t S);
 int st_kv_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv, int64_t nblocks,
                      int64_t Hkv, const uint32_t* pool, int64_t P, const int32_t* bt, int64_t btw, int64_t bts, const int32_t* lens,
                      const int32_t* starts, int64_t window, void* out, int64_t os, float* wo, float* wml, double scale, int64_t S,
-                     void* stream);
+                     int64_t whole, void* stream);
 
 /* Rotary positions of N tokens' queries [N, Hq, D] and keys [N, Hk, D] (either may have no heads): the pairs of the values offset ..
  * offset + part - 1 of every head, (2i, 2i + 1) of them (interleaved) or (i, i + part / 2), become (a c - b s, a s + b c) with the float32

@@ -392,7 +392,7 @@ py::object fused(const Library& lib, bool use_gemm, const at::Tensor& tree, cons
 
 // ---- lossless KV pages: attention of cu's rows (None: one query per sequence), pages uint8 [blocks, H, 2, 2, 1600], pool int32 [P, 16]
 py::object kv_chunk_attention(const Library& lib, const at::Tensor& pages, const at::Tensor& pool, const at::Tensor& q, const Maybe& cu,
-                              const at::Tensor& table, const at::Tensor& lens, double scale, int64_t splits, const Maybe& starts,
+                              const at::Tensor& table, const at::Tensor& lens, double scale, int64_t splits, int64_t whole, const Maybe& starts,
                               const Maybe& given, int64_t window) {
   constexpr int64_t D = 128;
   const at::Device device = pages.device();
@@ -420,7 +420,7 @@ py::object kv_chunk_attention(const Library& lib, const at::Tensor& pages, const
     }
     rc = lib.kv_chunk(q.const_data_ptr(), q.stride(0), T, Hq, of<int32_t>(cu), B, pages.const_data_ptr(), pages.size(0), H,
                       of<uint32_t>(pool), pool.size(0), of<int32_t>(table), table.size(1), table.stride(0), of<int32_t>(lens),
-                      of<int32_t>(starts), window, out.data_ptr(), out.stride(0), wo, wml, scale, splits,
+                      of<int32_t>(starts), window, out.data_ptr(), out.stride(0), wo, wml, scale, splits, whole,
                       c10::cuda::getCurrentCUDAStream(device.index()).stream());
   }
   check(lib, rc);

@@ -96,12 +96,11 @@ struct Work : Rows8 {
   int h, split, pos0;                                             // position of query 0
   int lo0, first_tile, tiles, count0, count1;                     // key tiles of the split; of those, how many each row tile needs
 };
-// false: the CTA has no rows.  Later tiles (of TILE rows) of a sequence see more keys: they go first
+// part `split` of `splits` of unit x (a tile of TILE rows and a KV head).  false: there are no such rows.  Later tiles of a sequence see more
+// keys: they go first
 template <int TILE>
-__device__ __forceinline__ bool chunk_work(const Attn8& a, int splits, int slots, int G, int lane, Work& w) {
-  int x = blockIdx.x;
-  w.split = x % splits;
-  x /= splits;
+__device__ __forceinline__ bool chunk_work(const Attn8& a, int x, int split, int splits, int slots, int G, int lane, Work& w) {
+  w.split = split;
   w.h = x % a.H;
   if (!find_rows<TILE>(a, G, slots - 1 - x / a.H, lane, w)) return false;
   const int start = w.start;

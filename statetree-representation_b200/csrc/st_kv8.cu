@@ -769,6 +769,7 @@ __global__ void __launch_bounds__(MERGE8 * 32) kv8_merge_kernel(const float* __r
   if (row >= rows) return;                                        // (WPR = 4: one row per CTA, never beyond)
   if (cu && (row / Hq < cu[0] || row / Hq >= cu[B])) return;      // rows of no sequence (the whole CTA with WPR = 4)
   const float* const ml = part_ml + row * splits * 2;
+  if (ml[1] < 0.f) return;                                        // a row that was not split: its output stands already
   const float* const po = part_o + row * splits * D + PL * lane;
   float top = -INFINITY;
   for (int j = lane; j < splits; j += 32) top = fmaxf(top, ml[2 * j]);

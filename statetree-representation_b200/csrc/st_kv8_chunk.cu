@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
   pdl_launch_dependents();
 
   Work w;
-  if (!chunk_work<2 * ROWS>(a, c.parts.splits, c.slots, G, lane, w)) return;
+  if (!chunk_work<2 * ROWS>(a, blockIdx.x / c.parts.splits, blockIdx.x % c.parts.splits, c.parts.splits, c.slots, G, lane, w)) return;
   const int tiles = max(w.count0, w.count1);
   // (pages behind the last key of the sequence, or behind its row of the table, may not exist: no key of theirs is seen)
   const int end_page = min((w.pos0 + w.n - 1) / PAGE + 1, a.table_width);

@@ -27,11 +27,11 @@ template <bool NARROW>
 struct Roles {
   static constexpr int CONV = NARROW ? 4 : 8, CONVERTERS = NARROW ? 2 * TILE_PAGES : TILE_PAGES;
   static constexpr int MMA = CONV + CONVERTERS, FETCH = MMA + 1, WARPS = MMA + 4, FETCHERS = WARPS - FETCH, GROUPS = WARPS / 4;
-  static constexpr int R_START = 65536 / (WARPS * 32) / 8 * 8, R_SOFTMAX = NARROW ? 112 : 160, R_CONV = NARROW ? 80 : 64, R_MMA = 32;
+  static constexpr int R_START = 65536 / (WARPS * 32) / 8 * 8, R_SOFTMAX = NARROW ? 112 : 152, R_CONV = NARROW ? 80 : 72, R_MMA = 32;
   static_assert(CONV / 4 * R_SOFTMAX + CONVERTERS / 4 * R_CONV + R_MMA <= GROUPS * R_START, "more registers than there are");
 };
 struct Pool { const uint32_t* at; int blocks; };
-struct ChunkArgs { Attn8 a; Parts8 parts; Pool pool; int* status; int slots; };
+struct ChunkArgs { Attn8 a; Parts8 parts; Pool pool; int* status; int slots, whole; };           // whole: units that are not split, the first ones
 
 // P is relative to a row's reference, the largest score seen up to RAISE before (base 2; BF16 has fp32's range: no lower bound is needed)
 constexpr float RAISE = 8.f;
@@ -123,10 +123,11 @@ __device__ __forceinline__ void page_edge(uint32_t (&A)[2][4][4], int first, int
 // takes some 270 cycles: one warp for all sixteen of a key tile would be the limit).
 // NARROW: keys and values have slots of their own (the second set where the second row tile's q would be), so that a page's values come in while
 // its keys are decoded: these pages are read once, from memory, not by many CTAs from L2.
+struct Kept { int row0, rows, first, h, split, splits; };        // of Work, for the way out; splits: of this unit
 struct LayX : Tiles<HD> {
   static constexpr int RAW = Tiles<HD>::END, SLOT_BYTES = 2 * RKV;                                 // a slot per page of a key tile
-  static constexpr int BARS = RAW + 8 * SLOT_BYTES, NBARS = ChunkBars::COUNT + 34, SLOT = BARS + NBARS * 8;
-  static constexpr int BYTES = SLOT + 16 + 1024;
+  static constexpr int BARS = RAW + 8 * SLOT_BYTES, NBARS = ChunkBars::COUNT + 34, SLOT = BARS + NBARS * 8, KEPT = SLOT + 16;
+  static constexpr int BYTES = KEPT + 48 + 1024;
   static __device__ __forceinline__ int slot(int set, int page) { return (set ? Q + TILE : RAW) + page * SLOT_BYTES; }
 };
 
@@ -200,13 +201,16 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
   pdl_wait();
   pdl_launch_dependents();
   Work w;
-  if (!chunk_work<NARROW ? FEW : 2 * ROWS>(a, c.parts.splits, c.slots, G, lane, w)) return;
+  // (a unit that is not split, among ones that are, leaves a mark for the join: no sum is negative)
+  const int splits = (int)blockIdx.x < c.whole ? 1 : c.parts.splits, x = (int)blockIdx.x - c.whole;
+  if (!chunk_work<NARROW ? FEW : 2 * ROWS>(a, x < 0 ? blockIdx.x : c.whole + x / splits, x < 0 ? 0 : x % splits, splits, c.slots, G, lane, w)) return;
   const int tiles = max(w.count0, w.count1);
   // (pages behind the last key of the sequence, or behind its row of the table, may not exist: no key of theirs is seen)
   const int end_page = min((w.pos0 + w.n - 1) / PAGE + 1, a.table_width);
   const uint64_t keep = policy_evict_last();                      // other row tiles of the sequence read the same pages
 
   if (warp == R::MMA) {
+    if (lane == 0) *reinterpret_cast<Kept*>(smem + L::KEPT) = {w.row0, w.rows, w.first, w.h, w.split, splits};
     if (elect_one()) {
       mbar_init(qfull, 4);
       mbar_init(qfull + 1, 4);
@@ -228,8 +232,7 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
     // ---------------------------------------------------------------- softmax: this thread's row
     const int t = warp >> 2, count = t ? w.count1 : w.count0, my = w.row0 + (NARROW ? lane : t * ROWS + (warp & 3) * 32 + lane);
     const bool live = my < w.row0 + w.rows;
-    const int token = live ? my / G : 0, head = live ? my % G : 0, hq = w.h * G + head;
-    const int pos = w.pos0 + token;
+    const int pos = w.pos0 + (live ? my / G : 0);
     // (a row that is none sees everything: its results go nowhere, and a warp with one does not take the masked way for it)
     const int hi = live ? min(pos, a.table_width * PAGE - 1) : 0x7FFFFFFF, lo = !live ? 0 : window_from(a.window, pos, w.lo0);
     const bool any = __any_sync(FULL, live);
@@ -346,11 +349,22 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
     }
     if (ok && count > 0) ok = mbar_wait(b.ofull + t, 0);
     if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_ACC);
-    // ---- out.  (a wait that ran out leaves the rows unwritten)
+    // ---- out (a wait that ran out leaves the rows unwritten).  Where the rows go comes back from shared memory: held across the loop it cost
+    // registers there (2048 queries behind 30000 tokens 1180 us, so 1117)
+    const Kept& kept = *reinterpret_cast<const Kept*>(smem + L::KEPT);
+    Work o;
+    Parts8 parts = c.parts;
+    o.row0 = kept.row0; o.rows = kept.rows; o.first = kept.first; o.h = kept.h; o.split = kept.split;
+    parts.splits = kept.splits;
+    const int row = o.row0 + (NARROW ? lane : t * ROWS + (warp & 3) * 32 + lane), of = a.Hq / a.H;
+    const bool mine = row < o.row0 + o.rows;
+    const int token = mine ? row / of : 0, hq = o.h * of + (mine ? row % of : 0);
+    if (kept.splits < c.parts.splits && mine && (!NARROW || warp == 0))
+      c.parts.ml[((long long)(o.first + token) * a.Hq + hq) * c.parts.splits * 2 + 1] = -1.f;
     if (NARROW) {
-      narrow_store(a, c.parts, w, smem, warp, lane, ok, count, to, m, l);
+      narrow_store(a, parts, o, smem, warp, lane, ok, count, to, m, l);
     } else if (ok && any) {
-      chunk_store<D>(a, c.parts, w, smem, t, warp, lane, live, token, hq, count, to, m, l);
+      chunk_store<D>(a, parts, o, smem, t, warp, lane, mine, token, hq, count, to, m, l);
     }
     tc_fence_before();
   } else if (warp < R::MMA) {
@@ -483,10 +497,12 @@ int opt_in(Kernel* kernel, int bytes, int regs, std::atomic<uint64_t>& set) {
   return 0;
 }
 template <bool NARROW>
-int chunk_launch(ChunkArgs& c, long long ctas, cudaStream_t st_) {
+int chunk_launch(ChunkArgs& c, long long units, cudaStream_t st_) {
   static std::atomic<uint64_t> set{0};
+  c.slots = (int)(units / c.a.H);
+  const long long whole = c.whole < units ? c.whole : units, ctas = whole + (units - whole) * c.parts.splits;
   ST_REQUIRE(ctas < (1ll << 31), "st_kv_chunk_attn: grid too large");
-  c.slots = (int)(ctas / c.a.H / c.parts.splits);
+  c.whole = (int)whole;
   if (int e = opt_in(kv_chunk_kernel<NARROW>, LayX::BYTES, Roles<NARROW>::R_START, set)) return e;
   return st::launch("st_kv_chunk_attn launch", kv_chunk_kernel<NARROW>, dim3((unsigned)ctas), dim3(Roles<NARROW>::WARPS * 32), (size_t)LayX::BYTES, st_, c);
 }
@@ -499,13 +515,13 @@ extern "C" int64_t st_kv_chunk_attn_workspace_bytes(int64_t T, int64_t Hq, int64
 extern "C" int st_kv_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq, const int32_t* cu, int64_t B, const void* kv, int64_t nblocks,
                                 int64_t Hkv, const uint32_t* pool, int64_t P, const int32_t* bt, int64_t btw, int64_t bts,
                                 const int32_t* lens, const int32_t* starts, int64_t window, void* out, int64_t os, float* wo, float* wml,
-                                double scale, int64_t S, void* stream) {
+                                double scale, int64_t S, int64_t whole, void* stream) {
   const char* who = "st_kv_chunk_attn";
   ChunkArgs c;
   if (int e = st::attn8_args(c.a, who, q, qs, T, Hq, cu, B, kv, (const int8_t*)kv, nblocks, Hkv, HD, bt, btw, bts, lens, starts, window, out, os,
                              scale))
     return e;
-  ST_REQUIRE(S >= 1 && S <= 1024, "%s: splits must be in [1, 1024]", who);
+  ST_REQUIRE(S >= 1 && S <= 1024 && whole >= 0, "%s: splits must be in [1, 1024], unsplit units not negative", who);
   if (T == 0 || B == 0) return 0;
   ST_REQUIRE(pool && P >= 0 && P < (1ll << 31), "%s: null pointer (pool)", who);
   ST_REQUIRE(S == 1 || (wo && wml && st::aligned16(wo)), "%s: split workspace (wo, wml) missing or unaligned", who);
@@ -514,13 +530,15 @@ extern "C" int st_kv_chunk_attn(const void* q, int64_t qs, int64_t T, int64_t Hq
   c.a.scale_log2 = fmaxf(c.a.scale_log2, FLT_MIN);                // (it multiplies the -inf of what a row does not see)
   c.parts = {wo, wml, (int)S, 1};
   c.pool = {pool, (int)P};
+  c.whole = S == 1 ? 0 : (int)(whole < (1ll << 30) ? whole : 1ll << 30);
   c.status = st::status_ptr();
   ST_REQUIRE(c.status != nullptr, "%s: no device status word", who);
   const long long G = Hq / Hkv;
   ST_REQUIRE(T * G < (1ll << 31), "%s: too large", who);
   const cudaStream_t st_ = (cudaStream_t)stream;
-  auto ctas_of = [&](long long rows) { return (T * G / rows + B) * Hkv * S; };                // (every sequence may leave a tile unfilled)
-  const int e = T * G <= FEW * B ? chunk_launch<true>(c, ctas_of(FEW), st_) : chunk_launch<false>(c, ctas_of(2 * ROWS), st_);
+  auto units_of = [&](long long rows) { return (T * G / rows + B) * Hkv; };                   // (every sequence may leave a tile unfilled)
+  ST_REQUIRE(units_of(FEW) < (1ll << 31), "%s: grid too large", who);
+  const int e = T * G <= FEW * B ? chunk_launch<true>(c, units_of(FEW), st_) : chunk_launch<false>(c, units_of(2 * ROWS), st_);
   if (e || S == 1) return e;
   return st::merge8("st_kv_chunk_attn merge launch", c.a, c.parts, HD, st_);
 }

@@ -80,11 +80,13 @@ class PageStore:
         sequence b's rows are cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1]; None: one each), the last of them at position lens[b] - 1 ->
         [T, Hq, 128].  A query at position p sees tokens [max(starts, p - window + 1), p] (window 0: from starts on), one that sees none
         gives zeros; rows behind cu[B] of a given `out` stay as they are.  splits: how many CTAs share a sequence (None: by the sizes)"""
+        whole = 0
         if splits is None:
-            splits = chunk_splits(q.shape[0], block_table.shape[0], self.H, q.shape[1] // self.H, block_table.shape[1])
+            splits, whole = chunk_splits(q.shape[0], block_table.shape[0], self.H, q.shape[1] // self.H, block_table.shape[1])
         host = calls()
         if host is not None:
-            done = host[0].kv_chunk_attention(host[1], self.pages, self.pool, q, cu, block_table, lens, scale, splits, starts, out, window)
+            done = host[0].kv_chunk_attention(host[1], self.pages, self.pool, q, cu, block_table, lens, scale, splits, whole, starts, out,
+                                              window)
             if done is not None:
                 return done
         q = _rows(q, 128)
@@ -93,7 +95,7 @@ class PageStore:
         need = lib().st_kv_chunk_attn_workspace_bytes(q.shape[0], q.shape[1], splits) // 4
         flat = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
         wo, wml = (flat[:need // 130 * 128], flat[need // 130 * 128:]) if need else (None, None)
-        kv_ext().chunk_attn(q, cu, self.pages, self.pool, block_table, lens, out, scale, splits, wo, wml, starts, window)
+        kv_ext().chunk_attn(q, cu, self.pages, self.pool, block_table, lens, out, scale, splits, wo, wml, starts, window, whole)
         return out
 
     def dense(self, blocks=None):
@@ -158,18 +160,33 @@ def chunk_splits8(tokens, seqs, kv_heads, group, max_pages, sms=148):
 
 
 def chunk_splits(tokens, seqs, kv_heads, group, max_pages, sms=148):
-    """How many CTAs share a sequence of the chunk attention over lossless pages, from what the host knows.  A CTA takes an SM: 32 rows for
-    sequences of at most as many on the mean, else 256 (st_kv_chunk.cu).  Split while that leaves SMs idle, down to 256 keys, and if the
-    steps of 128 keys that it saves (some 2 us each) are worth the join (a launch, and every row's partial results through memory: 512
-    queries of a prompt 21 us, in two splits 27; behind 4000 tokens 95 and 66)."""
+    """(splits, whole) of the chunk attention over lossless pages, from what the host knows: how many CTAs share a unit of it, and how many
+    units, the first ones, are not split.  A CTA takes an SM: 32 rows of a KV head for sequences of at most as many on the mean, else 256
+    (st_kv_chunk.cu).  A step of 128 keys takes some 2 us, a CTA 10 besides; a join takes a launch, and every row's partial results go through
+    memory.  Fewer units than SMs: split while that leaves SMs idle, down to 256 keys (512 queries behind 4000 tokens 95 us, in two 66;
+    behind none 21 and 27).  A last wave that is part-filled, behind a long context: the full waves whole, the rest in as many splits as
+    finish soonest (2048 queries behind 30000 tokens, 256 units on 148 SMs)."""
     seqs = max(1, seqs)
     rows = -(-tokens * group // seqs)                       # of a sequence, on the mean
-    ctas = kv_heads * seqs * -(-rows // (32 if rows <= 32 else 256))
-    n = min(sms // max(1, ctas), max_pages // 16, 64)
-    if n < 2:
-        return 1
-    steps = (16 * max_pages - tokens // (2 * seqs)) / 128
-    return n if 2.0 * steps * (1 - 1 / n) > 5 + 3e-4 * tokens * group * kv_heads * n else 1
+    tile = 32 if rows <= 32 else 256
+    units, steps = kv_heads * seqs * -(-rows // tile), (16 * max_pages - tokens // (2 * seqs)) / 128
+    if units < 1:
+        return 1, 0
+    n = min(sms // units, max_pages // 16, 64)
+    if n >= 2:
+        return (n, 0) if 2.0 * steps * (1 - 1 / n) > 5 + 3e-4 * tokens * group * kv_heads * n else (1, 0)
+    rest, before = units % sms, (16 * max_pages - tokens // seqs) / 128
+    if rest == 0 or units > 4 * sms or before < 32:
+        return 1, 0
+    best, saved = 1, 0.0
+    for n in (2, 3, 4, 5):
+        gain = (1 - -(-rest * n // sms) / n) * 2.0 * before - (-(-rest * n // sms) - 1) * 10 - 5 - 3e-4 * min(tokens * group * kv_heads, rest * tile) * n
+        if gain > saved:
+            best, saved = n, gain
+    if best == 1:
+        return 1, 0
+    empty = tokens * group // tile + seqs - units // kv_heads if seqs == 1 else 0      # (slots without rows come first)
+    return best, units - rest + empty * kv_heads
 
 
 class PageStore8:

@@ -80,7 +80,7 @@ _SIGNATURES = {
     "st_gemm_epilogue": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _i64, _vp]),
     "st_kv_chunk_attn_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "st_kv_chunk_attn": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp,
-                                _vp, _dbl, _i64, _vp]),
+                                _vp, _dbl, _i64, _i64, _vp]),
     "st_rotate": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _i64, _i64, _i64, _int, _int,
                          _vp, _vp, _dbl, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
     "st_moe_align": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
@@ -685,7 +685,7 @@ class _KV:
         return kv.shape[1]
 
     @staticmethod
-    def chunk_attn(q, cu, kv, pool, bt, lens, out, scale, S=1, wo=None, wml=None, starts=None, window=0):
+    def chunk_attn(q, cu, kv, pool, bt, lens, out, scale, S=1, wo=None, wml=None, starts=None, window=0, whole=0):
         """causal attention of the query rows cu[b] .. cu[b + 1] - 1 of every sequence b, q [T, Hq, 128], over the lossless pages"""
         who = "kv_chunk_attn"
         H = _KV._pages(who, kv, pool, q, cu, bt, lens, out, starts, wo, wml)
@@ -695,7 +695,7 @@ class _KV:
         if Hq % H or Hq == 0 or out.shape != q.shape:
             raise RuntimeError(f"{who}: q and out [tokens, a multiple of {H} heads, 128]")
         _KV._table(who, bt, lens, starts)
-        if window < 0 or S < 1:
+        if window < 0 or S < 1 or whole < 0:
             raise RuntimeError(f"{who}: window / splits")
         if cu is None and T != B:
             raise RuntimeError(f"{who}: without cu every sequence has one query")
@@ -709,7 +709,7 @@ class _KV:
         with _ctx(kv):
             _check(lib().st_kv_chunk_attn(q.data_ptr(), q.stride(0), T, Hq, _ptr(cu), B, kv.data_ptr(), kv.size(0), H, pool.data_ptr(),
                                           pool.size(0), bt.data_ptr(), bt.size(1), bt.stride(0), lens.data_ptr(), _ptr(starts), int(window),
-                                          out.data_ptr(), out.stride(0), _ptr(wo), _ptr(wml), float(scale), int(S), _stream(q)))
+                                          out.data_ptr(), out.stride(0), _ptr(wo), _ptr(wml), float(scale), int(S), int(whole), _stream(q)))
 
     @staticmethod
     def _table(who, bt, lens, starts):

@@ -137,6 +137,23 @@ def test_escapes_and_chains(new):
     assert torch.equal(out[0].view(4, 2, D)[:, 0], flat.V[0][0]) and torch.equal(out[0].view(4, 2, D)[:, 1], flat.V[0][0])
 
 
+@pytest.mark.parametrize("heads,kv,new,lens", [(8, 2, [300, 7, 0, 200], [400, 300, 9, 260]), (4, 2, [5, 3], [200, 90])])
+@pytest.mark.parametrize("whole", [1, 2, 5, 1000])
+def test_units_that_are_not_split(heads, kv, new, lens, whole, monkeypatch):
+    """some units whole, the others split, ragged; both host paths; rows behind the last sequence"""
+    from statetree_b200 import kvcache
+    s = Setup(heads, kv, new, lens, seed=16, tail=3)
+    for splits in (2, 3):
+        monkeypatch.setattr(kvcache, "chunk_splits", lambda *a: (splits, whole))
+        buf = torch.full((s.q.shape[0], heads, D), 3.0, dtype=torch.bfloat16, device="cuda")
+        s.check(s.call(out=buf))
+        assert bool((buf[sum(new):] == 3).all())
+        native = kvcache.calls
+        monkeypatch.setattr(kvcache, "calls", lambda: None)
+        assert torch.equal(s.call()[:sum(new)], buf[:sum(new)])
+        monkeypatch.setattr(kvcache, "calls", native)
+
+
 @pytest.mark.parametrize("new", [4, 90])
 @pytest.mark.parametrize("tiny", [3, 14, 40])
 def test_rows_that_were_appended_again(new, tiny):
