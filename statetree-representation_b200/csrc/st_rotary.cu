@@ -5,9 +5,10 @@
 // Bound by HBM: every value is read once and written once.  A lane owns VEC pairs (two 16-byte vectors) of a head, so that a pair
 // never crosses lanes in either layout and the norm needs one reduction over the head's lanes; a warp walks the heads of ONE token, whose
 // cosines and sines stay in registers.  Few tokens: the heads of a token are dealt to several warps.
-// Measured, us in a graph (BF16, heads of 128): 32764 tokens of 32 + 8 heads 111 = 6.1 TB/s (a copy of as many bytes 105), with norms 121;
-// 8190 tokens of 16 + 16 heads 26.7 (copy 24.7); 1261 tokens of 64 heads of 80, 32 of them rotated, 8.5; one token 2.9.  Two heads in flight
-// and 24 warps an SM; with norms one and 32 (two and 24: 129; the weights in registers 143; four in flight and 16 warps 159).
+// Measured, us in a graph (BF16, heads of 128): 32764 tokens of 32 + 8 heads 111 = 6.1 TB/s (a copy of as many bytes 105), with norms 118;
+// 8190 tokens of 16 + 16 heads 26.8 (copy 24.7); 1261 tokens of 64 heads of 80, 32 of them rotated, 8.9; one token 2.9.  Two heads in flight
+// and 24 warps an SM; with norms, whose arithmetic fills three quarters of the issue slots (two pairs an instruction: one 121), one and 32
+// (two and 24: 130; the weights in registers 143; four in flight and 16 warps 159).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -123,16 +124,16 @@ __global__ void __launch_bounds__(THREADS, NORM ? 4 : 3) rotate_kernel(const Rot
   };
 #pragma unroll
   for (int i = 0; i < U; ++i) load(p0 + i, u[i]);
-  float c[VEC], s[VEC];
+  uint64_t c[VEC / 2], s[VEC / 2];                 // of two pairs each: cosines, sines
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) { c[i] = 1.f; s[i] = 0.f; }
+  for (int i = 0; i < VEC / 2; ++i) { c[i] = pair2(1.f, 1.f); s[i] = 0; }
   if (rot && here) {
     const long long row = place(a, n) * half + s0;
 #pragma unroll
-    for (int i = 0; i < VEC; i += 4) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(a.cos_t + row + i)), y = __ldg(reinterpret_cast<const float4*>(a.sin_t + row + i));
-      c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
-      s[i] = a.sign * y.x; s[i + 1] = a.sign * y.y; s[i + 2] = a.sign * y.z; s[i + 3] = a.sign * y.w;
+    for (int i = 0; i < VEC / 2; i += 2) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(a.cos_t + row + 2 * i)), y = __ldg(reinterpret_cast<const float4*>(a.sin_t + row + 2 * i));
+      c[i] = pair2(x.x, x.y); c[i + 1] = pair2(x.z, x.w);
+      s[i] = pair2(a.sign * y.x, a.sign * y.y); s[i + 1] = pair2(a.sign * y.z, a.sign * y.w);
     }
   }
   for (int p = p0; p < p1; p += U) {
@@ -141,33 +142,53 @@ __global__ void __launch_bounds__(THREADS, NORM ? 4 : 3) rotate_kernel(const Rot
       float f[2 * VEC];
       unpack<T>(u[i][0], f);
       unpack<T>(u[i][1], f + VEC);
+      // pair k is (f[2k], f[2k + 1]) or (f[k], f[VEC + k]); two pairs at a time
+      auto first = [](int k) { return PAIRS ? 2 * k : k; };
+      auto other = [](int k) { return PAIRS ? 2 * k + 1 : VEC + k; };
+      uint64_t x[VEC / 2], y2[VEC / 2];
+#pragma unroll
+      for (int k = 0; k < VEC / 2; ++k) {
+        x[k] = pair2(f[first(2 * k)], f[first(2 * k + 1)]);
+        y2[k] = pair2(f[other(2 * k)], f[other(2 * k + 1)]);
+      }
       int kv;
       const int h = head_of(p + i, kv);
       load(p + i + U, u[i]);
       if constexpr (NORM) {
-        float ss = 0.f;
+        uint64_t sq = 0;
 #pragma unroll
-        for (int k = 0; k < 2 * VEC; ++k) ss = __fmaf_rn(f[k], f[k], ss);
+        for (int k = 0; k < VEC / 2; ++k) sq = fma2(y2[k], y2[k], fma2(x[k], x[k], sq));
+        float q0, q1;
+        unpair2(sq, q0, q1);
+        float ss = q0 + q1;
         for (int o = a.lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
         const T* const wt = reinterpret_cast<const T*>(a.s[kv].w);
         if (h >= 0 && wt) {                        // (from L1: held in registers they cost a quarter of the resident warps)
           const float r = rsqrtf(ss * inv_d + a.eps);
+          const uint64_t r2 = pair2(r, r);
           float g[2 * VEC];
           unpack<T>(__ldg(reinterpret_cast<const uint4*>(wt + d0)), g);
           unpack<T>(second ? __ldg(reinterpret_cast<const uint4*>(wt + d1)) : make_uint4(0, 0, 0, 0), g + VEC);
 #pragma unroll
-          for (int k = 0; k < 2 * VEC; ++k) f[k] = f[k] * r * g[k];
+          for (int k = 0; k < VEC / 2; ++k) {
+            x[k] = mul2f(mul2f(x[k], r2), pair2(g[first(2 * k)], g[first(2 * k + 1)]));
+            y2[k] = mul2f(mul2f(y2[k], r2), pair2(g[other(2 * k)], g[other(2 * k + 1)]));
+          }
         }
       }
       if (h < 0) continue;
       if (rot) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const int i0 = PAIRS ? 2 * k : k, i1 = PAIRS ? 2 * k + 1 : VEC + k;
-          const float x = f[i0], y = f[i1];
-          f[i0] = __fmaf_rn(x, c[k], -__fmul_rn(y, s[k]));
-          f[i1] = __fmaf_rn(x, s[k], __fmul_rn(y, c[k]));
+        for (int k = 0; k < VEC / 2; ++k) {
+          const uint64_t t = fma2(x[k], c[k], mul2f(y2[k], s[k]) ^ 0x8000000080000000ull);
+          y2[k] = fma2(x[k], s[k], mul2f(y2[k], c[k]));
+          x[k] = t;
         }
+      }
+#pragma unroll
+      for (int k = 0; k < VEC / 2; ++k) {
+        unpair2(x[k], f[first(2 * k)], f[first(2 * k + 1)]);
+        unpair2(y2[k], f[other(2 * k)], f[other(2 * k + 1)]);
       }
       T* const y = reinterpret_cast<T*>(a.s[kv].y) + n * a.s[kv].yt + h * a.s[kv].yh;
       *reinterpret_cast<uint4*>(y + d0) = pack<T>(f);

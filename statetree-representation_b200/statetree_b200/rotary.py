@@ -110,8 +110,10 @@ def rotate(q, k, positions, cos, sin, interleaved=True, offset=0, q_norm=None, k
     fp32 arithmetic, rounded once.  out: (q, k) outputs; an output may be its input.  inverse: by the opposite angles, so that it undoes
     a rotation (by tables without an amplitude).
 
-    Gradients flow to q and k (not through norms, and not with `out`, which are refused); they are the inverse rotation."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_norm, k_norm)):
+    Gradients flow to q and k (not through norms, and not with `out`, which are refused); they are the inverse rotation.  As for every
+    function: before backward() is captured into a CUDA graph, let go of eager graphs over the same leaves."""
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad) or (q_norm is not None and q_norm.requires_grad)
+                                    or (k_norm is not None and k_norm.requires_grad)):
         if q_norm is not None or k_norm is not None or out is not None:
             raise RuntimeError("rotate: gradients flow through the rotation alone (without norms and given outputs)")
         host = calls() if k is not None else None
