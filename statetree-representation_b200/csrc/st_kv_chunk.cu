@@ -1,13 +1,25 @@
 // Causal attention of several query tokens per sequence straight over the lossless KV pages: prompts, their chunks, speculative tokens.
 //     o = sum_j p_j v_j,  p = softmax_j(scale q . k_j),  j over [max(start, position - window + 1), position]
 // on tcgen05, 128 keys a step; pages are decoded into BF16 operand tiles in shared memory.  Two forms, by the rows (query token, head of the
-// group) per sequence: 256 rows a CTA, or (NARROW) 32.
-// Keys and values are exactly what was appended (BF16), scores are fp32 sums of exact products.  P is rounded to BF16 for the matrix
-// instruction that V's type asks for: 2^-9 of each probability at most, of either sign (its sum is of the fp32 values), below the rounding
-// of the output.  Everything else is fp32.
+// group) per sequence: 256 rows a CTA, or (NARROW) 32.  The division of the work, the tensor-memory columns, the hand-overs and the products are
+// those of the attention over 8-bit pages (st_chunk_tc.cuh, st_kv8_chunk.cu).
+// Keys and values are exactly what was appended (BF16), scores are fp32 sums of exact products.  P is rounded to BF16, the type that the matrix
+// instruction asks for beside V's: by 2^-8 of each probability at most, as the output's own rounding (its sum is of the fp32 values).
+// Everything else is fp32.
 //
 // Keys outside [start, len) of a sequence weigh nothing whatever their rows hold: scores are replaced, not shifted, and V's rows are zeroed
-// on the way into the operands (a probability of 0 times an infinity would be NaN).
+// on the way into the operands (a probability of 0 times an infinity would be NaN).  A value that is no number at a position that the
+// sequence has reaches every query whose keys lie in the same 128.
+//
+// Measured (32 query heads, 8 KV heads), us in a graph: 2048 queries behind 30000 tokens 1095-1120 = 0.94 PFLOP/s, a prompt of 4096 186, nine ragged
+// chunks with windows (7 heads a KV head) 101; 8 x 4 queries over 2900 tokens 33.
+// What bounds it.  A step of 256 rows takes 2.2 us, of which the MMAs fill 1.2: the chain scores -> softmax -> product of a row tile (with the
+// conversion left out 1.9 us a step) and the converters, which share the issue slots with it (50 % used; 250 instructions a page's keys or
+// values; escapes 0.2 us of the step).  A CTA costs some 12 us besides its steps (look-ups, q, filling and draining the two row tiles' chains,
+// output).  32 rows: 1.45 us a step, 4.5 TB/s of pages from 128 SMs, and as much outside the steps as in them.
+// Tried: four converter warps of two pages 1904 us (2048 behind 30000; they wait for one another's latencies), one producer warp 2241; P as high
+// part and residual is a product more; a CTA of 8 or 16 rows on mma.sync, three to an SM, for few rows: 8 x 4 queries 37 us, 32 x 4 over 2000
+// tokens 84 (here 70).
 #include <float.h>
 #include <math.h>
 
@@ -20,7 +32,10 @@
 namespace {
 using namespace st;
 
-constexpr int FEW = 32;                            // rows of a CTA of the narrow form, and per sequence (on the mean) up to which it is taken
+// Rows of a CTA of the narrow form, and per sequence (on the mean) up to which it is taken.  us with 32 / 256 rows a CTA, the better splits of
+// each: 8 rows of 8 sequences of 2900 tokens 32.3 / 33.6, 32 rows 36.7 / 36.7, 64 rows 51.6 / 37.9; 32 rows of 32 sequences 75.5 / 80.9, 64 rows
+// 143 / 82; 32 rows of one 21.9 / 20.0
+constexpr int FEW = 32;
 // Warps of kv_chunk_kernel: of softmax, of conversion (a page of a key tile each; NARROW: its keys or its values), one that issues the MMAs, three
 // producers.  Registers of a warpgroup: what they take up together is at most what the block starts with, a multiple of 8 a thread
 template <bool NARROW>
@@ -116,11 +131,10 @@ __device__ __forceinline__ void page_edge(uint32_t (&A)[2][4][4], int first, int
   for (int i = 0; i < 32; ++i) A[i >> 4][(i >> 2) & 3][i & 3] = ((i & 1) ? x8 : x0) ? A[i >> 4][(i >> 2) & 3][i & 3] : 0u;
 }
 
-// ------------------------------------------------------------------------------------------------ many rows
-// The division of the work, the hand-overs and the products are those of the attention over 8-bit pages (st_chunk_tc.cuh); what differs:
-// there is no factor per page, and the converter warps decode records.  A warp takes one page of every key tile, its keys and then its values,
-// from a slot of its own, which producer warps fill by bulk copies of 3200 bytes as soon as the records before are in registers (an issue
-// takes some 270 cycles: one warp for all sixteen of a key tile would be the limit).
+// ------------------------------------------------------------------------------------------------ the kernel
+// A converter warp takes one page of every key tile, its keys and its values, from a slot of its own (a waiter must never be two phases of a
+// barrier away: a slot has one producer and one consumer), which producer warps fill by bulk copies of 3200 bytes as soon as the records
+// before are in registers (an issue takes some 270 cycles: one warp for all sixteen of a key tile would be the limit).
 // NARROW: keys and values have slots of their own (the second set where the second row tile's q would be), so that a page's values come in while
 // its keys are decoded: these pages are read once, from memory, not by many CTAs from L2.
 struct Kept { int row0, rows, first, h, split, splits; };        // of Work, for the way out; splits: of this unit
