@@ -527,6 +527,16 @@ class _Weights:
         return gap % step >= row(a) and step - gap % step >= row(b)
 
     @staticmethod
+    def _own_memory(t):
+        """does every value of the rows t [N, heads, D] have memory of its own (tokens outside heads or heads outside tokens)"""
+        size = t.size(2)
+        for step, n in sorted((s, n) for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1):
+            if step < size and t.numel():
+                return False
+            size += (n - 1) * step
+        return True
+
+    @staticmethod
     def rotate(q, k, positions, cos, sin, interleaved, offset, inverse, wq, wk, eps, q_out, k_out):
         """q [N, Hq, D] and k [N, Hk, D] (or None) rotated into q_out and k_out"""
         who = "rotate"
@@ -558,8 +568,7 @@ class _Weights:
         outs = [o for _, o, _ in given]
         for i, (t, o, _) in enumerate(given):
             same = o.data_ptr() == t.data_ptr() and o.stride() == t.stride()
-            if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())) or (o.size(1) > 1 and o.stride(1) < D) or (
-                    o.size(0) > 1 and o.stride(0) < (o.size(1) - 1) * o.stride(1) + D):
+            if not _Weights._own_memory(o):
                 raise RuntimeError(f"{who}: an output whose values overlap")
             for j, (x, _, _) in enumerate(given):
                 if not (same if i == j else False) and not _Weights._apart(o, x):

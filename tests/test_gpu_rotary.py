@@ -240,3 +240,22 @@ def test_refusals():
         assert torch.equal(q, before[0]) and torch.equal(k, before[1])
     with pytest.raises(RuntimeError, match="gradients"):
         rotate(q.clone().requires_grad_(), k, pos, cos, sin, k_norm=w)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("N,D", [(1, 64), (2, 64), (37, 64), (37, 80), (130, 128)])
+def test_heads_outside_tokens_in_place(t, N, D):
+    """memory [heads, tokens, D], as attention modules hold it, rotated in place"""
+    from statetree_b200.rotary import rotate
+    q, k = (make(H, N, D, t).transpose(0, 1) for H in (5, 2))
+    before = q.clone(), k.clone()
+    cos, sin = tables(N, 64)
+    pos = torch.arange(N, device="cuda")
+    want = rotate(*before, pos, cos, sin)
+    got = rotate(q, k, pos, cos, sin, out=(q, k))
+    assert got[0] is q and got[1] is k and torch.equal(q, want[0]) and torch.equal(k, want[1])
+    both = make(7, N, D, t)                                  # (q and k beside one another in one buffer)
+    q, k = both[:5].transpose(0, 1), both[5:].transpose(0, 1)
+    want = rotate(q.clone(), k.clone(), pos, cos, sin)
+    rotate(q, k, pos, cos, sin, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])

@@ -92,3 +92,14 @@ def test_outputs_apart():
     assert not apart(buf[:, :3], buf[:, 2:5]) and not apart(buf, buf) and not apart(buf[:, :3], buf[1:, :3])
     assert not apart(buf[:, :, :8], buf[:, :, 4:12])
     assert apart(buf[:0], buf) and apart(torch.zeros(10, 8, 16), buf)
+
+
+def test_output_layouts():
+    """rows whose values have memory of their own, whichever of token and head lies further apart; shared ones are told"""
+    from statetree_b200.ops import _Weights
+    own = _Weights._own_memory
+    buf = torch.zeros(6, 10, 16)
+    assert own(buf) and own(buf.transpose(0, 1)) and own(buf[:, ::2]) and own(buf[:, :, :8]) and own(buf.transpose(0, 1)[:, 1:4])
+    assert own(buf[:1].expand(1, 10, 16)) and own(buf[:0]) and own(buf[:, :1].as_strided((6, 1, 16), (160, 0, 1)))
+    assert not own(buf[:, :1].expand(6, 10, 16)) and not own(buf[:1].expand(6, 10, 16)) and not own(buf.as_strided((6, 4, 16), (32, 16, 1)))
+    assert not own(buf.as_strided((6, 4, 16), (16, 32, 1))) and not own(buf.as_strided((6, 4, 16), (64, 8, 1)))
