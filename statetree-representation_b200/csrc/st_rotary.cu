@@ -7,7 +7,7 @@
 // cosines and sines stay in registers.  Few tokens: the heads of a token are dealt to several warps.
 // Measured, us in a graph (BF16, heads of 128): 32764 tokens of 32 + 8 heads 111 = 6.1 TB/s (a copy of as many bytes 105), with norms 118;
 // 8190 tokens of 16 + 16 heads 26.8 (copy 24.7); 1261 tokens of 64 heads of 80, 32 of them rotated, 8.9; one token 2.9.  Two heads in flight
-// and 24 warps an SM; with norms, whose arithmetic fills three quarters of the issue slots (two pairs an instruction: one 121), one and 32
+// and 24 warps an SM; with norms, whose arithmetic fills 70 % of the issue slots (two pairs an instruction: one 121), one and 32
 // (two and 24: 130; the weights in registers 143; four in flight and 16 warps 159).
 #include <cuda_fp16.h>
 

@@ -79,7 +79,9 @@ class PageStore:
         """causal attention of several query tokens per sequence, after their keys and values have been appended: q [T, Hq, 128] bf16,
         sequence b's rows are cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1]; None: one each), the last of them at position lens[b] - 1 ->
         [T, Hq, 128].  A query at position p sees tokens [max(starts, p - window + 1), p] (window 0: from starts on), one that sees none
-        gives zeros; rows behind cu[B] of a given `out` stay as they are.  splits: how many CTAs share a sequence (None: by the sizes)"""
+        gives zeros; rows behind cu[B] of a given `out`, which lies apart from q, stay as they are.  splits: how many CTAs share a unit of rows
+        (None: by the sizes).  Values that are no numbers at positions a sequence has not reached do no harm; at others they reach every query
+        whose keys lie in the same 128"""
         whole = 0
         if splits is None:
             splits, whole = chunk_splits(q.shape[0], block_table.shape[0], self.H, q.shape[1] // self.H, block_table.shape[1])
