@@ -21,9 +21,10 @@ def rotary_tables(part, length, theta=10000.0, scaling=None, device="cuda"):
       linear    factor: positions are divided by it
       dynamic   factor, original_max_position_embeddings: theta grows once `length` is beyond the trained length, so that the slowest
                 pair's angle grows by factor * length / trained - factor + 1 less
-      yarn      factor, original_max_position_embeddings [, beta_fast 32, beta_slow 1, attention_factor]: pairs that turn more than
-                beta_fast times over the trained length keep their speed, those below beta_slow are divided by factor, a line between;
-                cos and sin times attention_factor (0.1 ln(factor) + 1)
+      yarn      factor, original_max_position_embeddings [, beta_fast 32, beta_slow 1, truncate True, attention_factor]: pairs that turn
+                more than beta_fast times over the trained length keep their speed, those below beta_slow are divided by factor, a
+                line between, which begins and ends at whole pairs (truncate false: where the turns say); cos and sin times
+                attention_factor (0.1 ln(factor) + 1)
       llama3    factor, original_max_position_embeddings, low_freq_factor 1, high_freq_factor 4: the same by wavelength
       longrope  short_factor / long_factor (one number a pair; the long ones beyond the trained length), original_max_position_embeddings
                 [, attention_factor]: every pair divided by its own"""
@@ -47,8 +48,10 @@ def rotary_tables(part, length, theta=10000.0, scaling=None, device="cuda"):
         inv = inv / factor
     elif kind == "yarn":
         pair = lambda turns: part * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(theta))        # noqa: E731
-        lo = max(0, math.floor(pair(float(sc.get("beta_fast") or 32.0))))
-        hi = min(part - 1, math.ceil(pair(float(sc.get("beta_slow") or 1.0))))
+        lo, hi = pair(float(sc.get("beta_fast") or 32.0)), pair(float(sc.get("beta_slow") or 1.0))
+        if sc.get("truncate", True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(0, lo), min(part - 1, hi)
         slow = ((torch.arange(part // 2, **f64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         inv = inv * (1 - slow) + inv / factor * slow
         given = sc.get("attention_factor")

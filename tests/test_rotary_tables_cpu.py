@@ -1,0 +1,34 @@
+"""Tables of the rotary positions for the keys that model configurations carry beside the common ones: the tables that Hugging Face models make of
+the same configuration, and refusals of what would make another table."""
+import pytest
+import torch
+
+from statetree_b200.rotary import rotary_tables
+
+PART, THETA = 64, 1e4
+
+
+def models(scaling, length, max_length):
+    """(cos, sin) in 64 bits of the frequencies and the amplitude of a model whose configuration has `scaling` and `max_length` positions"""
+    pytest.importorskip("transformers")
+    from transformers import LlamaConfig
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+    cfg = LlamaConfig(hidden_size=256, num_attention_heads=4, head_dim=PART, max_position_embeddings=max_length,
+                      rope_parameters=dict({"rope_theta": THETA}, **scaling))
+    inv, amp = ROPE_INIT_FUNCTIONS[scaling["rope_type"]](cfg, "cpu", seq_len=length)
+    ang = torch.arange(length).double()[:, None] * inv.double()
+    return ang.cos() * amp, ang.sin() * amp
+
+
+def agree(got, want, amp=2.0):
+    """theirs are float32 frequencies: each is off by some 2^-22 of itself (a power, a division, sums), the angle by as much of up to
+    `length`, cosine and sine by as much as the angle, times the amplitude"""
+    tol = amp * got[0].shape[0] * 2.0 ** -20
+    assert all(float((g - w).abs().max()) < tol for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("factor", [2.0, 32.0])
+@pytest.mark.parametrize("truncate", [True, False])
+def test_yarn_with_and_without_whole_pairs(truncate, factor):
+    sc = dict(rope_type="yarn", factor=factor, original_max_position_embeddings=512, beta_fast=32.0, beta_slow=1.0, truncate=truncate)
+    agree(rotary_tables(PART, 600, THETA, sc, device="cpu"), models(sc, 600, 512))
