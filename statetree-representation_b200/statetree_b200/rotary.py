@@ -24,7 +24,8 @@ def rotary_tables(part, length, theta=10000.0, scaling=None, device="cuda"):
       yarn      factor, original_max_position_embeddings [, beta_fast 32, beta_slow 1, truncate True, attention_factor]: pairs that turn
                 more than beta_fast times over the trained length keep their speed, those below beta_slow are divided by factor, a
                 line between, which begins and ends at whole pairs (truncate false: where the turns say); cos and sin times
-                attention_factor (0.1 ln(factor) + 1)
+                attention_factor (0.1 ln(factor) + 1; with mscale m and mscale_all_dim a both given and not 0, (0.1 m ln(factor) + 1) /
+                (0.1 a ln(factor) + 1))
       llama3    factor, original_max_position_embeddings, low_freq_factor 1, high_freq_factor 4: the same by wavelength
       longrope  short_factor / long_factor (one number a pair; the long ones beyond the trained length), original_max_position_embeddings
                 [, attention_factor]: every pair divided by its own"""
@@ -54,8 +55,9 @@ def rotary_tables(part, length, theta=10000.0, scaling=None, device="cuda"):
         lo, hi = max(0, lo), min(part - 1, hi)
         slow = ((torch.arange(part // 2, **f64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         inv = inv * (1 - slow) + inv / factor * slow
-        given = sc.get("attention_factor")
-        amp = float(given) if given is not None else 0.1 * math.log(factor) + 1.0
+        given, m, a = sc.get("attention_factor"), sc.get("mscale"), sc.get("mscale_all_dim")
+        grown = lambda by: 0.1 * float(by) * math.log(factor) + 1.0                                          # noqa: E731
+        amp = float(given) if given is not None else grown(m) / grown(a) if m and a else grown(1.0)
     elif kind == "llama3":
         low, high = float(sc.get("low_freq_factor", 1.0)), float(sc.get("high_freq_factor", 4.0))
         turns = trained * inv / (2 * math.pi)

@@ -32,3 +32,11 @@ def agree(got, want, amp=2.0):
 def test_yarn_with_and_without_whole_pairs(truncate, factor):
     sc = dict(rope_type="yarn", factor=factor, original_max_position_embeddings=512, beta_fast=32.0, beta_slow=1.0, truncate=truncate)
     agree(rotary_tables(PART, 600, THETA, sc, device="cpu"), models(sc, 600, 512))
+
+
+@pytest.mark.parametrize("more", [dict(mscale=1.0, mscale_all_dim=1.0), dict(mscale=0.707, mscale_all_dim=1.0), dict(mscale=0.707),
+                                  dict(mscale_all_dim=0.707), dict(mscale=1.0, mscale_all_dim=0.0),
+                                  dict(mscale=0.5, mscale_all_dim=1.0, attention_factor=1.3), dict(mscale=0.5, mscale_all_dim=1.0, factor=1.0)], ids=str)
+def test_yarn_amplitudes(more):
+    sc = {**dict(rope_type="yarn", factor=40.0, original_max_position_embeddings=512), **more}
+    agree(rotary_tables(PART, 600, THETA, sc, device="cpu"), models(sc, 600, 512))
