@@ -27,8 +27,11 @@ def rotary_tables(part, length, theta=10000.0, scaling=None, device="cuda"):
                 attention_factor (0.1 ln(factor) + 1; with mscale m and mscale_all_dim a both given and not 0, (0.1 m ln(factor) + 1) /
                 (0.1 a ln(factor) + 1))
       llama3    factor, original_max_position_embeddings, low_freq_factor 1, high_freq_factor 4: the same by wavelength
-      longrope  short_factor / long_factor (one number a pair; the long ones beyond the trained length), original_max_position_embeddings
-                [, attention_factor]: every pair divided by its own"""
+      longrope  short_factor / long_factor (one number a pair; the long ones beyond the trained length), original_max_position_embeddings:
+                every pair divided by its own; cos and sin times attention_factor, by default sqrt(1 + ln(s) / ln(trained length)) for
+                a stretch s above 1, which is factor or, without one, max_position_embeddings / original_max_position_embeddings.
+                The stretch is the model's, whatever the `length` of a table: one of the three must be given (a configuration
+                keeps max_position_embeddings beside its rope_scaling: dict(rope_scaling, max_position_embeddings=...))"""
     if part < 2 or part % 2 or length < 1:
         raise ValueError(f"rotary_tables: an even number of values and at least one position, got {part} and {length}")
     sc = dict(scaling or {})
@@ -68,7 +71,11 @@ def rotary_tables(part, length, theta=10000.0, scaling=None, device="cuda"):
         if by is None or len(by) != part // 2:
             raise ValueError(f"rotary_tables: longrope needs {part // 2} factors")
         inv = inv / torch.tensor(by, **f64)
-        given, stretch = sc.get("attention_factor"), float(sc.get("factor") or max(1.0, length / trained))
+        given, stretch = sc.get("attention_factor"), sc.get("factor")
+        if stretch is None and sc.get("max_position_embeddings"):
+            stretch = sc["max_position_embeddings"] / trained
+        if given is None and stretch is None:
+            raise ValueError("rotary_tables: longrope needs factor, attention_factor or max_position_embeddings")
         amp = float(given) if given is not None else (math.sqrt(1 + math.log(stretch) / math.log(trained)) if stretch > 1 else 1.0)
     elif kind not in ("default", "linear", "dynamic"):
         raise ValueError(f"rotary_tables: unknown rope_type {kind!r}")

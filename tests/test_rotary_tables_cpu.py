@@ -40,3 +40,30 @@ def test_yarn_with_and_without_whole_pairs(truncate, factor):
 def test_yarn_amplitudes(more):
     sc = {**dict(rope_type="yarn", factor=40.0, original_max_position_embeddings=512), **more}
     agree(rotary_tables(PART, 600, THETA, sc, device="cpu"), models(sc, 600, 512))
+
+
+LONG = dict(rope_type="longrope", original_max_position_embeddings=512, short_factor=[1.0 + 0.1 * i for i in range(32)],
+            long_factor=[1.0 + i for i in range(32)])
+
+
+@pytest.mark.parametrize("length", [1, 300, 512, 513, 2000])
+@pytest.mark.parametrize("max_length", [600, 8192])
+def test_longrope_amplitude_is_the_models(max_length, length):
+    """... and no table's: tables of any length of one model have the same amplitude, in the row of position 0"""
+    got = rotary_tables(PART, length, THETA, dict(LONG, max_position_embeddings=max_length), device="cpu")
+    agree(got, models(LONG, length, max_length))
+    assert bool((got[0][0] == rotary_tables(PART, 4096, THETA, dict(LONG, max_position_embeddings=max_length), device="cpu")[0][0]).all())
+
+
+@pytest.mark.parametrize("more", [dict(factor=4.0), dict(factor=4.0, attention_factor=1.7), dict(attention_factor=1.25), dict(factor=1.0)], ids=str)
+def test_longrope_amplitudes(more):
+    """a factor goes before the lengths, an attention factor before both"""
+    sc = dict(LONG, **more)
+    agree(rotary_tables(PART, 600, THETA, dict(sc, max_position_embeddings=8192), device="cpu"), models(sc, 600, 8192))
+    agree(rotary_tables(PART, 600, THETA, sc, device="cpu"), models(sc, 600, 8192))
+
+
+def test_longrope_needs_the_models_stretch():
+    for length in (300, 2000):
+        with pytest.raises(ValueError, match="max_position_embeddings"):
+            rotary_tables(PART, length, THETA, LONG, device="cpu")
