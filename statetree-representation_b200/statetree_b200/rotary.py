@@ -12,10 +12,10 @@ import torch
 from .ops import calls, ext
 
 
-def rotary_tables(part, length, theta=10000.0, scaling=None, device="cuda"):
+def rotary_tables(part, length, theta=None, scaling=None, device="cuda"):
     """(cos, sin) float32 [length, part / 2] for positions 0 .. length - 1: angle position * theta^(-2i / part), formed in 64 bits (a far
-    position times a rounded frequency is off by whole radians in 32).  scaling: a model configuration's rope_scaling, a dict with
-    rope_type (or type)
+    position times a rounded frequency is off by whole radians in 32).  theta: by default scaling's rope_theta (where a configuration
+    keeps it there), else 10000; two that differ are refused.  scaling: a model configuration's rope_scaling, a dict with rope_type (or type)
 
       default   none
       linear    factor: positions are divided by it
@@ -35,6 +35,10 @@ def rotary_tables(part, length, theta=10000.0, scaling=None, device="cuda"):
     if part < 2 or part % 2 or length < 1:
         raise ValueError(f"rotary_tables: an even number of values and at least one position, got {part} and {length}")
     sc = dict(scaling or {})
+    known = sc.get("rope_theta")
+    if theta is not None and known is not None and float(theta) != float(known):
+        raise ValueError(f"rotary_tables: theta {theta}, and rope_theta {known} in the scaling")
+    theta = float(theta if theta is not None else known if known is not None else 10000.0)
     kind = sc.get("rope_type", sc.get("type", "default"))
     f64 = dict(dtype=torch.float64, device=device)
     trained = sc.get("original_max_position_embeddings") or sc.get("max_position_embeddings")

@@ -67,3 +67,27 @@ def test_longrope_needs_the_models_stretch():
     for length in (300, 2000):
         with pytest.raises(ValueError, match="max_position_embeddings"):
             rotary_tables(PART, length, THETA, LONG, device="cpu")
+
+
+@pytest.mark.parametrize("sc", [dict(rope_type="llama3", factor=8.0, original_max_position_embeddings=512, low_freq_factor=1.0, high_freq_factor=4.0),
+                                dict(rope_type="linear", factor=2.0), dict(LONG, factor=4.0),
+                                dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=512)], ids=lambda s: s["rope_type"])
+def test_theta_of_the_configuration(sc):
+    """a configuration that keeps its base beside the scaling"""
+    own = dict(sc, rope_theta=5e5)
+    got = rotary_tables(PART, 600, scaling=own, device="cpu")
+    agree(got, models(own, 600, 512))
+    assert all(bool((a == b).all()) for a, b in zip(got, rotary_tables(PART, 600, 5e5, sc, device="cpu")))
+    assert all(bool((a == b).all()) for a, b in zip(got, rotary_tables(PART, 600, 500000, own, device="cpu")))       # (the same, twice)
+
+
+def test_theta_by_default_and_by_the_plain_kind():
+    plain, base = rotary_tables(PART, 64, device="cpu"), rotary_tables(PART, 64, 1e4, device="cpu")
+    assert all(bool((a == b).all()) for a, b in zip(plain, base))
+    plain, base = rotary_tables(PART, 64, scaling=dict(rope_type="default", rope_theta=1e6), device="cpu"), rotary_tables(PART, 64, 1e6, device="cpu")
+    assert all(bool((a == b).all()) for a, b in zip(plain, base))
+
+
+def test_two_thetas_are_refused():
+    with pytest.raises(ValueError, match="rope_theta"):
+        rotary_tables(PART, 8, 1e4, dict(rope_type="default", rope_theta=5e5), device="cpu")
