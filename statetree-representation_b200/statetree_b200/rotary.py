@@ -12,10 +12,20 @@ import torch
 from .ops import calls, ext
 
 
+# what rotary_tables reads of a configuration's rope_scaling: of every kind, of its own.  (partial_rotary_factor is in `part`; a model's and its
+# trained length are looked at by the kinds that need them)
+_KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "original_max_position_embeddings", "max_position_embeddings"}
+_KIND_KEYS = {"default": set(), "linear": {"factor"}, "dynamic": {"factor"},
+              "yarn": {"factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"},
+              "llama3": {"factor", "low_freq_factor", "high_freq_factor"}, "longrope": {"factor", "attention_factor", "short_factor", "long_factor"}}
+
+
 def rotary_tables(part, length, theta=None, scaling=None, device="cuda"):
     """(cos, sin) float32 [length, part / 2] for positions 0 .. length - 1: angle position * theta^(-2i / part), formed in 64 bits (a far
     position times a rounded frequency is off by whole radians in 32).  theta: by default scaling's rope_theta (where a configuration
     keeps it there), else 10000; two that differ are refused.  scaling: a model configuration's rope_scaling, a dict with rope_type (or type)
+    and the keys of its kind; a key with a value that its kind does not read is refused, since a model that reads it has another table (one
+    dict per kind of layer: pass the layer's).  `part` is the head's dimension times the configuration's partial_rotary_factor
 
       default   none
       linear    factor: positions are divided by it
@@ -40,6 +50,11 @@ def rotary_tables(part, length, theta=None, scaling=None, device="cuda"):
         raise ValueError(f"rotary_tables: theta {theta}, and rope_theta {known} in the scaling")
     theta = float(theta if theta is not None else known if known is not None else 10000.0)
     kind = sc.get("rope_type", sc.get("type", "default"))
+    if kind not in _KIND_KEYS:
+        raise ValueError(f"rotary_tables: unknown rope_type {kind!r}")
+    unread = sorted(str(k) for k, v in sc.items() if v is not None and k not in _KEYS | _KIND_KEYS[kind])
+    if unread:
+        raise ValueError(f"rotary_tables: rope_type {kind!r} does not read {', '.join(unread)}")
     f64 = dict(dtype=torch.float64, device=device)
     trained = sc.get("original_max_position_embeddings") or sc.get("max_position_embeddings")
     if kind in ("dynamic", "yarn", "llama3", "longrope") and not trained:
@@ -81,8 +96,6 @@ def rotary_tables(part, length, theta=None, scaling=None, device="cuda"):
         if given is None and stretch is None:
             raise ValueError("rotary_tables: longrope needs factor, attention_factor or max_position_embeddings")
         amp = float(given) if given is not None else (math.sqrt(1 + math.log(stretch) / math.log(trained)) if stretch > 1 else 1.0)
-    elif kind not in ("default", "linear", "dynamic"):
-        raise ValueError(f"rotary_tables: unknown rope_type {kind!r}")
     cos, sin = torch.empty(2, length, part // 2, dtype=torch.float32, device=device)
     step = max(1, (1 << 24) // part)                        # (in parts: the angles take twice the tables' bytes)
     for at in range(0, length, step):

@@ -91,3 +91,24 @@ def test_theta_by_default_and_by_the_plain_kind():
 def test_two_thetas_are_refused():
     with pytest.raises(ValueError, match="rope_theta"):
         rotary_tables(PART, 8, 1e4, dict(rope_type="default", rope_theta=5e5), device="cpu")
+
+
+@pytest.mark.parametrize("sc", [
+    dict(factor=2.0), dict(rope_type="default", mrope_section=[16, 24, 24]), dict(rope_type="linear", factor=2.0, mscale=1.0),
+    dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=512, attn_factor=1.5),
+    dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=512, finetuned=True), dict(LONG, factor=4.0, short_mscale=1.2),
+    dict(full_attention=dict(rope_type="default"), sliding_attention=dict(rope_type="linear", factor=2.0))], ids=str)
+def test_keys_that_are_not_read_are_refused(sc):
+    """... they make another table in a model that reads them; a whole configuration of several kinds of layers is none of one kind"""
+    with pytest.raises(ValueError, match="does not read|unknown rope_type"):
+        rotary_tables(PART, 8, scaling=sc, device="cpu")
+
+
+def test_keys_without_a_value_and_of_the_models_sizes():
+    plain = rotary_tables(PART, 8, device="cpu")
+    same = rotary_tables(PART, 8, scaling=dict(rope_type="default", mrope_section=None, factor=None, partial_rotary_factor=0.5,
+                                               max_position_embeddings=4096), device="cpu")
+    assert all(bool((a == b).all()) for a, b in zip(plain, same))
+    sc = dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=512)
+    assert all(bool((a == b).all()) for a, b in zip(rotary_tables(PART, 8, scaling=sc, device="cpu"), rotary_tables(
+        PART, 8, scaling=dict(sc, attention_factor=None, mscale=None, beta_fast=None, max_position_embeddings=4096), device="cpu")))
