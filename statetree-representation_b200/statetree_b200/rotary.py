@@ -29,8 +29,8 @@ def rotary_tables(part, length, theta=None, scaling=None, device="cuda"):
 
       default   none
       linear    factor: positions are divided by it
-      dynamic   factor, original_max_position_embeddings: theta grows once `length` is beyond the trained length, so that the slowest
-                pair's angle grows by factor * length / trained - factor + 1 less
+      dynamic   factor, max_position_embeddings (without it original_max_position_embeddings): theta grows once `length` is beyond that
+                length, so that the slowest pair's angle grows by factor * length / trained - factor + 1 less
       yarn      factor, original_max_position_embeddings [, beta_fast 32, beta_slow 1, truncate True, attention_factor]: pairs that turn
                 more than beta_fast times over the trained length keep their speed, those below beta_slow are divided by factor, a
                 line between, which begins and ends at whole pairs (truncate false: where the turns say); cos and sin times
@@ -57,6 +57,8 @@ def rotary_tables(part, length, theta=None, scaling=None, device="cuda"):
         raise ValueError(f"rotary_tables: rope_type {kind!r} does not read {', '.join(unread)}")
     f64 = dict(dtype=torch.float64, device=device)
     trained = sc.get("original_max_position_embeddings") or sc.get("max_position_embeddings")
+    if kind == "dynamic":                                   # (what such a model counts from is its maximum)
+        trained = sc.get("max_position_embeddings") or trained
     if kind in ("dynamic", "yarn", "llama3", "longrope") and not trained:
         raise ValueError(f"rotary_tables: rope_type {kind!r} needs original_max_position_embeddings")
     if kind in ("linear", "dynamic", "yarn", "llama3") and not sc.get("factor", 0) >= 1:

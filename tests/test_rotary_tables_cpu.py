@@ -112,3 +112,11 @@ def test_keys_without_a_value_and_of_the_models_sizes():
     sc = dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=512)
     assert all(bool((a == b).all()) for a, b in zip(rotary_tables(PART, 8, scaling=sc, device="cpu"), rotary_tables(
         PART, 8, scaling=dict(sc, attention_factor=None, mscale=None, beta_fast=None, max_position_embeddings=4096), device="cpu")))
+
+
+@pytest.mark.parametrize("length", [600, 1024, 1500])
+def test_dynamic_counts_from_the_models_maximum(length):
+    sc = dict(rope_type="dynamic", factor=2.0, original_max_position_embeddings=512)
+    agree(rotary_tables(PART, length, THETA, dict(sc, max_position_embeddings=1024), device="cpu"), models(sc, length, 1024))
+    agree(rotary_tables(PART, length, THETA, dict(rope_type="dynamic", factor=2.0, max_position_embeddings=1024), device="cpu"),
+          models(sc, length, 1024))
