@@ -370,7 +370,7 @@ py::object fused(const Library& lib, bool use_gemm, const at::Tensor& tree, cons
                  const at::Tensor& x, const at::Tensor& ws, const Maybe& bias, int act, const Maybe& residual) {
   const int64_t M = tree.size(0) * 16, N = tree.size(1) * 64, B = plain_rows(x, N, tree.device()), width = act == 5 ? M / 2 : M;
   const at::Device device = tree.device();
-  if (B == 0 || !on(device, eo, el, eb) || (bias && (!flat(*bias, at::kBFloat16, device) || bias->numel() != M)) ||
+  if (B == 0 || !on(device, eo, el, eb) || (bias && (!flat(*bias, at::kBFloat16, device) || bias->dim() != 1 || bias->numel() != M)) ||
       (residual && (plain_rows(*residual, width, device) != B || residual->dim() != x.dim())))
     return py::none();
   at::Tensor y;

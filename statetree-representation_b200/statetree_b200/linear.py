@@ -527,7 +527,8 @@ def fused(self, x, activation=None, residual=None, out=None):
     the bias).  x as for forward: any leading shape (any number of rows), float type and device.  activation: None, "relu", "silu",
     "gelu", "gelu_tanh", or "swiglu" for a layer built from interleave_gate_up(gate, up) (its bias in that order too): silu(gate) * up, half
     as many columns.  residual: BF16 of the result's shape, on the layer's device.  out: a contiguous BF16 result, which may be the residual
-    itself (the residual stream is then added to in place), else apart from x and residual.  Inference only: no gradients, as forward."""
+    itself (the residual stream is then added to in place), else apart from x and residual.  A bias of another float type (a layer after
+    half() or float()) is rounded to BF16 first.  Inference only: no gradients, as forward."""
     home, M, N = self._buffers["tree"].device, self.out_features, self.in_features
     if activation not in ext().ACTIVATIONS:
         raise ValueError(f"TreeLinear.fused: activation {activation!r}; there are {', '.join(map(repr, ext().ACTIVATIONS))}")
@@ -539,7 +540,9 @@ def fused(self, x, activation=None, residual=None, out=None):
     if not x.shape or x.shape[-1] != N:
         raise RuntimeError(f"statetree_b200: the layer takes inputs of {N} columns, got {tuple(x.shape)}")
     shape, B = (*x.shape[:-1], width), x.shape[:-1].numel()
-    E = ext()
+    E, bias = ext(), self.bias
+    if bias is not None and bias.dtype != torch.bfloat16:
+        bias = bias.to(torch.bfloat16)
     st = _state(home)
     ws, use_gemm = st.scratch, True
     if 1 <= B <= min(GEMV_MAX, 32) and (activation != "swiglu" or (B <= 8 and st.swiglu_gemv(M, N, B))):
@@ -547,7 +550,7 @@ def fused(self, x, activation=None, residual=None, out=None):
     tables = self._tables or self.tables()
     host = calls() if out is None and B else None
     if host is not None:                                # one native call for inputs that need no conversion
-        done = host[0].fused(host[1], use_gemm, self._buffers["tree"], tables[0], tables[1], tables[2], x, ws, self.bias, act, residual)
+        done = host[0].fused(host[1], use_gemm, self._buffers["tree"], tables[0], tables[1], tables[2], x, ws, bias, act, residual)
         if done is not None:
             return done
     for name, t in (("residual", residual), ("out", out)):
@@ -571,7 +574,6 @@ def fused(self, x, activation=None, residual=None, out=None):
         elif B == 1:
             res = res.as_strided((1, width), (width, 1))
     if B:
-        bias = self.bias
         with on_device(home.index):
             if use_gemm:
                 E.gemm_epilogue(self._buffers["tree"], tables[0], tables[1], acts, out.view(B, width), bias, act, res)

@@ -494,8 +494,15 @@ class _Weights:
     ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "swiglu": 5}
 
     @staticmethod
+    def _bias(who, bias, T):
+        """a bias as the kernels read it: BF16, one value a row of the tree T, beside it"""
+        if bias is not None and not (bias.dtype == torch.bfloat16 and bias.shape == (T.shape[0] * 16,) and bias.is_contiguous() and bias.device == T.device):
+            raise RuntimeError(f"{who}: bias BF16 [{T.shape[0] * 16}] on {T.device}, got {bias.dtype} {list(bias.shape)} on {bias.device}")
+
+    @staticmethod
     def gemv_epilogue(T, EO, EB, EL, X, Y, bias, act, res, WS):
         """Y = act(X W^T + bias) + res, up to 32 rows; act: a value of ACTIVATIONS, res rows at any stride"""
+        _Weights._bias("gemv_epilogue", bias, T)
         with _ctx(T):
             _check(lib().st_gemv_epilogue(_ptr(T), _ptr(EO), _ptr(EB), _ptr(EL), _ptr(X), _ptr(Y), _ptr(bias), act, _ptr(res),
                                           0 if res is None else res.stride(0), X.shape[0], T.shape[0] * 16, X.shape[1], _ptr(WS),
@@ -504,6 +511,7 @@ class _Weights:
     @staticmethod
     def gemm_epilogue(T, EO, EL, X, Y, bias, act, res):
         """the same for any number of rows (tcgen05)"""
+        _Weights._bias("gemm_epilogue", bias, T)
         with _ctx(T):
             _check(lib().st_gemm_epilogue(_ptr(T), _ptr(EO), _ptr(EL), _ptr(X), _ptr(Y), _ptr(bias), act, _ptr(res),
                                           0 if res is None else res.stride(0), X.shape[0], T.shape[0] * 16, X.shape[1], _stream(T)))
