@@ -8,6 +8,7 @@ their own modules.
 import math
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from .ops import calls, ext
 
@@ -133,6 +134,13 @@ def _apply(q, k, positions, cos, sin, interleaved, offset, inverse, q_norm, k_no
     return q_out, k_out
 
 
+def _has_tangent(*tensors):
+    """is one of the tensors a dual one of forward-mode differentiation"""
+    if getattr(forward_ad, "_current_level", 0) < 0:        # (no level is open: there are none)
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def rotate(q, k, positions, cos, sin, interleaved=True, offset=0, q_norm=None, k_norm=None, eps=1e-6, inverse=False, out=None):
     """(q, k) rotated by their tokens' positions: q [N, Hq, D] and k [N, Hk, D] (or None) BF16, FP16 or float32, heads and tokens at any
     stride (parts of a fused q/k/v row); positions int64 [N] (or [1]: one for all; beyond the table: its last row); cos, sin float32
@@ -141,8 +149,10 @@ def rotate(q, k, positions, cos, sin, interleaved=True, offset=0, q_norm=None, k
     fp32 arithmetic, rounded once.  out: (q, k) outputs; an output may be its input.  inverse: by the opposite angles, so that it undoes
     a rotation (by tables without an amplitude).
 
-    Gradients flow to q and k (not through norms, and not with `out`, which are refused); they are the inverse rotation.  As for every
-    function: before backward() is captured into a CUDA graph, let go of eager graphs over the same leaves."""
+    Gradients flow to q and k (not through norms, and not with `out`, which are refused; nor are there forward-mode derivatives: dual
+    tensors are refused); they are the inverse rotation.  As for every function: before backward() is captured into a CUDA graph, let go of eager graphs over the same leaves."""
+    if _has_tangent(q, k, cos, sin, q_norm, k_norm, *(out or ())):
+        raise RuntimeError("rotate: no forward-mode derivatives")
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad) or (q_norm is not None and q_norm.requires_grad)
                                     or (k_norm is not None and k_norm.requires_grad)):
         if q_norm is not None or k_norm is not None or out is not None:
