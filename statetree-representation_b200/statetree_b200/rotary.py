@@ -149,14 +149,13 @@ def rotate(q, k, positions, cos, sin, interleaved=True, offset=0, q_norm=None, k
     fp32 arithmetic, rounded once.  out: (q, k) outputs; an output may be its input.  inverse: by the opposite angles, so that it undoes
     a rotation (by tables without an amplitude).
 
-    Gradients flow to q and k (not through norms, and not with `out`, which are refused; nor are there forward-mode derivatives: dual
+    Gradients flow to q and k (not to tables or through norms, and not with `out`, which are refused; nor are there forward-mode derivatives: dual
     tensors are refused); they are the inverse rotation.  As for every function: before backward() is captured into a CUDA graph, let go of eager graphs over the same leaves."""
     if _has_tangent(q, k, cos, sin, q_norm, k_norm, *(out or ())):
         raise RuntimeError("rotate: no forward-mode derivatives")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad) or (q_norm is not None and q_norm.requires_grad)
-                                    or (k_norm is not None and k_norm.requires_grad)):
-        if q_norm is not None or k_norm is not None or out is not None:
-            raise RuntimeError("rotate: gradients flow through the rotation alone (without norms and given outputs)")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, cos, sin, q_norm, k_norm, *(out or ()))):
+        if q_norm is not None or k_norm is not None or out is not None or cos.requires_grad or sin.requires_grad:
+            raise RuntimeError("rotate: gradients flow through the rotation of q and k alone (not to tables, norms and given outputs)")
         host = calls() if k is not None else None
         if host is not None:                                # (the same function in native code)
             done = host[0].rotate_grad(host[1], q, k, positions, cos, sin, interleaved, offset, inverse)

@@ -34,3 +34,22 @@ def test_forward_mode_into_an_output():
         args = dict(arguments(), k=None, k_norm=None)
         with pytest.raises(RuntimeError, match="forward-mode"):
             rotate(**args, out=(out, None))
+
+
+@pytest.mark.parametrize("name", ["cos", "sin", "q_norm", "k_norm", "out"])
+def test_gradients_to_what_gives_none(name):
+    """... whether q needs one or not; without gradients being recorded the call is one like any other"""
+    from statetree_b200.rotary import rotate
+    for q_too in (False, True):
+        args = arguments()
+        if name not in ("q_norm", "k_norm"):
+            args.update(q_norm=None, k_norm=None)
+        if name == "out":
+            args["out"] = (torch.empty(2, 2, 64).requires_grad_(), torch.empty(2, 1, 64))
+        else:
+            args[name].requires_grad_()
+        args["q"].requires_grad_(q_too)
+        with pytest.raises(RuntimeError, match="gradients"):
+            rotate(**args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            rotate(**args)
