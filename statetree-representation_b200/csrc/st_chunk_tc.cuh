@@ -1,6 +1,8 @@
 // What the two chunk attentions on the tensor cores share (st_kv8_chunk.cu: pages in 8 bits, st_kv_chunk.cu: lossless pages): the division of
 // the rows, shared- and tensor-memory operands, the loop that issues the MMAs, and the way out of a CTA's rows.
 #pragma once
+#include <type_traits>
+
 #include "st_kv8.cuh"
 #include "st_tc.cuh"
 
@@ -205,10 +207,14 @@ struct RowWalk {
   }
 };
 // A softmax warp's rows leave: this lane's row of O (tensor memory `to`, key tiles seen: count) over its sum l, or, of a split, as it is
-// with (reference m, l).  The whole warp calls
-template <int D>
+// with (reference m, l).  The whole warp calls.  last(q).to(v) has the last word on values 32 q .. 32 q + 31 of the lane's row
+struct AsTheyAre {
+  __device__ __forceinline__ AsTheyAre operator()(int) const { return {}; }
+  __device__ __forceinline__ void to(uint32_t*) const {}
+};
+template <int D, class Last = AsTheyAre>
 __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts, const Work& w, uint8_t* const smem, int t, int warp, int lane,
-                                            bool live, int token, int hq, int count, uint32_t to, float m, float l) {
+                                            bool live, int token, int hq, int count, uint32_t to, float m, float l, const Last last = Last()) {
   tc_fence_after();
   const long long r = (long long)(w.first + token) * a.Hq + hq;
   const float inv = parts.splits > 1 ? 1.f : (l > 0.f ? 1.f / l : l);
@@ -219,8 +225,10 @@ __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts,
   }
   if (parts.splits > 1) {
     float* const o = parts.o + (r * parts.splits + w.split) * D;
-#pragma unroll
+    constexpr int AT_ONCE = std::is_same_v<Last, AsTheyAre> ? D / 32 : 1;
+#pragma unroll AT_ONCE
     for (int q = 0; q < D / 32; ++q) {
+      const auto more = last(q);                                  // (while no values are held)
       uint32_t v[32];
       if (count > 0) {
         tm_ld32(to + 32 * q, v);
@@ -228,6 +236,7 @@ __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts,
       }
 #pragma unroll
       for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
+      more.to(v);
       if (live)
 #pragma unroll
         for (int k = 0; k < 8; ++k) reinterpret_cast<uint4*>(o + 32 * q)[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
@@ -239,6 +248,7 @@ __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts,
     uint8_t* const rows = smem + Tiles<D>::Q + t * Tiles<D>::TILE + (warp & 3) * (32 * 2 * D);
 #pragma unroll 1                                                  // (code that runs once: what it costs is to be fetched)
     for (int q = 0; q < D / 32; ++q) {
+      const auto more = last(q);                                  // (while no values are held)
       uint32_t v[32];
       if (count > 0) {
         tm_ld32(to + 32 * q, v);
@@ -246,6 +256,7 @@ __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts,
       }
 #pragma unroll
       for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? __float_as_uint(__uint_as_float(v[k]) * inv) : 0u;
+      more.to(v);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t u[4];

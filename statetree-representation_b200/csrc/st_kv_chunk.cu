@@ -8,11 +8,11 @@
 // Everything else is fp32.
 //
 // Keys outside [start, len) of a sequence weigh nothing whatever their rows hold: scores are replaced, not shifted, and V's rows are zeroed
-// on the way into the operands (a probability of 0 times an infinity would be NaN).  A value that is no number at a position that the
-// sequence has reaches every query whose keys lie in the same 128.
+// on the way into the operands (a probability of 0 times an infinity would be NaN).  Infinities and NaN of V at positions that the sequence has
+// are zeroed there too, and the rows that see them get them on their way out: an infinity of either sign gives itself, both or NaN give NaN.
 //
-// Measured (32 query heads, 8 KV heads), us in a graph: 2048 queries behind 30000 tokens 1095-1120 = 0.94 PFLOP/s, a prompt of 4096 186, nine ragged
-// chunks with windows (7 heads a KV head) 101; 8 x 4 queries over 2900 tokens 33.
+// Measured (32 query heads, 8 KV heads), us in a graph: 2048 queries behind 30000 tokens 1095-1120 = 0.94 PFLOP/s, a prompt of 4096 180, nine ragged
+// chunks with windows (7 heads a KV head) 103; 8 x 4 queries over 2900 tokens 34.
 // What bounds it.  A step of 256 rows takes 2.2 us, of which the MMAs fill 1.2: the chain scores -> softmax -> product of a row tile (with the
 // conversion left out 1.9 us a step) and the converters, which share the issue slots with it (50 % used; 250 instructions a page's keys or
 // values; escapes 0.2 us of the step).  A CTA costs some 12 us besides its steps (look-ups, q, filling and draining the two row tiles' chains,
@@ -57,12 +57,18 @@ constexpr float RAISE = 8.f;
 // unit (patching the fragments takes a serial step an entry: 2048 queries behind 30000 tokens 1.5 times as long).
 struct Lists {                                     // of a page's two units: what a lane holds of the list of unit lane / 16
   uint32_t heads, head, entry, word;               // both units' headers together, its own, an entry, a word of its chain's first block
-  bool listed, odd;
+  bool listed, odd, beyond;                        // beyond: a value may be NaN or an infinity
 };
 // Entries ascend unless a row has been appended again in place: does one not?
-__device__ __forceinline__ bool out_of_order(uint32_t entry, bool listed, int lane) {
+__device__ __forceinline__ bool entry_out_of_order(uint32_t entry, bool listed, int lane) {
   const uint32_t key = listed ? entry & 1023u : 0u, before = __shfl_up_sync(FULL, key, 1, 16);
-  return __any_sync(FULL, listed && (lane & 15) > 0 && key <= before);
+  return listed && (lane & 15) > 0 && key <= before;
+}
+__device__ __forceinline__ bool out_of_order(uint32_t entry, bool listed, int lane) { return __any_sync(FULL, entry_out_of_order(entry, listed, lane)); }
+// is one of a lane's nodes, those of rows lane / 4 and 8 more of either unit, the largest exponent (NaN, infinities)
+__device__ __forceinline__ bool node_beyond(const RecRegs (&r)[2]) {
+  const uint32_t x = ~(r[0].nodes | r[1].nodes << 16);
+  return ((x - 0x01010101u) & ~x & 0x80808080u) != 0u;
 }
 __device__ __forceinline__ void page_take(const uint8_t* unit, int lane, RecRegs (&r)[2], Lists& l) {
   l.heads = 0u;
@@ -76,9 +82,17 @@ __device__ __forceinline__ void page_take(const uint8_t* unit, int lane, RecRegs
   l.entry = *reinterpret_cast<const uint32_t*>(tail + 4 + 4 * min(lane & 15, NSLOT - 1));
 }
 // (ahead of the decoding: the chain's block is looked at behind it)
-__device__ __forceinline__ void page_lists(Lists& l, const Pool& pool, int lane) {
+template <bool NARROW>
+__device__ __forceinline__ void page_lists(Lists& l, const RecRegs (&r)[2], const Pool& pool, bool values, int lane) {
   l.listed = (lane & 15) < (int)min(l.head & 15u, (uint32_t)NSLOT);
-  l.odd = out_of_order(l.entry, l.listed, lane);
+  if (NARROW) {                                    // (a warp has either keys or values: 8 x 4 queries 34.3 us, with the one vote 34.5)
+    l.odd = out_of_order(l.entry, l.listed, lane);
+    l.beyond = values && __any_sync(FULL, node_beyond(r));
+  } else {
+    const uint32_t flags = __reduce_or_sync(FULL, (entry_out_of_order(l.entry, l.listed, lane) ? 1u : 0u) | (node_beyond(r) ? 2u : 0u));
+    l.odd = flags & 1u;
+    l.beyond = values && (flags & 2u);
+  }
   l.word = (l.head & 16u) && (int)(l.head >> 8) < pool.blocks ? __ldg(pool.at + (size_t)(l.head >> 8) * 16 + (lane & 15)) : 0u;
 }
 template <int HALF>
@@ -123,6 +137,44 @@ __device__ __forceinline__ void page_patch(uint8_t* tile, Lists& l, const Pool& 
     blk = more ? (int)(w0 >> 8) - 1 : -1;
   }
 }
+// What a CTA found among its values: first and last page with NaN or infinities, and for every dimension whether there is +inf or NaN, -inf or NaN
+struct Beyond { int page0, page1; uint32_t plus[HD / 32], minus[HD / 32]; };
+// A page's values that have the largest exponent (NaN, infinities): zeros instead, and a note.  Rare: such rows show in their nodes, which is all
+// that the other pages pay (8 x 4 queries over 2900 tokens 34.3 us, 33.2 without the look and the note)
+template <int HALF>
+__device__ __forceinline__ void page_finite(uint8_t* tile, int page, Beyond* note, int lane) {
+  bool found = false;
+  __syncwarp();
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {                    // four rows of a half at a time, eight lanes a row
+    uint4* const at = reinterpret_cast<uint4*>(tile + (i >> 2) * HALF) + (i & 3) * 32 + lane;
+    const uint32_t w[4] = {at->x, at->y, at->z, at->w};
+    uint32_t out[4], plus = 0u, minus = 0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      out[k] = w[k];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint32_t bits = w[k] >> (16 * b);
+        if ((bits & 0x7F80u) != 0x7F80u) continue;
+        const bool nan = bits & 0x7Fu, less = bits & 0x8000u;
+        plus |= nan || !less ? 1u << (2 * k + b) : 0u;
+        minus |= nan || less ? 1u << (2 * k + b) : 0u;
+        out[k] &= b ? 0xFFFFu : 0xFFFF0000u;
+      }
+    }
+    if ((plus | minus) == 0u) continue;
+    found = true;
+    *at = make_uint4(out[0], out[1], out[2], out[3]);
+    const int dim = 64 * (i >> 2) + 8 * ((lane & 7) ^ ((4 * (i & 3) + (lane >> 3)) & 7));
+    atomicOr(&note->plus[dim >> 5], plus << (dim & 31));
+    atomicOr(&note->minus[dim >> 5], minus << (dim & 31));
+  }
+  if (__any_sync(FULL, found) && lane == 0) {
+    atomicMin(&note->page0, page);
+    atomicMax(&note->page1, page);
+  }
+}
 // rows of positions outside [start, len) to zero
 __device__ __forceinline__ void page_edge(uint32_t (&A)[2][4][4], int first, int start, int len, int lane) {
   const int pos = first + (lane >> 2);
@@ -137,34 +189,113 @@ __device__ __forceinline__ void page_edge(uint32_t (&A)[2][4][4], int first, int
 // before are in registers (an issue takes some 270 cycles: one warp for all sixteen of a key tile would be the limit).
 // NARROW: keys and values have slots of their own (the second set where the second row tile's q would be), so that a page's values come in while
 // its keys are decoded: these pages are read once, from memory, not by many CTAs from L2.
-struct Kept { int row0, rows, first, h, split, splits; };        // of Work, for the way out; splits: of this unit
+struct Kept { int row0, rows, first, h, split, splits, b, pos0, start; Beyond beyond; };         // of Work, for the way out; splits: of this unit
 struct LayX : Tiles<HD> {
   static constexpr int RAW = Tiles<HD>::END, SLOT_BYTES = 2 * RKV;                                 // a slot per page of a key tile
   static constexpr int BARS = RAW + 8 * SLOT_BYTES, NBARS = ChunkBars::COUNT + 34, SLOT = BARS + NBARS * 8, KEPT = SLOT + 16;
-  static constexpr int BYTES = KEPT + 48 + 1024;
+  static constexpr int BYTES = KEPT + sizeof(Kept) + 1024;
   static __device__ __forceinline__ int slot(int set, int page) { return (set ? Q + TILE : RAW) + page * SLOT_BYTES; }
 };
+
+// A bit for every one of 32 values of a row: it gets +inf, -inf; NaN is both
+struct Seen {
+  uint32_t p, n;
+  __device__ __forceinline__ void to(uint32_t* v) const {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      if (p >> k & 1u) v[k] = __float_as_uint(__uint_as_float(v[k]) + INFINITY);
+      if (n >> k & 1u) v[k] = __float_as_uint(__uint_as_float(v[k]) - INFINITY);
+    }
+  }
+};
+// What values 32 q .. 32 q + 31 of this lane's row get: the infinities and NaN of the keys lo .. hi that it sees (`only` >= 0: of those in
+// the only-th 32 of every 128), which lie in pages page0 .. page1.  Lane l looks at value 32 q + l of a key.  It ends when no row can get more
+__device__ __forceinline__ Seen beyond_seen(const Attn8& a, const Pool& pool, const Kept& kept, int page0, int page1, int q, int lo, int hi, int only,
+                                            int lane) {
+  const int col = 32 * (q & 1) + lane;
+  const uint8_t* const values = a.kv + (size_t)kept.h * PAGE_BYTES + (2 + (q >> 1)) * RKV;
+  const size_t step = (size_t)a.H * PAGE_BYTES;
+  const int* const table = a.table + (long long)kept.b * a.table_stride;
+  const volatile Beyond& note = *const_cast<const volatile Beyond*>(&kept.beyond);
+  const uint32_t all_p = __shfl_sync(FULL, note.plus[q], 0), all_n = __shfl_sync(FULL, note.minus[q], 0);
+  uint32_t p = 0u, n = 0u;
+#pragma unroll 1
+  for (int p0 = page0; p0 <= page1; p0 += 32) {
+    if (__all_sync(FULL, lo > hi || (p == all_p && n == all_n))) break;
+    int e = 0;
+    bool has = false;
+    if (p0 + lane <= page1) {
+      e = __ldg(table + p0 + lane);
+      e = e < 0 ? 0 : (int)min((long long)e, a.nblocks - 1);
+      const uint4 nodes = __ldg(reinterpret_cast<const uint4*>(values + e * step + 1536));
+      has = ((__vcmpeq4(nodes.x, ~0u) | __vcmpeq4(nodes.y, ~0u)) | (__vcmpeq4(nodes.z, ~0u) | __vcmpeq4(nodes.w, ~0u))) != 0u;
+    }
+#pragma unroll 1
+    for (uint32_t todo = __ballot_sync(FULL, has); todo; todo &= todo - 1) {
+      const int i = __ffs(todo) - 1;
+      const uint8_t* const unit = values + __shfl_sync(FULL, e, i) * step;
+#pragma unroll 1
+      for (uint32_t rows = __ballot_sync(FULL, lane < 16 && __ldg(unit + 1536 + 2 * (lane & 7) + (lane >> 3 & 1)) == 255); rows; rows &= rows - 1) {
+        const int r = __ffs(rows) - 1, pos = (p0 + i) * PAGE + r;
+        const bool sees = pos >= lo && pos <= hi && (only < 0 || (pos >> 5 & 3) == only);
+        if (!__any_sync(FULL, sees)) continue;
+        // column 16 s + 8 i + 2 t + b of row r: its leaf (mantissa << 1 | its neighbour's sign) and its state's nibble
+        const int s = col >> 4, at = (r & 7) * 4 + (col & 7) / 2, two = (col >> 3 & 1) * 2;
+        const uint8_t* const leaf = unit + (s >> 1) * 512 + at * 16 + ((s & 1) * 2 + (r >> 3)) * 4 + two;
+        const uint32_t state = __ldg(unit + 1024 + at * 16 + s * 4 + two + (col & 1)) >> (4 * (r >> 3)) & 15u;
+        uint32_t bits = state ? 0u : 0x7F80u | __ldg(leaf + (col & 1)) >> 1 | (__ldg(leaf + ((col & 1) ^ 1)) & 1u) << 15;
+        uint32_t kp = 0u, kn = 0u;
+        auto bits_of = [&] {
+          const bool beyond = (bits & 0x7F80u) == 0x7F80u, nan = bits & 0x7Fu;
+          kp = __ballot_sync(FULL, beyond && (nan || !(bits & 0x8000u)));
+          kn = __ballot_sync(FULL, beyond && (nan || (bits & 0x8000u)));
+        };
+        bits_of();
+        if (!__any_sync(FULL, sees && ((kp & ~p) | (kn & ~n)))) continue;
+        // (an entry of a row that stood there before is what counts)
+        auto look = [&](uint32_t entry) { if ((int)(entry & 1023u) == r * 64 + col) bits = entry >> 16; };
+        const uint32_t head = __ldg(reinterpret_cast<const uint32_t*>(unit + REC));
+        for (int k = 0; k < (int)min(head & 15u, (uint32_t)NSLOT); ++k) look(__ldg(reinterpret_cast<const uint32_t*>(unit + REC) + 1 + k));
+        int blk = (head & 16u) ? (int)(head >> 8) : -1;
+        for (int hops = 0; blk >= 0 && blk < pool.blocks && hops < 4096; ++hops) {
+          const uint32_t w0 = __ldg(pool.at + (size_t)blk * 16);
+          for (int k = 0; k < (int)min(w0 & 0xFFu, (uint32_t)XSLOT); ++k) look(__ldg(pool.at + (size_t)blk * 16 + 1 + k));
+          blk = (int)(w0 >> 8) - 1;
+        }
+        bits_of();
+        p |= sees ? kp : 0u;
+        n |= sees ? kn : 0u;
+      }
+    }
+  }
+  return {p, n};
+}
 
 // NARROW: up to 32 rows, which stand four times in the first row tile, once for each of its softmax warps.  A warp forms P of 32 of a step's 128
 // keys (zeros elsewhere), so that the chain scores -> softmax -> product is a quarter of the exponentials long, and its copy of the rows
 // sums up those keys' values; here the four join.  (`ok` false: the rows stay unwritten)
+template <class Last>
 __device__ __forceinline__ void narrow_store(const Attn8& a, const Parts8& parts, const Work& w, uint8_t* const smem, int warp, int lane, bool ok,
-                                             int count, uint32_t to, float m, float l) {
+                                             int count, uint32_t to, float m, float l, const Last last) {
   constexpr int ROW = HD + 4;                                     // (rows 33 x 16 bytes apart: no two lanes of eight in one bank)
   float* const park = reinterpret_cast<float*>(smem);             // [warp][row][ROW]: where q, K and V were
   float2* const ml = reinterpret_cast<float2*>(park + 4 * FEW * ROW);
   tc_fence_after();
-#pragma unroll
+  constexpr int AT_ONCE = std::is_same_v<Last, AsTheyAre> ? HD / 32 : 1;
+#pragma unroll AT_ONCE
   for (int q = 0; q < HD / 32; ++q) {
+    const auto more = last(q);
     uint32_t v[32];
     if (count > 0) {
       tm_ld32(to + 32 * q, v);
       tm_wait_ld<32>(v);
     }
 #pragma unroll
+    for (int k = 0; k < 32; ++k) v[k] = count > 0 && l != 0.f ? v[k] : 0u;
+    more.to(v);
+#pragma unroll
     for (int k = 0; k < 8; ++k)
-      *reinterpret_cast<uint4*>(park + (warp * FEW + lane) * ROW + 32 * q + 4 * k) =
-          count > 0 && l != 0.f ? make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]) : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(park + (warp * FEW + lane) * ROW + 32 * q + 4 * k) = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
   }
   ml[warp * FEW + lane] = make_float2(l > 0.f || l != l ? m : -INFINITY, ok ? l : -1.f);      // (no sum is negative: a warp that gave up)
   named_bar_sync(1, 128);
@@ -224,7 +355,7 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
   const uint64_t keep = policy_evict_last();                      // other row tiles of the sequence read the same pages
 
   if (warp == R::MMA) {
-    if (lane == 0) *reinterpret_cast<Kept*>(smem + L::KEPT) = {w.row0, w.rows, w.first, w.h, w.split, splits};
+    if (lane == 0) *reinterpret_cast<Kept*>(smem + L::KEPT) = {w.row0, w.rows, w.first, w.h, w.split, splits, w.b, w.pos0, w.lo0, {0x7FFFFFFF, -1, {}, {}}};
     if (elect_one()) {
       mbar_init(qfull, 4);
       mbar_init(qfull + 1, 4);
@@ -375,10 +506,24 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
     const int token = mine ? row / of : 0, hq = o.h * of + (mine ? row % of : 0);
     if (kept.splits < c.parts.splits && mine && (!NARROW || warp == 0))
       c.parts.ml[((long long)(o.first + token) * a.Hq + hq) * c.parts.splits * 2 + 1] = -1.f;
-    if (NARROW) {
-      narrow_store(a, parts, o, smem, warp, lane, ok, count, to, m, l);
-    } else if (ok && any) {
-      chunk_store<D>(a, parts, o, smem, t, warp, lane, mine, token, hq, count, to, m, l);
+    auto leave = [&](const auto last) {
+      if (NARROW) {
+        narrow_store(a, parts, o, smem, warp, lane, ok, count, to, m, l, last);
+      } else if (ok && any) {
+        chunk_store<D>(a, parts, o, smem, t, warp, lane, mine, token, hq, count, to, m, l, last);
+      }
+    };
+    // (what the rows here see was noted before the arrivals that their products waited for; converters of the other row tile's later keys may
+    // still be at it, so that one lane reads for all.  The rare way out apart from the usual one: in its loops a prompt of 4096 took 4 us more)
+    const int page1 = __shfl_sync(FULL, *const_cast<const volatile int*>(&kept.beyond.page1), 0);
+    if (__builtin_expect(page1 < 0, 1)) {
+      leave(AsTheyAre());
+    } else {
+      const int page0 = __shfl_sync(FULL, *const_cast<const volatile int*>(&kept.beyond.page0), 0);
+      leave([&](int q) {
+        const int at = kept.pos0 + token, last_key = mine ? min(at, a.table_width * PAGE - 1) : -1;
+        return beyond_seen(a, c.pool, kept, page0, page1, q, window_from(a.window, at, kept.start), last_key, NARROW ? warp : -1, lane);
+      });
     }
     tc_fence_before();
   } else if (warp < R::MMA) {
@@ -398,12 +543,14 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
         const bool edge = kvi && (first < w.start || first + PAGE > w.len);
         uint32_t A[2][4][4];
         Lists l;
+        bool beyond = false;
         if (first < end_page * PAGE) {
           RecRegs r[2];
           page_take(smem + L::slot(set, cw), lane, r, l);
           __syncwarp();
           if (lane == 0) mbar_arrive(rempty + 8 * set + cw);
-          page_lists(l, c.pool, lane);
+          page_lists<NARROW>(l, r, c.pool, kvi, lane);
+          beyond = l.beyond;
           decode_frag(r[0], A[0]);
           decode_frag(r[1], A[1]);
           if (edge) page_edge(A, first, w.start, w.len, lane);
@@ -420,6 +567,7 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
         uint8_t* const tile = smem + (kvi ? L::V : L::K) + s * L::TILE + cw * (PAGE * 128);
         page_store<L::HALF>(tile, A, lane);
         page_patch<L::HALF>(tile, l, c.pool, edge, first, w.start, w.len, lane);
+        if (beyond) page_finite<L::HALF>(tile, first / PAGE, &reinterpret_cast<Kept*>(smem + L::KEPT)->beyond, lane);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive((kvi ? b.vfull : b.kfull) + s);

@@ -80,8 +80,9 @@ class PageStore:
         sequence b's rows are cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1]; None: one each), the last of them at position lens[b] - 1 ->
         [T, Hq, 128].  A query at position p sees tokens [max(starts, p - window + 1), p] (window 0: from starts on), one that sees none
         gives zeros; rows behind cu[B] of a given `out`, which lies apart from q, stay as they are.  splits: how many CTAs share a unit of rows
-        (None: by the sizes).  Values that are no numbers at positions a sequence has not reached do no harm; at others they reach every query
-        whose keys lie in the same 128"""
+        (None: by the sizes, with the table's width for the context: a table no wider than the longest sequence splits best).  Values that
+        are no numbers reach the queries that see them and no others (an infinity as itself, whatever it weighs).  Probabilities are rounded
+        to BF16 for the product with the values, 2^-8 of each at most, as the output (attention() keeps some sixteen bits of them).  No gradients"""
         whole = 0
         if splits is None:
             splits, whole = chunk_splits(q.shape[0], block_table.shape[0], self.H, q.shape[1] // self.H, block_table.shape[1])
