@@ -212,7 +212,10 @@ struct AsTheyAre {
   __device__ __forceinline__ AsTheyAre operator()(int) const { return {}; }
   __device__ __forceinline__ void to(uint32_t*) const {}
 };
-template <int D, class Last = AsTheyAre>
+// WALK: where the rows lie is walked to, from w, by code that is not unrolled; else it comes from the lanes that own them (live, token, hq).  Of two
+// ways to the same end each kernel has the one whose registers leave its loop alone: 8-bit pages 2048 queries behind 30000 tokens 1024 us walked,
+// 960 not, nine chunks of dimension 64 52.9 and 52.1; lossless pages, with w from shared memory, a prompt of 4096 179 and 184
+template <int D, bool WALK, class Last = AsTheyAre>
 __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts, const Work& w, uint8_t* const smem, int t, int warp, int lane,
                                             bool live, int token, int hq, int count, uint32_t to, float m, float l, const Last last = Last()) {
   tc_fence_after();
@@ -246,7 +249,8 @@ __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts,
     // the warp's rows leave through where its rows of q were (their last scores are done), D / 8 lanes a row
     constexpr int LANES = D / 8, PER = 32 / LANES;
     uint8_t* const rows = smem + Tiles<D>::Q + t * Tiles<D>::TILE + (warp & 3) * (32 * 2 * D);
-#pragma unroll 1                                                  // (code that runs once: what it costs is to be fetched)
+    constexpr int AT_ONCE = WALK ? 1 : D / 32;                    // (code that runs once: what it costs is to be fetched)
+#pragma unroll AT_ONCE
     for (int q = 0; q < D / 32; ++q) {
       const auto more = last(q);                                  // (while no values are held)
       uint32_t v[32];
@@ -266,14 +270,26 @@ __device__ __forceinline__ void chunk_store(const Attn8& a, const Parts8& parts,
       }
     }
     __syncwarp();
-    int row = lane / LANES;
-    const int at = t * ROWS + (warp & 3) * 32 + row, G = a.Hq / a.H;
-    RowWalk to_row(w.row0 + at, G);
+    if constexpr (WALK) {
+      int row = lane / LANES;
+      const int at = t * ROWS + (warp & 3) * 32 + row, G = a.Hq / a.H;
+      RowWalk to_row(w.row0 + at, G);
 #pragma unroll 4
-    for (int i = 0; i < LANES; ++i, row += PER, to_row.step(PER))
-      if (at + i * PER < w.rows)
-        *reinterpret_cast<uint4*>(a.out + (long long)(w.first + to_row.token) * a.out_stride + (w.h * G + to_row.head) * D + 8 * (lane % LANES)) =
-            *reinterpret_cast<const uint4*>(rows + row * (2 * D) + (((lane % LANES) ^ (row & 7)) << 4));
+      for (int i = 0; i < LANES; ++i, row += PER, to_row.step(PER))
+        if (at + i * PER < w.rows)
+          *reinterpret_cast<uint4*>(a.out + (long long)(w.first + to_row.token) * a.out_stride + (w.h * G + to_row.head) * D + 8 * (lane % LANES)) =
+              *reinterpret_cast<const uint4*>(rows + row * (2 * D) + (((lane % LANES) ^ (row & 7)) << 4));
+    } else {
+      const long long mine = live ? (long long)(w.first + token) * a.out_stride + (long long)hq * D : -1;
+#pragma unroll
+      for (int i = 0; i < LANES; ++i) {
+        const int row = i * PER + lane / LANES;
+        const long long to_row = __shfl_sync(FULL, mine, row);
+        if (to_row >= 0)
+          *reinterpret_cast<uint4*>(a.out + to_row + 8 * (lane % LANES)) =
+              *reinterpret_cast<const uint4*>(rows + row * (2 * D) + (((lane % LANES) ^ (row & 7)) << 4));
+      }
+    }
   }
 }
 }  // namespace st

@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_chunk_kernel(const Chunk8 c
     if (ok && count > 0) ok = mbar_wait(ofull + t, 0);
     if (!ok && lane == 0) atomicExch(c.status, ERR_WAIT_ACC);
     // ---- out.  (a wait that ran out leaves the rows unwritten)
-    if (ok && any) chunk_store<D>(a, c.parts, w, smem, t, warp, lane, live, token, hq, count, to, m, l);
+    if (ok && any) chunk_store<D, false>(a, c.parts, w, smem, t, warp, lane, live, token, hq, count, to, m, l);
     tc_fence_before();
   } else if (warp < W_MMA) {
     regs_down<R_CONV>();

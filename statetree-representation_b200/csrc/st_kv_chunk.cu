@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(Roles<NARROW>::WARPS * 32, 1) kv_chunk_kernel(
       if (NARROW) {
         narrow_store(a, parts, o, smem, warp, lane, ok, count, to, m, l, last);
       } else if (ok && any) {
-        chunk_store<D>(a, parts, o, smem, t, warp, lane, mine, token, hq, count, to, m, l, last);
+        chunk_store<D, true>(a, parts, o, smem, t, warp, lane, mine, token, hq, count, to, m, l, last);
       }
     };
     // (what the rows here see was noted before the arrivals that their products waited for; converters of the other row tile's later keys may
