@@ -136,8 +136,6 @@ def _apply(q, k, positions, cos, sin, interleaved, offset, inverse, q_norm, k_no
 
 def _has_tangent(*tensors):
     """is one of the tensors a dual one of forward-mode differentiation"""
-    if getattr(forward_ad, "_current_level", 0) < 0:        # (no level is open: there are none)
-        return False
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
@@ -151,9 +149,12 @@ def rotate(q, k, positions, cos, sin, interleaved=True, offset=0, q_norm=None, k
 
     Gradients flow to q and k (not to tables or through norms, and not with `out`, which are refused; nor are there forward-mode derivatives: dual
     tensors are refused); they are the inverse rotation.  As for every function: before backward() is captured into a CUDA graph, let go of eager graphs over the same leaves."""
-    if _has_tangent(q, k, cos, sin, q_norm, k_norm, *(out or ())):
+    # (a level of forward mode is open; where torch does not say so, it is looked for in the tensors)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and _has_tangent(q, k, cos, sin, q_norm, k_norm, *(out or ())):
         raise RuntimeError("rotate: no forward-mode derivatives")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, cos, sin, q_norm, k_norm, *(out or ()))):
+    if torch.is_grad_enabled() and (q.requires_grad or cos.requires_grad or sin.requires_grad or (k is not None and k.requires_grad)
+                                    or (q_norm is not None and q_norm.requires_grad) or (k_norm is not None and k_norm.requires_grad)
+                                    or (out is not None and any(t is not None and t.requires_grad for t in out))):
         if q_norm is not None or k_norm is not None or out is not None or cos.requires_grad or sin.requires_grad:
             raise RuntimeError("rotate: gradients flow through the rotation of q and k alone (not to tables, norms and given outputs)")
         host = calls() if k is not None else None
