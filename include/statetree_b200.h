@@ -314,7 +314,8 @@ int st_gemm_epilogue(const void* tree, const int32_t* eo, const uint32_t* el, co
  * (st_kv_append): q, out BF16 [T, Hq, 128] (16-byte aligned, token strides qs / os multiples of 8); cu int32 [B + 1]: sequence b's queries
  * are rows cu[b] .. cu[b + 1] - 1, the last at position lens[b] - 1 (cu NULL: one each).  A query at position p sees keys
  * [max(starts, p - window + 1), p] (starts int32 [B] or NULL; window 0: from starts on); one that sees none gives zeros.  bt int32: rows
- * of btw entries, bts apart (0: one row for all); keys beyond a row's pages take no part.  Rows of q behind cu[B] are left alone in
+ * of btw entries, bts apart (0: one row for all); keys beyond a row's pages take no part.  Infinities and NaN among the values reach the queries
+ * that see them and no others.  Rows of q behind cu[B] are left alone in
  * out.  S splits of every unit (a tile of 256 rows, or of 32 where sequences have at most as many on the mean, and a KV head) but the
  * first `whole`, which are the last tiles of the last sequences; wo float [T, Hq, S, 128] and wml float [T, Hq, S, 2] when S > 1
  * (st_kv_chunk_attn_workspace_bytes is what both take).  Any number of query heads per KV head.  No counterpart in the reference,

@@ -17,7 +17,8 @@ rotates and appends through their append, and a prompt runs in one pass (prefill
 
 `whole_prompts=True` runs prompts in one pass over the lossless pages too: q/k/v rows are normed and rotated (rotary.rotate), appended, and
 the queries attend to the pages (PageStore.chunk_attention); the o and down projections add the residual stream in their epilogue, and
-SwiGLU is the gate/up projection's (TreeLinear.fused).  Decode steps stay as they are.
+SwiGLU is the gate/up projection's (TreeLinear.fused).  Probabilities of that attention are rounded to BF16, 2^-8 of each at most; decode
+steps, which keep some sixteen bits of them, stay as they are.
 """
 import math
 from dataclasses import dataclass

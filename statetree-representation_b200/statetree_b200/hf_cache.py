@@ -19,7 +19,7 @@ cache then, since the keys of the refused pass have been appended.  Decode steps
 
 StateTreeKVCache(..., paged_prompts=True) does the same over the lossless pages (kvcache.PageStore.chunk_attention): a chunk of a prompt
 attends to the pages, which are no longer expanded to BF16 for it, sliding windows hold in decode steps too, and the same masks and
-modules are refused.
+modules are refused.  There, and in the decode steps of windowed layers, probabilities are rounded to BF16 (2^-8 of each at most).
 """
 import threading
 import weakref
